@@ -366,6 +366,69 @@ int hipenvs_legged_es_rollout_seeded(int32_t c, int32_t hidden, int32_t iters, i
                                      float height_gate, double assist, float* fitness, float* steps,
                                      void* workspace, int64_t workspace_bytes, hipenvs_stream_t stream);
 
+/* ---- Sequence policies (no reference counterpart) ----------------------- */
+
+/* Linear attention with a decay for each head. Per row (b, h), with lambda =
+ * exp(log_decay[h]) and a state S (dk, dv) f32:
+ *   S_t = (reset_t ? 0 : lambda S_{t-1}) + k_t v_t^T,   o_t = scale S_t^T q_t.
+ * dtype 0: q, k, v, out f32; 1: bfloat16 (raw 16 bits). q, k (b, t, h, dk) and v (b, t, h, dv)
+ * with unit stride in the last axis and any strides (in elements) in the others; `strides`, a
+ * host array, holds b, t, h of q, of k, of v, then b, t of reset. log_decay (h) f32; reset
+ * (b, t) u8 or NULL (none); state (b, h, dk, dv) f32 contiguous or NULL (zeros).
+ * -> out (b, t, h, dv) contiguous, final_state (b, h, dk, dv) f32 (may be `state`).
+ * 1 <= dk, dv <= 128. What a token before a reset or after t holds, a NaN or an infinity
+ * among it, does not reach o_t. */
+int hipenvs_decay_attention(int32_t dtype, const void* q, const void* k, const void* v,
+                            const int64_t* strides, const float* log_decay, const float* state,
+                            const uint8_t* reset, float scale, void* out, float* final_state,
+                            int64_t b, int64_t t, int32_t h, int32_t dk, int32_t dv,
+                            hipenvs_stream_t stream);
+
+/* Gradients of the above: dout like out with strides of its own, dfinal (b, h, dk, dv) f32
+ * contiguous or NULL (zeros) -> dq, dk_out, dv_out (b, t, h, dk or dv) contiguous in dtype,
+ * dstate (b, h, dk, dv) f32. `strides`: b, t, h of q, k, v, dout, then b, t of reset. The
+ * decays are constants of their heads and have no gradient. */
+int hipenvs_decay_attention_backward(int32_t dtype, const void* q, const void* k, const void* v,
+                                     const void* dout, const int64_t* strides, const float* log_decay,
+                                     const float* state, const uint8_t* reset, const float* dfinal,
+                                     float scale, void* dq, void* dk_out, void* dv_out, float* dstate,
+                                     int64_t b, int64_t t, int32_t h, int32_t dk, int32_t dv,
+                                     hipenvs_stream_t stream);
+
+/* One token of n environments: q, k (n, h, dk), v (n, h, dv) with strides of n and h and unit
+ * stride in the last axis, state (n, h, dk, dv) f32 contiguous, reset (n) u8 with stride
+ * reset_sn, or NULL -> out (n, h, dv) contiguous, next_state (n, h, dk, dv), which may be
+ * `state`. */
+int hipenvs_decay_attention_step(int32_t dtype, const void* q, int64_t q_sn, int64_t q_sh,
+                                 const void* k, int64_t k_sn, int64_t k_sh, const void* v,
+                                 int64_t v_sn, int64_t v_sh, const float* log_decay,
+                                 const float* state, const uint8_t* reset, int64_t reset_sn,
+                                 float scale, void* out, float* next_state, int64_t n, int32_t h,
+                                 int32_t dk, int32_t dv, hipenvs_stream_t stream);
+
+/* One AdamW step over `count` tensors, in place:
+ *   m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g^2,
+ *   p = keep p - (rates[k] m) / (sqrt(v) roots[k] + eps).
+ * params, grads, sizes, types, rates and roots are host arrays of `count`; types[k] is 1 for a
+ * bfloat16 parameter plus 2 for a bfloat16 gradient (float32 otherwise); a NULL gradient leaves
+ * its tensor and moments as they are. For AdamW, keep = 1 - lr * weight_decay, rates[k] =
+ * lr / (1 - beta1^t) and roots[k] = 1 / sqrt(1 - beta2^t) at that tensor's step t.
+ * The moments are flat, tensor after tensor, each beginning at a multiple of 256 values.
+ * bits 32: m, v f32, scales unused. bits 8: m i8 and v u8 codes (4-byte aligned) and a scale for
+ * every 256 values, m = scale t|t| with t = code / 127, v = scale t^4 with t = code / 255; the
+ * parameters are updated from the moments before they are rounded. A block with a NaN or
+ * an infinity in its moments reads back as NaN. */
+int hipenvs_adamw_step(int32_t bits, int32_t count, void* const* params, const void* const* grads,
+                       const int64_t* sizes, const int32_t* types, const double* rates,
+                       const double* roots, double beta1, double beta2, double eps, double keep,
+                       void* m, void* v, float* m_scales, float* v_scales, hipenvs_stream_t stream);
+
+/* The values 8-bit moments stand for: `blocks` blocks of 256 codes and their scales -> m, v
+ * (256 * blocks) f32, 16-byte aligned. */
+int hipenvs_adamw_decode(const void* m_codes, const void* v_codes, const float* m_scales,
+                         const float* v_scales, int64_t blocks, float* m, float* v,
+                         hipenvs_stream_t stream);
+
 /* ---- Diagnostics (no reference counterpart) ---------------------------- */
 
 /* Elementwise deterministic sin, cos, tanh of x (n) as the kernels compute them;

@@ -1,0 +1,312 @@
+// One AdamW step over many tensors at once, moments in 32 bits or in 8 bits with a scale for
+// every 256 values, and the read-back of 8-bit moments. No reference counterpart: the
+// reference's learners call their array library's optimizer.
+//
+//   m' = b1 m + (1 - b1) g          v' = b2 v + (1 - b2) g^2
+//   p' = keep p - (rate m') / (sqrt(v') root + eps),
+//   keep = 1 - lr wd, rate = lr / (1 - b1^t), root = 1 / sqrt(1 - b2^t)
+//
+// All arithmetic is float32, each operation rounded on its own (the library's
+// -ffp-contract=off), with correctly rounded division and square root, so the result is a
+// function of the inputs bit for bit. Parameters and gradients are float32 or bfloat16;
+// a bfloat16 parameter is rounded once, to nearest even, when it is written.
+#include "hipenvs_device.h"
+
+namespace hipenvs {
+namespace adamw {
+
+constexpr int kQuant = 256;          // values that share one scale, and the grain of the flat moments
+constexpr int kTile = 1024;          // values a block takes: four quant blocks, one for each wave
+constexpr int kMaxTensors = 64;      // of one launch: its descriptors are kernel arguments, below 4 KiB
+constexpr uint32_t kParamBf16 = 1, kGradBf16 = 2, kWide = 4;
+
+struct Tensor {
+  void* param;
+  const void* grad;
+  int64_t n;
+  int64_t at;       // where its moments begin, a multiple of kQuant
+  uint32_t tile0;   // the first of its tiles in this launch
+  uint32_t types;   // kParamBf16 | kGradBf16 | kWide: every pointer takes four values at once
+  float rate, root;
+};
+
+struct Batch {
+  Tensor t[kMaxTensors];
+  int32_t count;
+  float beta1, rest1, beta2, rest2, eps, keep;
+};
+
+__device__ __forceinline__ float bf16_to_f32(uint32_t u) { return __uint_as_float(u << 16); }
+
+// Nearest even; a NaN stays a NaN.
+__device__ __forceinline__ uint32_t f32_to_bf16(float x) {
+  const uint32_t u = __float_as_uint(x);
+  const uint32_t r = (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16;
+  return x != x ? ((u >> 16) | 0x40u) : r;
+}
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// Four values at `i` of a float32 or bfloat16 array of n; beyond n they are zero.
+__device__ __forceinline__ void load4(const void* base, int64_t i, int64_t n, bool bf16, bool wide, float (&x)[4]) {
+  if (wide && i + 4 <= n) {
+    if (bf16) {
+      const u32x2 w = *(const u32x2*)((const uint16_t*)base + i);
+      x[0] = bf16_to_f32(w.x & 0xFFFFu), x[1] = bf16_to_f32(w.x >> 16);
+      x[2] = bf16_to_f32(w.y & 0xFFFFu), x[3] = bf16_to_f32(w.y >> 16);
+    } else {
+      const f32x4 w = *(const f32x4*)((const float*)base + i);
+      x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    x[e] = 0.0f;
+    if (i + e < n) x[e] = bf16 ? bf16_to_f32(((const uint16_t*)base)[i + e]) : ((const float*)base)[i + e];
+  }
+}
+
+__device__ __forceinline__ void store4(void* base, int64_t i, int64_t n, bool bf16, bool wide, const float (&x)[4]) {
+  if (wide && i + 4 <= n) {
+    if (bf16) {
+      const u32x2 w = {f32_to_bf16(x[0]) | (f32_to_bf16(x[1]) << 16), f32_to_bf16(x[2]) | (f32_to_bf16(x[3]) << 16)};
+      *(u32x2*)((uint16_t*)base + i) = w;
+    } else {
+      const f32x4 w = {x[0], x[1], x[2], x[3]};
+      *(f32x4*)((float*)base + i) = w;
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (i + e < n) {
+      if (bf16)
+        ((uint16_t*)base)[i + e] = (uint16_t)f32_to_bf16(x[e]);
+      else
+        ((float*)base)[i + e] = x[e];
+    }
+}
+
+__device__ __forceinline__ float moved(float p, float m, float v, const Batch& b, const Tensor& t) {
+  return p * b.keep - (m * t.rate) / (sqrt_rn(v) * t.root + b.eps);
+}
+
+// The tensor whose tiles hold `tile`: the last one that begins at or before it. Uniform over
+// the block, over at most 64 descriptors in the kernel's arguments.
+__device__ __forceinline__ int find(const Batch& b, uint32_t tile) {
+  int lo = 0, hi = b.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (b.t[mid].tile0 <= tile)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
+__global__ __launch_bounds__(kBlock) void step32_kernel(Batch b, float* __restrict__ m_all, float* __restrict__ v_all) {
+  const Tensor& t = b.t[find(b, blockIdx.x)];
+  const int64_t i = (int64_t)(blockIdx.x - t.tile0) * kTile + 4 * threadIdx.x;
+  if (i >= t.n) return;
+  const bool wide = t.types & kWide, pb = t.types & kParamBf16, gb = t.types & kGradBf16;
+  float* m_at = m_all + t.at;
+  float* v_at = v_all + t.at;
+  float p[4], g[4], m[4], v[4];
+  load4(t.param, i, t.n, pb, wide, p);
+  load4(t.grad, i, t.n, gb, wide, g);
+  load4(m_at, i, t.n, false, wide, m);
+  load4(v_at, i, t.n, false, wide, v);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    m[e] = m[e] * b.beta1 + g[e] * b.rest1;
+    v[e] = v[e] * b.beta2 + (g[e] * g[e]) * b.rest2;
+    p[e] = moved(p[e], m[e], v[e], b, t);
+  }
+  store4(t.param, i, t.n, pb, wide, p);
+  store4(m_at, i, t.n, false, wide, m);
+  store4(v_at, i, t.n, false, wide, v);
+}
+
+// ---- 8-bit moments -------------------------------------------------------------------
+// A block of 256 values keeps its largest magnitude A (float32) and a code for each value:
+// of m, c in [-127, 127] for A t |t| with t = c / 127; of v, c in [0, 255] for A t^4 with
+// t = c / 255, so sqrt(v), which divides the update, is held as a square like m. Rounding is
+// to the nearest code of the root. No v above zero gets code 0: a denominator would fall to
+// eps, and the update would grow by orders of magnitude. A block with a NaN or an infinity
+// has that as its scale and reads back as NaN; one whose largest magnitude is subnormal has
+// the smallest normal number as its scale, whose reciprocal is finite.
+
+__device__ __forceinline__ float decode_m(int c, float scale) {
+  const float t = (float)c * (float)(1.0 / 127.0);
+  return (t * __builtin_fabsf(t)) * scale;
+}
+
+__device__ __forceinline__ float decode_v(uint32_t c, float scale) {
+  float t = (float)c * (float)(1.0 / 255.0);
+  t = t * t;
+  return (t * t) * scale;
+}
+
+// The largest of a wave's magnitudes, as bits, which order like the magnitudes with the
+// infinities and NaN above every number.
+__device__ __forceinline__ float wave_scale(const float (&x)[4]) {
+  uint32_t u = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t a = __float_as_uint(x[e]) & 0x7FFFFFFFu;
+    u = a > u ? a : u;
+  }
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) {
+    const uint32_t o = (uint32_t)__shfl_xor((int)u, s);
+    u = o > u ? o : u;
+  }
+  return __uint_as_float(u != 0 && u < 0x00800000u ? 0x00800000u : u);
+}
+
+// The nearest whole number in 0 .. top of y * top; 0 for a NaN.
+__device__ __forceinline__ int code_of(float y, float top) {
+  const float c = __builtin_rintf(y * top);
+  return c == c ? (int)__builtin_fminf(c, top) : 0;
+}
+
+__global__ __launch_bounds__(kBlock) void step8_kernel(Batch b, uint32_t* __restrict__ m_codes,
+                                                       uint32_t* __restrict__ v_codes, float* __restrict__ m_scales,
+                                                       float* __restrict__ v_scales) {
+  const Tensor& t = b.t[find(b, blockIdx.x)];
+  const int64_t first = (int64_t)(blockIdx.x - t.tile0) * kTile;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  if (first + wave * kQuant >= t.n) return;   // the whole wave: its quant block is past the tensor
+  const int64_t i = first + 4 * threadIdx.x;
+  const bool wide = t.types & kWide, pb = t.types & kParamBf16, gb = t.types & kGradBf16;
+  const int64_t word = (t.at + i) >> 2, block = (t.at + first) / kQuant + wave;
+  float p[4], g[4], m[4], v[4];
+  load4(t.param, i, t.n, pb, wide, p);
+  load4(t.grad, i, t.n, gb, wide, g);
+  const uint32_t mc = m_codes[word], vc = v_codes[word];
+  const float ms = m_scales[block], vs = v_scales[block];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    m[e] = decode_m((int)(int8_t)(mc >> (8 * e)), ms) * b.beta1 + g[e] * b.rest1;
+    v[e] = decode_v((vc >> (8 * e)) & 0xFFu, vs) * b.beta2 + (g[e] * g[e]) * b.rest2;
+    if (i + e >= t.n) m[e] = v[e] = 0.0f;   // the padding stays zero, also in a block that reads back as NaN
+  }
+  const float new_ms = wave_scale(m), new_vs = wave_scale(v);
+  const float m_inv = new_ms > 0.0f ? 1.0f / new_ms : 0.0f, v_inv = new_vs > 0.0f ? 1.0f / new_vs : 0.0f;
+  uint32_t new_mc = 0, new_vc = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int cm = code_of(sqrt_rn(__builtin_fabsf(m[e]) * m_inv), 127.0f);
+    int cv = code_of(sqrt_rn(sqrt_rn(v[e] * v_inv)), 255.0f);
+    cv = v[e] > 0.0f && cv < 1 ? 1 : cv;
+    new_mc |= ((uint32_t)(m[e] < 0.0f ? -cm : cm) & 0xFFu) << (8 * e);
+    new_vc |= (uint32_t)cv << (8 * e);
+    p[e] = moved(p[e], m[e], v[e], b, t);
+  }
+  store4(t.param, i, t.n, pb, wide, p);
+  m_codes[word] = new_mc;
+  v_codes[word] = new_vc;
+  if (lane == 0) {
+    m_scales[block] = new_ms;
+    v_scales[block] = new_vs;
+  }
+}
+
+__global__ __launch_bounds__(kBlock) void decode_kernel(const uint32_t* __restrict__ m_codes,
+                                                        const uint32_t* __restrict__ v_codes,
+                                                        const float* __restrict__ m_scales,
+                                                        const float* __restrict__ v_scales, int64_t words,
+                                                        float* __restrict__ m, float* __restrict__ v) {
+  const int64_t word = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  if (word >= words) return;
+  const int64_t block = word / (kQuant / 4);
+  const uint32_t mc = m_codes[word], vc = v_codes[word];
+  const float ms = m_scales[block], vs = v_scales[block];
+  float x[4], y[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    x[e] = decode_m((int)(int8_t)(mc >> (8 * e)), ms);
+    y[e] = decode_v((vc >> (8 * e)) & 0xFFu, vs);
+  }
+  store4(m, 4 * word, 4 * words, false, true, x);
+  store4(v, 4 * word, 4 * words, false, true, y);
+}
+
+bool aligned(const void* p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
+
+}  // namespace adamw
+}  // namespace hipenvs
+
+using namespace hipenvs;
+using namespace hipenvs::adamw;
+
+extern "C" int hipenvs_adamw_step(int32_t bits, int32_t count, void* const* params, const void* const* grads,
+                                  const int64_t* sizes, const int32_t* types, const double* rates,
+                                  const double* roots, double beta1, double beta2, double eps, double keep, void* m,
+                                  void* v, float* m_scales, float* v_scales, hipenvs_stream_t stream) {
+  if ((bits != 32 && bits != 8) || count < 0) return HIPENVS_E_ARG;
+  if (count == 0) return HIPENVS_OK;
+  if (!params || !grads || !sizes || !types || !rates || !roots) return HIPENVS_E_ARG;
+  int64_t total = 0;
+  for (int32_t k = 0; k < count; ++k) {
+    if (sizes[k] < 0 || sizes[k] > (int64_t)1 << 40 || (types[k] & ~3)) return HIPENVS_E_ARG;
+    if (sizes[k] > 0 && !params[k]) return HIPENVS_E_ARG;
+    total += sizes[k];
+  }
+  if (total == 0) return HIPENVS_OK;
+  if (!m || !v || !aligned(m, 4) || !aligned(v, 4)) return HIPENVS_E_ARG;
+  if (bits == 8 && (!m_scales || !v_scales)) return HIPENVS_E_ARG;
+  const bool moments_wide = bits == 8 || (aligned(m, 16) && aligned(v, 16));
+  Batch b;
+  b.beta1 = (float)beta1, b.rest1 = (float)(1.0 - beta1);
+  b.beta2 = (float)beta2, b.rest2 = (float)(1.0 - beta2);
+  b.eps = (float)eps, b.keep = (float)keep;
+  b.count = 0;
+  int64_t at = 0;
+  uint64_t tiles = 0;
+  const auto launch = [&]() {
+    const dim3 grid((unsigned)tiles), block(kBlock);
+    if (bits == 32)
+      hipLaunchKernelGGL(step32_kernel, grid, block, 0, as_stream(stream), b, (float*)m, (float*)v);
+    else
+      hipLaunchKernelGGL(step8_kernel, grid, block, 0, as_stream(stream), b, (uint32_t*)m, (uint32_t*)v, m_scales,
+                         v_scales);
+    b.count = 0;
+    tiles = 0;
+    return launch_status();
+  };
+  for (int32_t k = 0; k < count; ++k) {
+    const int64_t n = sizes[k];
+    if (n > 0 && grads[k]) {   // a tensor without a gradient keeps its parameters and its moments
+      const uint64_t own = (uint64_t)((n + kTile - 1) / kTile);
+      if (b.count == kMaxTensors || tiles + own > 0x7FFFFFFFu) {
+        const int status = launch();
+        if (status != HIPENVS_OK) return status;
+      }
+      const bool wide = moments_wide && aligned(params[k], (types[k] & 1) ? 8 : 16) &&
+                        aligned(grads[k], (types[k] & 2) ? 8 : 16);
+      b.t[b.count++] = {params[k], grads[k], n, at, (uint32_t)tiles, (uint32_t)types[k] | (wide ? kWide : 0u),
+                        (float)rates[k], (float)roots[k]};
+      tiles += own;
+    }
+    at += (n + kQuant - 1) / kQuant * kQuant;
+  }
+  return b.count ? launch() : HIPENVS_OK;
+}
+
+extern "C" int hipenvs_adamw_decode(const void* m_codes, const void* v_codes, const float* m_scales,
+                                    const float* v_scales, int64_t blocks, float* m, float* v,
+                                    hipenvs_stream_t stream) {
+  if (blocks < 0 || blocks > (int64_t)1 << 32) return HIPENVS_E_ARG;
+  if (blocks == 0) return HIPENVS_OK;
+  if (!m_codes || !v_codes || !m_scales || !v_scales || !m || !v) return HIPENVS_E_ARG;
+  if (!aligned(m_codes, 4) || !aligned(v_codes, 4) || !aligned(m, 16) || !aligned(v, 16)) return HIPENVS_E_ARG;
+  const int64_t words = blocks * (kQuant / 4);
+  hipLaunchKernelGGL(decode_kernel, dim3(grid_for(words)), dim3(kBlock), 0, as_stream(stream),
+                     (const uint32_t*)m_codes, (const uint32_t*)v_codes, m_scales, v_scales, words, m, v);
+  return launch_status();
+}

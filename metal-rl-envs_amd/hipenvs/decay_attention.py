@@ -1,0 +1,194 @@
+"""Linear attention with a decay for each head, for policies with a memory: over collected
+trajectories (``sequence``, with gradients) and for one step of every environment (``step``).
+The reference has no counterpart; its policies see the current observation only.
+
+A head of a row keeps a state S (dk, dv) in float32, with lambda = exp(log_decay[h]):
+
+    S_t = lambda S_{t-1} + k_t v_t^T          o_t = scale * S_t^T q_t
+
+and lambda S_{t-1} is left out where ``reset`` marks token t as the first of an episode (the
+``done`` of the environment step before it). ``scale`` defaults to 1 / sqrt(dk). Acting costs
+the same at every step, whatever the episode's length: the state is the whole memory.
+``sequence`` over a trajectory and ``step`` token by token compute the same thing.
+
+q, k, v are float32 or bfloat16 of one type, of any strides (views of one projection, rows
+collected time-major and transposed); a tensor whose last axis is not contiguous is copied.
+States, sums and log_decay are float32. Everything is asynchronous on the current stream, new
+tensors are returned and inputs are not written, except where ``next_state`` names one.
+"""
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+
+MAX_DIM = 128
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def _check(x, name, like, shape):
+    """A tensor of `like`'s type and device and of `shape`, its last axis contiguous."""
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(x).__name__}")
+    if x.dtype != like.dtype:
+        raise TypeError(f"{name} must be {like.dtype} as q is, got {x.dtype}")
+    if x.device != like.device:
+        raise ValueError(f"{name} is on {x.device}, q is on {like.device}")
+    if tuple(x.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape}, got {tuple(x.shape)}")
+    return x if x.stride(-1) == 1 or shape[-1] == 1 else x.contiguous()
+
+
+def _check_qkv(q, k, v, axes):
+    """(q, k, v, lead, h, dk, dv) of tensors (*lead, h, d) with `axes` axes in all."""
+    if not isinstance(q, torch.Tensor):
+        raise TypeError(f"q must be a torch.Tensor, got {type(q).__name__}")
+    if q.dtype not in _DTYPES:
+        raise TypeError(f"q must be float32 or bfloat16, got {q.dtype}")
+    if q.device.type != "cuda":
+        raise ValueError(f"q must be on a ROCm GPU, got device {q.device}")
+    if q.dim() != axes:
+        raise ValueError(f"q must have {axes} axes, got shape {tuple(q.shape)}")
+    if not isinstance(v, torch.Tensor) or v.dim() != axes:
+        raise ValueError(f"v must be a torch.Tensor with {axes} axes")
+    shape = tuple(q.shape)
+    lead, h, dk, dv = shape[:-2], shape[-2], shape[-1], v.shape[-1]
+    for name, d in (("dk", dk), ("dv", dv)):
+        if not 1 <= d <= MAX_DIM:
+            raise ValueError(f"{name} must be in 1..{MAX_DIM}, got {d}")
+    if not 1 <= h <= 65536:
+        raise ValueError(f"there must be 1 to 65536 heads, got {h}")
+    q = _check(q, "q", q, shape)
+    k = _check(k, "k", q, shape)
+    v = _check(v, "v", q, (*lead, h, dv))
+    return q, k, v, lead, h, dk, dv
+
+
+def _check_f32(x, name, shape, device):
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(x).__name__}")
+    if x.dtype != torch.float32:
+        raise TypeError(f"{name} must be float32, got {x.dtype}")
+    if tuple(x.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape}, got {tuple(x.shape)}")
+    if x.device != device:
+        raise ValueError(f"{name} is on {x.device}, q is on {device}")
+    return x.contiguous()
+
+
+def _check_decay(log_decay, h, device):
+    log_decay = _check_f32(log_decay, "log_decay", (h,), device)
+    if log_decay.requires_grad:
+        raise ValueError("log_decay is a constant of each head and has no gradient: pass it detached")
+    return log_decay
+
+
+def _check_reset(reset, shape, device):
+    if reset is None:
+        return None
+    if not isinstance(reset, torch.Tensor):
+        raise TypeError(f"reset must be a torch.Tensor, got {type(reset).__name__}")
+    if reset.dtype != torch.bool:
+        raise TypeError(f"reset must be bool, got {reset.dtype}")
+    if tuple(reset.shape) != shape:
+        raise ValueError(f"reset must have shape {shape}, got {tuple(reset.shape)}")
+    if reset.device != device:
+        raise ValueError(f"reset is on {reset.device}, q is on {device}")
+    return reset
+
+
+def _strides(rows, reset):
+    """The host array of strides: b, t, h of each tensor, then b, t of reset."""
+    flat = [s for x in rows for s in x.stride()[:3]]
+    flat += reset.stride() if reset is not None else (0, 0)
+    return (ctypes.c_int64 * len(flat))(*flat)
+
+
+def _scale(scale, dk):
+    return 1.0 / math.sqrt(dk) if scale is None else float(scale)
+
+
+def _forward(q, k, v, log_decay, state, reset, scale):
+    b, t, h, dk = q.shape
+    dv = v.shape[-1]
+    out = torch.empty((b, t, h, dv), dtype=q.dtype, device=q.device)
+    final = torch.empty((b, h, dk, dv), dtype=torch.float32, device=q.device)
+    with _lib.on(q.device):
+        _lib.call("hipenvs_decay_attention", _DTYPES[q.dtype], _lib.ptr(q), _lib.ptr(k), _lib.ptr(v),
+                  _strides((q, k, v), reset), _lib.ptr(log_decay), _lib.ptr(state), _lib.ptr(reset), scale,
+                  _lib.ptr(out), _lib.ptr(final), b, t, h, dk, dv, _lib.stream_of(q.device))
+    return out, final
+
+
+class _Sequence(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, state, reset, scale):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(q, k, v, log_decay, state, reset)
+        ctx.scale = scale
+        return _forward(q, k, v, log_decay, state, reset, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, dfinal):
+        q, k, v, log_decay, state, reset = ctx.saved_tensors
+        b, t, h, dk = q.shape
+        dv = v.shape[-1]
+        if dout is None:
+            dout = torch.zeros((b, t, h, dv), dtype=q.dtype, device=q.device)
+        elif dout.stride(-1) != 1 and dv != 1:
+            dout = dout.contiguous()
+        dfinal = dfinal.contiguous() if dfinal is not None else None
+        dq, dk_, dv_ = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
+        dstate = torch.empty((b, h, dk, dv), dtype=torch.float32, device=q.device)
+        with _lib.on(q.device):
+            _lib.call("hipenvs_decay_attention_backward", _DTYPES[q.dtype], _lib.ptr(q), _lib.ptr(k), _lib.ptr(v),
+                      _lib.ptr(dout), _strides((q, k, v, dout), reset), _lib.ptr(log_decay), _lib.ptr(state),
+                      _lib.ptr(reset), _lib.ptr(dfinal), ctx.scale, _lib.ptr(dq), _lib.ptr(dk_), _lib.ptr(dv_),
+                      _lib.ptr(dstate), b, t, h, dk, dv, _lib.stream_of(q.device))
+        return dq, dk_, dv_, None, dstate if state is not None else None, None, None
+
+
+def sequence(q, k, v, log_decay, state=None, reset=None, scale=None):
+    """Whole trajectories: q, k (b, t, h, dk), v (b, t, h, dv), log_decay (h,) float32, state
+    (b, h, dk, dv) float32 before the first token (None: zeros), reset (b, t) bool, True where
+    an episode begins at that token (None: nowhere). Returns (out (b, t, h, dv) of q's type,
+    final_state (b, h, dk, dv) float32), differentiable once in q, k, v and state."""
+    q, k, v, (b, t), h, dk, dv = _check_qkv(q, k, v, 4)
+    log_decay = _check_decay(log_decay, h, q.device)
+    reset = _check_reset(reset, (b, t), q.device)
+    if state is not None:
+        state = _check_f32(state, "state", (b, h, dk, dv), q.device)
+    scale = _scale(scale, dk)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                    or (state is not None and state.requires_grad)):
+        return _Sequence.apply(q, k, v, log_decay, state, reset, scale)
+    return _forward(q, k, v, log_decay, state, reset, scale)
+
+
+def step(q, k, v, log_decay, state, reset=None, scale=None, next_state=None):
+    """One token of every environment: q, k (n, h, dk), v (n, h, dv), state (n, h, dk, dv) float32
+    contiguous, reset (n,) bool, True where this token begins an episode. Returns
+    (out (n, h, dv) of q's type, next_state). ``next_state`` receives the new states and may be
+    ``state`` itself. Not differentiable: training goes through ``sequence``."""
+    q, k, v, (n,), h, dk, dv = _check_qkv(q, k, v, 3)
+    log_decay = _check_decay(log_decay, h, q.device)
+    reset = _check_reset(reset, (n,), q.device)
+    state = _check_f32(state, "state", (n, h, dk, dv), q.device)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
+        raise ValueError("step has no gradient: call it under torch.no_grad(), or use sequence")
+    if next_state is None:
+        next_state = torch.empty_like(state)
+    else:
+        if _check_f32(next_state, "next_state", (n, h, dk, dv), q.device) is not next_state:
+            raise ValueError("next_state must be contiguous")
+        torch.autograd.graph.increment_version(next_state)
+    out = torch.empty((n, h, dv), dtype=q.dtype, device=q.device)
+    with _lib.on(q.device):
+        _lib.call("hipenvs_decay_attention_step", _DTYPES[q.dtype], _lib.ptr(q), q.stride(0), q.stride(1), _lib.ptr(k),
+                  k.stride(0), k.stride(1), _lib.ptr(v), v.stride(0), v.stride(1), _lib.ptr(log_decay),
+                  _lib.ptr(state), _lib.ptr(reset), reset.stride(0) if reset is not None else 0, _scale(scale, dk),
+                  _lib.ptr(out), _lib.ptr(next_state), n, h, dk, dv, _lib.stream_of(q.device))
+    return out, next_state
