@@ -368,6 +368,10 @@ int hipenvs_legged_es_rollout_seeded(int32_t c, int32_t hidden, int32_t iters, i
 
 /* ---- Sequence policies (no reference counterpart) ----------------------- */
 
+/* Bytes of workspace the two calls below need on the current device; -1 for arguments they refuse. */
+int64_t hipenvs_decay_attention_workspace_bytes(int32_t dtype, int64_t b, int64_t t, int32_t h, int32_t dk,
+                                                int32_t dv);
+
 /* Linear attention with a decay for each head. Per row (b, h), with lambda =
  * exp(log_decay[h]) and a state S (dk, dv) f32:
  *   S_t = (reset_t ? 0 : lambda S_{t-1}) + k_t v_t^T,   o_t = scale S_t^T q_t.
@@ -376,13 +380,15 @@ int hipenvs_legged_es_rollout_seeded(int32_t c, int32_t hidden, int32_t iters, i
  * host array, holds b, t, h of q, of k, of v, then b, t of reset. log_decay (h) f32; reset
  * (b, t) u8 or NULL (none); state (b, h, dk, dv) f32 contiguous or NULL (zeros).
  * -> out (b, t, h, dv) contiguous, final_state (b, h, dk, dv) f32 (may be `state`).
+ * workspace: device memory of hipenvs_decay_attention_workspace_bytes bytes (states between
+ * the parts of long rows; 0 and NULL where rows alone fill the card).
  * 1 <= dk, dv <= 128. What a token before a reset or after t holds, a NaN or an infinity
  * among it, does not reach o_t. */
 int hipenvs_decay_attention(int32_t dtype, const void* q, const void* k, const void* v,
                             const int64_t* strides, const float* log_decay, const float* state,
                             const uint8_t* reset, float scale, void* out, float* final_state,
-                            int64_t b, int64_t t, int32_t h, int32_t dk, int32_t dv,
-                            hipenvs_stream_t stream);
+                            int64_t b, int64_t t, int32_t h, int32_t dk, int32_t dv, void* workspace,
+                            int64_t workspace_bytes, hipenvs_stream_t stream);
 
 /* Gradients of the above: dout like out with strides of its own, dfinal (b, h, dk, dv) f32
  * contiguous or NULL (zeros) -> dq, dk_out, dv_out (b, t, h, dk or dv) contiguous in dtype,
@@ -393,7 +399,7 @@ int hipenvs_decay_attention_backward(int32_t dtype, const void* q, const void* k
                                      const float* state, const uint8_t* reset, const float* dfinal,
                                      float scale, void* dq, void* dk_out, void* dv_out, float* dstate,
                                      int64_t b, int64_t t, int32_t h, int32_t dk, int32_t dv,
-                                     hipenvs_stream_t stream);
+                                     void* workspace, int64_t workspace_bytes, hipenvs_stream_t stream);
 
 /* One token of n environments: q, k (n, h, dk), v (n, h, dv) with strides of n and h and unit
  * stride in the last axis, state (n, h, dk, dv) f32 contiguous, reset (n) u8 with stride

@@ -1,117 +1,39 @@
-// Linear attention with a decay for each head and episodes inside its rows: over whole
-// sequences, with its gradients, and for one token of every environment. No reference
-// counterpart: the reference's policies have no memory.
-//
-//   S_t = (reset_t ? 0 : lambda S_{t-1}) + k_t v_t^T        o_t = scale S_t^T q_t
-//
-// lambda = exp(log_decay[h]); S is (dk, dv) in float32 for every row (b, h).
-//
-// One walk gives the outputs and every gradient. Forwards, it decays the state, adds
-// add * k v^T and reads read * S^T q; backwards, it adds and reads first and decays after. With
-// G_t = dL/dS_t = scale q_t do_t^T + (reset_{t+1} ? 0 : lambda G_{t+1}):
-//
-//   o  = walk(q, k, v) on S        dq = walk(do, v, k) on S^T            forwards
-//   dv = walk(k, q, do) on G       dk = walk(v, do, q) on G^T            backwards
-#include "hipenvs_device.h"
+// Linear attention with a decay for each head (decay_attention.h): the C entry points, the
+// joining of a sequence's parts, and one token of every environment.
+#include "decay_attention.h"
 
 namespace hipenvs {
 namespace da {
 
-constexpr int kMaxDim = 128;
-
-template <class T>
-__device__ __forceinline__ float to_f32(T x);
-template <>
-__device__ __forceinline__ float to_f32<float>(float x) {
-  return x;
-}
-template <>
-__device__ __forceinline__ float to_f32<uint16_t>(uint16_t x) {
-  return __uint_as_float((uint32_t)x << 16);
-}
-
-// Nearest even; a NaN stays a NaN.
-__device__ __forceinline__ uint16_t bf16_of(float x) {
-  const uint32_t u = __float_as_uint(x);
-  return (uint16_t)(x != x ? ((u >> 16) | 0x40u) : (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
-}
-template <class T>
-__device__ __forceinline__ T from_f32(float x);
-template <>
-__device__ __forceinline__ float from_f32<float>(float x) {
-  return x;
-}
-template <>
-__device__ __forceinline__ uint16_t from_f32<uint16_t>(float x) {
-  return bf16_of(x);
-}
-
-struct Rows {
-  const void* data;
-  int64_t sb, st, sh;   // strides in elements of a row's batch, token and head; the last is 1
-};
-
-struct Walk {
-  Rows q, k, v;            // roles: read with q, add k v^T
-  int32_t dk, dv;          // of these roles
-  const float* log_decay;  // (h)
-  const uint8_t* reset;    // (b, t) or null
-  int64_t reset_sb, reset_st;
-  const float* state_in;   // (b, h, dk, dv), or (b, h, dv, dk) when flipped; null: zeros
-  float* state_out;        // null: not wanted
-  bool flipped, backwards;
-  float read, add;
-  void* out;               // (b, t, h, dv) contiguous
-  int64_t t;
-  int32_t h;
-};
-
-// The walk, token by token: one wave for 16 columns of a row's state, a quarter of the rows of
-// the state in each 16 lanes.
-template <class T>
-__global__ __launch_bounds__(64) void walk_kernel(Walk w) {
-  const int col = blockIdx.y * 16 + (threadIdx.x & 15), part = threadIdx.x >> 4;
-  const int64_t row = blockIdx.x;
-  const int64_t b = row / w.h, h = row - b * w.h;
-  const int per = (w.dk + 3) / 4, r0 = part * per;
-  const bool live = col < w.dv;
-  const float lambda = expf(w.log_decay[h]);
-  const T* q = (const T*)w.q.data + b * w.q.sb + h * w.q.sh;
-  const T* k = (const T*)w.k.data + b * w.k.sb + h * w.k.sh;
-  const T* v = (const T*)w.v.data + b * w.v.sb + h * w.v.sh;
-  float s[kMaxDim / 4];
+// From each part's own state (what its tokens alone leave behind) to the state before each
+// part, in the order of the walk: carry' = lambda^tokens carry [no reset] + own. A thread for
+// each value of a row's state, eight parts' values read ahead of their use.
+__global__ __launch_bounds__(kBlock) void join_kernel(Walk w) {
+  const int size = w.dk * w.dv, at = blockIdx.y * kBlock + threadIdx.x;
+  if (at >= size) return;
+  const int64_t row = blockIdx.x, h = row % w.h;
+  const float ld = w.log_decay[h];
+  float* states = w.states + row * w.parts * size + at;
+  const uint8_t* flags = w.flags + row * w.parts;
+  float carry = w.state_in ? w.state_in[state_index(w, row, at / w.dv, at % w.dv)] : 0.0f;
+  constexpr int kAhead = 8;
+  for (int n0 = 0; n0 < w.parts; n0 += kAhead) {
+    float own[kAhead];
+    bool reset[kAhead];
 #pragma unroll
-  for (int i = 0; i < kMaxDim / 4; ++i) {
-    const int r = r0 + i;
-    s[i] = 0.0f;
-    if (w.state_in && i < per && r < w.dk && live)
-      s[i] = w.state_in[row * w.dk * w.dv + (w.flipped ? (int64_t)col * w.dk + r : (int64_t)r * w.dv + col)];
-  }
-  for (int64_t n = 0; n < w.t; ++n) {
-    const int64_t t = w.backwards ? w.t - 1 - n : n;
-    const bool fresh = w.reset && w.reset[b * w.reset_sb + t * w.reset_st];
-    const float x = live ? w.add * to_f32<T>(v[t * w.v.st + col]) : 0.0f;
-    float o = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kMaxDim / 4; ++i) {
-      const int r = r0 + i;
-      if (i < per && r < w.dk) {
-        if (!w.backwards) s[i] = fresh ? 0.0f : s[i] * lambda;
-        s[i] = __builtin_fmaf(to_f32<T>(k[t * w.k.st + r]), x, s[i]);
-        o = __builtin_fmaf(to_f32<T>(q[t * w.q.st + r]), s[i], o);
-        if (w.backwards) s[i] = fresh ? 0.0f : s[i] * lambda;
-      }
+    for (int e = 0; e < kAhead; ++e) {
+      const int n = n0 + e, p = w.backwards ? w.parts - 1 - n : n;
+      own[e] = n < w.parts ? states[(int64_t)p * size] : 0.0f;
+      reset[e] = n < w.parts ? flags[p] != 0 : false;
     }
-    o += __shfl_xor(o, 16);
-    o += __shfl_xor(o, 32);
-    if (part == 0 && live) ((T*)w.out)[((b * w.t + t) * w.h + h) * w.dv + col] = from_f32<T>(w.read * o);
-  }
-  if (!w.state_out || !live) return;
 #pragma unroll
-  for (int i = 0; i < kMaxDim / 4; ++i) {
-    const int r = r0 + i;
-    if (i < per && r < w.dk)
-      w.state_out[row * w.dk * w.dv + (w.flipped ? (int64_t)col * w.dk + r : (int64_t)r * w.dv + col)] = s[i];
+    for (int e = 0; e < kAhead; ++e) {
+      const int n = n0 + e, p = w.backwards ? w.parts - 1 - n : n;
+      if (n >= w.parts) break;
+      states[(int64_t)p * size] = carry;
+      const int64_t left = w.t - (int64_t)p * w.part, tokens = left < w.part ? left : w.part;
+      carry = (reset[e] ? 0.0f : carry * expf(ld * (float)tokens)) + own[e];
+    }
   }
 }
 
@@ -178,13 +100,30 @@ bool dims_ok(int32_t dtype, int64_t h, int64_t dk, int64_t dv) {
   return (dtype == 0 || dtype == 1) && h >= 1 && h <= 65536 && dk >= 1 && dk <= kMaxDim && dv >= 1 && dv <= kMaxDim;
 }
 
-int launch_walk(int32_t dtype, const Walk& w, int64_t b, hipStream_t s) {
-  const dim3 grid((unsigned)(b * w.h), (unsigned)((w.dv + 15) / 16)), block(64);
-  if (dtype == 0)
-    hipLaunchKernelGGL(walk_kernel<float>, grid, block, 0, s, w);
-  else
-    hipLaunchKernelGGL(walk_kernel<uint16_t>, grid, block, 0, s, w);
-  return launch_status();
+// A block walks a row, or a part of one where the rows are too few to fill the card: then a first
+// pass leaves each part's own state, the second joins them, the third walks every part from
+// the state before it.
+void divide(int64_t rows, int64_t t, int32_t chunk, int64_t cus, int32_t* parts, int64_t* part) {
+  const int64_t chunks = (t + chunk - 1) / chunk;
+  const int64_t want = (2 * cus + rows - 1) / rows, most = chunks / 4;
+  int64_t n = want < most ? want : most;
+  if (n < 2) n = 1;
+  const int64_t per = n > 1 ? (chunks + n - 1) / n : chunks;
+  *parts = n > 1 ? (int32_t)((chunks + per - 1) / per) : 1;
+  *part = (per > 0 ? per : 1) * chunk;
+}
+
+int32_t chunk_of(int32_t dtype) { return dtype == 1 ? Chunk<__bf16>::kTokens : Chunk<float>::kTokens; }
+
+int launch_walk(int32_t dtype, Walk w, hipStream_t s) {
+  if (w.parts > 1) {
+    int status = dtype == 1 ? launch_chunks<__bf16>(w, false, s) : launch_chunks<float>(w, false, s);
+    if (status != HIPENVS_OK) return status;
+    hipLaunchKernelGGL(join_kernel, dim3((unsigned)(w.b * w.h), grid_for(w.dk * w.dv)), dim3(kBlock), 0, s, w);
+    status = launch_status();
+    if (status != HIPENVS_OK) return status;
+  }
+  return dtype == 1 ? launch_chunks<__bf16>(w, true, s) : launch_chunks<float>(w, true, s);
 }
 
 }  // namespace da
@@ -199,21 +138,58 @@ bool sequence_ok(int32_t dtype, int64_t b, int64_t t, int64_t h, int64_t dk, int
   return dims_ok(dtype, h, dk, dv) && b >= 0 && t >= 0 && b * h <= 0x7FFFFFFF && b <= 0x7FFFFFFF && t <= 0x7FFFFFFF;
 }
 
-Rows rows(const void* data, const int64_t* strides) { return {data, strides[0], strides[1], strides[2]}; }
+// `d` values a row of `size` bytes each.
+Rows rows(const void* data, const int64_t* strides, int64_t size, int64_t d) {
+  const bool wide = (((uintptr_t)data | (uintptr_t)(strides[0] * size) | (uintptr_t)(strides[1] * size) |
+                      (uintptr_t)(strides[2] * size) | (uintptr_t)(d * size)) & 15) == 0;
+  return {data, strides[0], strides[1], strides[2], wide};
+}
+
+// The parts of a sequence and where in `workspace` their states and flags lie; the bytes used.
+int plan(int32_t dtype, int64_t b, int64_t t, int32_t h, int32_t dk, int32_t dv, void* workspace, Walk* w,
+         int64_t* bytes) {
+  int cus = 0;
+  const int status = device_cus(&cus);
+  if (status != HIPENVS_OK) return status;
+  divide(b * h, t, chunk_of(dtype), cus, &w->parts, &w->part);
+  const int64_t states = w->parts > 1 ? b * h * w->parts * dk * dv * (int64_t)sizeof(float) : 0;
+  w->states = (float*)workspace;
+  w->flags = (uint8_t*)workspace + states;
+  *bytes = w->parts > 1 ? states + b * h * w->parts : 0;
+  return HIPENVS_OK;
+}
 }  // namespace
+
+extern "C" int64_t hipenvs_decay_attention_workspace_bytes(int32_t dtype, int64_t b, int64_t t, int32_t h, int32_t dk,
+                                                           int32_t dv) {
+  if (!sequence_ok(dtype, b, t, h, dk, dv)) return -1;
+  if (b == 0) return 0;
+  Walk w = {};
+  int64_t bytes = 0;
+  return plan(dtype, b, t, h, dk, dv, nullptr, &w, &bytes) == HIPENVS_OK ? bytes : -1;
+}
 
 extern "C" int hipenvs_decay_attention(int32_t dtype, const void* q, const void* k, const void* v,
                                        const int64_t* strides, const float* log_decay, const float* state,
                                        const uint8_t* reset, float scale, void* out, float* final_state, int64_t b,
-                                       int64_t t, int32_t h, int32_t dk, int32_t dv, hipenvs_stream_t stream) {
+                                       int64_t t, int32_t h, int32_t dk, int32_t dv, void* workspace,
+                                       int64_t workspace_bytes, hipenvs_stream_t stream) {
   if (!sequence_ok(dtype, b, t, h, dk, dv)) return HIPENVS_E_ARG;
   if (b == 0) return HIPENVS_OK;
   if (!log_decay || !final_state || (t > 0 && (!q || !k || !v || !out || !strides))) return HIPENVS_E_ARG;
   static const int64_t none[11] = {};
   const int64_t* st = t > 0 ? strides : none;
-  Walk w = {rows(q, st), rows(k, st + 3), rows(v, st + 6), dk, dv, log_decay, reset, st[9], st[10],
-            state, final_state, false, false, scale, 1.0f, out, t, h};
-  return launch_walk(dtype, w, b, as_stream(stream));
+  const int64_t e = dtype == 1 ? 2 : 4;
+  Walk w = {};
+  int64_t need = 0;
+  const int status = plan(dtype, b, t, h, dk, dv, workspace, &w, &need);
+  if (status != HIPENVS_OK) return status;
+  if (need > 0 && (!workspace || workspace_bytes < need)) return HIPENVS_E_ARG;
+  w.q = rows(q, st, e, dk), w.k = rows(k, st + 3, e, dk), w.v = rows(v, st + 6, e, dv);
+  w.dk = dk, w.dv = dv, w.log_decay = log_decay, w.reset = reset, w.reset_sb = st[9], w.reset_st = st[10];
+  w.state_in = state, w.state_out = final_state, w.read = scale, w.add = 1.0f;
+  w.out = out, w.b = b, w.t = t, w.h = h;
+  return launch_walk(dtype, w, as_stream(stream));
 }
 
 extern "C" int hipenvs_decay_attention_backward(int32_t dtype, const void* q, const void* k, const void* v,
@@ -221,25 +197,36 @@ extern "C" int hipenvs_decay_attention_backward(int32_t dtype, const void* q, co
                                                 const float* state, const uint8_t* reset, const float* dfinal,
                                                 float scale, void* dq, void* dk_out, void* dv_out, float* dstate,
                                                 int64_t b, int64_t t, int32_t h, int32_t dk, int32_t dv,
-                                                hipenvs_stream_t stream) {
+                                                void* workspace, int64_t workspace_bytes, hipenvs_stream_t stream) {
   if (!sequence_ok(dtype, b, t, h, dk, dv)) return HIPENVS_E_ARG;
   if (b == 0) return HIPENVS_OK;
   if (!log_decay || !dstate || (t > 0 && (!q || !k || !v || !dout || !dq || !dk_out || !dv_out || !strides)))
     return HIPENVS_E_ARG;
   static const int64_t none[14] = {};
   const int64_t* st = t > 0 ? strides : none;
-  const Rows rq = rows(q, st), rk = rows(k, st + 3), rv = rows(v, st + 6), rdo = rows(dout, st + 9);
+  const int64_t e = dtype == 1 ? 2 : 4;
+  Walk w = {};
+  int64_t need = 0;
+  int status = plan(dtype, b, t, h, dk, dv, workspace, &w, &need);
+  if (status != HIPENVS_OK) return status;
+  if (need > 0 && (!workspace || workspace_bytes < need)) return HIPENVS_E_ARG;
+  const Rows rq = rows(q, st, e, dk), rk = rows(k, st + 3, e, dk), rv = rows(v, st + 6, e, dv),
+             rdo = rows(dout, st + 9, e, dv);
   const hipStream_t s = as_stream(stream);
-  const Walk by_q = {rdo, rv, rk, dv, dk, log_decay, reset, st[12], st[13], state, nullptr, true, false, scale, 1.0f,
-                     dq, t, h};
-  const Walk by_v = {rk, rq, rdo, dk, dv, log_decay, reset, st[12], st[13], dfinal, dstate, false, true, 1.0f, scale,
-                     dv_out, t, h};
-  const Walk by_k = {rv, rdo, rq, dv, dk, log_decay, reset, st[12], st[13], dfinal, nullptr, true, true, 1.0f, scale,
-                     dk_out, t, h};
-  int status = launch_walk(dtype, by_q, b, s);
-  if (status == HIPENVS_OK) status = launch_walk(dtype, by_v, b, s);
-  if (status == HIPENVS_OK) status = launch_walk(dtype, by_k, b, s);
-  return status;
+  w.log_decay = log_decay, w.reset = reset, w.reset_sb = st[12], w.reset_st = st[13], w.b = b, w.t = t, w.h = h;
+  // dq: forwards over the transposed states
+  w.q = rdo, w.k = rv, w.v = rk, w.dk = dv, w.dv = dk, w.state_in = state, w.state_out = nullptr;
+  w.flipped = true, w.backwards = false, w.read = scale, w.add = 1.0f, w.out = dq;
+  status = launch_walk(dtype, w, s);
+  if (status != HIPENVS_OK) return status;
+  // dv, and the gradient of the first state: backwards over the states' gradients
+  w.q = rk, w.k = rq, w.v = rdo, w.dk = dk, w.dv = dv, w.state_in = dfinal, w.state_out = dstate;
+  w.flipped = false, w.backwards = true, w.read = 1.0f, w.add = scale, w.out = dv_out;
+  status = launch_walk(dtype, w, s);
+  if (status != HIPENVS_OK) return status;
+  // dk: the same, transposed
+  w.q = rv, w.k = rdo, w.v = rq, w.dk = dv, w.dv = dk, w.state_out = nullptr, w.flipped = true, w.out = dk_out;
+  return launch_walk(dtype, w, s);
 }
 
 extern "C" int hipenvs_decay_attention_step(int32_t dtype, const void* q, int64_t q_sn, int64_t q_sh, const void* k,
@@ -257,7 +244,7 @@ extern "C" int hipenvs_decay_attention_step(int32_t dtype, const void* q, int64_
   const hipStream_t at = as_stream(stream);
   if (dtype == 0 && wide) hipLaunchKernelGGL((step_kernel<float, 4>), grid, block, 0, at, s);
   if (dtype == 0 && !wide) hipLaunchKernelGGL((step_kernel<float, 1>), grid, block, 0, at, s);
-  if (dtype == 1 && wide) hipLaunchKernelGGL((step_kernel<uint16_t, 4>), grid, block, 0, at, s);
-  if (dtype == 1 && !wide) hipLaunchKernelGGL((step_kernel<uint16_t, 1>), grid, block, 0, at, s);
+  if (dtype == 1 && wide) hipLaunchKernelGGL((step_kernel<__bf16, 4>), grid, block, 0, at, s);
+  if (dtype == 1 && !wide) hipLaunchKernelGGL((step_kernel<__bf16, 1>), grid, block, 0, at, s);
   return launch_status();
 }

@@ -70,9 +70,10 @@ SIGNATURES = {
     "hipenvs_acrobot_es_rollout_seeded": [_P, _P, _I64, _U32, ctypes.c_double, _I32, _I32, _P, _P, _I64, _P],
     "hipenvs_legged_es_rollout_seeded": [_I32, _I32, _I32, _I32, _P, _P, _I64, _U32, ctypes.c_double, _I32, _F32,
                                          _F32, _F32, ctypes.c_double, _P, _P, _P, _I64, _P],
-    "hipenvs_decay_attention": [_I32, _P, _P, _P, _P, _P, _P, _P, _F32, _P, _P, _I64, _I64, _I32, _I32, _I32, _P],
+    "hipenvs_decay_attention": [_I32, _P, _P, _P, _P, _P, _P, _P, _F32, _P, _P, _I64, _I64, _I32, _I32, _I32, _P, _I64,
+                                _P],
     "hipenvs_decay_attention_backward": [_I32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _F32, _P, _P, _P, _P, _I64, _I64,
-                                         _I32, _I32, _I32, _P],
+                                         _I32, _I32, _I32, _P, _I64, _P],
     "hipenvs_decay_attention_step": [_I32, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _F32, _P,
                                      _P, _I64, _I32, _I32, _I32, _P],
     "hipenvs_adamw_step": [_I32, _I32, _P, _P, _P, _P, _P, _P, ctypes.c_double, ctypes.c_double, ctypes.c_double,
@@ -84,6 +85,7 @@ SIGNATURES = {
 VALUE_SIGNATURES = {
     "hipenvs_legged_es_rollout_workspace_bytes": (ctypes.c_int64, [_I32, _I32, _I64]),
     "hipenvs_es_update_workspace_bytes": (ctypes.c_int64, [_I64, _I64]),
+    "hipenvs_decay_attention_workspace_bytes": (ctypes.c_int64, [_I32, _I64, _I64, _I32, _I32, _I32]),
 }
 
 

@@ -110,15 +110,25 @@ def _scale(scale, dk):
     return 1.0 / math.sqrt(dk) if scale is None else float(scale)
 
 
+def _workspace(dtype, b, t, h, dk, dv, device):
+    """(address, bytes, tensor) of the workspace of a sequence's calls."""
+    nbytes = _lib.lib().hipenvs_decay_attention_workspace_bytes(dtype, b, t, h, dk, dv)
+    if nbytes < 0:
+        raise _lib.HipEnvsError(f"hipenvs_decay_attention: unsupported sequence ({b}, {t}, {h}, {dk}, {dv})")
+    held = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    return _lib.ptr(held), nbytes, held
+
+
 def _forward(q, k, v, log_decay, state, reset, scale):
     b, t, h, dk = q.shape
     dv = v.shape[-1]
     out = torch.empty((b, t, h, dv), dtype=q.dtype, device=q.device)
     final = torch.empty((b, h, dk, dv), dtype=torch.float32, device=q.device)
     with _lib.on(q.device):
+        at, nbytes, _held = _workspace(_DTYPES[q.dtype], b, t, h, dk, dv, q.device)
         _lib.call("hipenvs_decay_attention", _DTYPES[q.dtype], _lib.ptr(q), _lib.ptr(k), _lib.ptr(v),
                   _strides((q, k, v), reset), _lib.ptr(log_decay), _lib.ptr(state), _lib.ptr(reset), scale,
-                  _lib.ptr(out), _lib.ptr(final), b, t, h, dk, dv, _lib.stream_of(q.device))
+                  _lib.ptr(out), _lib.ptr(final), b, t, h, dk, dv, at, nbytes, _lib.stream_of(q.device))
     return out, final
 
 
@@ -144,10 +154,11 @@ class _Sequence(torch.autograd.Function):
         dq, dk_, dv_ = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
         dstate = torch.empty((b, h, dk, dv), dtype=torch.float32, device=q.device)
         with _lib.on(q.device):
+            at, nbytes, _held = _workspace(_DTYPES[q.dtype], b, t, h, dk, dv, q.device)
             _lib.call("hipenvs_decay_attention_backward", _DTYPES[q.dtype], _lib.ptr(q), _lib.ptr(k), _lib.ptr(v),
                       _lib.ptr(dout), _strides((q, k, v, dout), reset), _lib.ptr(log_decay), _lib.ptr(state),
                       _lib.ptr(reset), _lib.ptr(dfinal), ctx.scale, _lib.ptr(dq), _lib.ptr(dk_), _lib.ptr(dv_),
-                      _lib.ptr(dstate), b, t, h, dk, dv, _lib.stream_of(q.device))
+                      _lib.ptr(dstate), b, t, h, dk, dv, at, nbytes, _lib.stream_of(q.device))
         return dq, dk_, dv_, None, dstate if state is not None else None, None, None
 
 

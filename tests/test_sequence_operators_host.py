@@ -18,7 +18,7 @@ def test_c_abi_checks_attention_arguments():
     strides = (ctypes.c_int64 * 14)()
 
     def forward(dtype=0, q=a, out=a, final=a, b=2, t=3, h=2, dk=8, dv=4):
-        return l.hipenvs_decay_attention(dtype, q, a, a, strides, a, None, None, 1.0, out, final, b, t, h, dk, dv, None)
+        return l.hipenvs_decay_attention(dtype, q, a, a, strides, a, None, None, 1.0, out, final, b, t, h, dk, dv, None, 0, None)
 
     for bad in (dict(dtype=2), dict(dtype=-1), dict(q=None), dict(out=None), dict(final=None), dict(b=-1), dict(t=-1),
                 dict(h=0), dict(dk=0), dict(dk=129), dict(dv=129), dict(dv=0), dict(b=1 << 31), dict(b=1 << 30, h=4),
@@ -26,9 +26,9 @@ def test_c_abi_checks_attention_arguments():
         assert forward(**bad) == _lib.E_ARG, bad
     assert forward(b=0) == _lib.OK
     assert l.hipenvs_decay_attention_backward(0, a, a, a, None, strides, a, None, None, None, 1.0, a, a, a, a, 2, 3, 2, 8,
-                                              4, None) == _lib.E_ARG
+                                              4, None, 0, None) == _lib.E_ARG
     assert l.hipenvs_decay_attention_backward(0, a, a, a, a, strides, a, None, None, None, 1.0, a, a, a, None, 2, 3, 2, 8,
-                                              4, None) == _lib.E_ARG
+                                              4, None, 0, None) == _lib.E_ARG
     step = l.hipenvs_decay_attention_step
     assert step(0, a, 1, 1, a, 1, 1, a, 1, 1, a, None, None, 0, 1.0, a, a, 4, 2, 8, 4, None) == _lib.E_ARG
     assert step(0, a, 1, 1, a, 1, 1, a, 1, 1, a, a, None, 0, 1.0, a, a, 4, 2, 200, 4, None) == _lib.E_ARG
