@@ -50,7 +50,6 @@ __device__ __forceinline__ T from_f32(float x) {
 struct Rows {
   const void* data;
   int64_t sb, st, sh;  // strides in elements of a row's batch, token and head; the last is 1
-  bool wide;           // every row begins at a multiple of 16 bytes and is whole 16-byte pieces
 };
 
 struct Walk {
@@ -62,6 +61,7 @@ struct Walk {
   const float* state_in;   // (b, h, dk, dv), or (b, h, dv, dk) when flipped; null: zeros
   float* state_out;        // null: not wanted
   bool flipped, backwards;
+  bool exact;              // the state is wanted in float32 to its last bits
   float read, add;
   void* out;               // (b, t, h, dv) contiguous
   int64_t b, t;
@@ -154,18 +154,22 @@ struct Chunk<float> {
   static constexpr int kTokens = 32, kPad = 4;
 };
 
-// One 16-byte piece of a token's row, zeros where the row has ended.
+// 16 bytes at any address that is a multiple of the value's size.
+typedef u32x4 __attribute__((aligned(2))) piece_at_2;
+typedef u32x2 __attribute__((aligned(2))) half_piece_at_2;
+
+// One 16-byte piece of a token's row from its column `col` on, zeros where the row has ended.
 template <class T>
-__device__ __forceinline__ u32x4 load_piece(const T* row, int col, int dim, bool wide) {
+__device__ __forceinline__ u32x4 load_piece(const T* at, int col, int dim) {
   constexpr int E = 16 / sizeof(T);
   u32x4 x = {0, 0, 0, 0};
-  if (wide) {
-    if (col < dim) x = *(const u32x4*)(row + col);
-  } else {
+  if (col + E <= dim) {
+    x = *(const piece_at_2*)at;
+  } else if (dim % E != 0) {
     T* y = (T*)&x;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (col + e < dim) y[e] = row[col + e];
+    for (int e = 0; e < E - 1; ++e)
+      if (col + e < dim) y[e] = at[e];
   }
   return x;
 }
@@ -203,48 +207,107 @@ __device__ __forceinline__ void split(float (&rest)[N], __bf16 (&parts)[M][N]) {
 // A wave takes 16 columns of the state, all of its rows: S[a][r] is row 16 a + 4 g + r, column
 // l, for lane 16 g + l. That is both a matrix instruction's result and, its rows
 // taken as the summed axis in that order, an operand of the read S^T q, so the state never
-// leaves its registers. The block's NW waves share a chunk's q, k, v (LDS, two buffers: while
-// one chunk is computed the next is on its way to registers) and its masked products
+// leaves its registers. The block's NW waves share a chunk's q, k, v (in LDS; while one
+// chunk is computed the next is on its way to registers) and its masked products
 // P[i][j], computed once.
 //
 // bfloat16 rows: the inputs are exact operands. P, the S that is read and the lambda^n v_j that
 // is added are float32, split for the matrix instructions into bfloat16 parts, each the
 // rounding of what the parts before it leave: two parts for P and S (16 bits, so a result's
-// error is that of its own rounding to bfloat16), three for what enters a state (all 24 bits: a
-// state is a float32 result). float32 rows use the float32 matrix instructions throughout.
-template <class T, int DK, int NW, bool kOut>
-__global__ __launch_bounds__(64 * NW) void chunk_kernel(Walk w) {
+// error is that of its own rounding to bfloat16) and for what enters a state that only results
+// are read from, three for one that is a float32 result itself (all 24 bits). float32 rows use the float32 matrix instructions throughout.
+template <class T, int DK, int NW, bool kOut, bool kBack>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) void chunk_kernel(Walk w) {
   constexpr bool kHalf = sizeof(T) == 2;
   constexpr int C = Chunk<T>::kTokens, PAD = Chunk<T>::kPad, E = 16 / sizeof(T), TH = 64 * NW, DV = 16 * NW;
   constexpr int SQ = DK + PAD, SV = DV + PAD, SP = C + PAD, NT = C / 16;
   constexpr int QP = DK / E, VP = DV / E;                               // pieces of a row
   constexpr int NQ = (C * QP + TH - 1) / TH, NV = (C * VP + TH - 1) / TH;  // pieces of a thread
-  __shared__ __attribute__((aligned(16))) T Qs[kOut ? 2 * C * SQ : 8];
-  __shared__ __attribute__((aligned(16))) T Ks[2 * C * SQ];
-  __shared__ __attribute__((aligned(16))) T Vs[2 * C * SV];
+  __shared__ __attribute__((aligned(16))) T Qs[kOut ? C * SQ : 8];
+  __shared__ __attribute__((aligned(16))) T Ks[C * SQ];
+  __shared__ __attribute__((aligned(16))) T Vs[C * SV];
   __shared__ __attribute__((aligned(16))) T Ps[kOut ? (kHalf ? 2 : 1) * C * SP : 8];
   __shared__ float pw[C + 1];
-  __shared__ __attribute__((aligned(16))) float wu[2 * C];
 
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, l = lane & 15;
   // blocks of one XCD (every eighth) take neighbouring rows, whose tokens share cache lines
-  const int64_t blocks = gridDim.x;
-  const int64_t id = blocks % 8 == 0 ? (int64_t)(blockIdx.x % 8) * (blocks / 8) + blockIdx.x / 8 : blockIdx.x;
-  const int64_t row = id / w.parts;
-  const int part = (int)(id - row * w.parts);
-  const int64_t b = row / w.h, h = row - b * w.h;
+  const uint32_t blocks = gridDim.x;
+  const uint32_t id = blocks % 8 == 0 ? (blockIdx.x % 8) * (blocks / 8) + blockIdx.x / 8 : blockIdx.x;
+  const uint32_t row = id / (uint32_t)w.parts, part = id - row * (uint32_t)w.parts;
+  const int64_t b = row / (uint32_t)w.h, h = row - (uint32_t)b * (uint32_t)w.h;
   const int64_t t0 = part * w.part, t1 = t0 + w.part < w.t ? t0 + w.part : w.t;
-  const int64_t chunks = (t1 - t0 + C - 1) / C;
-  const bool back = w.backwards;
-  const bool first = part == (back ? w.parts - 1 : 0), last = part == (back ? 0 : w.parts - 1);
+  const int chunks = (int)((t1 - t0 + C - 1) / C);
+  const bool last = part == (kBack ? 0 : (uint32_t)w.parts - 1);
+  const int tokens_of_last = (int)(t1 - t0) - (chunks - 1) * C;
+  float* local = w.parts > 1 ? w.states + ((int64_t)row * w.parts + part) * w.dk * w.dv : nullptr;
+
+  // where this thread's pieces of the first chunk lie, and how far on the next chunk's do
+  const int64_t start = t0 + (kBack ? (int64_t)(chunks - 1) * C : 0);
+  const T* qp[kOut ? NQ : 1];
+  const T* kp[NQ];
+  const T* vp[NV];
+#pragma unroll
+  for (int m = 0; m < NQ; ++m) {
+    const int p = tid + m * TH, r = p / QP, x = (p - r * QP) * E;
+    kp[m] = (const T*)w.k.data + b * w.k.sb + h * w.k.sh + (start + r) * w.k.st + x;
+    if constexpr (kOut) qp[m] = (const T*)w.q.data + b * w.q.sb + h * w.q.sh + (start + r) * w.q.st + x;
+  }
+#pragma unroll
+  for (int m = 0; m < NV; ++m) {
+    const int p = tid + m * TH, r = p / VP, x = (p - r * VP) * E;
+    vp[m] = (const T*)w.v.data + b * w.v.sb + h * w.v.sh + (start + r) * w.v.st + x;
+  }
+  const uint8_t* rp = w.reset ? w.reset + b * w.reset_sb + (start + lane) * w.reset_st : nullptr;
+  const int64_t q_on = (kBack ? -C : C) * w.q.st, k_on = (kBack ? -C : C) * w.k.st, v_on = (kBack ? -C : C) * w.v.st;
+
+  u32x4 xq[kOut ? NQ : 1], xk[NQ], xv[NV];
+  uint32_t xr = 0;
+  const bool filled = w.dk == DK && w.dv == DV && C * QP % TH == 0 && C * VP % TH == 0;
+  const auto load = [&](int n) {
+    if (filled && n == C) {
+#pragma unroll
+      for (int m = 0; m < NQ; ++m) {
+        xk[m] = *(const piece_at_2*)kp[m];
+        if constexpr (kOut) xq[m] = *(const piece_at_2*)qp[m];
+      }
+#pragma unroll
+      for (int m = 0; m < NV; ++m) xv[m] = *(const piece_at_2*)vp[m];
+    } else {
+      const u32x4 none = {0, 0, 0, 0};
+#pragma unroll
+      for (int m = 0; m < NQ; ++m) {
+        const int p = tid + m * TH, r = p / QP, x = (p - r * QP) * E;
+        xk[m] = none;
+        if constexpr (kOut) xq[m] = none;
+        if (r < n) {
+          xk[m] = load_piece<T>(kp[m], x, w.dk);
+          if constexpr (kOut) xq[m] = load_piece<T>(qp[m], x, w.dk);
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < NV; ++m) {
+        const int p = tid + m * TH, r = p / VP, x = (p - r * VP) * E;
+        xv[m] = none;
+        if (r < n) xv[m] = load_piece<T>(vp[m], x, w.dv);
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < NQ; ++m) {
+      kp[m] += k_on;
+      if constexpr (kOut) qp[m] += q_on;
+    }
+#pragma unroll
+    for (int m = 0; m < NV; ++m) vp[m] += v_on;
+    xr = 0;
+    if (rp) {
+      if (lane < n) xr = *rp;
+      rp += (kBack ? -C : C) * w.reset_st;
+    }
+  };
+  if (chunks > 0) load(kBack || chunks == 1 ? tokens_of_last : C);
+
   const float ld = w.log_decay[h];
-  const T* qrow = (const T*)w.q.data + b * w.q.sb + h * w.q.sh;
-  const T* krow = (const T*)w.k.data + b * w.k.sb + h * w.k.sh;
-  const T* vrow = (const T*)w.v.data + b * w.v.sb + h * w.v.sh;
-  float* local = w.parts > 1 ? w.states + (row * w.parts + part) * w.dk * w.dv : nullptr;
-
   for (int n = tid; n <= C; n += TH) pw[n] = n == 0 ? 1.0f : expf(ld * (float)n);
-
   f32x4 S[DK / 16];
   const int col = 16 * wave + l;
 #pragma unroll
@@ -257,147 +320,135 @@ __global__ __launch_bounds__(64 * NW) void chunk_kernel(Walk w) {
         x = local ? local[(int64_t)k * w.dv + col] : w.state_in ? w.state_in[state_index(w, row, k, col)] : 0.0f;
       S[a][r] = x;
     }
+  __syncthreads();   // pw
 
-  u32x4 xq[kOut ? NQ : 1], xk[NQ], xv[NV];
-  uint32_t xr = 0;
-  const auto load = [&](int64_t c) {
-    const int64_t at = t0 + c * C;
-    const int n = (int)(t1 - at < C ? t1 - at : C);
-#pragma unroll
-    for (int m = 0; m < NQ; ++m) {
-      const int p = tid + m * TH, r = p / QP, x = (p - r * QP) * E;
-      const u32x4 none = {0, 0, 0, 0};
-      xk[m] = none;
-      if constexpr (kOut) xq[m] = none;
-      if (r < n) {
-        xk[m] = load_piece<T>(krow + (at + r) * w.k.st, x, w.dk, w.k.wide);
-        if constexpr (kOut) xq[m] = load_piece<T>(qrow + (at + r) * w.q.st, x, w.dk, w.q.wide);
-      }
-    }
-#pragma unroll
-    for (int m = 0; m < NV; ++m) {
-      const int p = tid + m * TH, r = p / VP, x = (p - r * VP) * E;
-      const u32x4 none = {0, 0, 0, 0};
-      xv[m] = none;
-      if (r < n) xv[m] = load_piece<T>(vrow + (at + r) * w.v.st, x, w.dv, w.v.wide);
-    }
-    xr = 0;
-    if (w.reset && lane < n) xr = w.reset[b * w.reset_sb + (at + lane) * w.reset_st];
+  // The tiles of P, 16 queries x 16 keys, that some product uses, dealt to the waves: tile x of
+  // this wave is pair_of(x) = (query tile, key tile). bfloat16's products run over 32 keys, so
+  // the tiles beside the diagonal are among them, with decays of zero.
+  constexpr int kPairs = kHalf ? 12 : 4, kOwn = (kPairs + NW - 1) / NW;
+  const auto pair_of = [&](int x) {
+    const int y = wave + NW * x;
+    const int it = y < 4 ? y >> 1 : y < 8 ? 2 : 3, jt = y < 4 ? y & 1 : y & 3;
+    return kBack ? make_int2(NT - 1 - it, NT - 1 - jt) : make_int2(it, jt);
   };
 
+  // The decays of a whole chunk. of_pair[x][r]: of tile x of P, zero where the key is not yet
+  // there; of_read[it]: of the state, for query 16 it + l; of_add[x]: of the x-th token that
+  // this lane holds of v, which is held(x).
+  const auto held = [&](int x) { return kHalf ? 32 * (x / 8) + 8 * g + x % 8 : 16 * (x / 4) + 4 * g + x % 4; };
+  constexpr int NH = C / 4;
+  float of_pair[kOut ? kOwn : 1][4], of_read[kOut ? NT : 1], of_add[NH];
+  if constexpr (kOut) {
+#pragma unroll
+    for (int x = 0; x < kOwn; ++x) {
+      const int2 tile = pair_of(x);
+      const int ahead = 16 * (tile.x - tile.y) + l - 4 * g;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int gap = kBack ? r - ahead : ahead - r;
+        of_pair[x][r] = gap >= 0 && gap < C ? w.read * w.add * pw[gap] : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int it = 0; it < NT; ++it) of_read[it] = w.read * pw[kBack ? C - 1 - (16 * it + l) : 16 * it + l + 1];
+  }
+#pragma unroll
+  for (int x = 0; x < NH; ++x) of_add[x] = w.add * pw[kBack ? held(x) + 1 : C - 1 - held(x)];
+  const float of_chunk = pw[C];
+
+  T* op = nullptr;   // this lane's first output of the chunk
+  const int64_t o_row = (int64_t)w.h * w.dv;
+  if constexpr (kOut) op = (T*)w.out + (b * w.t + start + l) * o_row + h * w.dv + 16 * wave + 4 * g;
+
+  const bool idle = 16 * wave >= w.dv;   // no columns: this wave only moves and shares
+  const bool exact = w.exact;
   uint64_t any = 0;
   float bad = 0.0f;   // becomes NaN with the first value that is not finite
-  if (chunks > 0) load(back ? chunks - 1 : 0);
-  for (int64_t step = 0; step < chunks; ++step) {
-    const int64_t c = back ? chunks - 1 - step : step, at = t0 + c * C;
-    const int n = (int)(t1 - at < C ? t1 - at : C);
-    const int buf = (int)(step & 1);
-    T* Kb = Ks + buf * C * SQ;
-    T* Vb = Vs + buf * C * SV;
-    T* Qb = kOut ? Qs + buf * C * SQ : Qs;
-    float* wb = wu + buf * C;
+  for (int step = 0; step < chunks; ++step) {
+    const int n = (kBack ? step == 0 : step == chunks - 1) ? tokens_of_last : C;
+    if (step > 0) __syncthreads();   // the chunk before has been read
 #pragma unroll
     for (int m = 0; m < NQ; ++m) {
       const int p = tid + m * TH, r = p / QP, x = (p - r * QP) * E;
-      if (r < C) {
-        *(u32x4*)(Kb + r * SQ + x) = xk[m];
-        if constexpr (kOut) *(u32x4*)(Qb + r * SQ + x) = xq[m];
+      if (C * QP % TH == 0 || r < C) {
+        *(u32x4*)(Ks + r * SQ + x) = xk[m];
+        if constexpr (kOut) *(u32x4*)(Qs + r * SQ + x) = xq[m];
       }
     }
 #pragma unroll
     for (int m = 0; m < NV; ++m) {
       const int p = tid + m * TH, r = p / VP, x = (p - r * VP) * E;
-      if (r < C) *(u32x4*)(Vb + r * SV + x) = xv[m];
+      if (C * VP % TH == 0 || r < C) *(u32x4*)(Vs + r * SV + x) = xv[m];
     }
     // the chunk's resets, bit i for token i; the first and the last of them
     const uint64_t mask = __builtin_amdgcn_ballot_w64(xr != 0);
     any |= mask;
     const int r_first = mask ? __builtin_ctzll(mask) : C, r_last = mask ? 63 - __builtin_clzll(mask) : -1;
-    if (step == 0) __syncthreads();   // pw
-    if (tid < C) {
-      const int j = tid;
-      float x = 0.0f;
-      if (j < n) x = back ? (j < r_first ? w.add * pw[j + 1] : 0.0f) : (j >= r_last ? w.add * pw[n - 1 - j] : 0.0f);
-      wb[j] = x;
-    }
     __syncthreads();
-    if (step + 1 < chunks) load(back ? chunks - 2 - step : step + 1);
+    if (step + 1 < chunks) load(!kBack && step + 2 == chunks ? tokens_of_last : C);
 
+    f32x4 o[kOut ? NT : 1];
     if constexpr (kOut) {
-      // P[i][j], the tiles of 16 queries x 16 keys dealt to the waves
-      constexpr int H = NW > NT ? NW / NT : 1;
-      const int it0 = wave % NT, jt0 = wave / NT;
-      for (int it = it0; it < NT && jt0 < H; it += NW) {
-        const int i = 16 * it + l;
-        const uint64_t upto = mask & ((2ull << i) - 1), after = i < 63 ? mask >> (i + 1) : 0;
-        const int from = upto ? 63 - __builtin_clzll(upto) : 0, until = after ? i + 1 + __builtin_ctzll(after) : C;
+      f32x4 p[kOwn];
 #pragma unroll
-        for (int jt = 0; jt < NT; ++jt) {
-          if (jt % H != jt0) continue;
-          T* to = Ps + i * SP + 16 * jt + 4 * g;
-          if (back ? jt < it : jt > it) {
-            if constexpr (kHalf) {
-              if ((jt ^ it) == 1) {   // the other half of a 32-key product
-                const u32x2 none = {0, 0};
-                *(u32x2*)to = none;
-                *(u32x2*)(to + C * SP) = none;
-              }
-            }
-            continue;
-          }
-          f32x4 p = {0.0f, 0.0f, 0.0f, 0.0f};
-          if constexpr (kHalf) {
+      for (int x = 0; x < kOwn; ++x) {
+        const int2 tile = pair_of(x);
+        p[x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (kPairs % NW != 0 && wave + NW * x >= kPairs) break;
+        const T* kt = Ks + (16 * tile.y + l) * SQ;
+        const T* qt = Qs + (16 * tile.x + l) * SQ;
+        if constexpr (kHalf) {
 #pragma unroll
-            for (int s = 0; s < DK / 32; ++s) {
-              const bf16x8 kf = *(const bf16x8*)(Kb + (16 * jt + l) * SQ + 32 * s + 8 * g);
-              const bf16x8 qf = *(const bf16x8*)(Qb + i * SQ + 32 * s + 8 * g);
-              p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf, p, 0, 0, 0);
-            }
-          } else {
+          for (int m = 0; m < DK / 32; ++m)
+            p[x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8*)(kt + 32 * m + 8 * g),
+                                                           *(const bf16x8*)(qt + 32 * m + 8 * g), p[x], 0, 0, 0);
+        } else {
 #pragma unroll
-            for (int s = 0; s < DK / 16; ++s) {
-              const f32x4 kf = *(const f32x4*)(Kb + (16 * jt + l) * SQ + 16 * s + 4 * g);
-              const f32x4 qf = *(const f32x4*)(Qb + i * SQ + 16 * s + 4 * g);
+          for (int m = 0; m < DK / 16; ++m) {
+            const f32x4 kf = *(const f32x4*)(kt + 16 * m + 4 * g), qf = *(const f32x4*)(qt + 16 * m + 4 * g);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) p = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[e], p, 0, 0, 0);
-            }
-          }
-          f32x4 y;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int j = 16 * jt + 4 * g + r, gap = back ? j - i : i - j;
-            const bool seen = back ? j < until : j >= from;
-            y[r] = gap >= 0 && seen ? p[r] * (w.read * w.add * pw[gap < 0 ? 0 : gap]) : 0.0f;
-          }
-          if constexpr (kHalf) {
-            float rest[4] = {y[0], y[1], y[2], y[3]};
-            __bf16 of[2][4];
-            split(rest, of);
-            *(bf16x4*)to = __builtin_bit_cast(bf16x4, of[0]);
-            *(bf16x4*)(to + C * SP) = __builtin_bit_cast(bf16x4, of[1]);
-          } else {
-            *(f32x4*)to = y;
+            for (int e = 0; e < 4; ++e) p[x] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[e], p[x], 0, 0, 0);
           }
         }
       }
-      __syncthreads();
-    }
+#pragma unroll
+      for (int x = 0; x < kOwn; ++x)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) p[x][r] *= of_pair[x][r];
+      if (mask) {
+#pragma unroll
+        for (int x = 0; x < kOwn; ++x) {
+          const int2 tile = pair_of(x);
+          const int i = 16 * tile.x + l;
+          const uint64_t upto = mask & ((2ull << i) - 1), after = i < 63 ? mask >> (i + 1) : 0;
+          const int from = upto ? 63 - __builtin_clzll(upto) : 0, until = after ? i + 1 + __builtin_ctzll(after) : C;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int j = 16 * tile.y + 4 * g + r;
+            p[x][r] = (kBack ? j < until : j >= from) ? p[x][r] : 0.0f;
+          }
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < kOwn; ++x) {
+        const int2 tile = pair_of(x);
+        if (kPairs % NW != 0 && wave + NW * x >= kPairs) break;
+        T* to = Ps + (16 * tile.x + l) * SP + 16 * tile.y + 4 * g;
+        if constexpr (kHalf) {
+          float rest[4] = {p[x][0], p[x][1], p[x][2], p[x][3]};
+          __bf16 of[2][4];
+          split(rest, of);
+          *(bf16x4*)to = __builtin_bit_cast(bf16x4, of[0]);
+          *(bf16x4*)(to + C * SP) = __builtin_bit_cast(bf16x4, of[1]);
+        } else {
+          *(f32x4*)to = p[x];
+        }
+      }
 
-    // this wave's columns of v, and its share of the products
-    bf16x8 vh[kHalf ? C / 32 : 1];
-    float vf[kHalf ? 1 : C / 4];
-    if constexpr (kHalf) {
+      // what the state gives
 #pragma unroll
-      for (int s = 0; s < C / 32; ++s) vh[s] = read_columns(Vb, SV, 32 * s + 8 * g, 16 * wave);
-    } else {
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) vf[4 * t + e] = Vb[(16 * t + 4 * g + e) * SV + col];
-    }
-
-    if constexpr (kOut) {
-      bf16x8 sh[kHalf ? DK / 32 : 1][2];
+      for (int it = 0; it < NT; ++it) o[it] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (!idle) {
       if constexpr (kHalf) {
 #pragma unroll
         for (int a = 0; a < DK / 32; ++a) {
@@ -406,113 +457,161 @@ __global__ __launch_bounds__(64 * NW) void chunk_kernel(Walk w) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) rest[e] = S[2 * a + e / 4][e % 4];
           split(rest, of);
-          sh[a][0] = __builtin_bit_cast(bf16x8, of[0]), sh[a][1] = __builtin_bit_cast(bf16x8, of[1]);
+#pragma unroll
+          for (int it = 0; it < NT; ++it) {
+            const __bf16* q = Qs + (16 * it + l) * SQ + 32 * a + 4 * g;
+            const bf16x8 qf =
+                __builtin_shufflevector(*(const bf16x4*)q, *(const bf16x4*)(q + 16), 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+              o[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, of[m]), qf, o[it], 0, 0, 0);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int a = 0; a < DK / 16; ++a) {
+          f32x4 qf[NT];
+#pragma unroll
+          for (int it = 0; it < NT; ++it) qf[it] = *(const f32x4*)(Qs + (16 * it + l) * SQ + 16 * a + 4 * g);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int it = 0; it < NT; ++it)
+              o[it] = __builtin_amdgcn_mfma_f32_16x16x4f32(S[a][e], qf[it][e], o[it], 0, 0, 0);
         }
       }
 #pragma unroll
       for (int it = 0; it < NT; ++it) {
-        if (16 * it >= n) continue;
-        const int i = 16 * it + l;
-        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (back ? r_last < 16 * it + 16 : r_first > 16 * it) {   // some token of the tile sees S
-          if constexpr (kHalf) {
+        float f = of_read[it];
+        if (kBack && n < C) f = 16 * it + l < n ? w.read * pw[n - 1 - (16 * it + l)] : 0.0f;
 #pragma unroll
-            for (int a = 0; a < DK / 32; ++a) {
-              const __bf16* at_q = Qb + i * SQ + 32 * a + 4 * g;
-              const bf16x8 qf = __builtin_shufflevector(*(const bf16x4*)at_q, *(const bf16x4*)(at_q + 16), 0, 1, 2, 3,
-                                                        4, 5, 6, 7);
-              o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sh[a][0], qf, o, 0, 0, 0);
-              o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sh[a][1], qf, o, 0, 0, 0);
-            }
-          } else {
+        for (int r = 0; r < 4; ++r) o[it][r] *= f;
+      }
+      if (mask) {
 #pragma unroll
-            for (int a = 0; a < DK / 16; ++a) {
-              const f32x4 qf = *(const f32x4*)(Qb + i * SQ + 16 * a + 4 * g);
+        for (int it = 0; it < NT; ++it) {
+          const bool sees = kBack ? 16 * it + l >= r_last : 16 * it + l < r_first;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) o = __builtin_amdgcn_mfma_f32_16x16x4f32(S[a][e], qf[e], o, 0, 0, 0);
-            }
-          }
-          const bool sees = back ? i >= r_last : i < r_first;
-          const int gap = back ? n - 1 - i : i + 1;
-          const float f = w.read * pw[gap < 0 ? 0 : gap];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[r] = sees ? o[r] * f : 0.0f;
+          for (int r = 0; r < 4; ++r) o[it][r] = sees ? o[it][r] : 0.0f;
         }
-        if constexpr (kHalf) {
+      }
+      }
+      __syncthreads();
+    }
+    if (idle) continue;
+
+    // this wave's columns of v, and its share of the products
+    bf16x8 vh[kHalf ? C / 32 : 1];
+    float vf[kHalf ? 1 : NH];
+    if constexpr (kHalf) {
 #pragma unroll
-          for (int s = 0; s < C / 32; ++s)
-            if (back ? 2 * s + 1 >= it : 2 * s <= it) {
-              const T* p = Ps + i * SP + 32 * s + 8 * g;
-              o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vh[s], *(const bf16x8*)p, o, 0, 0, 0);
-              o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vh[s], *(const bf16x8*)(p + C * SP), o, 0, 0, 0);
+      for (int s = 0; s < C / 32; ++s) vh[s] = read_columns(Vs, SV, 32 * s + 8 * g, 16 * wave);
+    } else {
+#pragma unroll
+      for (int x = 0; x < NH; ++x) vf[x] = Vs[held(x) * SV + col];
+    }
+
+    if constexpr (kOut) {
+      if constexpr (kHalf) {
+#pragma unroll
+        for (int s = 0; s < C / 32; ++s)
+#pragma unroll
+          for (int it = 0; it < NT; ++it)
+            if (kBack ? 2 * s + 1 >= it : 2 * s <= it) {
+              const T* p = Ps + (16 * it + l) * SP + 32 * s + 8 * g;
+              o[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vh[s], *(const bf16x8*)p, o[it], 0, 0, 0);
+              o[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vh[s], *(const bf16x8*)(p + C * SP), o[it], 0, 0, 0);
             }
-        } else {
+      } else {
 #pragma unroll
-          for (int t = 0; t < NT; ++t)
-            if (back ? t >= it : t <= it) {
-              const f32x4 p = *(const f32x4*)(Ps + i * SP + 16 * t + 4 * g);
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) o = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[4 * t + e], p[e], o, 0, 0, 0);
+          for (int it = 0; it < NT; ++it)
+            if (kBack ? t >= it : t <= it) {
+              const f32x4 p = *(const f32x4*)(Ps + (16 * it + l) * SP + 16 * t + 4 * g);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                o[it] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[4 * t + e], p[e], o[it], 0, 0, 0);
             }
-        }
-        if (i < n) {
-          const int c0 = 16 * wave + 4 * g;
-          T* to = (T*)w.out + ((b * w.t + at + i) * w.h + h) * w.dv + c0;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) bad = __builtin_fmaf(o[r], 0.0f, bad);
-          if (w.dv % 4 == 0) {
-            if (c0 < w.dv) {
-              if constexpr (kHalf)
-                *(bf16x4*)to = __builtin_convertvector(o, bf16x4);
-              else
-                *(f32x4*)to = o;
-            }
-          } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (c0 + r < w.dv) to[r] = from_f32<T>(o[r]);
-          }
-        }
       }
     }
 
     // the state after the chunk
-    const float keep = pw[n];
+    float add[NH];
+    if (n == C) {
 #pragma unroll
-    for (int a = 0; a < DK / 16; ++a)
+      for (int x = 0; x < NH; ++x) add[x] = of_add[x];
+    } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) S[a][r] = mask ? 0.0f : S[a][r] * keep;
+      for (int x = 0; x < NH; ++x) add[x] = held(x) < n ? w.add * pw[kBack ? held(x) + 1 : n - 1 - held(x)] : 0.0f;
+    }
+    const float keep = n == C ? of_chunk : pw[n];
+    if (mask) {
+#pragma unroll
+      for (int x = 0; x < NH; ++x) add[x] = (kBack ? held(x) < r_first : held(x) >= r_last) ? add[x] : 0.0f;
+#pragma unroll
+      for (int a = 0; a < DK / 16; ++a) S[a] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    } else {
+#pragma unroll
+      for (int a = 0; a < DK / 16; ++a)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) S[a][r] *= keep;
+    }
     if constexpr (kHalf) {
 #pragma unroll
       for (int s = 0; s < C / 32; ++s) {
-        if (32 * s >= n) continue;
-        const f32x4 w0 = *(const f32x4*)(wb + 32 * s + 8 * g), w1 = *(const f32x4*)(wb + 32 * s + 8 * g + 4);
         float rest[8];
-        __bf16 of[3][8];
+        __bf16 of[2][8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) rest[e] = (float)vh[s][e] * (e < 4 ? w0[e & 3] : w1[e & 3]);
+        for (int e = 0; e < 8; ++e) rest[e] = (float)vh[s][e] * add[8 * s + e];
         split(rest, of);
+        bf16x8 kf[DK / 16];
 #pragma unroll
-        for (int a = 0; a < DK / 16; ++a) {
-          const bf16x8 kf = read_columns(Kb, SQ, 32 * s + 8 * g, 16 * a);
+        for (int a = 0; a < DK / 16; ++a) kf[a] = read_columns(Ks, SQ, 32 * s + 8 * g, 16 * a);
 #pragma unroll
-          for (int m = 0; m < 3; ++m)
-            S[a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, __builtin_bit_cast(bf16x8, of[m]), S[a], 0, 0, 0);
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int a = 0; a < DK / 16; ++a)
+            S[a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[a], __builtin_bit_cast(bf16x8, of[m]), S[a], 0, 0, 0);
+        if (exact) {
+          __bf16 least[1][8];
+          split(rest, least);
+#pragma unroll
+          for (int a = 0; a < DK / 16; ++a)
+            S[a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[a], __builtin_bit_cast(bf16x8, least[0]), S[a], 0, 0, 0);
         }
       }
     } else {
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        if (16 * t >= n) continue;
-        const f32x4 x = *(const f32x4*)(wb + 16 * t + 4 * g);
+      for (int x = 0; x < NH; ++x) {
+        const float y = vf[x] * add[x];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float y = vf[4 * t + e] * x[e];
+        for (int a = 0; a < DK / 16; ++a)
+          S[a] = __builtin_amdgcn_mfma_f32_16x16x4f32(Ks[held(x) * SQ + 16 * a + l], y, S[a], 0, 0, 0);
+      }
+    }
+
+    if constexpr (kOut) {
+      const int c0 = 16 * wave + 4 * g;
 #pragma unroll
-          for (int a = 0; a < DK / 16; ++a)
-            S[a] = __builtin_amdgcn_mfma_f32_16x16x4f32(Kb[(16 * t + 4 * g + e) * SQ + 16 * a + l], y, S[a], 0, 0, 0);
+      for (int it = 0; it < NT; ++it) {
+        T* to = op + it * 16 * o_row;
+        if (16 * it + l < n) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) bad = __builtin_fmaf(o[it][r], 0.0f, bad);
+          if (c0 + 4 <= w.dv) {
+            if constexpr (kHalf)
+              *(half_piece_at_2*)to = __builtin_bit_cast(u32x2, __builtin_convertvector(o[it], bf16x4));
+            else
+              *(piece_at_2*)to = __builtin_bit_cast(u32x4, o[it]);
+          } else if (w.dv % 4 != 0) {
+#pragma unroll
+            for (int r = 0; r < 3; ++r)
+              if (c0 + r < w.dv) to[r] = from_f32<T>(o[it][r]);
+          }
         }
       }
+      op += (kBack ? -C : C) * o_row;
     }
   }
 
@@ -520,13 +619,12 @@ __global__ __launch_bounds__(64 * NW) void chunk_kernel(Walk w) {
   for (int a = 0; a < DK / 16; ++a)
 #pragma unroll
     for (int r = 0; r < 4; ++r) bad = __builtin_fmaf(S[a][r], 0.0f, bad);
-  if (!kOut && tid == 0) w.flags[row * w.parts + part] = any != 0;
+  if (!kOut && tid == 0) w.flags[(int64_t)row * w.parts + part] = any != 0;
   if (16 * wave >= w.dv) return;
   if (__builtin_amdgcn_ballot_w64(bad != bad)) {
     serial<T, kOut>(w, row, 16 * wave, t0, t1, kOut ? local : nullptr, !kOut, kOut ? nullptr : local, kOut && last);
     return;
   }
-  (void)first;
 #pragma unroll
   for (int a = 0; a < DK / 16; ++a)
 #pragma unroll
@@ -542,10 +640,14 @@ __global__ __launch_bounds__(64 * NW) void chunk_kernel(Walk w) {
 template <class T, int DK, int NW>
 int launch_sized(const Walk& w, bool out, hipStream_t s) {
   const dim3 grid((unsigned)(w.b * w.h * w.parts)), block(64 * NW);
-  if (out)
-    hipLaunchKernelGGL((chunk_kernel<T, DK, NW, true>), grid, block, 0, s, w);
+  if (out && w.backwards)
+    hipLaunchKernelGGL((chunk_kernel<T, DK, NW, true, true>), grid, block, 0, s, w);
+  else if (out)
+    hipLaunchKernelGGL((chunk_kernel<T, DK, NW, true, false>), grid, block, 0, s, w);
+  else if (w.backwards)
+    hipLaunchKernelGGL((chunk_kernel<T, DK, NW, false, true>), grid, block, 0, s, w);
   else
-    hipLaunchKernelGGL((chunk_kernel<T, DK, NW, false>), grid, block, 0, s, w);
+    hipLaunchKernelGGL((chunk_kernel<T, DK, NW, false, false>), grid, block, 0, s, w);
   return launch_status();
 }
 

@@ -6,34 +6,65 @@ namespace hipenvs {
 namespace da {
 
 // From each part's own state (what its tokens alone leave behind) to the state before each
-// part, in the order of the walk: carry' = lambda^tokens carry [no reset] + own. A thread for
-// each value of a row's state, eight parts' values read ahead of their use.
-__global__ __launch_bounds__(kBlock) void join_kernel(Walk w) {
-  const int size = w.dk * w.dv, at = blockIdx.y * kBlock + threadIdx.x;
-  if (at >= size) return;
+// part, in the order of the walk: carry' = lambda^tokens carry [no reset] + own. `groups`
+// threads (1 to 8) take one value of a row's state, eight parts each: a thread reads its parts at
+// once and composes them into one step of the same form; the steps before it give it its
+// carry, and it writes its parts' states. One load's latency for up to 64 parts, and every
+// state read and written once. (A thread with all parts one after another took 31 us at
+// 64 parts of 8 rows of 64 x 64; eight threads for a value whatever the parts, 28 us at 4
+// parts of 150 rows of 48 x 80.)
+constexpr int kEach = 8, kGroups = 8;
+__global__ __launch_bounds__(kBlock) void join_kernel(Walk w, int groups) {
+  __shared__ float keeps[kBlock], owns[kBlock];
+  const int values = kBlock / groups, size = w.dk * w.dv;
+  const int group = threadIdx.x / values, x = threadIdx.x - group * values, at = blockIdx.y * values + x;
   const int64_t row = blockIdx.x, h = row % w.h;
+  const bool live = at < size;
   const float ld = w.log_decay[h];
-  float* states = w.states + row * w.parts * size + at;
+  float* states = w.states + row * w.parts * size + (live ? at : 0);
   const uint8_t* flags = w.flags + row * w.parts;
-  float carry = w.state_in ? w.state_in[state_index(w, row, at / w.dv, at % w.dv)] : 0.0f;
-  constexpr int kAhead = 8;
-  for (int n0 = 0; n0 < w.parts; n0 += kAhead) {
-    float own[kAhead];
-    bool reset[kAhead];
+  // a part's step; a keep below zero drops the state before it, whatever that holds
+  const auto stepped = [](float keep, float before, float own) { return (keep < 0.0f ? 0.0f : before * keep) + own; };
+  float carry = w.state_in && live ? w.state_in[state_index(w, row, at / w.dv, at % w.dv)] : 0.0f;
+  const float whole = expf(ld * (float)w.part);
+  for (int base = 0; base < w.parts; base += groups * kEach) {
+    const int n0 = base + group * kEach;
+    float own[kEach], of[kEach];
 #pragma unroll
-    for (int e = 0; e < kAhead; ++e) {
-      const int n = n0 + e, p = w.backwards ? w.parts - 1 - n : n;
-      own[e] = n < w.parts ? states[(int64_t)p * size] : 0.0f;
-      reset[e] = n < w.parts ? flags[p] != 0 : false;
+    for (int e = 0; e < kEach; ++e) {
+      own[e] = 0.0f, of[e] = 1.0f;
+      if (n0 + e < w.parts) {
+        const int p = w.backwards ? w.parts - 1 - n0 - e : n0 + e;
+        own[e] = states[(int64_t)p * size];
+        of[e] = flags[p] ? -1.0f : p < w.parts - 1 ? whole : expf(ld * (float)(w.t - (int64_t)p * w.part));
+      }
+    }
+    float mid = carry;
+    if (groups > 1) {
+      float keep = 1.0f, sum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        sum = stepped(of[e], sum, own[e]);
+        keep = of[e] < 0.0f || keep < 0.0f ? -1.0f : keep * of[e];
+      }
+      __syncthreads();   // the round before has been read
+      keeps[threadIdx.x] = keep;
+      owns[threadIdx.x] = sum;
+      __syncthreads();
+      for (int e = 0; e < groups; ++e) {
+        if (e == group) mid = carry;
+        carry = stepped(keeps[e * values + x], carry, owns[e * values + x]);
+      }
     }
 #pragma unroll
-    for (int e = 0; e < kAhead; ++e) {
-      const int n = n0 + e, p = w.backwards ? w.parts - 1 - n : n;
-      if (n >= w.parts) break;
-      states[(int64_t)p * size] = carry;
-      const int64_t left = w.t - (int64_t)p * w.part, tokens = left < w.part ? left : w.part;
-      carry = (reset[e] ? 0.0f : carry * expf(ld * (float)tokens)) + own[e];
+    for (int e = 0; e < kEach; ++e) {
+      if (n0 + e < w.parts && live) {
+        const int p = w.backwards ? w.parts - 1 - n0 - e : n0 + e;
+        states[(int64_t)p * size] = mid;
+      }
+      mid = stepped(of[e], mid, own[e]);
     }
+    if (groups == 1) carry = mid;
   }
 }
 
@@ -119,7 +150,10 @@ int launch_walk(int32_t dtype, Walk w, hipStream_t s) {
   if (w.parts > 1) {
     int status = dtype == 1 ? launch_chunks<__bf16>(w, false, s) : launch_chunks<float>(w, false, s);
     if (status != HIPENVS_OK) return status;
-    hipLaunchKernelGGL(join_kernel, dim3((unsigned)(w.b * w.h), grid_for(w.dk * w.dv)), dim3(kBlock), 0, s, w);
+    int groups = 1;
+    while (groups < kGroups && groups * kEach < w.parts) groups *= 2;
+    hipLaunchKernelGGL(join_kernel, dim3((unsigned)(w.b * w.h), grid_for(w.dk * w.dv, kBlock / groups)), dim3(kBlock),
+                       0, s, w, groups);
     status = launch_status();
     if (status != HIPENVS_OK) return status;
   }
@@ -138,12 +172,7 @@ bool sequence_ok(int32_t dtype, int64_t b, int64_t t, int64_t h, int64_t dk, int
   return dims_ok(dtype, h, dk, dv) && b >= 0 && t >= 0 && b * h <= 0x7FFFFFFF && b <= 0x7FFFFFFF && t <= 0x7FFFFFFF;
 }
 
-// `d` values a row of `size` bytes each.
-Rows rows(const void* data, const int64_t* strides, int64_t size, int64_t d) {
-  const bool wide = (((uintptr_t)data | (uintptr_t)(strides[0] * size) | (uintptr_t)(strides[1] * size) |
-                      (uintptr_t)(strides[2] * size) | (uintptr_t)(d * size)) & 15) == 0;
-  return {data, strides[0], strides[1], strides[2], wide};
-}
+Rows rows(const void* data, const int64_t* strides) { return {data, strides[0], strides[1], strides[2]}; }
 
 // The parts of a sequence and where in `workspace` their states and flags lie; the bytes used.
 int plan(int32_t dtype, int64_t b, int64_t t, int32_t h, int32_t dk, int32_t dv, void* workspace, Walk* w,
@@ -179,15 +208,14 @@ extern "C" int hipenvs_decay_attention(int32_t dtype, const void* q, const void*
   if (!log_decay || !final_state || (t > 0 && (!q || !k || !v || !out || !strides))) return HIPENVS_E_ARG;
   static const int64_t none[11] = {};
   const int64_t* st = t > 0 ? strides : none;
-  const int64_t e = dtype == 1 ? 2 : 4;
   Walk w = {};
   int64_t need = 0;
   const int status = plan(dtype, b, t, h, dk, dv, workspace, &w, &need);
   if (status != HIPENVS_OK) return status;
   if (need > 0 && (!workspace || workspace_bytes < need)) return HIPENVS_E_ARG;
-  w.q = rows(q, st, e, dk), w.k = rows(k, st + 3, e, dk), w.v = rows(v, st + 6, e, dv);
+  w.q = rows(q, st), w.k = rows(k, st + 3), w.v = rows(v, st + 6);
   w.dk = dk, w.dv = dv, w.log_decay = log_decay, w.reset = reset, w.reset_sb = st[9], w.reset_st = st[10];
-  w.state_in = state, w.state_out = final_state, w.read = scale, w.add = 1.0f;
+  w.state_in = state, w.state_out = final_state, w.exact = true, w.read = scale, w.add = 1.0f;
   w.out = out, w.b = b, w.t = t, w.h = h;
   return launch_walk(dtype, w, as_stream(stream));
 }
@@ -204,14 +232,13 @@ extern "C" int hipenvs_decay_attention_backward(int32_t dtype, const void* q, co
     return HIPENVS_E_ARG;
   static const int64_t none[14] = {};
   const int64_t* st = t > 0 ? strides : none;
-  const int64_t e = dtype == 1 ? 2 : 4;
   Walk w = {};
   int64_t need = 0;
   int status = plan(dtype, b, t, h, dk, dv, workspace, &w, &need);
   if (status != HIPENVS_OK) return status;
   if (need > 0 && (!workspace || workspace_bytes < need)) return HIPENVS_E_ARG;
-  const Rows rq = rows(q, st, e, dk), rk = rows(k, st + 3, e, dk), rv = rows(v, st + 6, e, dv),
-             rdo = rows(dout, st + 9, e, dv);
+  const Rows rq = rows(q, st), rk = rows(k, st + 3), rv = rows(v, st + 6),
+             rdo = rows(dout, st + 9);
   const hipStream_t s = as_stream(stream);
   w.log_decay = log_decay, w.reset = reset, w.reset_sb = st[12], w.reset_st = st[13], w.b = b, w.t = t, w.h = h;
   // dq: forwards over the transposed states
@@ -220,12 +247,13 @@ extern "C" int hipenvs_decay_attention_backward(int32_t dtype, const void* q, co
   status = launch_walk(dtype, w, s);
   if (status != HIPENVS_OK) return status;
   // dv, and the gradient of the first state: backwards over the states' gradients
-  w.q = rk, w.k = rq, w.v = rdo, w.dk = dk, w.dv = dv, w.state_in = dfinal, w.state_out = dstate;
+  w.q = rk, w.k = rq, w.v = rdo, w.dk = dk, w.dv = dv, w.state_in = dfinal, w.state_out = dstate, w.exact = true;
   w.flipped = false, w.backwards = true, w.read = 1.0f, w.add = scale, w.out = dv_out;
   status = launch_walk(dtype, w, s);
   if (status != HIPENVS_OK) return status;
   // dk: the same, transposed
-  w.q = rv, w.k = rdo, w.v = rq, w.dk = dv, w.dv = dk, w.state_out = nullptr, w.flipped = true, w.out = dk_out;
+  w.q = rv, w.k = rdo, w.v = rq, w.dk = dv, w.dv = dk, w.state_out = nullptr, w.exact = false, w.flipped = true;
+  w.out = dk_out;
   return launch_walk(dtype, w, s);
 }
 
