@@ -158,18 +158,46 @@ struct Chunk<float> {
 typedef u32x4 __attribute__((aligned(2))) piece_at_2;
 typedef u32x2 __attribute__((aligned(2))) half_piece_at_2;
 
-// One 16-byte piece of a token's row from its column `col` on, zeros where the row has ended.
+// A token's row of `dim` values is read in 16-byte pieces. The last one may be short: then the
+// row's last 16 bytes are read, which begin piece_begin(col) values into the row, and moved
+// down by `settled` once they are there (where they are written to LDS, so that no load waits
+// for another). A row shorter than a piece is read one value after another.
+template <class T>
+__device__ __forceinline__ int piece_begin(int col, int dim) {
+  constexpr int E = 16 / sizeof(T);
+  return dim < E ? 0 : col + E <= dim ? col : dim - E;
+}
+
 template <class T>
 __device__ __forceinline__ u32x4 load_piece(const T* at, int col, int dim) {
   constexpr int E = 16 / sizeof(T);
   u32x4 x = {0, 0, 0, 0};
-  if (col + E <= dim) {
-    x = *(const piece_at_2*)at;
-  } else if (dim % E != 0) {
-    T* y = (T*)&x;
-#pragma unroll
-    for (int e = 0; e < E - 1; ++e)
-      if (col + e < dim) y[e] = at[e];
+  if (col >= dim) return x;
+  if (dim < E) {
+    typedef uint32_t word __attribute__((aligned(2)));
+    if (sizeof(T) == 4) {
+#pragma unroll 1
+      for (int e = dim - 1; e >= 0; --e) x = u32x4{((const word*)at)[e], x[0], x[1], x[2]};
+    } else {
+#pragma unroll 1
+      for (int e = dim - 1; e >= 0; --e)
+        x = u32x4{(x[0] << 16) | ((const uint16_t*)at)[e], (x[1] << 16) | (x[0] >> 16), (x[2] << 16) | (x[1] >> 16),
+                  (x[3] << 16) | (x[2] >> 16)};
+    }
+    return x;
+  }
+  return *(const piece_at_2*)at;
+}
+
+template <class T>
+__device__ __forceinline__ u32x4 settled(u32x4 x, int col, int dim) {
+  constexpr int E = 16 / sizeof(T);
+  if (dim % E != 0 && dim > E) {
+    const int over = col + E > dim ? col + E - dim : 0, bytes = over * (int)sizeof(T);
+    if (bytes & 8) x = u32x4{x[2], x[3], 0, 0};
+    if (bytes & 4) x = u32x4{x[1], x[2], x[3], 0};
+    if (bytes & 2)
+      x = u32x4{(x[0] >> 16) | (x[1] << 16), (x[1] >> 16) | (x[2] << 16), (x[2] >> 16) | (x[3] << 16), x[3] >> 16};
   }
   return x;
 }
@@ -249,13 +277,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
 #pragma unroll
   for (int m = 0; m < NQ; ++m) {
     const int p = tid + m * TH, r = p / QP, x = (p - r * QP) * E;
-    kp[m] = (const T*)w.k.data + b * w.k.sb + h * w.k.sh + (start + r) * w.k.st + x;
-    if constexpr (kOut) qp[m] = (const T*)w.q.data + b * w.q.sb + h * w.q.sh + (start + r) * w.q.st + x;
+    const int y = piece_begin<T>(x, w.dk);
+    kp[m] = (const T*)w.k.data + b * w.k.sb + h * w.k.sh + (start + r) * w.k.st + y;
+    if constexpr (kOut) qp[m] = (const T*)w.q.data + b * w.q.sb + h * w.q.sh + (start + r) * w.q.st + y;
   }
 #pragma unroll
   for (int m = 0; m < NV; ++m) {
     const int p = tid + m * TH, r = p / VP, x = (p - r * VP) * E;
-    vp[m] = (const T*)w.v.data + b * w.v.sb + h * w.v.sh + (start + r) * w.v.st + x;
+    vp[m] = (const T*)w.v.data + b * w.v.sb + h * w.v.sh + (start + r) * w.v.st + piece_begin<T>(x, w.dv);
   }
   const uint8_t* rp = w.reset ? w.reset + b * w.reset_sb + (start + lane) * w.reset_st : nullptr;
   const int64_t q_on = (kBack ? -C : C) * w.q.st, k_on = (kBack ? -C : C) * w.k.st, v_on = (kBack ? -C : C) * w.v.st;
@@ -311,15 +340,23 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
   f32x4 S[DK / 16];
   const int col = 16 * wave + l;
 #pragma unroll
-  for (int a = 0; a < DK / 16; ++a)
+  for (int a = 0; a < DK / 16; ++a) S[a] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  if (kOut && (local || w.state_in)) {   // every value in flight at once: none behind a condition of its own
+    const float* from = local ? local : w.state_in + (int64_t)row * w.dk * w.dv;
+    const bool turned = !local && w.flipped;
+    const int on_row = turned ? 1 : w.dv, on_col = turned ? w.dk : 1, c = col < w.dv ? col : 0;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int k = 16 * a + 4 * g + r;
-      float x = 0.0f;
-      if (kOut && k < w.dk && col < w.dv)
-        x = local ? local[(int64_t)k * w.dv + col] : w.state_in ? w.state_in[state_index(w, row, k, col)] : 0.0f;
-      S[a][r] = x;
-    }
+    for (int a = 0; a < DK / 16; ++a)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int k = 16 * a + 4 * g + r;
+        S[a][r] = from[(k < w.dk ? k : 0) * on_row + c * on_col];
+      }
+#pragma unroll
+    for (int a = 0; a < DK / 16; ++a)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) S[a][r] = 16 * a + 4 * g + r < w.dk && col < w.dv ? S[a][r] : 0.0f;
+  }
   __syncthreads();   // pw
 
   // The tiles of P, 16 queries x 16 keys, that some product uses, dealt to the waves: tile x of
@@ -371,14 +408,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     for (int m = 0; m < NQ; ++m) {
       const int p = tid + m * TH, r = p / QP, x = (p - r * QP) * E;
       if (C * QP % TH == 0 || r < C) {
-        *(u32x4*)(Ks + r * SQ + x) = xk[m];
-        if constexpr (kOut) *(u32x4*)(Qs + r * SQ + x) = xq[m];
+        *(u32x4*)(Ks + r * SQ + x) = settled<T>(xk[m], x, w.dk);
+        if constexpr (kOut) *(u32x4*)(Qs + r * SQ + x) = settled<T>(xq[m], x, w.dk);
       }
     }
 #pragma unroll
     for (int m = 0; m < NV; ++m) {
       const int p = tid + m * TH, r = p / VP, x = (p - r * VP) * E;
-      if (C * VP % TH == 0 || r < C) *(u32x4*)(Vs + r * SV + x) = xv[m];
+      if (C * VP % TH == 0 || r < C) *(u32x4*)(Vs + r * SV + x) = settled<T>(xv[m], x, w.dv);
     }
     // the chunk's resets, bit i for token i; the first and the last of them
     const uint64_t mask = __builtin_amdgcn_ballot_w64(xr != 0);
