@@ -141,22 +141,34 @@ __device__ __forceinline__ void serial(const Walk& w, int64_t row, int col0, int
 
 // ---- the chunked walk -------------------------------------------------------------------
 
-// Tokens a chunk holds and the padding of its LDS rows, which keeps 16 rows read at one column
-// on different banks.
+// Tokens a chunk holds and the padding of LDS rows of `width` values: 16 rows read at one column
+// in 16 bytes lie on different banks, and so do, nearly, the 8 bytes of 8 rows that the
+// transposing reads of bfloat16 take at once (rows 12, 28, 36 or 52 banks apart).
 template <class T>
 struct Chunk;
 template <>
 struct Chunk<__bf16> {
-  static constexpr int kTokens = 64, kPad = 8;
+  static constexpr int kTokens = 64;
+  static constexpr int pad(int width) { return width == 32 || width == 128 ? 24 : 8; }
 };
 template <>
 struct Chunk<float> {
-  static constexpr int kTokens = 32, kPad = 4;
+  static constexpr int kTokens = 32;
+  static constexpr int pad(int) { return 4; }
 };
 
 // 16 bytes at any address that is a multiple of the value's size.
 typedef u32x4 __attribute__((aligned(2))) piece_at_2;
-typedef u32x2 __attribute__((aligned(2))) half_piece_at_2;
+template <class T>
+struct Fours;   // four values
+template <>
+struct Fours<__bf16> {
+  typedef u32x2 type;
+};
+template <>
+struct Fours<float> {
+  typedef u32x4 type;
+};
 
 // A token's row of `dim` values is read in 16-byte pieces. The last one may be short: then the
 // row's last 16 bytes are read, which begin piece_begin(col) values into the row, and moved
@@ -169,24 +181,20 @@ __device__ __forceinline__ int piece_begin(int col, int dim) {
 }
 
 template <class T>
-__device__ __forceinline__ u32x4 load_piece(const T* at, int col, int dim) {
+__device__ __forceinline__ u32x4 load_short_row(const T* at, int col, int dim) {
   constexpr int E = 16 / sizeof(T);
   u32x4 x = {0, 0, 0, 0};
   if (col >= dim) return x;
-  if (dim < E) {
-    typedef uint32_t word __attribute__((aligned(2)));
-    if (sizeof(T) == 4) {
+  if (dim >= E) return *(const piece_at_2*)at;
 #pragma unroll 1
-      for (int e = dim - 1; e >= 0; --e) x = u32x4{((const word*)at)[e], x[0], x[1], x[2]};
-    } else {
-#pragma unroll 1
-      for (int e = dim - 1; e >= 0; --e)
-        x = u32x4{(x[0] << 16) | ((const uint16_t*)at)[e], (x[1] << 16) | (x[0] >> 16), (x[2] << 16) | (x[1] >> 16),
-                  (x[3] << 16) | (x[2] >> 16)};
-    }
-    return x;
+  for (int e = dim - 1; e >= 0; --e) {
+    if (sizeof(T) == 4)
+      x = u32x4{((const uint32_t*)at)[e], x[0], x[1], x[2]};
+    else
+      x = u32x4{(x[0] << 16) | ((const uint16_t*)at)[e], (x[1] << 16) | (x[0] >> 16), (x[2] << 16) | (x[1] >> 16),
+                (x[3] << 16) | (x[2] >> 16)};
   }
-  return *(const piece_at_2*)at;
+  return x;
 }
 
 template <class T>
@@ -207,15 +215,29 @@ __device__ __forceinline__ bf16x8 join(i16x4 a, i16x4 b) {
   return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// Columns col .. col + 15 of rows row .. row + 7 of a bfloat16 tile, rows differing between
-// the four groups of 16 lanes: lane l of a group gets column col + l, its 8 rows in order. A
+// Columns col .. col + 15 of rows row .. row + 3 and row + 16 .. row + 19 of a bfloat16 tile,
+// rows differing between the four groups of 16 lanes: lane l of a group gets column col + l. A
 // transposing read gives a group 16 columns of 4 rows, each of its lanes addressing 4 values.
 __device__ __forceinline__ bf16x8 read_columns(const __bf16* tile, int stride, int row, int col) {
   const int l = threadIdx.x & 15;
   const __bf16* p = tile + (row + (l >> 2)) * stride + col + 4 * (l & 3);
   typedef __attribute__((address_space(3))) i16x4* lds4;
   return join(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p),
-              __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 4 * stride)));
+              __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 16 * stride)));
+}
+
+// Four values and the four 16 further on: an operand whose summed axis is ordered like
+// read_columns' and like a result's rows.
+__device__ __forceinline__ bf16x8 read_pair(const __bf16* p) {
+  return __builtin_shufflevector(*(const bf16x4*)p, *(const bf16x4*)(p + 16), 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// A lane's index, in a branch that few chunks take: what is computed from it there is computed
+// there. Otherwise the compiler computes it all before the loop and holds it in registers that
+// the loop itself needs (248 of 256 at bfloat16 heads of 64, its reads waiting for each other).
+__device__ __forceinline__ int here(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
 }
 
 // The bfloat16 parts of N (even) float32 values: of each, the rounding of what is left.
@@ -244,11 +266,18 @@ __device__ __forceinline__ void split(float (&rest)[N], __bf16 (&parts)[M][N]) {
 // rounding of what the parts before it leave: two parts for P and S (16 bits, so a result's
 // error is that of its own rounding to bfloat16) and for what enters a state that only results
 // are read from, three for one that is a float32 result itself (all 24 bits). float32 rows use the float32 matrix instructions throughout.
+// Waves a SIMD holds at once, which bounds their registers (512 over that many): three where
+// that many registers suffice without spilling, two elsewhere.
+template <class T>
+constexpr int waves_of(int dk, int nw) {
+  return sizeof(T) == 4 && (dk == 32 || (dk == 64 && nw >= 4)) ? 3 : 2;
+}
+
 template <class T, int DK, int NW, bool kOut, bool kBack>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) void chunk_kernel(Walk w) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_of<T>(DK, NW)))) void chunk_kernel(Walk w) {
   constexpr bool kHalf = sizeof(T) == 2;
-  constexpr int C = Chunk<T>::kTokens, PAD = Chunk<T>::kPad, E = 16 / sizeof(T), TH = 64 * NW, DV = 16 * NW;
-  constexpr int SQ = DK + PAD, SV = DV + PAD, SP = C + PAD, NT = C / 16;
+  constexpr int C = Chunk<T>::kTokens, E = 16 / sizeof(T), TH = 64 * NW, DV = 16 * NW, NT = C / 16;
+  constexpr int SQ = DK + Chunk<T>::pad(DK), SV = DV + Chunk<T>::pad(DV), SP = C + Chunk<T>::pad(C);
   constexpr int QP = DK / E, VP = DV / E;                               // pieces of a row
   constexpr int NQ = (C * QP + TH - 1) / TH, NV = (C * VP + TH - 1) / TH;  // pieces of a thread
   __shared__ __attribute__((aligned(16))) T Qs[kOut ? C * SQ : 8];
@@ -271,62 +300,63 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
 
   // where this thread's pieces of the first chunk lie, and how far on the next chunk's do
   const int64_t start = t0 + (kBack ? (int64_t)(chunks - 1) * C : 0);
-  const T* qp[kOut ? NQ : 1];
-  const T* kp[NQ];
-  const T* vp[NV];
-#pragma unroll
-  for (int m = 0; m < NQ; ++m) {
-    const int p = tid + m * TH, r = p / QP, x = (p - r * QP) * E;
-    const int y = piece_begin<T>(x, w.dk);
-    kp[m] = (const T*)w.k.data + b * w.k.sb + h * w.k.sh + (start + r) * w.k.st + y;
-    if constexpr (kOut) qp[m] = (const T*)w.q.data + b * w.q.sb + h * w.q.sh + (start + r) * w.q.st + y;
-  }
-#pragma unroll
-  for (int m = 0; m < NV; ++m) {
-    const int p = tid + m * TH, r = p / VP, x = (p - r * VP) * E;
-    vp[m] = (const T*)w.v.data + b * w.v.sb + h * w.v.sh + (start + r) * w.v.st + piece_begin<T>(x, w.dv);
-  }
+  static_assert(TH % QP == 0 && TH % VP == 0, "a thread's pieces lie in one column of a chunk");
+  const int qx = tid % QP * E, qr = tid / QP, vx = tid % VP * E, vr = tid / VP;
+  constexpr int QR = TH / QP, VR = TH / VP;   // rows between a thread's pieces
+  const int ky = piece_begin<T>(qx, w.dk);
+  const T* kp = (const T*)w.k.data + b * w.k.sb + h * w.k.sh + (start + qr) * w.k.st + ky;
+  const T* qp = kOut ? (const T*)w.q.data + b * w.q.sb + h * w.q.sh + (start + qr) * w.q.st + ky : nullptr;
+  const T* vp = (const T*)w.v.data + b * w.v.sb + h * w.v.sh + (start + vr) * w.v.st + piece_begin<T>(vx, w.dv);
   const uint8_t* rp = w.reset ? w.reset + b * w.reset_sb + (start + lane) * w.reset_st : nullptr;
   const int64_t q_on = (kBack ? -C : C) * w.q.st, k_on = (kBack ? -C : C) * w.k.st, v_on = (kBack ? -C : C) * w.v.st;
 
   u32x4 xq[kOut ? NQ : 1], xk[NQ], xv[NV];
   uint32_t xr = 0;
-  const bool filled = w.dk == DK && w.dv == DV && C * QP % TH == 0 && C * VP % TH == 0;
+  const bool tiny = w.dk < E || w.dv < E;
+  const bool filled = w.dk == DK && w.dv == DV && C % QR == 0 && C % VR == 0;
   const auto load = [&](int n) {
     if (filled && n == C) {
 #pragma unroll
       for (int m = 0; m < NQ; ++m) {
-        xk[m] = *(const piece_at_2*)kp[m];
-        if constexpr (kOut) xq[m] = *(const piece_at_2*)qp[m];
+        xk[m] = *(const piece_at_2*)(kp + m * QR * w.k.st);
+        if constexpr (kOut) xq[m] = *(const piece_at_2*)(qp + m * QR * w.q.st);
       }
 #pragma unroll
-      for (int m = 0; m < NV; ++m) xv[m] = *(const piece_at_2*)vp[m];
+      for (int m = 0; m < NV; ++m) xv[m] = *(const piece_at_2*)(vp + m * VR * w.v.st);
     } else {
       const u32x4 none = {0, 0, 0, 0};
 #pragma unroll
       for (int m = 0; m < NQ; ++m) {
-        const int p = tid + m * TH, r = p / QP, x = (p - r * QP) * E;
         xk[m] = none;
         if constexpr (kOut) xq[m] = none;
-        if (r < n) {
-          xk[m] = load_piece<T>(kp[m], x, w.dk);
-          if constexpr (kOut) xq[m] = load_piece<T>(qp[m], x, w.dk);
-        }
       }
 #pragma unroll
-      for (int m = 0; m < NV; ++m) {
-        const int p = tid + m * TH, r = p / VP, x = (p - r * VP) * E;
-        xv[m] = none;
-        if (r < n) xv[m] = load_piece<T>(vp[m], x, w.dv);
+      for (int m = 0; m < NV; ++m) xv[m] = none;
+      if (!tiny) {
+#pragma unroll
+        for (int m = 0; m < NQ; ++m)
+          if (qr + m * QR < n && qx < w.dk) {
+            xk[m] = *(const piece_at_2*)(kp + m * QR * w.k.st);
+            if constexpr (kOut) xq[m] = *(const piece_at_2*)(qp + m * QR * w.q.st);
+          }
+#pragma unroll
+        for (int m = 0; m < NV; ++m)
+          if (vr + m * VR < n && vx < w.dv) xv[m] = *(const piece_at_2*)(vp + m * VR * w.v.st);
+      } else {
+#pragma unroll
+        for (int m = 0; m < NQ; ++m)
+          if (qr + m * QR < n) {
+            xk[m] = load_short_row<T>(kp + m * QR * w.k.st, qx, w.dk);
+            if constexpr (kOut) xq[m] = load_short_row<T>(qp + m * QR * w.q.st, qx, w.dk);
+          }
+#pragma unroll
+        for (int m = 0; m < NV; ++m)
+          if (vr + m * VR < n) xv[m] = load_short_row<T>(vp + m * VR * w.v.st, vx, w.dv);
       }
     }
-#pragma unroll
-    for (int m = 0; m < NQ; ++m) {
-      kp[m] += k_on;
-      if constexpr (kOut) qp[m] += q_on;
-    }
-#pragma unroll
-    for (int m = 0; m < NV; ++m) vp[m] += v_on;
+    kp += k_on;
+    if constexpr (kOut) qp += q_on;
+    vp += v_on;
     xr = 0;
     if (rp) {
       if (lane < n) xr = *rp;
@@ -372,7 +402,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
   // The decays of a whole chunk. of_pair[x][r]: of tile x of P, zero where the key is not yet
   // there; of_read[it]: of the state, for query 16 it + l; of_add[x]: of the x-th token that
   // this lane holds of v, which is held(x).
-  const auto held = [&](int x) { return kHalf ? 32 * (x / 8) + 8 * g + x % 8 : 16 * (x / 4) + 4 * g + x % 4; };
+  const auto held = [](int x, int g) { return 16 * (x / 4) + 4 * g + x % 4; };
   constexpr int NH = C / 4;
   float of_pair[kOut ? kOwn : 1][4], of_read[kOut ? NT : 1], of_add[NH];
   if constexpr (kOut) {
@@ -390,12 +420,43 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     for (int it = 0; it < NT; ++it) of_read[it] = w.read * pw[kBack ? C - 1 - (16 * it + l) : 16 * it + l + 1];
   }
 #pragma unroll
-  for (int x = 0; x < NH; ++x) of_add[x] = w.add * pw[kBack ? held(x) + 1 : C - 1 - held(x)];
+  for (int x = 0; x < NH; ++x) of_add[x] = w.add * pw[kBack ? held(x, g) + 1 : C - 1 - held(x, g)];
   const float of_chunk = pw[C];
 
   T* op = nullptr;   // this lane's first output of the chunk
   const int64_t o_row = (int64_t)w.h * w.dv;
   if constexpr (kOut) op = (T*)w.out + (b * w.t + start + l) * o_row + h * w.dv + 16 * wave + 4 * g;
+
+  // The outputs of a chunk are stored while the next one is on its way to LDS: after the wait
+  // for that one's loads, which would otherwise be a wait for the stores as well.
+  typedef typename Fours<T>::type Four;
+  Four done[kOut ? NT : 1];
+  int done_n = 0;
+  const auto store = [&]() {
+    typedef Four __attribute__((aligned(2))) at_2;
+    if (done_n == C && 16 * wave + 16 <= w.dv) {
+#pragma unroll
+      for (int it = 0; it < NT; ++it) *(at_2*)(op + it * 16 * o_row) = done[it];
+    } else {
+      const int lh = here(l), c0 = here(16 * wave + 4 * g);
+#pragma unroll
+      for (int it = 0; it < NT; ++it) {
+        T* to = op + it * 16 * o_row;
+        if (16 * it + lh < done_n) {
+          if (c0 + 4 <= w.dv) {
+            *(at_2*)to = done[it];
+          } else if (w.dv % 4 != 0) {
+            T y[4];
+            __builtin_memcpy(y, &done[it], sizeof(y));
+#pragma unroll
+            for (int r = 0; r < 3; ++r)
+              if (c0 + r < w.dv) to[r] = y[r];
+          }
+        }
+      }
+    }
+    if (done_n > 0) op += (kBack ? -C : C) * o_row;
+  };
 
   const bool idle = 16 * wave >= w.dv;   // no columns: this wave only moves and shares
   const bool exact = w.exact;
@@ -404,19 +465,25 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
   for (int step = 0; step < chunks; ++step) {
     const int n = (kBack ? step == 0 : step == chunks - 1) ? tokens_of_last : C;
     if (step > 0) __syncthreads();   // the chunk before has been read
+    if (w.dk % E != 0 || w.dv % E != 0) {
 #pragma unroll
-    for (int m = 0; m < NQ; ++m) {
-      const int p = tid + m * TH, r = p / QP, x = (p - r * QP) * E;
-      if (C * QP % TH == 0 || r < C) {
-        *(u32x4*)(Ks + r * SQ + x) = settled<T>(xk[m], x, w.dk);
-        if constexpr (kOut) *(u32x4*)(Qs + r * SQ + x) = settled<T>(xq[m], x, w.dk);
+      for (int m = 0; m < NQ; ++m) {
+        xk[m] = settled<T>(xk[m], qx, w.dk);
+        if constexpr (kOut) xq[m] = settled<T>(xq[m], qx, w.dk);
       }
+#pragma unroll
+      for (int m = 0; m < NV; ++m) xv[m] = settled<T>(xv[m], vx, w.dv);
     }
 #pragma unroll
-    for (int m = 0; m < NV; ++m) {
-      const int p = tid + m * TH, r = p / VP, x = (p - r * VP) * E;
-      if (C * VP % TH == 0 || r < C) *(u32x4*)(Vs + r * SV + x) = settled<T>(xv[m], x, w.dv);
-    }
+    for (int m = 0; m < NQ; ++m)
+      if (C % QR == 0 || qr + m * QR < C) {
+        *(u32x4*)(Ks + (qr + m * QR) * SQ + qx) = xk[m];
+        if constexpr (kOut) *(u32x4*)(Qs + (qr + m * QR) * SQ + qx) = xq[m];
+      }
+#pragma unroll
+    for (int m = 0; m < NV; ++m)
+      if (C % VR == 0 || vr + m * VR < C) *(u32x4*)(Vs + (vr + m * VR) * SV + vx) = xv[m];
+    if constexpr (kOut) store();
     // the chunk's resets, bit i for token i; the first and the last of them
     const uint64_t mask = __builtin_amdgcn_ballot_w64(xr != 0);
     any |= mask;
@@ -453,15 +520,16 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
 #pragma unroll
         for (int r = 0; r < 4; ++r) p[x][r] *= of_pair[x][r];
       if (mask) {
+        const int lh = here(l), gh = here(g);
 #pragma unroll
         for (int x = 0; x < kOwn; ++x) {
           const int2 tile = pair_of(x);
-          const int i = 16 * tile.x + l;
+          const int i = 16 * tile.x + lh;
           const uint64_t upto = mask & ((2ull << i) - 1), after = i < 63 ? mask >> (i + 1) : 0;
           const int from = upto ? 63 - __builtin_clzll(upto) : 0, until = after ? i + 1 + __builtin_ctzll(after) : C;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int j = 16 * tile.y + 4 * g + r;
+            const int j = 16 * tile.y + 4 * gh + r;
             p[x][r] = (kBack ? j < until : j >= from) ? p[x][r] : 0.0f;
           }
         }
@@ -483,55 +551,63 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
       }
 
       // what the state gives
-#pragma unroll
-      for (int it = 0; it < NT; ++it) o[it] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       if (!idle) {
-      if constexpr (kHalf) {
+        if constexpr (kHalf) {
 #pragma unroll
-        for (int a = 0; a < DK / 32; ++a) {
-          float rest[8];
-          __bf16 of[2][8];
+          for (int a = 0; a < DK / 32; ++a) {
+            float rest[8];
+            __bf16 of[2][8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) rest[e] = S[2 * a + e / 4][e % 4];
-          split(rest, of);
+            for (int e = 0; e < 8; ++e) rest[e] = S[2 * a + e / 4][e % 4];
+            split(rest, of);
 #pragma unroll
-          for (int it = 0; it < NT; ++it) {
-            const __bf16* q = Qs + (16 * it + l) * SQ + 32 * a + 4 * g;
-            const bf16x8 qf =
-                __builtin_shufflevector(*(const bf16x4*)q, *(const bf16x4*)(q + 16), 0, 1, 2, 3, 4, 5, 6, 7);
+            for (int it = 0; it < NT; ++it) {
+              const bf16x8 qf = read_pair(Qs + (16 * it + l) * SQ + 32 * a + 4 * g);
+              const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+              o[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, of[0]), qf,
+                                                              a == 0 ? zero : o[it], 0, 0, 0);
+              o[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, of[1]), qf, o[it], 0, 0, 0);
+            }
+          }
+        } else {
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
-              o[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, of[m]), qf, o[it], 0, 0, 0);
+          for (int a = 0; a < DK / 16; ++a) {
+            f32x4 qf[NT];
+#pragma unroll
+            for (int it = 0; it < NT; ++it) qf[it] = *(const f32x4*)(Qs + (16 * it + l) * SQ + 16 * a + 4 * g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int it = 0; it < NT; ++it) {
+                const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+                o[it] = __builtin_amdgcn_mfma_f32_16x16x4f32(S[a][e], qf[it][e], a == 0 && e == 0 ? zero : o[it], 0, 0,
+                                                             0);
+              }
           }
         }
-      } else {
+        if (!kBack || n == C) {
 #pragma unroll
-        for (int a = 0; a < DK / 16; ++a) {
-          f32x4 qf[NT];
+          for (int it = 0; it < NT; ++it)
 #pragma unroll
-          for (int it = 0; it < NT; ++it) qf[it] = *(const f32x4*)(Qs + (16 * it + l) * SQ + 16 * a + 4 * g);
+            for (int r = 0; r < 4; ++r) o[it][r] *= of_read[it];
+        } else {
+          const int lh = here(l);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+          for (int it = 0; it < NT; ++it) {
+            const float f = 16 * it + lh < n ? w.read * pw[n - 1 - (16 * it + lh)] : 0.0f;
 #pragma unroll
-            for (int it = 0; it < NT; ++it)
-              o[it] = __builtin_amdgcn_mfma_f32_16x16x4f32(S[a][e], qf[it][e], o[it], 0, 0, 0);
+            for (int r = 0; r < 4; ++r) o[it][r] *= f;
+          }
         }
-      }
+        if (mask) {
+          const int lh = here(l);
 #pragma unroll
-      for (int it = 0; it < NT; ++it) {
-        float f = of_read[it];
-        if (kBack && n < C) f = 16 * it + l < n ? w.read * pw[n - 1 - (16 * it + l)] : 0.0f;
+          for (int it = 0; it < NT; ++it) {
+            const bool sees = kBack ? 16 * it + lh >= r_last : 16 * it + lh < r_first;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[it][r] *= f;
-      }
-      if (mask) {
-#pragma unroll
-        for (int it = 0; it < NT; ++it) {
-          const bool sees = kBack ? 16 * it + l >= r_last : 16 * it + l < r_first;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[it][r] = sees ? o[it][r] : 0.0f;
+            for (int r = 0; r < 4; ++r) o[it][r] = sees ? o[it][r] : 0.0f;
+          }
         }
-      }
       }
       __syncthreads();
     }
@@ -542,10 +618,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     float vf[kHalf ? 1 : NH];
     if constexpr (kHalf) {
 #pragma unroll
-      for (int s = 0; s < C / 32; ++s) vh[s] = read_columns(Vs, SV, 32 * s + 8 * g, 16 * wave);
+      for (int s = 0; s < C / 32; ++s) vh[s] = read_columns(Vs, SV, 32 * s + 4 * g, 16 * wave);
     } else {
 #pragma unroll
-      for (int x = 0; x < NH; ++x) vf[x] = Vs[held(x) * SV + col];
+      for (int x = 0; x < NH; ++x) vf[x] = Vs[held(x, g) * SV + col];
     }
 
     if constexpr (kOut) {
@@ -555,9 +631,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
 #pragma unroll
           for (int it = 0; it < NT; ++it)
             if (kBack ? 2 * s + 1 >= it : 2 * s <= it) {
-              const T* p = Ps + (16 * it + l) * SP + 32 * s + 8 * g;
-              o[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vh[s], *(const bf16x8*)p, o[it], 0, 0, 0);
-              o[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vh[s], *(const bf16x8*)(p + C * SP), o[it], 0, 0, 0);
+              const T* p = Ps + (16 * it + l) * SP + 32 * s + 4 * g;
+              o[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vh[s], read_pair(p), o[it], 0, 0, 0);
+              o[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vh[s], read_pair(p + C * SP), o[it], 0, 0, 0);
             }
       } else {
 #pragma unroll
@@ -579,13 +655,18 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
 #pragma unroll
       for (int x = 0; x < NH; ++x) add[x] = of_add[x];
     } else {
+      const int gh = here(g);
 #pragma unroll
-      for (int x = 0; x < NH; ++x) add[x] = held(x) < n ? w.add * pw[kBack ? held(x) + 1 : n - 1 - held(x)] : 0.0f;
+      for (int x = 0; x < NH; ++x) {
+        const int j = held(x, gh);
+        add[x] = j < n ? w.add * pw[kBack ? j + 1 : n - 1 - j] : 0.0f;
+      }
     }
     const float keep = n == C ? of_chunk : pw[n];
     if (mask) {
+      const int gh = here(g);
 #pragma unroll
-      for (int x = 0; x < NH; ++x) add[x] = (kBack ? held(x) < r_first : held(x) >= r_last) ? add[x] : 0.0f;
+      for (int x = 0; x < NH; ++x) add[x] = (kBack ? held(x, gh) < r_first : held(x, gh) >= r_last) ? add[x] : 0.0f;
 #pragma unroll
       for (int a = 0; a < DK / 16; ++a) S[a] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     } else {
@@ -604,7 +685,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         split(rest, of);
         bf16x8 kf[DK / 16];
 #pragma unroll
-        for (int a = 0; a < DK / 16; ++a) kf[a] = read_columns(Ks, SQ, 32 * s + 8 * g, 16 * a);
+        for (int a = 0; a < DK / 16; ++a) kf[a] = read_columns(Ks, SQ, 32 * s + 4 * g, 16 * a);
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -624,33 +705,24 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         const float y = vf[x] * add[x];
 #pragma unroll
         for (int a = 0; a < DK / 16; ++a)
-          S[a] = __builtin_amdgcn_mfma_f32_16x16x4f32(Ks[held(x) * SQ + 16 * a + l], y, S[a], 0, 0, 0);
+          S[a] = __builtin_amdgcn_mfma_f32_16x16x4f32(Ks[held(x, g) * SQ + 16 * a + l], y, S[a], 0, 0, 0);
       }
     }
 
     if constexpr (kOut) {
-      const int c0 = 16 * wave + 4 * g;
 #pragma unroll
       for (int it = 0; it < NT; ++it) {
-        T* to = op + it * 16 * o_row;
-        if (16 * it + l < n) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) bad = __builtin_fmaf(o[it][r], 0.0f, bad);
-          if (c0 + 4 <= w.dv) {
-            if constexpr (kHalf)
-              *(half_piece_at_2*)to = __builtin_bit_cast(u32x2, __builtin_convertvector(o[it], bf16x4));
-            else
-              *(piece_at_2*)to = __builtin_bit_cast(u32x4, o[it]);
-          } else if (w.dv % 4 != 0) {
-#pragma unroll
-            for (int r = 0; r < 3; ++r)
-              if (c0 + r < w.dv) to[r] = from_f32<T>(o[it][r]);
-          }
-        }
+        for (int r = 0; r < 4; ++r) bad = __builtin_fmaf(o[it][r], 0.0f, bad);
+        if constexpr (kHalf)
+          done[it] = __builtin_bit_cast(Four, __builtin_convertvector(o[it], bf16x4));
+        else
+          done[it] = __builtin_bit_cast(Four, o[it]);
       }
-      op += (kBack ? -C : C) * o_row;
+      done_n = n;
     }
   }
+  if constexpr (kOut) store();
 
 #pragma unroll
   for (int a = 0; a < DK / 16; ++a)
