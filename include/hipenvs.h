@@ -391,13 +391,14 @@ int hipenvs_decay_attention(int32_t dtype, const void* q, const void* k, const v
                             int64_t workspace_bytes, hipenvs_stream_t stream);
 
 /* Gradients of the above: dout like out with strides of its own, dfinal (b, h, dk, dv) f32
- * contiguous or NULL (zeros) -> dq, dk_out, dv_out (b, t, h, dk or dv) contiguous in dtype,
+ * contiguous or NULL (zeros); states: the workspace that hipenvs_decay_attention was given for
+ * these inputs, as it left it, or NULL (computed again; also where its size is 0) -> dq, dk_out, dv_out (b, t, h, dk or dv) contiguous in dtype,
  * dstate (b, h, dk, dv) f32. `strides`: b, t, h of q, k, v, dout, then b, t of reset. The
  * decays are constants of their heads and have no gradient. */
 int hipenvs_decay_attention_backward(int32_t dtype, const void* q, const void* k, const void* v,
                                      const void* dout, const int64_t* strides, const float* log_decay,
                                      const float* state, const uint8_t* reset, const float* dfinal,
-                                     float scale, void* dq, void* dk_out, void* dv_out, float* dstate,
+                                     const float* states, float scale, void* dq, void* dk_out, void* dv_out, float* dstate,
                                      int64_t b, int64_t t, int32_t h, int32_t dk, int32_t dv,
                                      void* workspace, int64_t workspace_bytes, hipenvs_stream_t stream);
 

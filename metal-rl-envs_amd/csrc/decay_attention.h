@@ -70,8 +70,16 @@ struct Walk {
   // own from the state before it; one part: states and flags are not used
   int32_t parts;
   int64_t part;
-  float* states;           // (b h, parts, dk, dv)
+  float* states;           // (b h, parts, dk, dv), or (b h, parts, dv, dk) when turned
   uint8_t* flags;          // (b h, parts): a reset in the part
+  bool turned;
+};
+
+// One walk, or two of the same kind over the same rows: their blocks for a row lie side by side
+// on one XCD and read what they share (q and dout, for the gradients of k and v) once.
+struct Walks {
+  Walk w[2];
+  int32_t count;
 };
 
 // Values of a state in its caller's layout.
@@ -83,12 +91,12 @@ __device__ __forceinline__ int64_t state_index(const Walk& w, int64_t row, int r
 // column c of the four in each 16 lanes, an eighth of 128 rows of the state in each lane. The
 // chunked form meets zero weights with whatever their tokens hold, and 0 * NaN is not 0; so a
 // wave that finds anything but finite numbers in its outputs or its state walks its part
-// again here, where a token takes part only where it counts. It starts from what the
-// chunked form started from: `from` (rows, columns), else the caller's state, or zeros. A path
-// for data that has gone wrong: small in registers, not fast.
+// again here, where a token takes part only where it counts, from the state that the chunked
+// form started from: `from`, with its strides of rows and columns (null: zeros). A path for
+// data that has gone wrong: small in registers, not fast.
 template <class T, bool kOut>
-__device__ __forceinline__ void serial(const Walk& w, int64_t row, int col0, int64_t t0, int64_t t1, const float* from,
-                                    bool zero, float* to, bool last) {
+__device__ __forceinline__ void serial(const Walk& w, int64_t row, int col0, int64_t t0, int64_t t1,
+                                       const float* from, int on_row, int on_col, float* to, bool last) {
   constexpr int N = kMaxDim / 16;
   const int lane = threadIdx.x & 63, l = lane & 15;
   const int64_t b = row / w.h, h = row - b * w.h;
@@ -104,8 +112,7 @@ __device__ __forceinline__ void serial(const Walk& w, int64_t row, int col0, int
     for (int i = 0; i < N; ++i) {
       const int r = 16 * i + l;
       s[i] = 0.0f;
-      if (!zero && r < w.dk && live)
-        s[i] = from ? from[(int64_t)r * w.dv + col] : w.state_in ? w.state_in[state_index(w, row, r, col)] : 0.0f;
+      if (from && r < w.dk && live) s[i] = from[r * on_row + col * on_col];
     }
     for (int64_t n = 0; n < t1 - t0; ++n) {
       const int64_t t = w.backwards ? t1 - 1 - n : t0 + n;
@@ -274,7 +281,7 @@ constexpr int waves_of(int dk, int nw) {
 }
 
 template <class T, int DK, int NW, bool kOut, bool kBack>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_of<T>(DK, NW)))) void chunk_kernel(Walk w) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_of<T>(DK, NW)))) void chunk_kernel(Walks walks) {
   constexpr bool kHalf = sizeof(T) == 2;
   constexpr int C = Chunk<T>::kTokens, E = 16 / sizeof(T), TH = 64 * NW, DV = 16 * NW, NT = C / 16;
   constexpr int SQ = DK + Chunk<T>::pad(DK), SV = DV + Chunk<T>::pad(DV), SP = C + Chunk<T>::pad(C);
@@ -289,7 +296,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, l = lane & 15;
   // blocks of one XCD (every eighth) take neighbouring rows, whose tokens share cache lines
   const uint32_t blocks = gridDim.x;
-  const uint32_t id = blocks % 8 == 0 ? (blockIdx.x % 8) * (blocks / 8) + blockIdx.x / 8 : blockIdx.x;
+  const uint32_t at = blocks % 8 == 0 ? (blockIdx.x % 8) * (blocks / 8) + blockIdx.x / 8 : blockIdx.x;
+  const uint32_t id = walks.count == 2 ? at / 2 : at;
+  const Walk& w = walks.w[walks.count == 2 ? at % 2 : 0];
   const uint32_t row = id / (uint32_t)w.parts, part = id - row * (uint32_t)w.parts;
   const int64_t b = row / (uint32_t)w.h, h = row - (uint32_t)b * (uint32_t)w.h;
   const int64_t t0 = part * w.part, t1 = t0 + w.part < w.t ? t0 + w.part : w.t;
@@ -371,10 +380,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
   const int col = 16 * wave + l;
 #pragma unroll
   for (int a = 0; a < DK / 16; ++a) S[a] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  if (kOut && (local || w.state_in)) {   // every value in flight at once: none behind a condition of its own
-    const float* from = local ? local : w.state_in + (int64_t)row * w.dk * w.dv;
-    const bool turned = !local && w.flipped;
-    const int on_row = turned ? 1 : w.dv, on_col = turned ? w.dk : 1, c = col < w.dv ? col : 0;
+  // where the state before the first token lies, and its strides of rows and columns
+  const float* from = !kOut ? nullptr : local ? local : w.state_in ? w.state_in + (int64_t)row * w.dk * w.dv : nullptr;
+  const bool turned = local ? w.turned : w.flipped;
+  const int on_row = turned ? 1 : w.dv, on_col = turned ? w.dk : 1;
+  if (from) {   // every value in flight at once: none behind a condition of its own
+    const int c = col < w.dv ? col : 0;
 #pragma unroll
     for (int a = 0; a < DK / 16; ++a)
 #pragma unroll
@@ -731,7 +742,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
   if (!kOut && tid == 0) w.flags[(int64_t)row * w.parts + part] = any != 0;
   if (16 * wave >= w.dv) return;
   if (__builtin_amdgcn_ballot_w64(bad != bad)) {
-    serial<T, kOut>(w, row, 16 * wave, t0, t1, kOut ? local : nullptr, !kOut, kOut ? nullptr : local, kOut && last);
+    serial<T, kOut>(w, row, 16 * wave, t0, t1, from, on_row, on_col, kOut ? nullptr : local, kOut && last);
     return;
   }
 #pragma unroll
@@ -747,36 +758,45 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
 }
 
 template <class T, int DK, int NW>
-int launch_sized(const Walk& w, bool out, hipStream_t s) {
-  const dim3 grid((unsigned)(w.b * w.h * w.parts)), block(64 * NW);
+int launch_sized(const Walks& walks, bool out, hipStream_t s) {
+  const Walk& w = walks.w[0];
+  const dim3 grid((unsigned)(w.b * w.h * w.parts * walks.count)), block(64 * NW);
   if (out && w.backwards)
-    hipLaunchKernelGGL((chunk_kernel<T, DK, NW, true, true>), grid, block, 0, s, w);
+    hipLaunchKernelGGL((chunk_kernel<T, DK, NW, true, true>), grid, block, 0, s, walks);
   else if (out)
-    hipLaunchKernelGGL((chunk_kernel<T, DK, NW, true, false>), grid, block, 0, s, w);
+    hipLaunchKernelGGL((chunk_kernel<T, DK, NW, true, false>), grid, block, 0, s, walks);
   else if (w.backwards)
-    hipLaunchKernelGGL((chunk_kernel<T, DK, NW, false, true>), grid, block, 0, s, w);
+    hipLaunchKernelGGL((chunk_kernel<T, DK, NW, false, true>), grid, block, 0, s, walks);
   else
-    hipLaunchKernelGGL((chunk_kernel<T, DK, NW, false, false>), grid, block, 0, s, w);
+    hipLaunchKernelGGL((chunk_kernel<T, DK, NW, false, false>), grid, block, 0, s, walks);
   return launch_status();
 }
 
+inline int rows_of(int dk) { return dk <= 32 ? 32 : dk <= 64 ? 64 : 128; }
+inline int waves_for(int dv) { return dv <= 32 ? 2 : dv <= 64 ? 4 : 8; }
+
 template <class T, int DK>
-int launch_rows(const Walk& w, bool out, hipStream_t s) {
-  if (w.dv <= 32) return launch_sized<T, DK, 2>(w, out, s);
-  if (w.dv <= 64) return launch_sized<T, DK, 4>(w, out, s);
-  return launch_sized<T, DK, 8>(w, out, s);
+int launch_rows(const Walks& walks, bool out, hipStream_t s) {
+  switch (waves_for(walks.w[0].dv)) {
+    case 2: return launch_sized<T, DK, 2>(walks, out, s);
+    case 4: return launch_sized<T, DK, 4>(walks, out, s);
+    default: return launch_sized<T, DK, 8>(walks, out, s);
+  }
 }
 
-// The walk's kernel for w.dk and w.dv: with outputs, or each part's own state alone.
+// The kernel for these walks, all of one size of kernel: with outputs, or each part's own state
+// alone.
 template <class T>
-int launch_chunks(const Walk& w, bool out, hipStream_t s) {
-  if (w.dk <= 32) return launch_rows<T, 32>(w, out, s);
-  if (w.dk <= 64) return launch_rows<T, 64>(w, out, s);
-  return launch_rows<T, 128>(w, out, s);
+int launch_chunks(const Walks& walks, bool out, hipStream_t s) {
+  switch (rows_of(walks.w[0].dk)) {
+    case 32: return launch_rows<T, 32>(walks, out, s);
+    case 64: return launch_rows<T, 64>(walks, out, s);
+    default: return launch_rows<T, 128>(walks, out, s);
+  }
 }
 
-extern template int launch_chunks<__bf16>(const Walk&, bool, hipStream_t);
-extern template int launch_chunks<float>(const Walk&, bool, hipStream_t);
+extern template int launch_chunks<__bf16>(const Walks&, bool, hipStream_t);
+extern template int launch_chunks<float>(const Walks&, bool, hipStream_t);
 
 }  // namespace da
 }  // namespace hipenvs

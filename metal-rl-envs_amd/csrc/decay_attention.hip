@@ -146,18 +146,20 @@ void divide(int64_t rows, int64_t t, int32_t chunk, int64_t cus, int32_t* parts,
 
 int32_t chunk_of(int32_t dtype) { return dtype == 1 ? Chunk<__bf16>::kTokens : Chunk<float>::kTokens; }
 
-int launch_walk(int32_t dtype, Walk w, hipStream_t s) {
-  if (w.parts > 1) {
-    int status = dtype == 1 ? launch_chunks<__bf16>(w, false, s) : launch_chunks<float>(w, false, s);
-    if (status != HIPENVS_OK) return status;
-    int groups = 1;
-    while (groups < kGroups && groups * kEach < w.parts) groups *= 2;
-    hipLaunchKernelGGL(join_kernel, dim3((unsigned)(w.b * w.h), grid_for(w.dk * w.dv, kBlock / groups)), dim3(kBlock),
-                       0, s, w, groups);
-    status = launch_status();
-    if (status != HIPENVS_OK) return status;
-  }
-  return dtype == 1 ? launch_chunks<__bf16>(w, true, s) : launch_chunks<float>(w, true, s);
+int launch(int32_t dtype, const Walks& walks, bool out, hipStream_t s) {
+  return dtype == 1 ? launch_chunks<__bf16>(walks, out, s) : launch_chunks<float>(walks, out, s);
+}
+
+// The states before the parts of a walk whose rows are walked in parts.
+int launch_states(int32_t dtype, const Walk& w, hipStream_t s) {
+  if (w.parts == 1) return HIPENVS_OK;
+  const int status = launch(dtype, {{w, w}, 1}, false, s);
+  if (status != HIPENVS_OK) return status;
+  int groups = 1;
+  while (groups < kGroups && groups * kEach < w.parts) groups *= 2;
+  hipLaunchKernelGGL(join_kernel, dim3((unsigned)(w.b * w.h), grid_for(w.dk * w.dv, kBlock / groups)), dim3(kBlock), 0,
+                     s, w, groups);
+  return launch_status();
 }
 
 }  // namespace da
@@ -217,13 +219,14 @@ extern "C" int hipenvs_decay_attention(int32_t dtype, const void* q, const void*
   w.dk = dk, w.dv = dv, w.log_decay = log_decay, w.reset = reset, w.reset_sb = st[9], w.reset_st = st[10];
   w.state_in = state, w.state_out = final_state, w.exact = true, w.read = scale, w.add = 1.0f;
   w.out = out, w.b = b, w.t = t, w.h = h;
-  return launch_walk(dtype, w, as_stream(stream));
+  const int walked = launch_states(dtype, w, as_stream(stream));
+  return walked == HIPENVS_OK ? launch(dtype, {{w, w}, 1}, true, as_stream(stream)) : walked;
 }
 
 extern "C" int hipenvs_decay_attention_backward(int32_t dtype, const void* q, const void* k, const void* v,
                                                 const void* dout, const int64_t* strides, const float* log_decay,
                                                 const float* state, const uint8_t* reset, const float* dfinal,
-                                                float scale, void* dq, void* dk_out, void* dv_out, float* dstate,
+                                                const float* states, float scale, void* dq, void* dk_out, void* dv_out, float* dstate,
                                                 int64_t b, int64_t t, int32_t h, int32_t dk, int32_t dv,
                                                 void* workspace, int64_t workspace_bytes, hipenvs_stream_t stream) {
   if (!sequence_ok(dtype, b, t, h, dk, dv)) return HIPENVS_E_ARG;
@@ -237,24 +240,37 @@ extern "C" int hipenvs_decay_attention_backward(int32_t dtype, const void* q, co
   int status = plan(dtype, b, t, h, dk, dv, workspace, &w, &need);
   if (status != HIPENVS_OK) return status;
   if (need > 0 && (!workspace || workspace_bytes < need)) return HIPENVS_E_ARG;
+  float* own_states = w.states;
   const Rows rq = rows(q, st), rk = rows(k, st + 3), rv = rows(v, st + 6),
              rdo = rows(dout, st + 9);
   const hipStream_t s = as_stream(stream);
   w.log_decay = log_decay, w.reset = reset, w.reset_sb = st[12], w.reset_st = st[13], w.b = b, w.t = t, w.h = h;
-  // dq: forwards over the transposed states
+  // dq: forwards over the transposed states, which the forward pass has left, or are computed
+  // again (transposed) where it has not
   w.q = rdo, w.k = rv, w.v = rk, w.dk = dv, w.dv = dk, w.state_in = state, w.state_out = nullptr;
   w.flipped = true, w.backwards = false, w.read = scale, w.add = 1.0f, w.out = dq;
-  status = launch_walk(dtype, w, s);
+  if (states) {
+    w.states = const_cast<float*>(states);
+    w.turned = true;
+  } else {
+    status = launch_states(dtype, w, s);
+    if (status != HIPENVS_OK) return status;
+  }
+  status = launch(dtype, {{w, w}, 1}, true, s);
   if (status != HIPENVS_OK) return status;
   // dv, and the gradient of the first state: backwards over the states' gradients
   w.q = rk, w.k = rq, w.v = rdo, w.dk = dk, w.dv = dv, w.state_in = dfinal, w.state_out = dstate, w.exact = true;
+  w.states = own_states, w.turned = false;
   w.flipped = false, w.backwards = true, w.read = 1.0f, w.add = scale, w.out = dv_out;
-  status = launch_walk(dtype, w, s);
+  status = launch_states(dtype, w, s);
   if (status != HIPENVS_OK) return status;
   // dk: the same, transposed
-  w.q = rv, w.k = rdo, w.v = rq, w.dk = dv, w.dv = dk, w.state_out = nullptr, w.exact = false, w.flipped = true;
-  w.out = dk_out;
-  return launch_walk(dtype, w, s);
+  Walk u = w;
+  u.q = rv, u.k = rdo, u.v = rq, u.dk = dv, u.dv = dk, u.state_out = nullptr, u.exact = false, u.flipped = true;
+  u.turned = true, u.out = dk_out;
+  if (rows_of(dk) == rows_of(dv) && waves_for(dk) == waves_for(dv)) return launch(dtype, {{w, u}, 2}, true, s);
+  status = launch(dtype, {{w, w}, 1}, true, s);
+  return status == HIPENVS_OK ? launch(dtype, {{u, u}, 1}, true, s) : status;
 }
 
 extern "C" int hipenvs_decay_attention_step(int32_t dtype, const void* q, int64_t q_sn, int64_t q_sh, const void* k,

@@ -3,6 +3,6 @@
 
 namespace hipenvs {
 namespace da {
-template int launch_chunks<__bf16>(const Walk&, bool, hipStream_t);
+template int launch_chunks<__bf16>(const Walks&, bool, hipStream_t);
 }  // namespace da
 }  // namespace hipenvs

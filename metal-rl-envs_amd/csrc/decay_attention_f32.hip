@@ -3,6 +3,6 @@
 
 namespace hipenvs {
 namespace da {
-template int launch_chunks<float>(const Walk&, bool, hipStream_t);
+template int launch_chunks<float>(const Walks&, bool, hipStream_t);
 }  // namespace da
 }  // namespace hipenvs

@@ -72,7 +72,7 @@ SIGNATURES = {
                                          _F32, _F32, ctypes.c_double, _P, _P, _P, _I64, _P],
     "hipenvs_decay_attention": [_I32, _P, _P, _P, _P, _P, _P, _P, _F32, _P, _P, _I64, _I64, _I32, _I32, _I32, _P, _I64,
                                 _P],
-    "hipenvs_decay_attention_backward": [_I32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _F32, _P, _P, _P, _P, _I64, _I64,
+    "hipenvs_decay_attention_backward": [_I32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _F32, _P, _P, _P, _P, _I64, _I64,
                                          _I32, _I32, _I32, _P, _I64, _P],
     "hipenvs_decay_attention_step": [_I32, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _F32, _P,
                                      _P, _I64, _I32, _I32, _I32, _P],

@@ -120,30 +120,32 @@ def _workspace(dtype, b, t, h, dk, dv, device):
 
 
 def _forward(q, k, v, log_decay, state, reset, scale):
+    """(out, final_state, workspace): the workspace holds the states between a long row's parts."""
     b, t, h, dk = q.shape
     dv = v.shape[-1]
     out = torch.empty((b, t, h, dv), dtype=q.dtype, device=q.device)
     final = torch.empty((b, h, dk, dv), dtype=torch.float32, device=q.device)
     with _lib.on(q.device):
-        at, nbytes, _held = _workspace(_DTYPES[q.dtype], b, t, h, dk, dv, q.device)
+        at, nbytes, workspace = _workspace(_DTYPES[q.dtype], b, t, h, dk, dv, q.device)
         _lib.call("hipenvs_decay_attention", _DTYPES[q.dtype], _lib.ptr(q), _lib.ptr(k), _lib.ptr(v),
                   _strides((q, k, v), reset), _lib.ptr(log_decay), _lib.ptr(state), _lib.ptr(reset), scale,
                   _lib.ptr(out), _lib.ptr(final), b, t, h, dk, dv, at, nbytes, _lib.stream_of(q.device))
-    return out, final
+    return out, final, workspace
 
 
 class _Sequence(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, state, reset, scale):
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(q, k, v, log_decay, state, reset)
+        out, final, workspace = _forward(q, k, v, log_decay, state, reset, scale)
+        ctx.save_for_backward(q, k, v, log_decay, state, reset, workspace)
         ctx.scale = scale
-        return _forward(q, k, v, log_decay, state, reset, scale)
+        return out, final
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, dfinal):
-        q, k, v, log_decay, state, reset = ctx.saved_tensors
+        q, k, v, log_decay, state, reset, states = ctx.saved_tensors
         b, t, h, dk = q.shape
         dv = v.shape[-1]
         if dout is None:
@@ -157,7 +159,7 @@ class _Sequence(torch.autograd.Function):
             at, nbytes, _held = _workspace(_DTYPES[q.dtype], b, t, h, dk, dv, q.device)
             _lib.call("hipenvs_decay_attention_backward", _DTYPES[q.dtype], _lib.ptr(q), _lib.ptr(k), _lib.ptr(v),
                       _lib.ptr(dout), _strides((q, k, v, dout), reset), _lib.ptr(log_decay), _lib.ptr(state),
-                      _lib.ptr(reset), _lib.ptr(dfinal), ctx.scale, _lib.ptr(dq), _lib.ptr(dk_), _lib.ptr(dv_),
+                      _lib.ptr(reset), _lib.ptr(dfinal), _lib.ptr(states), ctx.scale, _lib.ptr(dq), _lib.ptr(dk_), _lib.ptr(dv_),
                       _lib.ptr(dstate), b, t, h, dk, dv, at, nbytes, _lib.stream_of(q.device))
         return dq, dk_, dv_, None, dstate if state is not None else None, None, None
 
@@ -176,7 +178,7 @@ def sequence(q, k, v, log_decay, state=None, reset=None, scale=None):
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or (state is not None and state.requires_grad)):
         return _Sequence.apply(q, k, v, log_decay, state, reset, scale)
-    return _forward(q, k, v, log_decay, state, reset, scale)
+    return _forward(q, k, v, log_decay, state, reset, scale)[:2]
 
 
 def step(q, k, v, log_decay, state, reset=None, scale=None, next_state=None):

@@ -25,9 +25,9 @@ def test_c_abi_checks_attention_arguments():
                 dict(t=1 << 31)):
         assert forward(**bad) == _lib.E_ARG, bad
     assert forward(b=0) == _lib.OK
-    assert l.hipenvs_decay_attention_backward(0, a, a, a, None, strides, a, None, None, None, 1.0, a, a, a, a, 2, 3, 2, 8,
+    assert l.hipenvs_decay_attention_backward(0, a, a, a, None, strides, a, None, None, None, None, 1.0, a, a, a, a, 2, 3, 2, 8,
                                               4, None, 0, None) == _lib.E_ARG
-    assert l.hipenvs_decay_attention_backward(0, a, a, a, a, strides, a, None, None, None, 1.0, a, a, a, None, 2, 3, 2, 8,
+    assert l.hipenvs_decay_attention_backward(0, a, a, a, a, strides, a, None, None, None, None, 1.0, a, a, a, None, 2, 3, 2, 8,
                                               4, None, 0, None) == _lib.E_ARG
     step = l.hipenvs_decay_attention_step
     assert step(0, a, 1, 1, a, 1, 1, a, 1, 1, a, None, None, 0, 1.0, a, a, 4, 2, 8, 4, None) == _lib.E_ARG
