@@ -168,10 +168,23 @@ __device__ __forceinline__ float wave_scale(const float (&x)[4]) {
   return __uint_as_float(u != 0 && u < 0x00800000u ? 0x00800000u : u);
 }
 
-// The nearest whole number in 0 .. top of y * top; 0 for a NaN.
-__device__ __forceinline__ int code_of(float y, float top) {
-  const float c = __builtin_rintf(y * top);
+// A code: the nearest whole number in 0 .. top of root * top; 0 for a NaN. The roots that
+// decide are the correctly rounded ones, but only a product next to the border of two codes
+// depends on their last bits. The hardware's root is within 1 ulp, and a root of such a root
+// within 1.5; the exact ones within 0.5 and 0.75: so the products differ by at most
+// 255 * 2.25 * 2^-23 and their own roundings, 2^-16, together below 8.5e-5, and give the same
+// code unless they lie within kBorder of a half. A wave that holds such a one (about one in
+// ten) takes the exact roots for all of it. Three exact roots for every value took 322 us for
+// 87 million, bound by their float64 instructions.
+constexpr float kBorder = 1e-4f;
+
+__device__ __forceinline__ int code_of(float product, float top) {
+  const float c = __builtin_rintf(product);
   return c == c ? (int)__builtin_fminf(c, top) : 0;
+}
+
+__device__ __forceinline__ bool near_border(float product) {
+  return __builtin_fabsf(__builtin_fabsf(product - __builtin_rintf(product)) - 0.5f) < kBorder;
 }
 
 __global__ __launch_bounds__(kBlock) void step8_kernel(Batch b, uint32_t* __restrict__ m_codes,
@@ -197,11 +210,26 @@ __global__ __launch_bounds__(kBlock) void step8_kernel(Batch b, uint32_t* __rest
   }
   const float new_ms = wave_scale(m), new_vs = wave_scale(v);
   const float m_inv = new_ms > 0.0f ? 1.0f / new_ms : 0.0f, v_inv = new_vs > 0.0f ? 1.0f / new_vs : 0.0f;
+  float of_m[4], of_v[4];
+  bool unsure = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    of_m[e] = __builtin_amdgcn_sqrtf(__builtin_fabsf(m[e]) * m_inv) * 127.0f;
+    of_v[e] = __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(v[e] * v_inv)) * 255.0f;
+    unsure = unsure || near_border(of_m[e]) || near_border(of_v[e]);
+  }
+  if (__builtin_amdgcn_ballot_w64(unsure)) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      of_m[e] = sqrt_rn(__builtin_fabsf(m[e]) * m_inv) * 127.0f;
+      of_v[e] = sqrt_rn(sqrt_rn(v[e] * v_inv)) * 255.0f;
+    }
+  }
   uint32_t new_mc = 0, new_vc = 0;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const int cm = code_of(sqrt_rn(__builtin_fabsf(m[e]) * m_inv), 127.0f);
-    int cv = code_of(sqrt_rn(sqrt_rn(v[e] * v_inv)), 255.0f);
+    const int cm = code_of(of_m[e], 127.0f);
+    int cv = code_of(of_v[e], 255.0f);
     cv = v[e] > 0.0f && cv < 1 ? 1 : cv;
     new_mc |= ((uint32_t)(m[e] < 0.0f ? -cm : cm) & 0xFFu) << (8 * e);
     new_vc |= (uint32_t)cv << (8 * e);

@@ -280,12 +280,18 @@ constexpr int waves_of(int dk, int nw) {
   return sizeof(T) == 4 && (dk == 32 || (dk == 64 && nw >= 4)) ? 3 : 2;
 }
 
+constexpr int power_of_two(int n) {   // the least that is not below n
+  int p = 1;
+  while (p < n) p *= 2;
+  return p;
+}
+
 template <class T, int DK, int NW, bool kOut, bool kBack>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_of<T>(DK, NW)))) void chunk_kernel(Walks walks) {
   constexpr bool kHalf = sizeof(T) == 2;
   constexpr int C = Chunk<T>::kTokens, E = 16 / sizeof(T), TH = 64 * NW, DV = 16 * NW, NT = C / 16;
   constexpr int SQ = DK + Chunk<T>::pad(DK), SV = DV + Chunk<T>::pad(DV), SP = C + Chunk<T>::pad(C);
-  constexpr int QP = DK / E, VP = DV / E;                               // pieces of a row
+  constexpr int QP = power_of_two(DK / E), VP = power_of_two(DV / E);      // pieces of a row, rounded up
   constexpr int NQ = (C * QP + TH - 1) / TH, NV = (C * VP + TH - 1) / TH;  // pieces of a thread
   __shared__ __attribute__((aligned(16))) T Qs[kOut ? C * SQ : 8];
   __shared__ __attribute__((aligned(16))) T Ks[C * SQ];
@@ -322,7 +328,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
   u32x4 xq[kOut ? NQ : 1], xk[NQ], xv[NV];
   uint32_t xr = 0;
   const bool tiny = w.dk < E || w.dv < E;
-  const bool filled = w.dk == DK && w.dv == DV && C % QR == 0 && C % VR == 0;
+  const bool filled = w.dk == DK && w.dv == DV && QP * E == DK && VP * E == DV && C % QR == 0 && C % VR == 0;
   const auto load = [&](int n) {
     if (filled && n == C) {
 #pragma unroll
@@ -487,13 +493,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
     }
 #pragma unroll
     for (int m = 0; m < NQ; ++m)
-      if (C % QR == 0 || qr + m * QR < C) {
+      if ((C % QR == 0 || qr + m * QR < C) && (QP * E == DK || qx < DK)) {
         *(u32x4*)(Ks + (qr + m * QR) * SQ + qx) = xk[m];
         if constexpr (kOut) *(u32x4*)(Qs + (qr + m * QR) * SQ + qx) = xq[m];
       }
 #pragma unroll
     for (int m = 0; m < NV; ++m)
-      if (C % VR == 0 || vr + m * VR < C) *(u32x4*)(Vs + (vr + m * VR) * SV + vx) = xv[m];
+      if ((C % VR == 0 || vr + m * VR < C) && (VP * E == DV || vx < DV)) *(u32x4*)(Vs + (vr + m * VR) * SV + vx) = xv[m];
     if constexpr (kOut) store();
     // the chunk's resets, bit i for token i; the first and the last of them
     const uint64_t mask = __builtin_amdgcn_ballot_w64(xr != 0);
@@ -772,31 +778,49 @@ int launch_sized(const Walks& walks, bool out, hipStream_t s) {
   return launch_status();
 }
 
-inline int rows_of(int dk) { return dk <= 32 ? 32 : dk <= 64 ? 64 : 128; }
-inline int waves_for(int dv) { return dv <= 32 ? 2 : dv <= 64 ? 4 : 8; }
+// The kernel that takes dk rows and dv columns of a state: its rows, and its waves.
+inline int rows_of(int dk) { return dk <= 32 ? 32 : dk <= 64 ? 64 : dk <= 96 ? 96 : 128; }
+inline int waves_for(int dv) {
+  const int waves = (dv + 15) / 16;
+  return waves == 7 ? 8 : waves;
+}
 
 template <class T, int DK>
-int launch_rows(const Walks& walks, bool out, hipStream_t s) {
+int of_rows(const Walks& walks, bool out, hipStream_t s) {
   switch (waves_for(walks.w[0].dv)) {
+    case 1: return launch_sized<T, DK, 1>(walks, out, s);
     case 2: return launch_sized<T, DK, 2>(walks, out, s);
+    case 3: return launch_sized<T, DK, 3>(walks, out, s);
     case 4: return launch_sized<T, DK, 4>(walks, out, s);
+    case 5: return launch_sized<T, DK, 5>(walks, out, s);
+    case 6: return launch_sized<T, DK, 6>(walks, out, s);
     default: return launch_sized<T, DK, 8>(walks, out, s);
   }
 }
 
-// The kernel for these walks, all of one size of kernel: with outputs, or each part's own state
-// alone.
+// These walks, all of one size of kernel: with outputs, or each part's own state alone.
 template <class T>
-int launch_chunks(const Walks& walks, bool out, hipStream_t s) {
+int launch_walks(const Walks& walks, bool out, hipStream_t s) {
   switch (rows_of(walks.w[0].dk)) {
-    case 32: return launch_rows<T, 32>(walks, out, s);
-    case 64: return launch_rows<T, 64>(walks, out, s);
-    default: return launch_rows<T, 128>(walks, out, s);
+    case 32: return of_rows<T, 32>(walks, out, s);
+    case 64: return of_rows<T, 64>(walks, out, s);
+    case 96: return of_rows<T, 96>(walks, out, s);
+    default: return of_rows<T, 128>(walks, out, s);
   }
 }
 
-extern template int launch_chunks<__bf16>(const Walks&, bool, hipStream_t);
-extern template int launch_chunks<float>(const Walks&, bool, hipStream_t);
+// Each in a file of its own, which compile side by side.
+#define HIPENVS_DA_ROWS(of, T, DK) of template int of_rows<T, DK>(const Walks&, bool, hipStream_t);
+#ifndef HIPENVS_DA_DEFINE
+HIPENVS_DA_ROWS(extern, __bf16, 32)
+HIPENVS_DA_ROWS(extern, __bf16, 64)
+HIPENVS_DA_ROWS(extern, __bf16, 96)
+HIPENVS_DA_ROWS(extern, __bf16, 128)
+HIPENVS_DA_ROWS(extern, float, 32)
+HIPENVS_DA_ROWS(extern, float, 64)
+HIPENVS_DA_ROWS(extern, float, 96)
+HIPENVS_DA_ROWS(extern, float, 128)
+#endif
 
 }  // namespace da
 }  // namespace hipenvs

@@ -69,9 +69,12 @@ __global__ __launch_bounds__(kBlock) void join_kernel(Walk w, int groups) {
 }
 
 // One token of every environment: a block for each (n, h), the state read once and written
-// once. `V` values of a state row at a time: L = ceil(dv / V) threads hold a row, 256 / L
-// rows at a time; the rows' shares of the output meet in LDS. next may be state itself: a
-// thread writes only what it has read.
+// once, bound by that. Four values of a state row at a time, at whatever address they lie:
+// L = ceil(dv / 4) threads hold a row (the last one its one to four last values), 256 / L rows at a
+// time; the rows' shares of the output meet in LDS. next may be state itself: a thread writes
+// only what it has read. 4,096 environments x 8 heads of 64: 188 us, 5.8 TB/s. (One value at a
+// time where dv is no multiple of four: 39 us at 8,364 states of 16 x 127, where this takes
+// 30.)
 struct Step {
   Rows q, k, v;   // sb: stride of the environment; st is not read
   const float* log_decay;
@@ -84,45 +87,72 @@ struct Step {
   int32_t h, dk, dv;
 };
 
-template <class T, int V>
+template <class T>
 __global__ __launch_bounds__(kBlock) void step_kernel(Step s) {
-  typedef float vec __attribute__((ext_vector_type(V)));
-  __shared__ float share[kBlock * V];
+  typedef f32x4 __attribute__((aligned(4))) four;
+  __shared__ __attribute__((aligned(16))) float share[kBlock * 4];
   const int64_t item = blockIdx.x, n = item / s.h, h = item - n * s.h;
-  const int L = (s.dv + V - 1) / V, R = kBlock / L;
-  const int r0 = threadIdx.x / L, c = (threadIdx.x - r0 * L) * V;
+  const int L = (s.dv + 3) / 4, R = kBlock / L;
+  const int r0 = threadIdx.x / L, c = (threadIdx.x - r0 * L) * 4;
+  const int left = s.dv - c;   // values of the row from c on
   const T* q = (const T*)s.q.data + n * s.q.sb + h * s.q.sh;
   const T* k = (const T*)s.k.data + n * s.k.sb + h * s.k.sh;
   const T* v = (const T*)s.v.data + n * s.v.sb + h * s.v.sh;
   const bool fresh = s.reset && s.reset[n * s.reset_sn];
   const float lambda = expf(s.log_decay[h]);
-  float x[V], o[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) o[e] = 0.0f;
+  f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
   if (r0 < R) {
+    float x[4];
 #pragma unroll
-    for (int e = 0; e < V; ++e) x[e] = to_f32<T>(v[c + e]);
+    for (int e = 0; e < 4; ++e) x[e] = to_f32<T>(v[e < left ? c + e : c]);
     const int64_t base = item * s.dk * s.dv + c;
-    for (int r = r0; r < s.dk; r += R) {
-      const float kr = to_f32<T>(k[r]), qr = to_f32<T>(q[r]);
-      vec y = 0.0f;
-      if (!fresh) y = *(const vec*)(s.state + base + (int64_t)r * s.dv);
+    constexpr int kAhead = 4;   // rows in flight: next may be state, so no read passes a write by itself
+    for (int first = r0; first < s.dk; first += kAhead * R) {
+      f32x4 y[kAhead];
+      float kr[kAhead], qr[kAhead];
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float kept = fresh ? 0.0f : y[e] * lambda;
-        y[e] = __builtin_fmaf(kr, x[e], kept);
-        o[e] = __builtin_fmaf(qr, y[e], o[e]);
+      for (int m = 0; m < kAhead; ++m) {
+        const int r = first + m * R;
+        y[m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        kr[m] = qr[m] = 0.0f;
+        if (r < s.dk) {
+          kr[m] = to_f32<T>(k[r]), qr[m] = to_f32<T>(q[r]);
+          const float* from = s.state + base + (int64_t)r * s.dv;
+          if (!fresh) {
+            if (left >= 4)
+              y[m] = *(const four*)from;
+            else
+              y[m] = f32x4{from[0], from[left > 1 ? 1 : 0], from[left > 2 ? 2 : 0], 0.0f};
+          }
+        }
       }
-      *(vec*)(s.next + base + (int64_t)r * s.dv) = y;
-    }
 #pragma unroll
-    for (int e = 0; e < V; ++e) share[r0 * L * V + c + e] = o[e];
+      for (int m = 0; m < kAhead; ++m) {
+        const int r = first + m * R;
+        if (r < s.dk) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            y[m][e] = __builtin_fmaf(kr[m], x[e], fresh ? 0.0f : y[m][e] * lambda);
+            o[e] = __builtin_fmaf(qr[m], y[m][e], o[e]);
+          }
+          float* to = s.next + base + (int64_t)r * s.dv;
+          if (left >= 4) {
+            *(four*)to = y[m];
+          } else {
+            to[0] = y[m][0];
+            if (left > 1) to[1] = y[m][1];
+            if (left > 2) to[2] = y[m][2];
+          }
+        }
+      }
+    }
+    *(f32x4*)(share + (r0 * L * 4 + c)) = o;
   }
   __syncthreads();
   for (int j = threadIdx.x; j < s.dv; j += kBlock) {
     float sum = 0.0f;
     const int rows = R < s.dk ? R : s.dk;
-    for (int r = 0; r < rows; ++r) sum += share[r * L * V + j];
+    for (int r = 0; r < rows; ++r) sum += share[r * L * 4 + j];
     ((T*)s.out)[item * s.dv + j] = from_f32<T>(s.scale * sum);
   }
 }
@@ -131,23 +161,32 @@ bool dims_ok(int32_t dtype, int64_t h, int64_t dk, int64_t dv) {
   return (dtype == 0 || dtype == 1) && h >= 1 && h <= 65536 && dk >= 1 && dk <= kMaxDim && dv >= 1 && dv <= kMaxDim;
 }
 
+int launch(int32_t dtype, const Walks& walks, bool out, hipStream_t s) {
+  return dtype == 1 ? launch_walks<__bf16>(walks, out, s) : launch_walks<float>(walks, out, s);
+}
+
 // A block walks a row, or a part of one where the rows are too few to fill the card: then a first
 // pass leaves each part's own state, the second joins them, the third walks every part from
-// the state before it.
-void divide(int64_t rows, int64_t t, int32_t chunk, int64_t cus, int32_t* parts, int64_t* part) {
-  const int64_t chunks = (t + chunk - 1) / chunk;
-  const int64_t want = (2 * cus + rows - 1) / rows, most = chunks / 4;
-  int64_t n = want < most ? want : most;
-  if (n < 2) n = 1;
+// the state before it. The card is full at eight waves a CU: two blocks of four waves take
+// 4.1 us a chunk where one takes 3.1 (bfloat16 heads of 64), two of eight waves as long as one
+// after the other (heads of 128: 209 us at 512 rows, 106 at 256). As many parts as fill it
+// once are the fastest (32 rows of 8,192 tokens in heads of 128: 148 us in 8 parts, 165 in
+// 16, 645 in one; 8 rows of 16,381 in heads of 64: 44 us in 64 parts, 77 in 16), of two
+// chunks at least, where they save more than the passes cost: the first pass takes about 0.45 of
+// the third, joining and launching about five chunks.
+int divide(int32_t dtype, int64_t rows, int64_t t, int32_t widest, int32_t* parts, int64_t* part) {
+  int cus = 0;
+  const int status = device_cus(&cus);
+  if (status != HIPENVS_OK) return status;
+  const int64_t chunk = dtype == 1 ? Chunk<__bf16>::kTokens : Chunk<float>::kTokens;
+  const int64_t chunks = (t + chunk - 1) / chunk, waves = waves_for(widest);
+  const int64_t fill = cus * (waves > 4 ? 1 : 8 / waves) / rows, most = chunks / 2;
+  int64_t n = fill < most ? fill : most;
+  if (n < 2 || chunks * (20 * n - 29) <= 100 * n) n = 1;
   const int64_t per = n > 1 ? (chunks + n - 1) / n : chunks;
   *parts = n > 1 ? (int32_t)((chunks + per - 1) / per) : 1;
   *part = (per > 0 ? per : 1) * chunk;
-}
-
-int32_t chunk_of(int32_t dtype) { return dtype == 1 ? Chunk<__bf16>::kTokens : Chunk<float>::kTokens; }
-
-int launch(int32_t dtype, const Walks& walks, bool out, hipStream_t s) {
-  return dtype == 1 ? launch_chunks<__bf16>(walks, out, s) : launch_chunks<float>(walks, out, s);
+  return HIPENVS_OK;
 }
 
 // The states before the parts of a walk whose rows are walked in parts.
@@ -179,10 +218,8 @@ Rows rows(const void* data, const int64_t* strides) { return {data, strides[0], 
 // The parts of a sequence and where in `workspace` their states and flags lie; the bytes used.
 int plan(int32_t dtype, int64_t b, int64_t t, int32_t h, int32_t dk, int32_t dv, void* workspace, Walk* w,
          int64_t* bytes) {
-  int cus = 0;
-  const int status = device_cus(&cus);
+  const int status = divide(dtype, b * h, t, dk < dv ? dv : dk, &w->parts, &w->part);
   if (status != HIPENVS_OK) return status;
-  divide(b * h, t, chunk_of(dtype), cus, &w->parts, &w->part);
   const int64_t states = w->parts > 1 ? b * h * w->parts * dk * dv * (int64_t)sizeof(float) : 0;
   w->states = (float*)workspace;
   w->flags = (uint8_t*)workspace + states;
@@ -283,12 +320,10 @@ extern "C" int hipenvs_decay_attention_step(int32_t dtype, const void* q, int64_
   if (!q || !k || !v || !log_decay || !state || !out || !next_state) return HIPENVS_E_ARG;
   const Step s = {{q, q_sn, 0, q_sh}, {k, k_sn, 0, k_sh}, {v, v_sn, 0, v_sh}, log_decay, reset, reset_sn,
                   state, next_state, out, scale, h, dk, dv};
-  const bool wide = dv % 4 == 0 && (((uintptr_t)state | (uintptr_t)next_state) & 15) == 0;
   const dim3 grid((unsigned)(n * h)), block(kBlock);
-  const hipStream_t at = as_stream(stream);
-  if (dtype == 0 && wide) hipLaunchKernelGGL((step_kernel<float, 4>), grid, block, 0, at, s);
-  if (dtype == 0 && !wide) hipLaunchKernelGGL((step_kernel<float, 1>), grid, block, 0, at, s);
-  if (dtype == 1 && wide) hipLaunchKernelGGL((step_kernel<__bf16, 4>), grid, block, 0, at, s);
-  if (dtype == 1 && !wide) hipLaunchKernelGGL((step_kernel<__bf16, 1>), grid, block, 0, at, s);
+  if (dtype == 1)
+    hipLaunchKernelGGL(step_kernel<__bf16>, grid, block, 0, as_stream(stream), s);
+  else
+    hipLaunchKernelGGL(step_kernel<float>, grid, block, 0, as_stream(stream), s);
   return launch_status();
 }

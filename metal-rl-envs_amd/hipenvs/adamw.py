@@ -16,8 +16,8 @@ where a code c stands for scale * t|t|, t = c / 127 (m), or scale * t^4, t = c /
 Asynchronous on the current stream.
 """
 
-import ctypes
 import math
+from array import array
 
 import torch
 
@@ -25,6 +25,7 @@ from . import _lib
 
 BLOCK = 256
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
+_OF_GRAD = {torch.float32: 0, torch.bfloat16: 2}
 
 
 def _padded(n):
@@ -61,6 +62,33 @@ def _check_moments(moments, n, device):
     return 32 if len(moments) == 2 else 8
 
 
+def _corrections(t, lr, beta1, beta2):
+    """(lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t))."""
+    return lr / (1.0 - beta1 ** t), 1.0 / math.sqrt(1.0 - beta2 ** t)
+
+
+def _refused_param(params, device):
+    for i, p in enumerate(params):
+        if p.dtype not in _TYPES:
+            return TypeError(f"params[{i}] must be float32 or bfloat16, got {p.dtype}")
+        if p.device != device:
+            return ValueError(f"params[{i}] is on {p.device}, params[0] is on {device}")
+        if not p.is_contiguous():
+            return ValueError(f"params[{i}] must be contiguous")
+
+
+def _refused_grad(params, grads, device):
+    for i, (p, g) in enumerate(zip(params, grads)):
+        if g is None:
+            continue
+        if g.dtype not in _OF_GRAD:
+            return TypeError(f"grads[{i}] must be float32 or bfloat16, got {g.dtype}")
+        if g.device != device:
+            return ValueError(f"grads[{i}] is on {g.device}, params[0] is on {device}")
+        if g.shape != p.shape:
+            return ValueError(f"grads[{i}] must have shape {tuple(p.shape)}, got {tuple(g.shape)}")
+
+
 def step(params, grads, moments, t, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01):
     """One step in place: params and moments change, grads do not. `grads` holds a tensor for each
     parameter, or None where it has none (that parameter and its moments stay). `t` is the
@@ -80,51 +108,49 @@ def step(params, grads, moments, t, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weigh
     device = params[0].device
     if device.type != "cuda":
         raise ValueError(f"params must be on a ROCm GPU, got device {device}")
+    index, kinds, grad_kinds = params[0].get_device(), _TYPES, _OF_GRAD
     ptrs, grad_ptrs, sizes, types, held, flat = [], [], [], [], [], 0
-    for i in range(count):
-        p, g = params[i], grads[i]
-        kind = _TYPES.get(p.dtype)
-        if kind is None:
-            raise TypeError(f"params[{i}] must be float32 or bfloat16, got {p.dtype}")
-        if p.device != device:
-            raise ValueError(f"params[{i}] is on {p.device}, params[0] is on {device}")
-        if not p.is_contiguous():
-            raise ValueError(f"params[{i}] must be contiguous")
-        n = p.numel()
+    for p, g in zip(params, grads):
+        kind = kinds.get(p.dtype)
+        if kind is None or p.get_device() != index or not p.is_contiguous():
+            raise _refused_param(params, device)
         if g is None:
-            grad_ptrs.append(None)
+            grad_ptrs.append(0)
         else:
-            of_grad = _TYPES.get(g.dtype)
-            if of_grad is None:
-                raise TypeError(f"grads[{i}] must be float32 or bfloat16, got {g.dtype}")
-            if g.shape != p.shape:
-                raise ValueError(f"grads[{i}] must have shape {tuple(p.shape)}, got {tuple(g.shape)}")
-            if g.device != device:
-                raise ValueError(f"grads[{i}] is on {g.device}, params[0] is on {device}")
+            of_grad = grad_kinds.get(g.dtype)
+            if of_grad is None or g.get_device() != index or g.shape != p.shape:
+                raise _refused_grad(params, grads, device)
             if not g.is_contiguous():
                 g = g.contiguous()
-                held.append(g)
-            kind |= of_grad << 1
+                held.append(g)   # until the launch: the stream's next allocation may take its memory then
+            kind += of_grad
             grad_ptrs.append(g.data_ptr())
+        n = p.numel()
         ptrs.append(p.data_ptr())
         sizes.append(n)
         types.append(kind)
-        flat += _padded(n)
+        flat += -(-n // BLOCK) * BLOCK
     if len(set(ptrs)) != count and len({a for a, n in zip(ptrs, sizes) if n}) != sum(n > 0 for n in sizes):
         raise ValueError("a parameter is listed twice")
     bits = _check_moments(moments, flat, device)
-    steps = [t] * count if isinstance(t, int) else [int(x) for x in t]
-    if len(steps) != count or min(steps) < 1:
-        raise ValueError("t must be a step number from 1, or one for each parameter")
-    of_step = {n: (lr / (1.0 - beta1 ** n), 1.0 / math.sqrt(1.0 - beta2 ** n)) for n in set(steps)}
-    pointers, doubles = ctypes.c_void_p * count, ctypes.c_double * count
+    if isinstance(t, int):
+        if t < 1:
+            raise ValueError(f"t must be a step number from 1, got {t}")
+        rate, root = _corrections(t, lr, beta1, beta2)
+        rates, roots = array("d", [rate]) * count, array("d", [root]) * count
+    else:
+        steps = [int(x) for x in t]
+        if len(steps) != count or min(steps) < 1:
+            raise ValueError("t must be a step number from 1, or one for each parameter")
+        of_step = {n: _corrections(n, lr, beta1, beta2) for n in set(steps)}
+        rates = array("d", [of_step[n][0] for n in steps])
+        roots = array("d", [of_step[n][1] for n in steps])
     m, v, *scales = (x.data_ptr() for x in moments)
     m_scales, v_scales = scales if scales else (None, None)
+    arrays = (array("Q", ptrs), array("Q", grad_ptrs), array("q", sizes), array("i", types), rates, roots)
     with _lib.on(device):
-        _lib.call("hipenvs_adamw_step", bits, count, pointers(*ptrs), pointers(*grad_ptrs),
-                  (ctypes.c_int64 * count)(*sizes), (ctypes.c_int32 * count)(*types),
-                  doubles(*(of_step[n][0] for n in steps)), doubles(*(of_step[n][1] for n in steps)), beta1, beta2,
-                  eps, 1.0 - lr * weight_decay, m, v, m_scales, v_scales, _lib.stream_of(device))
+        _lib.call("hipenvs_adamw_step", bits, count, *(a.buffer_info()[0] for a in arrays), beta1, beta2, eps,
+                  1.0 - lr * weight_decay, m, v, m_scales, v_scales, _lib.stream_of(device))
     torch.autograd.graph.increment_version((*params, *moments))
 
 

@@ -28,53 +28,55 @@ MAX_DIM = 128
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 
-def _check(x, name, like, shape):
-    """A tensor of `like`'s type and device and of `shape`, its last axis contiguous."""
+def _tensor(x, name):
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor, got {type(x).__name__}")
-    if x.dtype != like.dtype:
-        raise TypeError(f"{name} must be {like.dtype} as q is, got {x.dtype}")
-    if x.device != like.device:
-        raise ValueError(f"{name} is on {x.device}, q is on {like.device}")
-    if tuple(x.shape) != shape:
+    return x
+
+
+def _check(x, name, dtype, device, shape):
+    """A tensor of that type, shape and device (a GPU's index), its last axis contiguous."""
+    if _tensor(x, name).dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, got {x.dtype}")
+    if x.shape != shape:
         raise ValueError(f"{name} must have shape {shape}, got {tuple(x.shape)}")
+    if x.get_device() != device:
+        raise ValueError(f"{name} is on {x.device}, q is on GPU {device}")
     return x if x.stride(-1) == 1 or shape[-1] == 1 else x.contiguous()
 
 
 def _check_qkv(q, k, v, axes):
-    """(q, k, v, lead, h, dk, dv) of tensors (*lead, h, d) with `axes` axes in all."""
-    if not isinstance(q, torch.Tensor):
-        raise TypeError(f"q must be a torch.Tensor, got {type(q).__name__}")
-    if q.dtype not in _DTYPES:
-        raise TypeError(f"q must be float32 or bfloat16, got {q.dtype}")
-    if q.device.type != "cuda":
+    """(q, k, v, the GPU's index, lead, h, dk, dv) of tensors (*lead, h, d) with `axes` axes in all."""
+    dtype = _tensor(q, "q").dtype
+    if dtype not in _DTYPES:
+        raise TypeError(f"q must be float32 or bfloat16, got {dtype}")
+    device = q.get_device()
+    if not q.is_cuda:
         raise ValueError(f"q must be on a ROCm GPU, got device {q.device}")
-    if q.dim() != axes:
-        raise ValueError(f"q must have {axes} axes, got shape {tuple(q.shape)}")
-    if not isinstance(v, torch.Tensor) or v.dim() != axes:
-        raise ValueError(f"v must be a torch.Tensor with {axes} axes")
     shape = tuple(q.shape)
+    if len(shape) != axes:
+        raise ValueError(f"q must have {axes} axes, got shape {shape}")
+    if _tensor(v, "v").dim() != axes:
+        raise ValueError(f"v must have {axes} axes, got shape {tuple(v.shape)}")
     lead, h, dk, dv = shape[:-2], shape[-2], shape[-1], v.shape[-1]
-    for name, d in (("dk", dk), ("dv", dv)):
-        if not 1 <= d <= MAX_DIM:
-            raise ValueError(f"{name} must be in 1..{MAX_DIM}, got {d}")
+    if not (1 <= dk <= MAX_DIM and 1 <= dv <= MAX_DIM):
+        raise ValueError(f"dk and dv must be in 1..{MAX_DIM}, got {dk} and {dv}")
     if not 1 <= h <= 65536:
         raise ValueError(f"there must be 1 to 65536 heads, got {h}")
-    q = _check(q, "q", q, shape)
-    k = _check(k, "k", q, shape)
-    v = _check(v, "v", q, (*lead, h, dv))
-    return q, k, v, lead, h, dk, dv
+    if q.stride(-1) != 1 and dk != 1:
+        q = q.contiguous()
+    k = _check(k, "k", dtype, device, shape)
+    v = _check(v, "v", dtype, device, (*lead, h, dv))
+    return q, k, v, device, lead, h, dk, dv
 
 
 def _check_f32(x, name, shape, device):
-    if not isinstance(x, torch.Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor, got {type(x).__name__}")
-    if x.dtype != torch.float32:
+    if _tensor(x, name).dtype is not torch.float32:
         raise TypeError(f"{name} must be float32, got {x.dtype}")
-    if tuple(x.shape) != shape:
+    if x.shape != shape:
         raise ValueError(f"{name} must have shape {shape}, got {tuple(x.shape)}")
-    if x.device != device:
-        raise ValueError(f"{name} is on {x.device}, q is on {device}")
+    if x.get_device() != device:
+        raise ValueError(f"{name} is on {x.device}, q is on GPU {device}")
     return x.contiguous()
 
 
@@ -88,14 +90,12 @@ def _check_decay(log_decay, h, device):
 def _check_reset(reset, shape, device):
     if reset is None:
         return None
-    if not isinstance(reset, torch.Tensor):
-        raise TypeError(f"reset must be a torch.Tensor, got {type(reset).__name__}")
-    if reset.dtype != torch.bool:
+    if _tensor(reset, "reset").dtype is not torch.bool:
         raise TypeError(f"reset must be bool, got {reset.dtype}")
-    if tuple(reset.shape) != shape:
+    if reset.shape != shape:
         raise ValueError(f"reset must have shape {shape}, got {tuple(reset.shape)}")
-    if reset.device != device:
-        raise ValueError(f"reset is on {reset.device}, q is on {device}")
+    if reset.get_device() != device:
+        raise ValueError(f"reset is on {reset.device}, q is on GPU {device}")
     return reset
 
 
@@ -169,11 +169,11 @@ def sequence(q, k, v, log_decay, state=None, reset=None, scale=None):
     (b, h, dk, dv) float32 before the first token (None: zeros), reset (b, t) bool, True where
     an episode begins at that token (None: nowhere). Returns (out (b, t, h, dv) of q's type,
     final_state (b, h, dk, dv) float32), differentiable once in q, k, v and state."""
-    q, k, v, (b, t), h, dk, dv = _check_qkv(q, k, v, 4)
-    log_decay = _check_decay(log_decay, h, q.device)
-    reset = _check_reset(reset, (b, t), q.device)
+    q, k, v, device, (b, t), h, dk, dv = _check_qkv(q, k, v, 4)
+    log_decay = _check_decay(log_decay, h, device)
+    reset = _check_reset(reset, (b, t), device)
     if state is not None:
-        state = _check_f32(state, "state", (b, h, dk, dv), q.device)
+        state = _check_f32(state, "state", (b, h, dk, dv), device)
     scale = _scale(scale, dk)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or (state is not None and state.requires_grad)):
@@ -186,22 +186,23 @@ def step(q, k, v, log_decay, state, reset=None, scale=None, next_state=None):
     contiguous, reset (n,) bool, True where this token begins an episode. Returns
     (out (n, h, dv) of q's type, next_state). ``next_state`` receives the new states and may be
     ``state`` itself. Not differentiable: training goes through ``sequence``."""
-    q, k, v, (n,), h, dk, dv = _check_qkv(q, k, v, 3)
-    log_decay = _check_decay(log_decay, h, q.device)
-    reset = _check_reset(reset, (n,), q.device)
-    state = _check_f32(state, "state", (n, h, dk, dv), q.device)
+    q, k, v, device, (n,), h, dk, dv = _check_qkv(q, k, v, 3)
+    log_decay = _check_decay(log_decay, h, device)
+    reset = _check_reset(reset, (n,), device)
+    state = _check_f32(state, "state", (n, h, dk, dv), device)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
         raise ValueError("step has no gradient: call it under torch.no_grad(), or use sequence")
     if next_state is None:
         next_state = torch.empty_like(state)
     else:
-        if _check_f32(next_state, "next_state", (n, h, dk, dv), q.device) is not next_state:
+        if _check_f32(next_state, "next_state", (n, h, dk, dv), device) is not next_state:
             raise ValueError("next_state must be contiguous")
         torch.autograd.graph.increment_version(next_state)
-    out = torch.empty((n, h, dv), dtype=q.dtype, device=q.device)
-    with _lib.on(q.device):
-        _lib.call("hipenvs_decay_attention_step", _DTYPES[q.dtype], _lib.ptr(q), q.stride(0), q.stride(1), _lib.ptr(k),
-                  k.stride(0), k.stride(1), _lib.ptr(v), v.stride(0), v.stride(1), _lib.ptr(log_decay),
-                  _lib.ptr(state), _lib.ptr(reset), reset.stride(0) if reset is not None else 0, _scale(scale, dk),
-                  _lib.ptr(out), _lib.ptr(next_state), n, h, dk, dv, _lib.stream_of(q.device))
+    on = q.device
+    out = torch.empty((n, h, dv), dtype=q.dtype, device=on)
+    with _lib.on(on):
+        _lib.call("hipenvs_decay_attention_step", _DTYPES[q.dtype], q.data_ptr(), q.stride(0), q.stride(1),
+                  k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                  log_decay.data_ptr(), state.data_ptr(), _lib.ptr(reset), reset.stride(0) if reset is not None else 0,
+                  _scale(scale, dk), out.data_ptr(), next_state.data_ptr(), n, h, dk, dv, _lib.stream_of(on))
     return out, next_state
