@@ -424,7 +424,7 @@ int hipenvs_decay_attention_step(int32_t dtype, const void* q, int64_t q_sn, int
  * bits 32: m, v f32, scales unused. bits 8: m i8 and v u8 codes (4-byte aligned) and a scale for
  * every 256 values, m = scale t|t| with t = code / 127, v = scale t^4 with t = code / 255; the
  * parameters are updated from the moments before they are rounded. A block with a NaN or
- * an infinity in its moments reads back as NaN. */
+ * an infinity in its moments reads back as no number. */
 int hipenvs_adamw_step(int32_t bits, int32_t count, void* const* params, const void* const* grads,
                        const int64_t* sizes, const int32_t* types, const double* rates,
                        const double* roots, double beta1, double beta2, double eps, double keep,

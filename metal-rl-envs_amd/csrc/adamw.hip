@@ -26,7 +26,7 @@ struct Tensor {
   int64_t n;
   int64_t at;       // where its moments begin, a multiple of kQuant
   uint32_t tile0;   // the first of its tiles in this launch
-  uint32_t types;   // kParamBf16 | kGradBf16 | kWide: every pointer takes four values at once
+  uint32_t types;   // kParamBf16 | kGradBf16 | kWide: every pointer can take four values at once
   float rate, root;
 };
 
@@ -36,55 +36,43 @@ struct Batch {
   float beta1, rest1, beta2, rest2, eps, keep;
 };
 
-__device__ __forceinline__ float bf16_to_f32(uint32_t u) { return __uint_as_float(u << 16); }
-
-// Nearest even; a NaN stays a NaN.
-__device__ __forceinline__ uint32_t f32_to_bf16(float x) {
-  const uint32_t u = __float_as_uint(x);
-  const uint32_t r = (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16;
-  return x != x ? ((u >> 16) | 0x40u) : r;
-}
-
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 
-// Four values at `i` of a float32 or bfloat16 array of n; beyond n they are zero.
-__device__ __forceinline__ void load4(const void* base, int64_t i, int64_t n, bool bf16, bool wide, float (&x)[4]) {
-  if (wide && i + 4 <= n) {
-    if (bf16) {
-      const u32x2 w = *(const u32x2*)((const uint16_t*)base + i);
-      x[0] = bf16_to_f32(w.x & 0xFFFFu), x[1] = bf16_to_f32(w.x >> 16);
-      x[2] = bf16_to_f32(w.y & 0xFFFFu), x[3] = bf16_to_f32(w.y >> 16);
-    } else {
-      const f32x4 w = *(const f32x4*)((const float*)base + i);
-      x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
-    }
+// Four values at `i` of a float32 or bfloat16 array of n; beyond n they are zero. `whole`: they
+// are all there, and lie where four are read at once (the same for a wave).
+__device__ __forceinline__ void load4(const void* base, int64_t i, int64_t n, bool bf16, bool whole, float (&x)[4]) {
+  if (whole) {
+    f32x4 w;
+    if (bf16)
+      w = __builtin_convertvector(*(const bf16x4*)((const __bf16*)base + i), f32x4);
+    else
+      w = *(const f32x4*)((const float*)base + i);
+    x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
     return;
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     x[e] = 0.0f;
-    if (i + e < n) x[e] = bf16 ? bf16_to_f32(((const uint16_t*)base)[i + e]) : ((const float*)base)[i + e];
+    if (i + e < n) x[e] = bf16 ? (float)((const __bf16*)base)[i + e] : ((const float*)base)[i + e];
   }
 }
 
-__device__ __forceinline__ void store4(void* base, int64_t i, int64_t n, bool bf16, bool wide, const float (&x)[4]) {
-  if (wide && i + 4 <= n) {
-    if (bf16) {
-      const u32x2 w = {f32_to_bf16(x[0]) | (f32_to_bf16(x[1]) << 16), f32_to_bf16(x[2]) | (f32_to_bf16(x[3]) << 16)};
-      *(u32x2*)((uint16_t*)base + i) = w;
-    } else {
-      const f32x4 w = {x[0], x[1], x[2], x[3]};
+__device__ __forceinline__ void store4(void* base, int64_t i, int64_t n, bool bf16, bool whole, const float (&x)[4]) {
+  const f32x4 w = {x[0], x[1], x[2], x[3]};
+  if (whole) {
+    if (bf16)
+      *(bf16x4*)((__bf16*)base + i) = __builtin_convertvector(w, bf16x4);   // to nearest even
+    else
       *(f32x4*)((float*)base + i) = w;
-    }
     return;
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (i + e < n) {
       if (bf16)
-        ((uint16_t*)base)[i + e] = (uint16_t)f32_to_bf16(x[e]);
+        ((__bf16*)base)[i + e] = (__bf16)x[e];
       else
         ((float*)base)[i + e] = x[e];
     }
@@ -110,9 +98,9 @@ __device__ __forceinline__ int find(const Batch& b, uint32_t tile) {
 
 __global__ __launch_bounds__(kBlock) void step32_kernel(Batch b, float* __restrict__ m_all, float* __restrict__ v_all) {
   const Tensor& t = b.t[find(b, blockIdx.x)];
-  const int64_t i = (int64_t)(blockIdx.x - t.tile0) * kTile + 4 * threadIdx.x;
+  const int64_t first = (int64_t)(blockIdx.x - t.tile0) * kTile, i = first + 4 * threadIdx.x;
   if (i >= t.n) return;
-  const bool wide = t.types & kWide, pb = t.types & kParamBf16, gb = t.types & kGradBf16;
+  const bool wide = (t.types & kWide) && first + kTile <= t.n, pb = t.types & kParamBf16, gb = t.types & kGradBf16;
   float* m_at = m_all + t.at;
   float* v_at = v_all + t.at;
   float p[4], g[4], m[4], v[4];
@@ -137,7 +125,7 @@ __global__ __launch_bounds__(kBlock) void step32_kernel(Batch b, float* __restri
 // t = c / 255, so sqrt(v), which divides the update, is held as a square like m. Rounding is
 // to the nearest code of the root. No v above zero gets code 0: a denominator would fall to
 // eps, and the update would grow by orders of magnitude. A block with a NaN or an infinity
-// has that as its scale and reads back as NaN; one whose largest magnitude is subnormal has
+// has that as its scale and reads back as no number; one whose largest magnitude is subnormal has
 // the smallest normal number as its scale, whose reciprocal is finite.
 
 __device__ __forceinline__ float decode_m(int c, float scale) {
@@ -160,15 +148,18 @@ __device__ __forceinline__ float wave_scale(const float (&x)[4]) {
     const uint32_t a = __float_as_uint(x[e]) & 0x7FFFFFFFu;
     u = a > u ? a : u;
   }
-#pragma unroll
-  for (int s = 32; s > 0; s >>= 1) {
-    const uint32_t o = (uint32_t)__shfl_xor((int)u, s);
-    u = o > u ? o : u;
-  }
+  // within 16 lanes by data-parallel moves, between the four rows by scalars
+  const auto larger = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+  u = larger(u, (uint32_t)__builtin_amdgcn_mov_dpp((int)u, 0xB1, 0xF, 0xF, true));    // the neighbour of two
+  u = larger(u, (uint32_t)__builtin_amdgcn_mov_dpp((int)u, 0x4E, 0xF, 0xF, true));    // of four
+  u = larger(u, (uint32_t)__builtin_amdgcn_mov_dpp((int)u, 0x141, 0xF, 0xF, true));   // mirrored in eight
+  u = larger(u, (uint32_t)__builtin_amdgcn_mov_dpp((int)u, 0x140, 0xF, 0xF, true));   // mirrored in sixteen
+  u = larger(larger((uint32_t)__builtin_amdgcn_readlane((int)u, 0), (uint32_t)__builtin_amdgcn_readlane((int)u, 16)),
+             larger((uint32_t)__builtin_amdgcn_readlane((int)u, 32), (uint32_t)__builtin_amdgcn_readlane((int)u, 48)));
   return __uint_as_float(u != 0 && u < 0x00800000u ? 0x00800000u : u);
 }
 
-// A code: the nearest whole number in 0 .. top of root * top; 0 for a NaN. The roots that
+// A code: the nearest whole number in 0 .. top of root * top. The roots that
 // decide are the correctly rounded ones, but only a product next to the border of two codes
 // depends on their last bits. The hardware's root is within 1 ulp, and a root of such a root
 // within 1.5; the exact ones within 0.5 and 0.75: so the products differ by at most
@@ -178,13 +169,8 @@ __device__ __forceinline__ float wave_scale(const float (&x)[4]) {
 // 87 million, bound by their float64 instructions.
 constexpr float kBorder = 1e-4f;
 
-__device__ __forceinline__ int code_of(float product, float top) {
-  const float c = __builtin_rintf(product);
-  return c == c ? (int)__builtin_fminf(c, top) : 0;
-}
-
 __device__ __forceinline__ bool near_border(float product) {
-  return __builtin_fabsf(__builtin_fabsf(product - __builtin_rintf(product)) - 0.5f) < kBorder;
+  return __builtin_fabsf(__builtin_amdgcn_fractf(product) - 0.5f) < kBorder;
 }
 
 __global__ __launch_bounds__(kBlock) void step8_kernel(Batch b, uint32_t* __restrict__ m_codes,
@@ -195,7 +181,8 @@ __global__ __launch_bounds__(kBlock) void step8_kernel(Batch b, uint32_t* __rest
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   if (first + wave * kQuant >= t.n) return;   // the whole wave: its quant block is past the tensor
   const int64_t i = first + 4 * threadIdx.x;
-  const bool wide = t.types & kWide, pb = t.types & kParamBf16, gb = t.types & kGradBf16;
+  const bool inside = first + (wave + 1) * kQuant <= t.n;
+  const bool wide = (t.types & kWide) && inside, pb = t.types & kParamBf16, gb = t.types & kGradBf16;
   const int64_t word = (t.at + i) >> 2, block = (t.at + first) / kQuant + wave;
   float p[4], g[4], m[4], v[4];
   load4(t.param, i, t.n, pb, wide, p);
@@ -206,7 +193,11 @@ __global__ __launch_bounds__(kBlock) void step8_kernel(Batch b, uint32_t* __rest
   for (int e = 0; e < 4; ++e) {
     m[e] = decode_m((int)(int8_t)(mc >> (8 * e)), ms) * b.beta1 + g[e] * b.rest1;
     v[e] = decode_v((vc >> (8 * e)) & 0xFFu, vs) * b.beta2 + (g[e] * g[e]) * b.rest2;
-    if (i + e >= t.n) m[e] = v[e] = 0.0f;   // the padding stays zero, also in a block that reads back as NaN
+  }
+  if (!inside) {   // the padding stays zero, also in a block that does not read back as numbers
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (i + e >= t.n) m[e] = v[e] = 0.0f;
   }
   const float new_ms = wave_scale(m), new_vs = wave_scale(v);
   const float m_inv = new_ms > 0.0f ? 1.0f / new_ms : 0.0f, v_inv = new_vs > 0.0f ? 1.0f / new_vs : 0.0f;
@@ -225,14 +216,15 @@ __global__ __launch_bounds__(kBlock) void step8_kernel(Batch b, uint32_t* __rest
       of_v[e] = sqrt_rn(sqrt_rn(v[e] * v_inv)) * 255.0f;
     }
   }
+  // the codes as float32 and into their bytes: a code of m below zero as 256 more, its two's
+  // complement
   uint32_t new_mc = 0, new_vc = 0;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const int cm = code_of(of_m[e], 127.0f);
-    int cv = code_of(of_v[e], 255.0f);
-    cv = v[e] > 0.0f && cv < 1 ? 1 : cv;
-    new_mc |= ((uint32_t)(m[e] < 0.0f ? -cm : cm) & 0xFFu) << (8 * e);
-    new_vc |= (uint32_t)cv << (8 * e);
+    const float cm = __builtin_copysignf(__builtin_fminf(__builtin_rintf(of_m[e]), 127.0f), m[e]);
+    const float cv = __builtin_fmaxf(__builtin_fminf(__builtin_rintf(of_v[e]), 255.0f), v[e] > 0.0f ? 1.0f : 0.0f);
+    new_mc = __builtin_amdgcn_cvt_pk_u8_f32(cm < 0.0f ? cm + 256.0f : cm, e, new_mc);
+    new_vc = __builtin_amdgcn_cvt_pk_u8_f32(cv, e, new_vc);
     p[e] = moved(p[e], m[e], v[e], b, t);
   }
   store4(t.param, i, t.n, pb, wide, p);
