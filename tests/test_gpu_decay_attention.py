@@ -231,6 +231,87 @@ def test_what_an_earlier_episode_or_a_later_token_holds_does_not_reach(dev, dtyp
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+def test_bad_values_in_rows_walked_in_parts(dev, dtype):
+    """A long row: a NaN in its value rows inside one part, an infinity in another, each ended by a
+    reset: everything after the resets, and every other head and row, is as without them."""
+    from hipenvs import decay_attention
+
+    c = case(dev, 30, 2, 3000, 2, 32, 48, dtype, "apart", 0)
+    c["reset"] = torch.zeros(2, 3000, dtype=torch.bool, device=dev)
+    c["reset"][0, 700] = c["reset"][0, 1500] = c["reset"][0, 2200] = True
+    clean = decay_attention.sequence(**c)
+    spoilt = {**c, "v": c["v"].clone(), "k": c["k"].clone()}
+    spoilt["v"][0, 650, 1, 3] = float("nan")
+    spoilt["k"][0, 1490, 1, 5] = float("inf")
+    got = decay_attention.sequence(**spoilt)
+    touched = torch.zeros(2, 3000, 2, dtype=torch.bool, device=dev)
+    touched[0, 650:700, 1] = touched[0, 1490:1500, 1] = True
+    assert not torch.isfinite(got[0][touched].float()).all()
+    args = [to_np(c[n]) for n in ("q", "k", "v", "log_decay", "state", "reset")]
+    want, size = oda.sequence(*args, 32 ** -0.5), oda.magnitudes(*args, 32 ** -0.5)
+    mask = touched.cpu().numpy()
+    for x in (got, clean):
+        close(x[0][~touched], want[0][~mask], size[0][~mask], dtype, 3000, 32, 48)
+        close(x[1], want[1], size[1], F32, 3000, 32, 48)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_backward_with_and_without_the_forward_s_states(dev, dtype):
+    """The C entry point computes the states between parts again where it is given none."""
+    import ctypes
+
+    from hipenvs import _lib, decay_attention
+
+    b, t, h, dk, dv = 2, 3000, 2, 32, 48
+    c = case(dev, 31, b, t, h, dk, dv, dtype, "fused", 700)
+    code = decay_attention._DTYPES[dtype]
+    need = _lib.lib().hipenvs_decay_attention_workspace_bytes(code, b, t, h, dk, dv)
+    assert need > 0
+    gen = torch.Generator().manual_seed(2)
+    dout = torch.randn(b, t, h, dv, generator=gen).to(dtype).to(dev)
+    out, final, states = decay_attention._forward(c["q"], c["k"], c["v"], c["log_decay"], c["state"], c["reset"], 0.2)
+    assert states.numel() == need
+    args = [to_np(c[n]) for n in ("q", "k", "v", "log_decay", "state", "reset")]
+    want = oda.gradients(*args, 0.2, to_np(dout), None)
+    size = oda.magnitudes(*args, 0.2, to_np(dout), None)[2:]
+    for given in (states, None):
+        grads = [torch.empty(b, t, h, d, dtype=dtype, device=dev) for d in (dk, dk, dv)]
+        dstate = torch.empty(b, h, dk, dv, device=dev)
+        work = torch.empty(need, dtype=torch.uint8, device=dev)
+        strides = decay_attention._strides((c["q"], c["k"], c["v"], dout), c["reset"])
+        _lib.call("hipenvs_decay_attention_backward", code, *(_lib.ptr(c[n]) for n in "qkv"), _lib.ptr(dout), strides,
+                  _lib.ptr(c["log_decay"]), _lib.ptr(c["state"]), _lib.ptr(c["reset"]), None, _lib.ptr(given), 0.2,
+                  *(_lib.ptr(g) for g in grads), _lib.ptr(dstate), b, t, h, dk, dv, _lib.ptr(work), need,
+                  _lib.stream_of(dev))
+        for x, w, s in zip((*grads, dstate), want, size):
+            close(x, w, s, x.dtype, t, dk, dv)
+    rc = _lib.lib().hipenvs_decay_attention(code, *(_lib.ptr(c[n]) for n in "qkv"), strides, _lib.ptr(c["log_decay"]),
+                                            None, None, 0.2, _lib.ptr(out), _lib.ptr(final), b, t, h, dk, dv,
+                                            _lib.ptr(states), need - 1, None)
+    assert rc == _lib.E_ARG   # a workspace too small
+
+
+def test_a_captured_sequence(dev):
+    """A long row's three launches in a graph, replayed with the program's own work between."""
+    from hipenvs import decay_attention
+
+    c = case(dev, 32, 1, 2500, 2, 32, 32, BF16, "apart", 300)
+    decay_attention.sequence(**c)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, final = decay_attention.sequence(**c)
+    for seed in range(4):
+        other = case(dev, 33 + seed, 1, 2500, 2, 32, 32, BF16, "apart", 300)
+        for n in ("q", "k", "v", "state", "reset"):
+            c[n].copy_(other[n])
+        graph.replay()
+        torch.cuda.synchronize()
+        want = decay_attention.sequence(**other)
+        assert torch.equal(out, want[0]) and torch.equal(final, want[1])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_a_state_that_is_not_finite_ends_at_the_reset(dev, dtype):
     c = case(dev, 11, 2, 90, 2, 16, 16, dtype, "apart", 0)
     c["state"][0, 1] = float("nan")
