@@ -17,6 +17,7 @@ Asynchronous on the current stream.
 """
 
 import math
+import operator
 from array import array
 
 import torch
@@ -26,6 +27,13 @@ from . import _lib
 BLOCK = 256
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
 _OF_GRAD = {torch.float32: 0, torch.bfloat16: 2}
+_dtype, _shape, _add = operator.attrgetter("dtype"), operator.attrgetter("shape"), operator.add
+_device, _contiguous = torch.Tensor.get_device, torch.Tensor.is_contiguous
+_address, _numel = torch.Tensor.data_ptr, torch.Tensor.numel
+
+
+def _is_tensor(x):
+    return x is not None
 
 
 def _padded(n):
@@ -108,28 +116,29 @@ def step(params, grads, moments, t, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weigh
     device = params[0].device
     if device.type != "cuda":
         raise ValueError(f"params must be on a ROCm GPU, got device {device}")
-    index, kinds, grad_kinds = params[0].get_device(), _TYPES, _OF_GRAD
-    ptrs, grad_ptrs, sizes, types, held, flat = [], [], [], [], [], 0
-    for p, g in zip(params, grads):
-        kind = kinds.get(p.dtype)
-        if kind is None or p.get_device() != index or not p.is_contiguous():
-            raise _refused_param(params, device)
-        if g is None:
-            grad_ptrs.append(0)
-        else:
-            of_grad = grad_kinds.get(g.dtype)
-            if of_grad is None or g.get_device() != index or g.shape != p.shape:
-                raise _refused_grad(params, grads, device)
-            if not g.is_contiguous():
-                g = g.contiguous()
-                held.append(g)   # until the launch: the stream's next allocation may take its memory then
-            kind += of_grad
-            grad_ptrs.append(g.data_ptr())
-        n = p.numel()
-        ptrs.append(p.data_ptr())
-        sizes.append(n)
-        types.append(kind)
-        flat += -(-n // BLOCK) * BLOCK
+    # one pass of a C function over the list for each property: a loop over the tensors in Python
+    # costs twice as much, and more than the launch at a few dozen tensors
+    index = params[0].get_device()
+    types = list(map(_TYPES.get, map(_dtype, params)))
+    if None in types or set(map(_device, params)) != {index} or not all(map(_contiguous, params)):
+        raise _refused_param(params, device)
+    given = grads if all(map(_is_tensor, grads)) else [g for g in grads if g is not None]
+    of_grads = list(map(_OF_GRAD.get, map(_dtype, given)))
+    whole = len(given) == count
+    if (None in of_grads or (given and set(map(_device, given)) != {index})
+            or list(map(_shape, given)) != list(map(_shape, params if whole else
+                                                    [p for p, g in zip(params, grads) if g is not None]))):
+        raise _refused_grad(params, grads, device)
+    if not all(map(_contiguous, given)):   # the copies live until the launch: their memory may go to the next tensor then
+        given = [g.contiguous() for g in given]
+    grad_ptrs = list(map(_address, given))
+    if not whole:
+        ptr_of, kind_of = iter(grad_ptrs), iter(of_grads)
+        grad_ptrs = [0 if g is None else next(ptr_of) for g in grads]
+        of_grads = [0 if g is None else next(kind_of) for g in grads]
+    types = list(map(_add, types, of_grads))
+    ptrs, sizes = list(map(_address, params)), list(map(_numel, params))
+    flat = sum(-(-n // BLOCK) for n in sizes) * BLOCK
     if len(set(ptrs)) != count and len({a for a, n in zip(ptrs, sizes) if n}) != sum(n > 0 for n in sizes):
         raise ValueError("a parameter is listed twice")
     bits = _check_moments(moments, flat, device)

@@ -99,11 +99,18 @@ def _check_reset(reset, shape, device):
     return reset
 
 
+_STRIDES = {n: ctypes.c_int64 * n for n in (11, 14)}
+
+
+def _flat_strides(rows):
+    return [s for x in rows for s in x.stride()[:3]]
+
+
 def _strides(rows, reset):
     """The host array of strides: b, t, h of each tensor, then b, t of reset."""
-    flat = [s for x in rows for s in x.stride()[:3]]
+    flat = _flat_strides(rows)
     flat += reset.stride() if reset is not None else (0, 0)
-    return (ctypes.c_int64 * len(flat))(*flat)
+    return _STRIDES[len(flat)](*flat)
 
 
 def _scale(scale, dk):
@@ -134,34 +141,51 @@ def _forward(q, k, v, log_decay, state, reset, scale):
 
 
 class _Sequence(torch.autograd.Function):
+    # The backward runs in the engine's own thread, where Python costs several times what it does here:
+    # whatever it can be given ready, the forward makes.
     @staticmethod
     def forward(ctx, q, k, v, log_decay, state, reset, scale):
         ctx.set_materialize_grads(False)
         out, final, workspace = _forward(q, k, v, log_decay, state, reset, scale)
         ctx.save_for_backward(q, k, v, log_decay, state, reset, workspace)
-        ctx.scale = scale
+        b, t, h, dk = q.shape
+        flat = _flat_strides((q, k, v))
+        tail = reset.stride() if reset is not None else (0, 0)
+        ctx.ready = (_DTYPES[q.dtype], q.dtype, q.device, b, t, h, dk, v.shape[-1], flat, tail, scale,
+                     workspace.numel() if workspace is not None else 0)
         return out, final
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout, dfinal):
-        q, k, v, log_decay, state, reset, states = ctx.saved_tensors
-        b, t, h, dk = q.shape
-        dv = v.shape[-1]
-        if dout is None:
-            dout = torch.zeros((b, t, h, dv), dtype=q.dtype, device=q.device)
-        elif dout.stride(-1) != 1 and dv != 1:
-            dout = dout.contiguous()
-        dfinal = dfinal.contiguous() if dfinal is not None else None
-        dq, dk_, dv_ = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
-        dstate = torch.empty((b, h, dk, dv), dtype=torch.float32, device=q.device)
-        with _lib.on(q.device):
-            at, nbytes, _held = _workspace(_DTYPES[q.dtype], b, t, h, dk, dv, q.device)
-            _lib.call("hipenvs_decay_attention_backward", _DTYPES[q.dtype], _lib.ptr(q), _lib.ptr(k), _lib.ptr(v),
-                      _lib.ptr(dout), _strides((q, k, v, dout), reset), _lib.ptr(log_decay), _lib.ptr(state),
-                      _lib.ptr(reset), _lib.ptr(dfinal), _lib.ptr(states), ctx.scale, _lib.ptr(dq), _lib.ptr(dk_), _lib.ptr(dv_),
-                      _lib.ptr(dstate), b, t, h, dk, dv, at, nbytes, _lib.stream_of(q.device))
-        return dq, dk_, dv_, None, dstate if state is not None else None, None, None
+        if torch.is_grad_enabled():
+            return _backward_once(ctx, dout, dfinal)
+        return _backward(ctx, dout, dfinal)
+
+
+def _backward(ctx, dout, dfinal):
+    q, k, v, log_decay, state, reset, states = ctx.saved_tensors
+    code, dtype, device, b, t, h, dk, dv, flat, tail, scale, nbytes = ctx.ready
+    if dout is None:
+        dout = torch.zeros((b, t, h, dv), dtype=dtype, device=device)
+    elif dout.stride(-1) != 1 and dv != 1:
+        dout = dout.contiguous()
+    if dfinal is not None:
+        dfinal = dfinal.contiguous()
+    dq = torch.empty((b, t, h, dk), dtype=dtype, device=device)
+    dk_ = torch.empty((b, t, h, dk), dtype=dtype, device=device)
+    dv_ = torch.empty((b, t, h, dv), dtype=dtype, device=device)
+    dstate = torch.empty((b, h, dk, dv), dtype=torch.float32, device=device)
+    held = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    with _lib.on(device):
+        _lib.call("hipenvs_decay_attention_backward", code, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(),
+                  _STRIDES[14](*flat, *dout.stride()[:3], *tail), log_decay.data_ptr(), _lib.ptr(state),
+                  _lib.ptr(reset), _lib.ptr(dfinal), _lib.ptr(states), scale, dq.data_ptr(), dk_.data_ptr(),
+                  dv_.data_ptr(), dstate.data_ptr(), b, t, h, dk, dv, _lib.ptr(held), nbytes, _lib.stream_of(device))
+    return dq, dk_, dv_, None, dstate if state is not None else None, None, None
+
+
+# where a graph of the gradient is asked for: the gradients are without one, and say so when used
+_backward_once = torch.autograd.function.once_differentiable(_backward)
 
 
 def sequence(q, k, v, log_decay, state=None, reset=None, scale=None):

@@ -529,3 +529,17 @@ def test_refusals_on_the_device(dev):
         decay_attention.step(one[0].clone().requires_grad_(), *one[1:], ok[3], ok[4])
     with pytest.raises(TypeError):
         decay_attention.step(*one, ok[3], None)
+
+
+def test_a_second_derivative_is_refused(dev):
+    """create_graph gives the gradient; differentiating that raises."""
+    from hipenvs import decay_attention
+
+    c = case(dev, 40, 1, 9, 1, 4, 4, F32, "apart", 0)
+    q = c["q"].detach().requires_grad_()
+    out, _ = decay_attention.sequence(**{**c, "q": q})
+    once, = torch.autograd.grad(out.square().sum(), q, create_graph=True)
+    plain, = torch.autograd.grad(decay_attention.sequence(**{**c, "q": q})[0].square().sum(), q)
+    assert torch.equal(once.detach(), plain)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(once.sum(), q)
