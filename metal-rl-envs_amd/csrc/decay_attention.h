@@ -261,18 +261,6 @@ __device__ __forceinline__ void split(float (&rest)[N], __bf16 (&parts)[M][N]) {
     }
 }
 
-// A wave takes 16 columns of the state, all of its rows: S[a][r] is row 16 a + 4 g + r, column
-// l, for lane 16 g + l. That is both a matrix instruction's result and, its rows
-// taken as the summed axis in that order, an operand of the read S^T q, so the state never
-// leaves its registers. The block's NW waves share a chunk's q, k, v (in LDS; while one
-// chunk is computed the next is on its way to registers) and its masked products
-// P[i][j], computed once.
-//
-// bfloat16 rows: the inputs are exact operands. P, the S that is read and the lambda^n v_j that
-// is added are float32, split for the matrix instructions into bfloat16 parts, each the
-// rounding of what the parts before it leave: two parts for P and S (16 bits, so a result's
-// error is that of its own rounding to bfloat16) and for what enters a state that only results
-// are read from, three for one that is a float32 result itself (all 24 bits). float32 rows use the float32 matrix instructions throughout.
 // Waves a SIMD holds at once, which bounds their registers (512 over that many): three where
 // that many registers suffice without spilling, two elsewhere.
 template <class T>
@@ -286,6 +274,27 @@ constexpr int power_of_two(int n) {   // the least that is not below n
   return p;
 }
 
+// A wave takes 16 columns of the state, all of its rows: S[a][r] is row 16 a + 4 g + r, column
+// l, for lane 16 g + l. That is both a matrix instruction's result and, its rows
+// taken as the summed axis in that order, an operand of the read S^T q, so the state never
+// leaves its registers. The block's NW waves share a chunk's q, k, v (in LDS; while one
+// chunk is computed the next is on its way to registers) and its masked products
+// P[i][j], computed once.
+//
+// bfloat16 rows: the inputs are exact operands. P, the S that is read and the lambda^n v_j that
+// is added are float32, split for the matrix instructions into bfloat16 parts, each the
+// rounding of what the parts before it leave: two parts for P and S (16 bits, so a result's
+// error is that of its own rounding to bfloat16) and for what enters a state that only results
+// are read from, three for one that is a float32 result itself (all 24 bits). float32 rows
+// use the float32 matrix instructions throughout.
+//
+// What bounds it: with many rows of 128 tokens memory, at 4.7 TB/s (float32 heads of 32), 4.2 (of
+// 64) and 3.8 (bfloat16 heads of 32 and 64), where a large copy reaches 4.9; in heads of 128 the
+// chain of a chunk's loads, barriers and products, eight waves being all that 233 registers
+// leave a CU (3.1 TB/s bfloat16, 2.9 float32, there mostly float32 products). A chunk of 64
+// tokens takes a block of four waves 3.1 us alone on a CU and 4.1 beside another (bfloat16
+// heads of 64), of eight waves 6.5 (heads of 128). Chunks of 64 are one wave's reset mask and
+// two products' depth; float32's 32 keep a block's q, k, v and P below 56 KB of LDS.
 template <class T, int DK, int NW, bool kOut, bool kBack>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_of<T>(DK, NW)))) void chunk_kernel(Walks walks) {
   constexpr bool kHalf = sizeof(T) == 2;
