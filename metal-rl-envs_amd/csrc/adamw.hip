@@ -18,6 +18,10 @@ namespace adamw {
 constexpr int kQuant = 256;          // values that share one scale, and the grain of the flat moments
 constexpr int kTile = 1024;          // values a block takes: four quant blocks, one for each wave
 constexpr int kMaxTensors = 64;      // of one launch: its descriptors are kernel arguments, below 4 KiB
+// A launch's threads stay below 2^32, the most a grid's axis takes: a tensor goes in pieces of
+// kPiece values, at most kMostTiles tiles to a launch.
+constexpr int64_t kPiece = (int64_t)1 << 32;
+constexpr uint64_t kMostTiles = (uint64_t)1 << 23;
 constexpr uint32_t kParamBf16 = 1, kGradBf16 = 2, kWide = 4;
 
 struct Tensor {
@@ -247,9 +251,10 @@ __global__ __launch_bounds__(kBlock) void step8_kernel(Batch b, uint32_t* __rest
 __global__ __launch_bounds__(kBlock) void decode_kernel(const uint32_t* __restrict__ m_codes,
                                                         const uint32_t* __restrict__ v_codes,
                                                         const float* __restrict__ m_scales,
-                                                        const float* __restrict__ v_scales, int64_t words,
-                                                        float* __restrict__ m, float* __restrict__ v) {
-  const int64_t word = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+                                                        const float* __restrict__ v_scales, int64_t word0,
+                                                        int64_t words, float* __restrict__ m,
+                                                        float* __restrict__ v) {
+  const int64_t word = word0 + (int64_t)blockIdx.x * kBlock + threadIdx.x;
   if (word >= words) return;
   const int64_t block = word / (kQuant / 4);
   const uint32_t mc = m_codes[word], vc = v_codes[word];
@@ -308,20 +313,23 @@ extern "C" int hipenvs_adamw_step(int32_t bits, int32_t count, void* const* para
     return launch_status();
   };
   for (int32_t k = 0; k < count; ++k) {
-    const int64_t n = sizes[k];
-    if (n > 0 && grads[k]) {   // a tensor without a gradient keeps its parameters and its moments
-      const uint64_t own = (uint64_t)((n + kTile - 1) / kTile);
-      if (b.count == kMaxTensors || tiles + own > 0x7FFFFFFFu) {
-        const int status = launch();
+    const int64_t n = grads[k] ? sizes[k] : 0;   // a tensor without a gradient keeps its parameters and its moments
+    const int64_t p_size = (types[k] & 1) ? 2 : 4, g_size = (types[k] & 2) ? 2 : 4;
+    for (int64_t done = 0; done < n; done += kPiece) {
+      char* param = (char*)params[k] + done * p_size;
+      const char* grad = (const char*)grads[k] + done * g_size;
+      const int64_t own_n = n - done < kPiece ? n - done : kPiece;
+      const uint64_t own = (uint64_t)((own_n + kTile - 1) / kTile);
+      if (b.count == kMaxTensors || tiles + own > kMostTiles) {
+        const int status = b.count ? launch() : HIPENVS_OK;
         if (status != HIPENVS_OK) return status;
       }
-      const bool wide = moments_wide && aligned(params[k], (types[k] & 1) ? 8 : 16) &&
-                        aligned(grads[k], (types[k] & 2) ? 8 : 16);
-      b.t[b.count++] = {params[k], grads[k], n, at, (uint32_t)tiles, (uint32_t)types[k] | (wide ? kWide : 0u),
+      const bool wide = moments_wide && aligned(param, 4 * p_size) && aligned(grad, 4 * g_size);
+      b.t[b.count++] = {param, grad, own_n, at + done, (uint32_t)tiles, (uint32_t)types[k] | (wide ? kWide : 0u),
                         (float)rates[k], (float)roots[k]};
       tiles += own;
     }
-    at += (n + kQuant - 1) / kQuant * kQuant;
+    at += (sizes[k] + kQuant - 1) / kQuant * kQuant;
   }
   return b.count ? launch() : HIPENVS_OK;
 }
@@ -334,7 +342,13 @@ extern "C" int hipenvs_adamw_decode(const void* m_codes, const void* v_codes, co
   if (!m_codes || !v_codes || !m_scales || !v_scales || !m || !v) return HIPENVS_E_ARG;
   if (!aligned(m_codes, 4) || !aligned(v_codes, 4) || !aligned(m, 16) || !aligned(v, 16)) return HIPENVS_E_ARG;
   const int64_t words = blocks * (kQuant / 4);
-  hipLaunchKernelGGL(decode_kernel, dim3(grid_for(words)), dim3(kBlock), 0, as_stream(stream),
-                     (const uint32_t*)m_codes, (const uint32_t*)v_codes, m_scales, v_scales, words, m, v);
-  return launch_status();
+  constexpr int64_t kMostWords = (int64_t)1 << 30;
+  for (int64_t word0 = 0; word0 < words; word0 += kMostWords) {
+    const int64_t own = words - word0 < kMostWords ? words - word0 : kMostWords;
+    hipLaunchKernelGGL(decode_kernel, dim3(grid_for(own)), dim3(kBlock), 0, as_stream(stream),
+                       (const uint32_t*)m_codes, (const uint32_t*)v_codes, m_scales, v_scales, word0, words, m, v);
+    const int status = launch_status();
+    if (status != HIPENVS_OK) return status;
+  }
+  return HIPENVS_OK;
 }

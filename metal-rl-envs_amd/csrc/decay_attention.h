@@ -73,7 +73,11 @@ struct Walk {
   float* states;           // (b h, parts, dk, dv), or (b h, parts, dv, dk) when turned
   uint8_t* flags;          // (b h, parts): a reset in the part
   bool turned;
+  uint32_t row0;           // the first row of this launch
 };
+
+// Threads of a launch stay below 2^32, the most a grid's axis takes.
+constexpr int64_t kMostThreads = 0xFFFFFFFFll;
 
 // One walk, or two of the same kind over the same rows: their blocks for a row lie side by side
 // on one XCD and read what they share (q and dout, for the gradients of k and v) once.
@@ -314,7 +318,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
   const uint32_t at = blocks % 8 == 0 ? (blockIdx.x % 8) * (blocks / 8) + blockIdx.x / 8 : blockIdx.x;
   const uint32_t id = walks.count == 2 ? at / 2 : at;
   const Walk& w = walks.w[walks.count == 2 ? at % 2 : 0];
-  const uint32_t row = id / (uint32_t)w.parts, part = id - row * (uint32_t)w.parts;
+  const uint32_t piece = id / (uint32_t)w.parts, part = id - piece * (uint32_t)w.parts, row = w.row0 + piece;
   const int64_t b = row / (uint32_t)w.h, h = row - (uint32_t)b * (uint32_t)w.h;
   const int64_t t0 = part * w.part, t1 = t0 + w.part < w.t ? t0 + w.part : w.t;
   const int chunks = (int)((t1 - t0 + C - 1) / C);
@@ -773,18 +777,24 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
 }
 
 template <class T, int DK, int NW>
-int launch_sized(const Walks& walks, bool out, hipStream_t s) {
+int launch_sized(Walks walks, bool out, hipStream_t s) {
   const Walk& w = walks.w[0];
-  const dim3 grid((unsigned)(w.b * w.h * w.parts * walks.count)), block(64 * NW);
-  if (out && w.backwards)
-    hipLaunchKernelGGL((chunk_kernel<T, DK, NW, true, true>), grid, block, 0, s, walks);
-  else if (out)
-    hipLaunchKernelGGL((chunk_kernel<T, DK, NW, true, false>), grid, block, 0, s, walks);
-  else if (w.backwards)
-    hipLaunchKernelGGL((chunk_kernel<T, DK, NW, false, true>), grid, block, 0, s, walks);
-  else
-    hipLaunchKernelGGL((chunk_kernel<T, DK, NW, false, false>), grid, block, 0, s, walks);
-  return launch_status();
+  const int64_t rows = w.b * w.h, per = (int64_t)w.parts * walks.count, most = kMostThreads / (64 * NW) / per;
+  for (int64_t row0 = 0; row0 < rows; row0 += most) {
+    walks.w[0].row0 = walks.w[1].row0 = (uint32_t)row0;
+    const dim3 grid((unsigned)((rows - row0 < most ? rows - row0 : most) * per)), block(64 * NW);
+    if (out && w.backwards)
+      hipLaunchKernelGGL((chunk_kernel<T, DK, NW, true, true>), grid, block, 0, s, walks);
+    else if (out)
+      hipLaunchKernelGGL((chunk_kernel<T, DK, NW, true, false>), grid, block, 0, s, walks);
+    else if (w.backwards)
+      hipLaunchKernelGGL((chunk_kernel<T, DK, NW, false, true>), grid, block, 0, s, walks);
+    else
+      hipLaunchKernelGGL((chunk_kernel<T, DK, NW, false, false>), grid, block, 0, s, walks);
+    const int status = launch_status();
+    if (status != HIPENVS_OK) return status;
+  }
+  return HIPENVS_OK;
 }
 
 // The kernel that takes dk rows and dv columns of a state: its rows, and its waves.

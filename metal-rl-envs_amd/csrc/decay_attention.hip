@@ -85,13 +85,14 @@ struct Step {
   void* out;      // (n, h, dv) contiguous
   float scale;
   int32_t h, dk, dv;
+  int64_t item0;  // the first state of this launch
 };
 
 template <class T>
 __global__ __launch_bounds__(kBlock) void step_kernel(Step s) {
   typedef f32x4 __attribute__((aligned(4))) four;
   __shared__ __attribute__((aligned(16))) float share[kBlock * 4];
-  const int64_t item = blockIdx.x, n = item / s.h, h = item - n * s.h;
+  const int64_t item = s.item0 + blockIdx.x, n = item / s.h, h = item - n * s.h;
   const int L = (s.dv + 3) / 4, R = kBlock / L;
   const int r0 = threadIdx.x / L, c = (threadIdx.x - r0 * L) * 4;
   const int left = s.dv - c;   // values of the row from c on
@@ -251,7 +252,7 @@ extern "C" int hipenvs_decay_attention(int32_t dtype, const void* q, const void*
   int64_t need = 0;
   const int status = plan(dtype, b, t, h, dk, dv, workspace, &w, &need);
   if (status != HIPENVS_OK) return status;
-  if (need > 0 && (!workspace || workspace_bytes < need)) return HIPENVS_E_ARG;
+  if (need > 0 && (!workspace || ((uintptr_t)workspace & 3) || workspace_bytes < need)) return HIPENVS_E_ARG;
   w.q = rows(q, st), w.k = rows(k, st + 3), w.v = rows(v, st + 6);
   w.dk = dk, w.dv = dv, w.log_decay = log_decay, w.reset = reset, w.reset_sb = st[9], w.reset_st = st[10];
   w.state_in = state, w.state_out = final_state, w.exact = true, w.read = scale, w.add = 1.0f;
@@ -276,7 +277,7 @@ extern "C" int hipenvs_decay_attention_backward(int32_t dtype, const void* q, co
   int64_t need = 0;
   int status = plan(dtype, b, t, h, dk, dv, workspace, &w, &need);
   if (status != HIPENVS_OK) return status;
-  if (need > 0 && (!workspace || workspace_bytes < need)) return HIPENVS_E_ARG;
+  if (need > 0 && (!workspace || ((uintptr_t)workspace & 3) || workspace_bytes < need)) return HIPENVS_E_ARG;
   float* own_states = w.states;
   const Rows rq = rows(q, st), rk = rows(k, st + 3), rv = rows(v, st + 6),
              rdo = rows(dout, st + 9);
@@ -318,12 +319,17 @@ extern "C" int hipenvs_decay_attention_step(int32_t dtype, const void* q, int64_
   if (!dims_ok(dtype, h, dk, dv) || n < 0 || n > 0x7FFFFFFF || n * h > 0x7FFFFFFF) return HIPENVS_E_ARG;
   if (n == 0) return HIPENVS_OK;
   if (!q || !k || !v || !log_decay || !state || !out || !next_state) return HIPENVS_E_ARG;
-  const Step s = {{q, q_sn, 0, q_sh}, {k, k_sn, 0, k_sh}, {v, v_sn, 0, v_sh}, log_decay, reset, reset_sn,
-                  state, next_state, out, scale, h, dk, dv};
-  const dim3 grid((unsigned)(n * h)), block(kBlock);
-  if (dtype == 1)
-    hipLaunchKernelGGL(step_kernel<__bf16>, grid, block, 0, as_stream(stream), s);
-  else
-    hipLaunchKernelGGL(step_kernel<float>, grid, block, 0, as_stream(stream), s);
-  return launch_status();
+  Step s = {{q, q_sn, 0, q_sh}, {k, k_sn, 0, k_sh}, {v, v_sn, 0, v_sh}, log_decay, reset, reset_sn,
+            state, next_state, out, scale, h, dk, dv, 0};
+  const int64_t items = n * h, most = kMostThreads / kBlock;
+  for (s.item0 = 0; s.item0 < items; s.item0 += most) {
+    const dim3 grid((unsigned)(items - s.item0 < most ? items - s.item0 : most)), block(kBlock);
+    if (dtype == 1)
+      hipLaunchKernelGGL(step_kernel<__bf16>, grid, block, 0, as_stream(stream), s);
+    else
+      hipLaunchKernelGGL(step_kernel<float>, grid, block, 0, as_stream(stream), s);
+    const int status = launch_status();
+    if (status != HIPENVS_OK) return status;
+  }
+  return HIPENVS_OK;
 }

@@ -311,6 +311,12 @@ def test_a_tensor_past_32_bits(dev):
     adamw.step([short_p], [short_g], adamw.init([short_p], 8), 1, lr=0.1)
     assert torch.equal(p[:1025], short_p) and torch.equal(p[-1025:], short_p)
     assert int(moments[0][1 << 20]) == 0 and float(p[1 << 31]) == float(p[1 << 22])
+    m, v = adamw.decode(moments)
+    short = adamw.init([short_p], 8)
+    adamw.step([short_p], [short_g], short, 1, lr=0.1)
+    for x, y in zip((m, v), adamw.decode(short)):   # the last 1025 values share their blocks' scale with zeros
+        assert torch.equal(x[:1025], y[:1025]) and torch.equal(x[-1280:][:1025], x[n - 1025:n])
+    assert m[n - 1025:n].abs().max() == m[:1025].abs().max() and not m[1 << 31:(1 << 31) + 4096].any()
 
 
 def test_refusals_on_the_device(dev):
@@ -331,3 +337,25 @@ def test_refusals_on_the_device(dev):
         with pytest.raises(TypeError):
             bad()
     adamw.step([], [], (), 1)
+
+
+def test_a_captured_step(dev):
+    """adamw.step in a graph (its step number the captured one), replayed with new gradients and the
+    program's own work between, against the same calls made eagerly."""
+    from hipenvs import adamw
+
+    for bits in (32, 8):
+        params, grads = tensors(dev, 11)
+        twin = [p.clone() for p in params]
+        a, b = adamw.init(params, bits), adamw.init(params, bits)
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            adamw.step(params, grads, a, 7, **HYPER)
+        for k in range(4):
+            for g in grads:
+                g.mul_(-0.8 - 0.1 * k)
+            graph.replay()
+            torch.cuda.synchronize()
+            adamw.step(twin, grads, b, 7, **HYPER)
+            assert all(torch.equal(x, y) for x, y in zip((*params, *a), (*twin, *b))), (bits, k)

@@ -543,3 +543,34 @@ def test_a_second_derivative_is_refused(dev):
     assert torch.equal(once.detach(), plain)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(once.sum(), q)
+
+
+def test_more_states_than_a_launch_takes(dev):
+    """17 million states of 1 x 1 a step, and 34 million rows of one token with their gradients: more
+    threads than one grid holds. o = q (lambda s + k v), and the products' derivatives."""
+    from hipenvs import decay_attention
+
+    n = 17_000_011
+    gen = torch.Generator(device=dev)
+    gen.manual_seed(1)
+
+    def draw(count, *shape):
+        return torch.randn(count, *shape, generator=gen, device=dev)
+
+    ld = torch.zeros(1, device=dev)
+    q, k, v, s = draw(n, 1, 1), draw(n, 1, 1), draw(n, 1, 1), draw(n, 1, 1, 1)
+    out, nxt = decay_attention.step(q, k, v, ld, s, scale=1.0)
+    want = s.flatten() + k.flatten() * v.flatten()
+    assert torch.allclose(nxt.flatten(), want, rtol=1e-6, atol=1e-6)
+    assert torch.allclose(out.flatten(), q.flatten() * want, rtol=1e-5, atol=1e-5)
+
+    n = 34_000_003
+    q, k, v = (draw(n, 1, 1, 1).requires_grad_() for _ in range(3))
+    s = draw(n, 1, 1, 1).requires_grad_()
+    out, final = decay_attention.sequence(q, k, v, ld, s, scale=1.0)
+    do = draw(n, 1, 1, 1)
+    grads = torch.autograd.grad(out, (q, k, v, s), do)
+    with torch.no_grad():
+        state = s + k * v
+        for x, y in zip((out, final, *grads), (q * state, state, do * state, do * q * v, do * q * k, do * q)):
+            assert torch.allclose(x, y, rtol=1e-5, atol=1e-5)
