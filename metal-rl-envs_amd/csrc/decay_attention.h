@@ -309,7 +309,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
   __shared__ __attribute__((aligned(16))) T Qs[kOut ? C * SQ : 8];
   __shared__ __attribute__((aligned(16))) T Ks[C * SQ];
   __shared__ __attribute__((aligned(16))) T Vs[C * SV];
-  __shared__ __attribute__((aligned(16))) T Ps[kOut ? (kHalf ? 2 : 1) * C * SP : 8];
+  // Where dv <= 16 the block is one wave, which has all of P, and P's tiles are operands as they lie
+  // in its registers: no copy in shared memory, no wait for it, and the smaller block (17.7 kB, not
+  // 36, in bf16 with dk = 32) runs more often per CU. 2^24 values of q, k and v by 16 x 16 heads,
+  // 128 tokens: bf16 106 -> 51 us, with gradients 413 -> 204; f32 108 -> 75 and 376 -> 277; at
+  // dk = 128 50 -> 39 and 77 -> 49. With more waves each has a share of P only and reads the rest.
+  constexpr bool kOwnP = NW == 1;
+  __shared__ __attribute__((aligned(16))) T Ps[kOut && !kOwnP ? (kHalf ? 2 : 1) * C * SP : 8];
   __shared__ float pw[C + 1];
 
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, l = lane & 15;
@@ -424,9 +430,15 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
   // the tiles beside the diagonal are among them, with decays of zero.
   constexpr int kPairs = kHalf ? 12 : 4, kOwn = (kPairs + NW - 1) / NW;
   const auto pair_of = [&](int x) {
-    const int y = wave + NW * x;
+    const int y = kOwnP ? x : wave + NW * x;
     const int it = y < 4 ? y >> 1 : y < 8 ? 2 : 3, jt = y < 4 ? y & 1 : y & 3;
     return kBack ? make_int2(NT - 1 - it, NT - 1 - jt) : make_int2(it, jt);
+  };
+
+  // and the other way round, where one wave has them all
+  const auto own_of = [](int it, int jt) {
+    const int i = kBack ? NT - 1 - it : it, j = kBack ? NT - 1 - jt : jt;
+    return i < 2 ? 2 * i + j : 4 * (i - 1) + j;
   };
 
   // The decays of a whole chunk. of_pair[x][r]: of tile x of P, zero where the key is not yet
@@ -522,6 +534,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
     if (step + 1 < chunks) load(!kBack && step + 2 == chunks ? tokens_of_last : C);
 
     f32x4 o[kOut ? NT : 1];
+    bf16x4 own_p[kOut && kOwnP && kHalf ? kOwn : 1][2];
+    f32x4 own_f[kOut && kOwnP && !kHalf ? kOwn : 1];
     if constexpr (kOut) {
       f32x4 p[kOwn];
 #pragma unroll
@@ -573,8 +587,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
           float rest[4] = {p[x][0], p[x][1], p[x][2], p[x][3]};
           __bf16 of[2][4];
           split(rest, of);
-          *(bf16x4*)to = __builtin_bit_cast(bf16x4, of[0]);
-          *(bf16x4*)(to + C * SP) = __builtin_bit_cast(bf16x4, of[1]);
+          if constexpr (kOwnP) {
+            own_p[x][0] = __builtin_bit_cast(bf16x4, of[0]), own_p[x][1] = __builtin_bit_cast(bf16x4, of[1]);
+          } else {
+            *(bf16x4*)to = __builtin_bit_cast(bf16x4, of[0]);
+            *(bf16x4*)(to + C * SP) = __builtin_bit_cast(bf16x4, of[1]);
+          }
+        } else if constexpr (kOwnP) {
+          own_f[x] = p[x];
         } else {
           *(f32x4*)to = p[x];
         }
@@ -639,7 +659,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
           }
         }
       }
-      __syncthreads();
+      if constexpr (!kOwnP) __syncthreads();
     }
     if (idle) continue;
 
@@ -662,8 +682,16 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
           for (int it = 0; it < NT; ++it)
             if (kBack ? 2 * s + 1 >= it : 2 * s <= it) {
               const T* p = Ps + (16 * it + l) * SP + 32 * s + 4 * g;
-              o[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vh[s], read_pair(p), o[it], 0, 0, 0);
-              o[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vh[s], read_pair(p + C * SP), o[it], 0, 0, 0);
+#pragma unroll
+              for (int m = 0; m < 2; ++m) {
+                bf16x8 pf;
+                if constexpr (kOwnP)
+                  pf = __builtin_shufflevector(own_p[own_of(it, 2 * s)][m], own_p[own_of(it, 2 * s + 1)][m], 0, 1, 2, 3,
+                                               4, 5, 6, 7);
+                else
+                  pf = read_pair(p + m * C * SP);
+                o[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vh[s], pf, o[it], 0, 0, 0);
+              }
             }
       } else {
 #pragma unroll
@@ -671,7 +699,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
 #pragma unroll
           for (int it = 0; it < NT; ++it)
             if (kBack ? t >= it : t <= it) {
-              const f32x4 p = *(const f32x4*)(Ps + (16 * it + l) * SP + 16 * t + 4 * g);
+              f32x4 p;
+              if constexpr (kOwnP)
+                p = own_f[own_of(it, t)];
+              else
+                p = *(const f32x4*)(Ps + (16 * it + l) * SP + 16 * t + 4 * g);
 #pragma unroll
               for (int e = 0; e < 4; ++e)
                 o[it] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[4 * t + e], p[e], o[it], 0, 0, 0);

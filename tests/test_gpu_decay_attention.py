@@ -136,6 +136,38 @@ def test_many_short_rows(dev, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dk, dv", [(9, 16), (16, 8), (40, 16), (96, 1), (128, 16), (16, 100)])
+def test_a_narrow_side(dev, dk, dv, dtype):
+    """Keys or values of at most 16 columns, whose walks have blocks of one wave: short, with a
+    ragged end, and long enough for parts."""
+    for b, t, episode in ((3, 95, 0), (2, 161, 11), (1, 2500, 400)):
+        c = case(dev, 12, b, t, 2, dk, dv, dtype, "fused", episode)
+        check_forward(c)
+        check_backward(c)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_bad_values_of_narrow_heads(dev, dtype):
+    """A NaN in a value row stays within its episode and its column; nothing before it changes."""
+    from hipenvs import decay_attention
+
+    c = case(dev, 13, 2, 200, 2, 32, 16, dtype, "apart", 0)
+    c["reset"] = torch.zeros(2, 200, dtype=torch.bool, device=dev)
+    c["reset"][:, 90] = c["reset"][:, 150] = True
+    spoilt = {**c, "v": c["v"].clone()}
+    spoilt["v"][0, 100, 1, 5] = float("nan")
+    out, final = decay_attention.sequence(**spoilt)
+    touched = torch.zeros(2, 200, 2, 16, dtype=torch.bool, device=dev)
+    touched[0, 100:150, 1, 5] = True
+    assert torch.isnan(out[touched]).all()
+    args = [to_np(c[n]) for n in ("q", "k", "v", "log_decay", "state", "reset")]
+    want, size = oda.sequence(*args, 32 ** -0.5), oda.magnitudes(*args, 32 ** -0.5)
+    mask = touched.cpu().numpy()
+    close(out[~touched], want[0][~mask], size[0][~mask], dtype, 200, 32, 16)
+    close(final, want[1], size[1], F32, 200, 32, 16)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_only_one_of_the_results_is_used(dev, dtype):
     c = case(dev, 6, 2, 100, 2, 32, 32, dtype, "apart", 30)
     check_backward(c, use_final=False)
