@@ -314,8 +314,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
   // 36, in bf16 with dk = 32) runs more often per CU. 2^24 values of q, k and v by 16 x 16 heads,
   // 128 tokens: bf16 106 -> 51 us, with gradients 413 -> 204; f32 108 -> 75 and 376 -> 277; at
   // dk = 128 50 -> 39 and 77 -> 49. With more waves each has a share of P only and reads the rest:
-  // two that make all of P each gain and lose up to 7 % by shape, and spill at dk = 128 in bf16
-  // (45 -> 74 us).
+  // two that make all of P each take 21 % less to 9 % more by shape and length, and spill at
+  // dk = 128 in bf16 (45 -> 74 us).
   constexpr bool kOwnP = NW == 1;
   __shared__ __attribute__((aligned(16))) T Ps[kOut && !kOwnP ? (kHalf ? 2 : 1) * C * SP : 8];
   __shared__ float pw[C + 1];
