@@ -61,7 +61,6 @@ struct Walk {
   const float* state_in;   // (b, h, dk, dv), or (b, h, dv, dk) when flipped; null: zeros
   float* state_out;        // null: not wanted
   bool flipped, backwards;
-  bool exact;              // the state is wanted in float32 to its last bits
   float read, add;
   void* out;               // (b, t, h, dv) contiguous
   int64_t b, t;
@@ -168,6 +167,18 @@ struct Chunk<float> {
   static constexpr int pad(int) { return 4; }
 };
 
+// What P is stored as: float32, or T's parts.
+template <bool kSplit, class T>
+struct Stored {
+  typedef float type;
+  static constexpr int kPad = Chunk<float>::pad(0);
+};
+template <class T>
+struct Stored<true, T> {
+  typedef T type;
+  static constexpr int kPad = Chunk<T>::pad(Chunk<T>::kTokens);
+};
+
 // 16 bytes at any address that is a multiple of the value's size.
 typedef u32x4 __attribute__((aligned(2))) piece_at_2;
 template <class T>
@@ -251,11 +262,13 @@ __device__ __forceinline__ int here(int x) {
   return x;
 }
 
-// The bfloat16 parts of N (even) float32 values: of each, the rounding of what is left.
-template <int M, int N>
-__device__ __forceinline__ void split(float (&rest)[N], __bf16 (&parts)[M][N]) {
+// The bfloat16 parts of N (even) float32 values: of each, the rounding of what is left. Three
+// parts of 8 bits hold all 24.
+constexpr int kParts = 3;
+template <int N>
+__device__ __forceinline__ void split(float (&rest)[N], __bf16 (&parts)[kParts][N]) {
 #pragma unroll
-  for (int m = 0; m < M; ++m)
+  for (int m = 0; m < kParts; ++m)
 #pragma unroll
     for (int e = 0; e < N; e += 2) {
       const f32x2 x = {rest[e], rest[e + 1]};
@@ -286,24 +299,24 @@ constexpr int power_of_two(int n) {   // the least that is not below n
 // P[i][j], computed once.
 //
 // bfloat16 rows: the inputs are exact operands. P, the S that is read and the lambda^n v_j that
-// is added are float32, split for the matrix instructions into bfloat16 parts, each the
-// rounding of what the parts before it leave: two parts for P and S (16 bits, so a result's
-// error is that of its own rounding to bfloat16) and for what enters a state that only results
-// are read from, three for one that is a float32 result itself (all 24 bits). float32 rows
-// use the float32 matrix instructions throughout.
+// is added are float32, split for the matrix instructions into three bfloat16 parts, each the
+// rounding of what the parts before it leave: all 24 bits, so nothing but a result is rounded to
+// fewer. float32 rows use the float32 matrix instructions throughout.
 //
-// What bounds it: with many rows of 128 tokens memory, at 4.7 TB/s (float32 heads of 32), 4.2 (of
-// 64) and 3.8 (bfloat16 heads of 32 and 64), where a large copy reaches 4.9; in heads of 128 the
-// chain of a chunk's loads, barriers and products, eight waves being all that 233 registers
-// leave a CU (3.1 TB/s bfloat16, 2.9 float32, there mostly float32 products). A chunk of 64
-// tokens takes a block of four waves 3.1 us alone on a CU and 4.1 beside another (bfloat16
-// heads of 64), of eight waves 6.5 (heads of 128). Chunks of 64 are one wave's reset mask and
+// What bounds it: with many rows of 128 tokens memory, at 4.8 TB/s (float32 heads of 32), 4.3 (of
+// 64), 3.6 and 3.8 (bfloat16 heads of 32 and 64), where a large copy reaches 4.9; in heads of 128 the
+// chain of a chunk's loads, barriers and products, eight waves being all that 239 registers
+// leave a CU (3.2 TB/s bfloat16, 3.0 float32, there mostly float32 products). A chunk of 64
+// tokens takes a block of four waves 3.4 us alone on a CU and 4.2 beside another (bfloat16
+// heads of 64), of eight waves 5.8 (heads of 128). Parts of 24 bits, where two (16 bits) would be
+// within a result's own rounding, cost 1 to 13 % (sequence of 8 heads of 64 x 16,381 41.7 -> 43.5 us,
+// 512 rows of 1,000 with gradients 272 -> 294). Chunks of 64 are one wave's reset mask and
 // two products' depth; float32's 32 keep a block's q, k, v and P below 56 KB of LDS.
 template <class T, int DK, int NW, bool kOut, bool kBack>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_of<T>(DK, NW)))) void chunk_kernel(Walks walks) {
   constexpr bool kHalf = sizeof(T) == 2;
   constexpr int C = Chunk<T>::kTokens, E = 16 / sizeof(T), TH = 64 * NW, DV = 16 * NW, NT = C / 16;
-  constexpr int SQ = DK + Chunk<T>::pad(DK), SV = DV + Chunk<T>::pad(DV), SP = C + Chunk<T>::pad(C);
+  constexpr int SQ = DK + Chunk<T>::pad(DK), SV = DV + Chunk<T>::pad(DV);
   constexpr int QP = power_of_two(DK / E), VP = power_of_two(DV / E);      // pieces of a row, rounded up
   constexpr int NQ = (C * QP + TH - 1) / TH, NV = (C * VP + TH - 1) / TH;  // pieces of a thread
   __shared__ __attribute__((aligned(16))) T Qs[kOut ? C * SQ : 8];
@@ -311,13 +324,21 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
   __shared__ __attribute__((aligned(16))) T Vs[C * SV];
   // Where dv <= 16 the block is one wave, which has all of P, and P's tiles are operands as they lie
   // in its registers: no copy in shared memory, no wait for it, and the smaller block (17.7 kB, not
-  // 36, in bf16 with dk = 32) runs more often per CU. 2^24 values of q, k and v by 16 x 16 heads,
-  // 128 tokens: bf16 106 -> 51 us, with gradients 413 -> 204; f32 108 -> 75 and 376 -> 277; at
-  // dk = 128 50 -> 39 and 77 -> 49. With more waves each has a share of P only and reads the rest:
-  // two that make all of P each take 21 % less to 9 % more by shape and length, and spill at
-  // dk = 128 in bf16 (45 -> 74 us).
+  // 45, in bf16 with dk = 32) runs more often per CU. 2^24 values of q, k and v by 16 x 16 heads,
+  // 128 tokens: bf16 145 -> 55 us, with gradients 588 -> 217; f32 113 -> 76 and 376 -> 287; at
+  // dk = 128 56 -> 41 and 75 -> 48. With more waves each has a share of P only and reads the rest:
+  // two that make all of P each took 21 % less to 9 % more by shape and length (bf16 in two parts),
+  // and spilled at dk = 128 in bf16 (45 -> 74 us).
   constexpr bool kOwnP = NW == 1;
-  __shared__ __attribute__((aligned(16))) T Ps[kOut && !kOwnP ? (kHalf ? 2 : 1) * C * SP : 8];
+  // bfloat16's parts of P are made once, by the wave that made its tile, but in blocks of two waves
+  // and at most 32 rows: these read P as float32 and split it themselves, so that four of them fit a CU's
+  // LDS (39 kB, not 49). 32 x 32 heads, 2^24 values each of q, k and v, 128 tokens: 58 us, not 67,
+  // with gradients 213, not 256; 1,000 tokens 66, not 64, and 237, not 248. With more rows three fit
+  // either way (64 x 32: 50 and 49 us).
+  constexpr bool kSplitP = kHalf && !kOwnP && !(NW == 2 && DK == 32);
+  typedef Stored<kSplitP, T> P;
+  constexpr int SP = C + P::kPad, kPs = kSplitP ? kParts : 1;
+  __shared__ __attribute__((aligned(16))) typename P::type Ps[kOut && !kOwnP ? kPs * C * SP : 8];
   __shared__ float pw[C + 1];
 
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, l = lane & 15;
@@ -503,7 +524,6 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
   };
 
   const bool idle = 16 * wave >= w.dv;   // no columns: this wave only moves and shares
-  const bool exact = w.exact;
   uint64_t any = 0;
   float bad = 0.0f;   // becomes NaN with the first value that is not finite
   for (int step = 0; step < chunks; ++step) {
@@ -536,8 +556,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
     if (step + 1 < chunks) load(!kBack && step + 2 == chunks ? tokens_of_last : C);
 
     f32x4 o[kOut ? NT : 1];
-    bf16x4 own_p[kOut && kOwnP && kHalf ? kOwn : 1][2];
-    f32x4 own_f[kOut && kOwnP && !kHalf ? kOwn : 1];
+    f32x4 own_p[kOut && kOwnP ? kOwn : 1];
     if constexpr (kOut) {
       f32x4 p[kOwn];
 #pragma unroll
@@ -584,19 +603,15 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
       for (int x = 0; x < kOwn; ++x) {
         const int2 tile = pair_of(x);
         if (kPairs % NW != 0 && wave + NW * x >= kPairs) break;
-        T* to = Ps + (16 * tile.x + l) * SP + 16 * tile.y + 4 * g;
-        if constexpr (kHalf) {
+        typename P::type* to = Ps + (16 * tile.x + l) * SP + 16 * tile.y + 4 * g;
+        if constexpr (kOwnP) {
+          own_p[x] = p[x];
+        } else if constexpr (kSplitP) {
           float rest[4] = {p[x][0], p[x][1], p[x][2], p[x][3]};
-          __bf16 of[2][4];
+          __bf16 of[kParts][4];
           split(rest, of);
-          if constexpr (kOwnP) {
-            own_p[x][0] = __builtin_bit_cast(bf16x4, of[0]), own_p[x][1] = __builtin_bit_cast(bf16x4, of[1]);
-          } else {
-            *(bf16x4*)to = __builtin_bit_cast(bf16x4, of[0]);
-            *(bf16x4*)(to + C * SP) = __builtin_bit_cast(bf16x4, of[1]);
-          }
-        } else if constexpr (kOwnP) {
-          own_f[x] = p[x];
+#pragma unroll
+          for (int m = 0; m < kParts; ++m) *(bf16x4*)(to + m * C * SP) = __builtin_bit_cast(bf16x4, of[m]);
         } else {
           *(f32x4*)to = p[x];
         }
@@ -608,7 +623,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
 #pragma unroll
           for (int a = 0; a < DK / 32; ++a) {
             float rest[8];
-            __bf16 of[2][8];
+            __bf16 of[kParts][8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) rest[e] = S[2 * a + e / 4][e % 4];
             split(rest, of);
@@ -616,9 +631,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
             for (int it = 0; it < NT; ++it) {
               const bf16x8 qf = read_pair(Qs + (16 * it + l) * SQ + 32 * a + 4 * g);
               const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-              o[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, of[0]), qf,
-                                                              a == 0 ? zero : o[it], 0, 0, 0);
-              o[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, of[1]), qf, o[it], 0, 0, 0);
+#pragma unroll
+              for (int m = 0; m < kParts; ++m)
+                o[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, of[m]), qf,
+                                                                a == 0 && m == 0 ? zero : o[it], 0, 0, 0);
             }
           }
         } else {
@@ -683,15 +699,28 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
 #pragma unroll
           for (int it = 0; it < NT; ++it)
             if (kBack ? 2 * s + 1 >= it : 2 * s <= it) {
-              const T* p = Ps + (16 * it + l) * SP + 32 * s + 4 * g;
+              const typename P::type* p = Ps + (16 * it + l) * SP + 32 * s + 4 * g;
+              __bf16 of[kParts][8];
+              if constexpr (!kSplitP) {
+                float rest[8];
 #pragma unroll
-              for (int m = 0; m < 2; ++m) {
+                for (int e = 0; e < 8; e += 4) {
+                  f32x4 four;
+                  if constexpr (kOwnP)
+                    four = own_p[own_of(it, 2 * s + e / 4)];
+                  else
+                    four = *(const f32x4*)(p + 4 * e);
+                  rest[e] = four[0], rest[e + 1] = four[1], rest[e + 2] = four[2], rest[e + 3] = four[3];
+                }
+                split(rest, of);
+              }
+#pragma unroll
+              for (int m = 0; m < kParts; ++m) {
                 bf16x8 pf;
-                if constexpr (kOwnP)
-                  pf = __builtin_shufflevector(own_p[own_of(it, 2 * s)][m], own_p[own_of(it, 2 * s + 1)][m], 0, 1, 2, 3,
-                                               4, 5, 6, 7);
-                else
+                if constexpr (kSplitP)
                   pf = read_pair(p + m * C * SP);
+                else
+                  pf = __builtin_bit_cast(bf16x8, of[m]);
                 o[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vh[s], pf, o[it], 0, 0, 0);
               }
             }
@@ -703,7 +732,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
             if (kBack ? t >= it : t <= it) {
               f32x4 p;
               if constexpr (kOwnP)
-                p = own_f[own_of(it, t)];
+                p = own_p[own_of(it, t)];
               else
                 p = *(const f32x4*)(Ps + (16 * it + l) * SP + 16 * t + 4 * g);
 #pragma unroll
@@ -743,7 +772,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
 #pragma unroll
       for (int s = 0; s < C / 32; ++s) {
         float rest[8];
-        __bf16 of[2][8];
+        __bf16 of[kParts][8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) rest[e] = (float)vh[s][e] * add[8 * s + e];
         split(rest, of);
@@ -751,17 +780,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_o
 #pragma unroll
         for (int a = 0; a < DK / 16; ++a) kf[a] = read_columns(Ks, SQ, 32 * s + 4 * g, 16 * a);
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int m = 0; m < kParts; ++m)
 #pragma unroll
           for (int a = 0; a < DK / 16; ++a)
             S[a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[a], __builtin_bit_cast(bf16x8, of[m]), S[a], 0, 0, 0);
-        if (exact) {
-          __bf16 least[1][8];
-          split(rest, least);
-#pragma unroll
-          for (int a = 0; a < DK / 16; ++a)
-            S[a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[a], __builtin_bit_cast(bf16x8, least[0]), S[a], 0, 0, 0);
-        }
       }
     } else {
 #pragma unroll

@@ -169,10 +169,10 @@ int launch(int32_t dtype, const Walks& walks, bool out, hipStream_t s) {
 // A block walks a row, or a part of one where the rows are too few to fill the card: then a first
 // pass leaves each part's own state, the second joins them, the third walks every part from
 // the state before it. The card is full at eight waves a CU: two blocks of four waves take
-// 4.1 us a chunk where one takes 3.1 (bfloat16 heads of 64), two of eight waves as long as one
-// after the other (heads of 128: 209 us at 512 rows, 106 at 256). As many parts as fill it
-// once are the fastest (32 rows of 8,192 tokens in heads of 128: 148 us in 8 parts, 165 in
-// 16, 645 in one; 8 rows of 16,381 in heads of 64: 44 us in 64 parts, 77 in 16), of two
+// 4.2 us a chunk where one takes 3.4 (bfloat16 heads of 64), two of eight waves as long as one
+// after the other (heads of 128: 228 us at 512 rows, 117 at 256). As many parts as fill it
+// once are the fastest (32 rows of 8,192 tokens in heads of 128: 158 us in 8 parts, 173 in
+// 16, 724 in one; 8 rows of 16,381 in heads of 64: 46 us in 64 parts, 81 in 16), of two
 // chunks at least, where they save more than the passes cost: the first pass takes about 0.45 of
 // the third, joining and launching about five chunks.
 int divide(int32_t dtype, int64_t rows, int64_t t, int32_t widest, int32_t* parts, int64_t* part) {
@@ -255,7 +255,7 @@ extern "C" int hipenvs_decay_attention(int32_t dtype, const void* q, const void*
   if (need > 0 && (!workspace || ((uintptr_t)workspace & 3) || workspace_bytes < need)) return HIPENVS_E_ARG;
   w.q = rows(q, st), w.k = rows(k, st + 3), w.v = rows(v, st + 6);
   w.dk = dk, w.dv = dv, w.log_decay = log_decay, w.reset = reset, w.reset_sb = st[9], w.reset_st = st[10];
-  w.state_in = state, w.state_out = final_state, w.exact = true, w.read = scale, w.add = 1.0f;
+  w.state_in = state, w.state_out = final_state, w.read = scale, w.add = 1.0f;
   w.out = out, w.b = b, w.t = t, w.h = h;
   const int walked = launch_states(dtype, w, as_stream(stream));
   return walked == HIPENVS_OK ? launch(dtype, {{w, w}, 1}, true, as_stream(stream)) : walked;
@@ -297,14 +297,14 @@ extern "C" int hipenvs_decay_attention_backward(int32_t dtype, const void* q, co
   status = launch(dtype, {{w, w}, 1}, true, s);
   if (status != HIPENVS_OK) return status;
   // dv, and the gradient of the first state: backwards over the states' gradients
-  w.q = rk, w.k = rq, w.v = rdo, w.dk = dk, w.dv = dv, w.state_in = dfinal, w.state_out = dstate, w.exact = true;
+  w.q = rk, w.k = rq, w.v = rdo, w.dk = dk, w.dv = dv, w.state_in = dfinal, w.state_out = dstate;
   w.states = own_states, w.turned = false;
   w.flipped = false, w.backwards = true, w.read = 1.0f, w.add = scale, w.out = dv_out;
   status = launch_states(dtype, w, s);
   if (status != HIPENVS_OK) return status;
   // dk: the same, transposed
   Walk u = w;
-  u.q = rv, u.k = rdo, u.v = rq, u.dk = dv, u.dv = dk, u.state_out = nullptr, u.exact = false, u.flipped = true;
+  u.q = rv, u.k = rdo, u.v = rq, u.dk = dv, u.dv = dk, u.state_out = nullptr, u.flipped = true;
   u.turned = true, u.out = dk_out;
   if (rows_of(dk) == rows_of(dv) && waves_for(dk) == waves_for(dv)) return launch(dtype, {{w, u}, 2}, true, s);
   status = launch(dtype, {{w, w}, 1}, true, s);
