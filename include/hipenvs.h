@@ -392,7 +392,7 @@ int hipenvs_decay_attention(int32_t dtype, const void* q, const void* k, const v
 
 /* Gradients of the above: dout like out with strides of its own, dfinal (b, h, dk, dv) f32
  * contiguous or NULL (zeros); states: the workspace that hipenvs_decay_attention was given for
- * these inputs, as it left it, or NULL (computed again; also where its size is 0) -> dq, dk_out, dv_out (b, t, h, dk or dv) contiguous in dtype,
+ * these inputs, as it left it and 4-byte aligned, or NULL (computed again; also where its size is 0) -> dq, dk_out, dv_out (b, t, h, dk or dv) contiguous in dtype,
  * dstate (b, h, dk, dv) f32. `strides`: b, t, h of q, k, v, dout, then b, t of reset. The
  * decays are constants of their heads and have no gradient. */
 int hipenvs_decay_attention_backward(int32_t dtype, const void* q, const void* k, const void* v,

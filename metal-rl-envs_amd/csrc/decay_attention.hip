@@ -271,6 +271,7 @@ extern "C" int hipenvs_decay_attention_backward(int32_t dtype, const void* q, co
   if (b == 0) return HIPENVS_OK;
   if (!log_decay || !dstate || (t > 0 && (!q || !k || !v || !dout || !dq || !dk_out || !dv_out || !strides)))
     return HIPENVS_E_ARG;
+  if ((uintptr_t)states & 3) return HIPENVS_E_ARG;
   static const int64_t none[14] = {};
   const int64_t* st = t > 0 ? strides : none;
   Walk w = {};

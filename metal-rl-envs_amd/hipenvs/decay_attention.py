@@ -102,13 +102,9 @@ def _check_reset(reset, shape, device):
 _STRIDES = {n: ctypes.c_int64 * n for n in (11, 14)}
 
 
-def _flat_strides(rows):
-    return [s for x in rows for s in x.stride()[:3]]
-
-
 def _strides(rows, reset):
     """The host array of strides: b, t, h of each tensor, then b, t of reset."""
-    flat = _flat_strides(rows)
+    flat = [s for x in rows for s in x.stride()[:3]]
     flat += reset.stride() if reset is not None else (0, 0)
     return _STRIDES[len(flat)](*flat)
 
@@ -142,16 +138,15 @@ def _forward(q, k, v, log_decay, state, reset, scale):
 
 class _Sequence(torch.autograd.Function):
     # The backward runs in the engine's own thread, where Python costs several times what it does here:
-    # whatever it can be given ready, the forward makes.
+    # what it can be given ready, the forward makes. Not the layout of what is saved: hooks on saved
+    # tensors may hand back others of the same values (a copy on the host and back packs a view).
     @staticmethod
     def forward(ctx, q, k, v, log_decay, state, reset, scale):
         ctx.set_materialize_grads(False)
         out, final, workspace = _forward(q, k, v, log_decay, state, reset, scale)
         ctx.save_for_backward(q, k, v, log_decay, state, reset, workspace)
         b, t, h, dk = q.shape
-        flat = _flat_strides((q, k, v))
-        tail = reset.stride() if reset is not None else (0, 0)
-        ctx.ready = (_DTYPES[q.dtype], q.dtype, q.device, b, t, h, dk, v.shape[-1], flat, tail, scale,
+        ctx.ready = (_DTYPES[q.dtype], q.dtype, q.device, q.get_device(), b, t, h, dk, v.shape[-1], scale,
                      workspace.numel() if workspace is not None else 0)
         return out, final
 
@@ -164,7 +159,16 @@ class _Sequence(torch.autograd.Function):
 
 def _backward(ctx, dout, dfinal):
     q, k, v, log_decay, state, reset, states = ctx.saved_tensors
-    code, dtype, device, b, t, h, dk, dv, flat, tail, scale, nbytes = ctx.ready
+    code, dtype, device, index, b, t, h, dk, dv, scale, nbytes = ctx.ready
+    q = _check(q, "the saved q", dtype, index, (b, t, h, dk))
+    k = _check(k, "the saved k", dtype, index, (b, t, h, dk))
+    v = _check(v, "the saved v", dtype, index, (b, t, h, dv))
+    log_decay = _check_f32(log_decay, "the saved log_decay", (h,), index)
+    reset = _check_reset(reset, (b, t), index)
+    if state is not None:
+        state = _check_f32(state, "the saved state", (b, h, dk, dv), index)
+    if states is not None:
+        states = _check(states, "the saved workspace", torch.uint8, index, (nbytes,))
     if dout is None:
         dout = torch.zeros((b, t, h, dv), dtype=dtype, device=device)
     elif dout.stride(-1) != 1 and dv != 1:
@@ -178,7 +182,7 @@ def _backward(ctx, dout, dfinal):
     held = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     with _lib.on(device):
         _lib.call("hipenvs_decay_attention_backward", code, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(),
-                  _STRIDES[14](*flat, *dout.stride()[:3], *tail), log_decay.data_ptr(), _lib.ptr(state),
+                  _strides((q, k, v, dout), reset), log_decay.data_ptr(), _lib.ptr(state),
                   _lib.ptr(reset), _lib.ptr(dfinal), _lib.ptr(states), scale, dq.data_ptr(), dk_.data_ptr(),
                   dv_.data_ptr(), dstate.data_ptr(), b, t, h, dk, dv, _lib.ptr(held), nbytes, _lib.stream_of(device))
     return dq, dk_, dv_, None, dstate if state is not None else None, None, None
