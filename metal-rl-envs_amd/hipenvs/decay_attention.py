@@ -21,6 +21,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -99,6 +100,15 @@ def _check_reset(reset, shape, device):
     return reset
 
 
+def _refuse_tangents(name, *tensors):
+    """Forward-mode derivatives are not there, and outputs without one would read as a derivative of
+    zero. Outside every dual level, which torch counts from 0, there is nothing to look for."""
+    if getattr(forward_ad, "_current_level", 0) < 0:
+        return
+    if any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in tensors):
+        raise ValueError(f"{name} has no forward-mode derivative: pass it tensors without tangents")
+
+
 _STRIDES = {n: ctypes.c_int64 * n for n in (11, 14)}
 
 
@@ -169,6 +179,7 @@ def _backward(ctx, dout, dfinal):
         state = _check_f32(state, "the saved state", (b, h, dk, dv), index)
     if states is not None:
         states = _check(states, "the saved workspace", torch.uint8, index, (nbytes,))
+    _refuse_tangents("the gradient of sequence", dout, dfinal)
     if dout is None:
         dout = torch.zeros((b, t, h, dv), dtype=dtype, device=device)
     elif dout.stride(-1) != 1 and dv != 1:
@@ -196,12 +207,13 @@ def sequence(q, k, v, log_decay, state=None, reset=None, scale=None):
     """Whole trajectories: q, k (b, t, h, dk), v (b, t, h, dv), log_decay (h,) float32, state
     (b, h, dk, dv) float32 before the first token (None: zeros), reset (b, t) bool, True where
     an episode begins at that token (None: nowhere). Returns (out (b, t, h, dv) of q's type,
-    final_state (b, h, dk, dv) float32), differentiable once in q, k, v and state."""
+    final_state (b, h, dk, dv) float32), differentiable once in q, k, v and state, in reverse mode."""
     q, k, v, device, (b, t), h, dk, dv = _check_qkv(q, k, v, 4)
     log_decay = _check_decay(log_decay, h, device)
     reset = _check_reset(reset, (b, t), device)
     if state is not None:
         state = _check_f32(state, "state", (b, h, dk, dv), device)
+    _refuse_tangents("sequence", q, k, v, log_decay, state)
     scale = _scale(scale, dk)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or (state is not None and state.requires_grad)):
@@ -220,11 +232,12 @@ def step(q, k, v, log_decay, state, reset=None, scale=None, next_state=None):
     state = _check_f32(state, "state", (n, h, dk, dv), device)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
         raise ValueError("step has no gradient: call it under torch.no_grad(), or use sequence")
+    if next_state is not None and _check_f32(next_state, "next_state", (n, h, dk, dv), device) is not next_state:
+        raise ValueError("next_state must be contiguous")
+    _refuse_tangents("step", q, k, v, log_decay, state, next_state)
     if next_state is None:
         next_state = torch.empty_like(state)
     else:
-        if _check_f32(next_state, "next_state", (n, h, dk, dv), device) is not next_state:
-            raise ValueError("next_state must be contiguous")
         torch.autograd.graph.increment_version(next_state)
     on = q.device
     out = torch.empty((n, h, dv), dtype=q.dtype, device=on)

@@ -151,3 +151,17 @@ def test_c_abi_refuses_states_that_floats_do_not_lie_in():
     a, strides = ctypes.c_void_p(4096), (ctypes.c_int64 * 14)()
     assert _lib.lib().hipenvs_decay_attention_backward(0, a, a, a, a, strides, a, None, None, None, ctypes.c_void_p(4098), 1.0,
                                                        a, a, a, a, 2, 3, 2, 8, 4, None, 0, None) == _lib.E_ARG
+
+
+def test_tangents_are_found():
+    from torch.autograd import forward_ad
+
+    from hipenvs import decay_attention
+
+    x = torch.ones(3)
+    decay_attention._refuse_tangents("it", x, None)
+    with forward_ad.dual_level():
+        decay_attention._refuse_tangents("it", x, None)
+        dual = forward_ad.make_dual(x, x)
+        with pytest.raises(ValueError, match="it has no forward-mode derivative"):
+            decay_attention._refuse_tangents("it", x, None, dual[1:])

@@ -57,3 +57,40 @@ def test_saved_tensors_left_on_the_host_are_refused(dev):
     with pytest.raises(ValueError):
         gradients(long, torch.autograd.graph.saved_tensors_hooks(
             lambda x: x, lambda x: x.cpu() if x.dtype == torch.uint8 else x))
+
+
+def test_forward_mode_derivatives_are_refused(dev):
+    """A dual tensor asks for a derivative along its tangent, which nothing here gives; a level without
+    dual tensors changes nothing."""
+    from torch.autograd import forward_ad
+
+    from hipenvs import decay_attention
+
+    c = case(dev, 63, 2, 9, 2, 8, 4, F32, "apart", 3)
+    want = decay_attention.sequence(**c)
+    one = [c[n][:, 0].contiguous() for n in ("q", "k", "v")] + [c["log_decay"], c["state"].clone()]
+    stepped = decay_attention.step(*one)
+    with forward_ad.dual_level():
+        assert all(torch.equal(x, y) for x, y in zip(decay_attention.sequence(**c), want))
+        assert all(torch.equal(x, y) for x, y in zip(decay_attention.step(*one), stepped))
+        for n in ("q", "k", "v", "log_decay", "state"):
+            dual = forward_ad.make_dual(c[n], torch.ones_like(c[n]))
+            with pytest.raises(ValueError, match="forward-mode"):
+                decay_attention.sequence(**{**c, n: dual})
+            leaf = c["q"].detach().requires_grad_()
+            if n != "q":
+                with pytest.raises(ValueError, match="forward-mode"):
+                    decay_attention.sequence(**{**c, "q": leaf, n: dual})
+        for i in range(5):
+            dual = forward_ad.make_dual(one[i], torch.ones_like(one[i]))
+            with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
+                decay_attention.step(*one[:i], dual, *one[i + 1:])
+        into = forward_ad.make_dual(one[4].clone(), torch.ones_like(one[4]))
+        version = into._version
+        with pytest.raises(ValueError, match="forward-mode"):
+            decay_attention.step(*one, next_state=into)
+        assert into._version == version
+        leaf = c["q"].detach().requires_grad_()
+        out, _ = decay_attention.sequence(**{**c, "q": leaf})
+        with pytest.raises(ValueError, match="forward-mode"):
+            torch.autograd.grad(out, leaf, forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out)))
