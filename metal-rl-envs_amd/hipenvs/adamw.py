@@ -160,7 +160,9 @@ def step(params, grads, moments, t, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weigh
     with _lib.on(device):
         _lib.call("hipenvs_adamw_step", bits, count, *(a.buffer_info()[0] for a in arrays), beta1, beta2, eps,
                   1.0 - lr * weight_decay, m, v, m_scales, v_scales, _lib.stream_of(device))
-    torch.autograd.graph.increment_version((*params, *moments))
+    changed = params if whole else [p for p, g in zip(params, grads) if g is not None]
+    if changed:   # the others are as they were: a graph that holds them stays good
+        torch.autograd.graph.increment_version((*changed, *moments))
 
 
 def decode(moments):
