@@ -104,12 +104,13 @@ class Learner:
             raise ValueError(f"task must be one of {sorted(TASKS)}, got {cfg.task}")
         self.cfg = cfg
         device = torch.device(device) if device is not None else _lib.default_device()
-        body, self.seen, actions = TASKS[cfg.task]
+        body, seen, actions = TASKS[cfg.task]
+        self.seen = torch.tensor(seen, device=device)   # a list would be uploaded, and waited for, at every step
         body.reseed(cfg.seed)
         self.env = adapter.DeviceEnv(body, cfg.envs, seed=cfg.seed + 1, device=device)
         self.generator = torch.Generator(device=device)
         self.generator.manual_seed(cfg.seed)
-        self.policy = Policy(len(self.seen), actions, cfg.width, cfg.heads, cfg.layers, self.generator)
+        self.policy = Policy(len(seen), actions, cfg.width, cfg.heads, cfg.layers, self.generator)
         self.optimizer = adamw.AdamW(self.policy.parameters(), lr=cfg.lr, weight_decay=cfg.weight_decay, bits=cfg.bits)
         self.memory = self.policy.initial_state(cfg.envs)
         self.begins = torch.ones(cfg.envs, dtype=torch.bool, device=device)
@@ -120,7 +121,7 @@ class Learner:
         before = [s.clone() for s in self.memory]
         steps = []
         for _ in range(self.cfg.horizon):
-            obs = self.env.obs()[:, list(self.seen)]
+            obs = self.env.obs().index_select(1, self.seen)
             logits = self.policy.act(obs, self.memory, self.begins)
             noise = torch.rand(logits.shape, generator=self.generator, device=logits.device)
             action = (logits - torch.log(-torch.log(noise.clamp(1e-12, 1 - 1e-7)))).argmax(-1)   # Gumbel's maximum
