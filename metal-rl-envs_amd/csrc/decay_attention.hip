@@ -23,8 +23,14 @@ __global__ __launch_bounds__(kBlock) void join_kernel(Walk w, int groups) {
   const float ld = w.log_decay[h];
   float* states = w.states + row * w.parts * size + (live ? at : 0);
   const uint8_t* flags = w.flags + row * w.parts;
-  // a part's step; a keep below zero drops the state before it, whatever that holds
-  const auto stepped = [](float keep, float before, float own) { return (keep < 0.0f ? 0.0f : before * keep) + own; };
+  // A part's step; a keep below zero drops the state before it, whatever that holds. lambda^n over
+  // a part's n tokens may underflow or overflow where lambda does not: token by token an
+  // infinity stays what it is under any lambda above zero, and zero under any.
+  const bool lasting = expf(ld) > 0.0f;
+  const auto stepped = [lasting](float keep, float before, float own) {
+    const float kept = lasting && __builtin_isinf(before) ? before : before * keep;
+    return (keep < 0.0f || before == 0.0f ? 0.0f : kept) + own;
+  };
   float carry = w.state_in && live ? w.state_in[state_index(w, row, at / w.dv, at % w.dv)] : 0.0f;
   const float whole = expf(ld * (float)w.part);
   for (int base = 0; base < w.parts; base += groups * kEach) {
