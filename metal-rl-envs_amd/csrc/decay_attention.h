@@ -304,7 +304,7 @@ constexpr int power_of_two(int n) {   // the least that is not below n
 // fewer. float32 rows use the float32 matrix instructions throughout.
 //
 // What bounds it: with many rows of 128 tokens memory, at 4.8 TB/s (float32 heads of 32), 4.3 (of
-// 64), 3.6 and 3.8 (bfloat16 heads of 32 and 64), where a large copy reaches 4.9; in heads of 128 the
+// 64), 3.6 and 3.8 (bfloat16 heads of 32 and 64), where `step` reaches 5.8; in heads of 128 the
 // chain of a chunk's loads, barriers and products, eight waves being all that 239 registers
 // leave a CU (3.2 TB/s bfloat16, 3.0 float32, there mostly float32 products). A chunk of 64
 // tokens takes a block of four waves 3.4 us alone on a CU and 4.2 beside another (bfloat16

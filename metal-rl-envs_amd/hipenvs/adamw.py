@@ -1,5 +1,5 @@
-"""AdamW over all tensors of a policy in one launch, moments in 32 bits or in 8 bits with a
-scale for every 256 values. The reference has no counterpart: its gradient learners call
+"""AdamW over all tensors of a policy, one launch for every 64 of them, moments in 32 bits or in
+8 bits with a scale for every 256 values. The reference has no counterpart: its gradient learners call
 their array library's optimizer.
 
     m = b1 m + (1 - b1) g          v = b2 v + (1 - b2) g^2
