@@ -436,6 +436,115 @@ int hipenvs_adamw_decode(const void* m_codes, const void* v_codes, const float* 
                          const float* v_scales, int64_t blocks, float* m, float* v,
                          hipenvs_stream_t stream);
 
+/* ---- Policies over tokens (no reference counterpart) --------------------- */
+
+/* Bytes on the current device, -1 for arguments that are refused: of the workspace of the forward
+ * pass (which 0) and of the backward pass (2), and of the states that the forward pass keeps for the
+ * backward pass (1). */
+int64_t hipenvs_selective_scan_workspace_bytes(int32_t which, int64_t b, int64_t t, int32_t d, int32_t n,
+                                               int32_t g);
+
+/* The selective state space scan. Per row b and channel c of d, with n states h in f32:
+ *   delta = softplus(dt_t + dt_bias),  h_t = (reset_t ? 0 : exp(delta rate) h_{t-1}) + delta x_t write_t,
+ *   out_t = (read_t . h_t + skip x_t) silu(gate_t).
+ * dtype 0: x, dt, gate (b, t, d), write, read (b, t, g, n) and out f32; 1: bfloat16 (raw 16 bits), each
+ * with unit stride in the last axis and any strides (in elements) in the others; channel c reads
+ * group c / (d / g). `strides`, a host array: b, t of x, of dt, of gate, then b, t, g of write, of
+ * read, then b, t of reset. rate (d, n), skip, dt_bias (d) f32 contiguous; skip, gate, dt_bias, reset
+ * (b, t) u8 or NULL (left out); state (b, d, n) f32 contiguous or NULL (zeros).
+ * -> out (b, t, d) contiguous, final_state (b, d, n) f32 (not `state`), checks (which 1 above, 16-byte
+ * aligned) or NULL. 1 <= n <= 64, d <= 65536, g divides d. workspace: 16-byte aligned. What a token
+ * before a reset or after t holds, a NaN or an infinity among it, does not reach out_t. */
+int hipenvs_selective_scan(int32_t dtype, const void* x, const void* dt, const float* rate, const void* write,
+                           const void* read, const float* skip, const void* gate, const float* dt_bias,
+                           const float* state, const uint8_t* reset, const int64_t* strides, void* out,
+                           float* final_state, float* checks, int64_t b, int64_t t, int32_t d, int32_t n, int32_t g,
+                           void* workspace, int64_t workspace_bytes, hipenvs_stream_t stream);
+
+/* Gradients of the above from dout like out with strides of its own (two more in `strides`), dfinal
+ * (b, d, n) f32 contiguous or NULL (zeros) and the checks that the forward pass left -> dx, ddt, dgate
+ * (b, t, d), dwrite, dread (b, t, g, n) contiguous in dtype (dgate only with gate), dparams (d (n + 2))
+ * f32: of rate (d, n), then skip (d), then dt_bias (d); dstate (b, d, n) f32. */
+int hipenvs_selective_scan_backward(int32_t dtype, const void* x, const void* dt, const float* rate,
+                                    const void* write, const void* read, const float* skip, const void* gate,
+                                    const float* dt_bias, const uint8_t* reset, const void* dout, const float* dfinal,
+                                    const float* checks, const int64_t* strides, void* dx, void* ddt, void* dwrite,
+                                    void* dread, void* dgate, float* dparams, float* dstate, int64_t b, int64_t t,
+                                    int32_t d, int32_t n, int32_t g, void* workspace, int64_t workspace_bytes,
+                                    hipenvs_stream_t stream);
+
+/* One token of `count` environments: x, dt, gate (count, d), write, read (count, g, n), state
+ * (count, d, n) f32 contiguous, reset (count) u8 or NULL -> out (count, d) contiguous, next_state, which
+ * may be `state`. `strides`: of the environment in x, dt, gate, then of the environment and the group
+ * in write, in read, then of reset. */
+int hipenvs_selective_scan_step(int32_t dtype, const void* x, const void* dt, const float* rate, const void* write,
+                                const void* read, const float* skip, const void* gate, const float* dt_bias,
+                                const float* state, const uint8_t* reset, const int64_t* strides, void* out,
+                                float* next_state, int64_t count, int32_t d, int32_t n, int32_t g,
+                                hipenvs_stream_t stream);
+
+/* The short causal convolution of each channel, w taps of 1 to 4:
+ *   pre_t = bias + sum_{j < w} weight[j] x_{t-w+1+j},  out = silu ? silu(pre) : pre,
+ * without the taps that reach before the first token of t's episode. x (b, t, d) in dtype with unit
+ * stride in the last axis; weight (d, w), bias (d) or NULL f32; state (b, w - 1, d) f32 contiguous, the
+ * values before the row, or NULL (zeros); `strides`: b, t of x, then of reset (u8 or NULL)
+ * -> out (b, t, d) contiguous, final_state (b, w - 1, d) f32 (not `state`). */
+int hipenvs_causal_conv(int32_t dtype, const void* x, const float* weight, const float* bias, const float* state,
+                        const uint8_t* reset, const int64_t* strides, int32_t silu, void* out, float* final_state,
+                        int64_t b, int64_t t, int32_t d, int32_t w, hipenvs_stream_t stream);
+
+/* Bytes of workspace of the gradients below on the current device; -1 for arguments they refuse. */
+int64_t hipenvs_causal_conv_workspace_bytes(int64_t b, int64_t t, int32_t d, int32_t w);
+
+/* Gradients of the above from dout like out with strides of its own (two more in `strides`) and dfinal
+ * (b, w - 1, d) f32 contiguous or NULL (zeros) -> dx (b, t, d) contiguous in dtype, dparams (d (w + 1))
+ * f32: of weight (d, w), then bias (d); dstate (b, w - 1, d) f32. workspace: 16-byte aligned. */
+int hipenvs_causal_conv_backward(int32_t dtype, const void* x, const float* weight, const float* bias,
+                                 const float* state, const uint8_t* reset, const void* dout, const float* dfinal,
+                                 const int64_t* strides, int32_t silu, void* dx, float* dparams, float* dstate,
+                                 int64_t b, int64_t t, int32_t d, int32_t w, void* workspace, int64_t workspace_bytes,
+                                 hipenvs_stream_t stream);
+
+/* One token of n environments: x (n, d) with stride x_sn, state (n, w - 1, d) f32 contiguous -> out
+ * (n, d) contiguous, next_state, which may be `state`. */
+int hipenvs_causal_conv_step(int32_t dtype, const void* x, int64_t x_sn, const float* weight, const float* bias,
+                             const float* state, const uint8_t* reset, int64_t reset_sn, int32_t silu, void* out,
+                             float* next_state, int64_t n, int32_t d, int32_t w, hipenvs_stream_t stream);
+
+/* out (count, d) = scale * rows of table (v, d) in dtype, table_sv elements apart, for `count` tokens of
+ * token_bytes 4 or 8. A negative token: zeros; one past the table: NaN. */
+int hipenvs_embedding(int32_t dtype, const void* tokens, int32_t token_bytes, const void* table, int64_t table_sv,
+                      float scale, void* out, int64_t count, int64_t v, int32_t d, hipenvs_stream_t stream);
+
+/* Bytes of workspace of the gradient below; -1 for arguments it refuses. */
+int64_t hipenvs_embedding_workspace_bytes(int64_t count, int64_t v, int32_t d);
+
+/* dtable (v, d) = scale * the sums of the rows of dout (count, d), dout_s elements apart, over equal
+ * tokens, zeros where there is none; f32 sums in an order that depends on the tokens alone. Tokens that
+ * are negative or past the table add to nothing. workspace: 16-byte aligned. */
+int hipenvs_embedding_backward(int32_t dtype, const void* tokens, int32_t token_bytes, const void* dout,
+                               int64_t dout_s, float scale, void* dtable, int64_t count, int64_t v, int32_t d,
+                               void* workspace, int64_t workspace_bytes, hipenvs_stream_t stream);
+
+/* Bytes of workspace of hipenvs_log_probs on the current device; -1 for arguments it refuses. */
+int64_t hipenvs_log_probs_workspace_bytes(int64_t rows, int64_t v, int32_t top);
+
+/* Per row of logits (rows, v) in dtype, logits_s elements apart: log_prob = log softmax at the token
+ * (0 for a negative token, NaN for one past the row), entropy = -sum p log p, stats (rows, 2) for the
+ * gradient or NULL; with top > 0 (at most 64, at most v) the `top` most likely tokens in order, of equals
+ * the lowest first: top_log_prob, top_index (rows, top). A logit of -inf has probability 0; a row of
+ * nothing else has log probabilities of -inf and entropy 0. workspace: 16-byte aligned. */
+int hipenvs_log_probs(int32_t dtype, const void* logits, int64_t logits_s, const int64_t* tokens, float* log_prob,
+                      float* entropy, float* stats, int32_t top, float* top_log_prob, int64_t* top_index,
+                      int64_t rows, int64_t v, void* workspace, int64_t workspace_bytes, hipenvs_stream_t stream);
+
+/* dlogits (rows, v) contiguous in dtype, from the stats and entropy that hipenvs_log_probs left and the
+ * gradients of log_prob and entropy (rows) f32, either NULL (zeros). */
+int hipenvs_log_probs_backward(int32_t dtype, const void* logits, int64_t logits_s, const int64_t* tokens,
+                               const float* stats, const float* entropy, const float* dlog_prob,
+                               const float* dentropy, void* dlogits, int64_t rows, int64_t v,
+                               hipenvs_stream_t stream);
+
 /* ---- Diagnostics (no reference counterpart) ---------------------------- */
 
 /* Elementwise deterministic sin, cos, tanh of x (n) as the kernels compute them;

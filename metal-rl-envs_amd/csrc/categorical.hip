@@ -1,0 +1,467 @@
+// Log probabilities of given tokens under rows of logits, with entropies, the most likely tokens, and
+// the gradient of the logits. No reference counterpart.
+//
+//   m = max x, s = sum exp(x - m), w = sum exp(x - m) (x - m)
+//   log p(token) = x[token] - m - log s        H = log s - w / s
+//   dx_j = dlog_prob ([j = token] - p_j) - dentropy p_j (log p_j + H)
+//
+// A logit of -inf is a token that is not allowed: it adds nothing to any sum. A row of nothing else
+// has log probabilities of -inf, entropy 0 and a gradient of zeros; a row with a NaN or +inf is no
+// number throughout. A negative token is none: log probability 0, no gradient of its own.
+// Everything is float32 but the logits, which may be bfloat16, and their gradient.
+#include "row_ops.h"
+
+namespace hipenvs {
+namespace categorical {
+
+using namespace rows;
+
+constexpr int kMaxTop = 64;
+
+struct LogProbs {
+  const void* logits;
+  const int64_t* tokens;
+  int64_t logits_s, rows, v, part;   // part: values of a row that one block takes
+  float *log_prob, *entropy, *stats;   // stats (rows, 2): m and log2 s
+  float* top_log_prob;               // (rows, top)
+  int64_t* top_index;
+  float* partial;                    // (rows, parts, 4): m, s, w
+  uint64_t* tops;                    // (rows, parts, top)
+  int32_t parts, top;
+  int64_t item0;
+};
+
+// Differences of logits reach -inf, and a zero times that is no number; exp(-160) and
+// 2^-160 are 0 in float32.
+__device__ __forceinline__ float at_least(float x) { return x < -160.0f ? -160.0f : x; }
+
+// m, s and w of some of a row's values.
+struct Sums {
+  float m, s, w;
+
+  __device__ __forceinline__ void raise(float to) {
+    if (to > m) {
+      const float step = at_least(m - to), k = exp2_of(step * kLog2e);
+      if (m != -__builtin_inff()) {
+        w = k * __builtin_fmaf(s, step, w);
+        s *= k;
+      }
+      m = to;
+    }
+  }
+
+  __device__ __forceinline__ void add(float x) {   // after raise(x)
+    const float t = at_least(x - (m == -__builtin_inff() ? 0.0f : m)), e = exp2_of(t * kLog2e);
+    s += e;
+    w = __builtin_fmaf(e, t, w);
+  }
+
+  __device__ __forceinline__ void join(Sums o) {
+    raise(o.m);
+    o.raise(m);
+    s += o.s;
+    w += o.w;
+  }
+};
+
+__device__ __forceinline__ Sums none() { return {-__builtin_inff(), 0.0f, 0.0f}; }
+
+template <int kXor>
+__device__ __forceinline__ float from_lane_xor(float v) {
+  if constexpr (kXor < 16) return from_xor<kXor>(v);
+  else return __shfl_xor(v, kXor);
+}
+
+template <int kLanes>
+__device__ __forceinline__ Sums joined(Sums a) {
+  const auto with = [&](auto step) {
+    constexpr int kXor = decltype(step)::value;
+    if constexpr (kXor < kLanes)
+      a.join({from_lane_xor<kXor>(a.m), from_lane_xor<kXor>(a.s), from_lane_xor<kXor>(a.w)});
+  };
+  with(std::integral_constant<int, 1>()), with(std::integral_constant<int, 2>()), with(std::integral_constant<int, 4>());
+  with(std::integral_constant<int, 8>()), with(std::integral_constant<int, 16>()), with(std::integral_constant<int, 32>());
+  return a;
+}
+
+// A value and its place as one number: larger ones first, NaN before all, of equals the lowest place.
+__device__ __forceinline__ uint64_t ranked(float x, uint32_t index) {
+  const uint32_t u = __float_as_uint(x + 0.0f);   // -0 as 0
+  const uint32_t key = x != x ? 0xFFFFFFFFu : u & 0x80000000u ? ~u : u | 0x80000000u;
+  return (uint64_t)key << 32 | (0xFFFFFFFFu - index);
+}
+
+__device__ __forceinline__ uint32_t place_in(uint64_t r) { return 0xFFFFFFFFu - (uint32_t)r; }
+
+__device__ __forceinline__ float value_in(uint64_t r) {
+  const uint32_t key = (uint32_t)(r >> 32);
+  if (key == 0xFFFFFFFFu) return __builtin_nanf("");
+  return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
+}
+
+__device__ __forceinline__ uint64_t lane_value(uint64_t v, int lane) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+
+// The most likely so far, one a lane, in order; empty places are 0.
+struct Best {
+  uint64_t own, least;   // least: the last that is kept, in all lanes
+
+  // takes each lane's candidate, if it is among the best
+  __device__ __forceinline__ void offer(uint64_t candidate, int top, int lane) {
+    uint64_t better = __builtin_amdgcn_ballot_w64(candidate > least);
+    while (better) {
+      const uint64_t v = lane_value(candidate, __builtin_ctzll(better));
+      const int at = __popcll(__builtin_amdgcn_ballot_w64(own > v));
+      const uint64_t before = __shfl_up(own, 1);
+      own = lane < at ? own : lane == at ? v : before;
+      least = lane_value(own, top - 1);
+      better &= better - 1;
+      better &= __builtin_amdgcn_ballot_w64(candidate > least);
+    }
+  }
+};
+
+// What a row's sums say: its outputs, by one lane.
+__device__ __forceinline__ void write_row(const LogProbs& p, int64_t row, Sums a, float chosen, int64_t token) {
+  const bool empty = a.m == -__builtin_inff() && a.s == 0.0f;
+  const float log_s = __builtin_amdgcn_logf(a.s);   // to the base of 2
+  const float l = log_s * kLn2;
+  float lp = empty ? -__builtin_inff() : (chosen - a.m) - l;
+  if (token >= p.v) lp = __builtin_nanf("");
+  p.log_prob[row] = token < 0 ? 0.0f : lp;
+  p.entropy[row] = empty ? 0.0f : l - a.w / a.s;
+  if (p.stats) {
+    p.stats[2 * row] = empty ? 0.0f : a.m;
+    p.stats[2 * row + 1] = empty ? __builtin_inff() : log_s;   // every p = 0
+  }
+}
+
+__device__ __forceinline__ float top_log_prob(uint64_t ranked, Sums a) {
+  const float x = value_in(ranked);
+  if (a.m == -__builtin_inff() && a.s == 0.0f) return x;   // every token is out: -inf
+  return (x - a.m) - __builtin_amdgcn_logf(a.s) * kLn2;
+}
+
+// Short rows: G lanes hold a row in registers, E values each.
+template <class T, int G, int E>
+__global__ __launch_bounds__(kBlock) void short_kernel(LogProbs p) {
+  const int64_t row = p.item0 + (int64_t)blockIdx.x * (kBlock / G) + threadIdx.x / G;
+  const int lane = threadIdx.x % G;
+  if (row >= p.rows) return;   // all of a row's lanes
+  const T* x = (const T*)p.logits + row * p.logits_s;
+  const int v = (int)p.v;
+  const int64_t token = p.tokens[row];
+  float own[E];
+  Sums a = none();
+#pragma unroll
+  for (int e = 0; e < E; ++e) own[e] = e * G + lane < v ? (float)x[e * G + lane] : -__builtin_inff();
+#pragma unroll
+  for (int e = 0; e < E; ++e) a.m = own[e] > a.m ? own[e] : a.m;
+#pragma unroll
+  for (int e = 0; e < E; ++e) a.add(own[e]);
+  a = joined<G>(a);
+  if (lane == 0) write_row(p, row, a, token >= 0 && token < p.v ? (float)x[token] : 0.0f, token);
+  uint32_t taken = 0;
+  for (int k = 0; k < p.top; ++k) {
+    uint64_t best = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const uint64_t r = e * G + lane < v && !(taken >> e & 1) ? ranked(own[e], e * G + lane) : 0;
+      best = r > best ? r : best;
+    }
+    uint64_t all = best;
+#pragma unroll
+    for (int step = 1; step < G; step *= 2) {
+      const uint64_t other = __shfl_xor(all, step);
+      all = other > all ? other : all;
+    }
+    const uint32_t at = place_in(all);
+    if (at % G == (uint32_t)lane) taken |= 1u << (at / G);
+    if (lane == 0) {
+      p.top_log_prob[row * p.top + k] = top_log_prob(all, a);
+      p.top_index[row * p.top + k] = at;
+    }
+  }
+}
+
+// Long rows: a block takes a part of a row, every wave with its own sums and its own best.
+template <class T>
+__global__ __launch_bounds__(kBlock) void long_kernel(LogProbs p) {
+  __shared__ Sums sums[4];
+  __shared__ uint64_t best[4][kMaxTop];
+  const int64_t item = p.item0 + blockIdx.x, row = item / p.parts;
+  const int part = (int)(item - row * p.parts), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const T* x = (const T*)p.logits + row * p.logits_s;
+  const int64_t first = part * p.part, end = first + p.part < p.v ? first + p.part : p.v;
+  Sums a = none();
+  Best b = {0, 0};
+  for (int64_t at = first; at < end; at += kBlock * 4) {
+    const int64_t i = at + threadIdx.x * 4;
+    f32x4 own = load_upto(x + i, end - i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (i + e >= end) own[e] = -__builtin_inff();
+    float m = own[0];
+#pragma unroll
+    for (int e = 1; e < 4; ++e) m = own[e] > m ? own[e] : m;
+    a.raise(m);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a.add(own[e]);
+    if (p.top)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) b.offer(i + e < end ? ranked(own[e], (uint32_t)(i + e)) : 0, p.top, lane);
+  }
+  a = joined<64>(a);
+  if (lane == 0) sums[wave] = a;
+  if (lane < p.top) best[wave][lane] = b.own;
+  __syncthreads();
+  if (wave != 0) return;
+  for (int k = 1; k < 4; ++k) {
+    a.join(sums[k]);
+    if (p.top) b.offer(lane < p.top ? best[k][lane] : 0, p.top, lane);
+  }
+  if (p.parts == 1) {
+    const int64_t token = p.tokens[row];
+    if (lane == 0) write_row(p, row, a, token >= 0 && token < p.v ? (float)x[token] : 0.0f, token);
+    if (lane < p.top) {
+      p.top_log_prob[row * p.top + lane] = top_log_prob(b.own, a);
+      p.top_index[row * p.top + lane] = place_in(b.own);
+    }
+    return;
+  }
+  if (lane == 0) {
+    float* to = p.partial + item * 4;
+    to[0] = a.m, to[1] = a.s, to[2] = a.w;
+  }
+  if (lane < p.top) p.tops[item * p.top + lane] = b.own;
+}
+
+// The parts of a row together, a wave for each.
+template <class T>
+__global__ __launch_bounds__(64) void join_kernel(LogProbs p) {
+  const int64_t row = p.item0 + blockIdx.x;
+  const int lane = threadIdx.x;
+  Sums a = none();
+  Best b = {0, 0};
+  for (int k0 = 0; k0 < p.parts; k0 += 64) {
+    const int k = k0 + lane;
+    if (k < p.parts) {
+      const float* from = p.partial + (row * p.parts + k) * 4;
+      a.join({from[0], from[1], from[2]});
+    }
+  }
+  a = joined<64>(a);
+  if (p.top)
+    for (int64_t k0 = 0; k0 < (int64_t)p.parts * p.top; k0 += 64) {
+      const int64_t k = k0 + lane;
+      b.offer(k < (int64_t)p.parts * p.top ? p.tops[row * p.parts * p.top + k] : 0, p.top, lane);
+    }
+  const int64_t token = p.tokens[row];
+  if (lane == 0)
+    write_row(p, row, a, token >= 0 && token < p.v ? (float)((const T*)p.logits)[row * p.logits_s + token] : 0.0f, token);
+  if (lane < p.top) {
+    p.top_log_prob[row * p.top + lane] = top_log_prob(b.own, a);
+    p.top_index[row * p.top + lane] = place_in(b.own);
+  }
+}
+
+struct Gradient {
+  const void* logits;
+  const int64_t* tokens;
+  const float *stats, *entropy, *dlog_prob, *dentropy;
+  void* dlogits;   // (rows, v) contiguous
+  int64_t logits_s, rows, v, item0;
+  int32_t pieces;
+};
+
+// What a row's gradient takes: dx = chosen dlog_prob - p (dlog_prob + dentropy (log p + H)).
+struct RowGradient {
+  float m, log_s, h, dlp, dh;
+  int64_t token;
+
+  __device__ __forceinline__ RowGradient(const Gradient& g, int64_t row) {
+    m = g.stats[2 * row], log_s = g.stats[2 * row + 1];
+    token = g.tokens[row];
+    h = g.entropy[row];
+    dlp = g.dlog_prob && token >= 0 && log_s != __builtin_inff() ? g.dlog_prob[row] : 0.0f;
+    dh = g.dentropy ? g.dentropy[row] : 0.0f;
+  }
+
+  __device__ __forceinline__ float of(float x, int64_t j) const {
+    const float log2_p = at_least(__builtin_fmaf(x - m, kLog2e, -log_s));
+    const float through = -exp2_of(log2_p) * __builtin_fmaf(dh, __builtin_fmaf(log2_p, kLn2, h), dlp);
+    return j == token ? through + dlp : through;
+  }
+};
+
+template <class T, int G, int E>
+__global__ __launch_bounds__(kBlock) void short_gradient_kernel(Gradient g) {
+  const int64_t row = g.item0 + (int64_t)blockIdx.x * (kBlock / G) + threadIdx.x / G;
+  const int lane = threadIdx.x % G;
+  if (row >= g.rows) return;
+  const T* x = (const T*)g.logits + row * g.logits_s;
+  T* dx = (T*)g.dlogits + row * g.v;
+  const RowGradient of(g, row);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int j = e * G + lane;
+    if (j < (int)g.v) dx[j] = (T)of.of((float)x[j], j);
+  }
+}
+
+constexpr int kPiece = 4096;   // values of a row that a block takes
+
+template <class T>
+__global__ __launch_bounds__(kBlock) void long_gradient_kernel(Gradient g) {
+  const int64_t item = g.item0 + blockIdx.x, row = item / g.pieces, first = (item - row * g.pieces) * kPiece;
+  const T* x = (const T*)g.logits + row * g.logits_s;
+  T* dx = (T*)g.dlogits + row * g.v;
+  const RowGradient of(g, row);
+#pragma unroll
+  for (int k = 0; k < kPiece / (kBlock * 4); ++k) {
+    const int64_t j = first + k * (kBlock * 4) + threadIdx.x * 4;
+    if (j >= g.v) break;
+    f32x4 own = load_upto(x + j, g.v - j);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) own[e] = of.of(own[e], j + e);
+    store_upto(dx + j, own, g.v - j);
+  }
+}
+
+namespace {
+constexpr int64_t kShort = 1024;   // values of a row that a wave holds in registers
+
+bool sizes_ok(int32_t dtype, int64_t rows, int64_t v, int64_t top) {
+  return (dtype == 0 || dtype == 1) && rows >= 0 && rows <= 0x7FFFFFFF && v >= 1 && v <= 0x7FFFFFFF && top >= 0 &&
+         top <= kMaxTop && top <= v;
+}
+
+// The parts of a long row: as many as give the card eight waves a CU, none below 4,096 values.
+int plan(LogProbs* p, int64_t rows, int64_t v) {
+  int cus = 0;
+  const int status = device_cus(&cus);
+  if (status != HIPENVS_OK) return status;
+  p->rows = rows, p->v = v;
+  int64_t parts = 1;
+  if (v > kShort && rows < cus * 2) {
+    parts = (cus * 2 + rows - 1) / rows;
+    if (parts > (v + 4095) / 4096) parts = (v + 4095) / 4096;
+  }
+  p->part = ((v + parts - 1) / parts + 3) / 4 * 4;
+  p->parts = (int32_t)((v + p->part - 1) / p->part);
+  return HIPENVS_OK;
+}
+
+int64_t round16(int64_t x) { return (x + 15) / 16 * 16; }
+
+int64_t lay(LogProbs* p, char* at, int32_t top) {
+  if (p->parts <= 1) return 0;
+  const int64_t partial = round16(p->rows * p->parts * 16);
+  p->partial = (float*)at;
+  p->tops = (uint64_t*)(at + partial);
+  return partial + p->rows * p->parts * top * 8;
+}
+
+template <class S, class F>
+int in_launches(S s, int64_t blocks, int threads, const F& launch) {
+  const int64_t most = kMostThreads / threads;
+  for (int64_t done = 0; done < blocks; done += most) {
+    launch(s, done, dim3((unsigned)(blocks - done < most ? blocks - done : most)));
+    const int status = launch_status();
+    if (status != HIPENVS_OK) return status;
+  }
+  return HIPENVS_OK;
+}
+
+// f(lanes of a row, values a lane) for rows of up to kShort values
+template <class F>
+int for_short(int64_t v, const F& f) {
+  using std::integral_constant;
+  if (v <= 4) return f(integral_constant<int, 1>(), integral_constant<int, 4>());
+  if (v <= 16) return f(integral_constant<int, 4>(), integral_constant<int, 4>());
+  if (v <= 64) return f(integral_constant<int, 16>(), integral_constant<int, 4>());
+  if (v <= 256) return f(integral_constant<int, 64>(), integral_constant<int, 4>());
+  return f(integral_constant<int, 64>(), integral_constant<int, 16>());
+}
+
+template <class T>
+int forward(const LogProbs& p, hipStream_t stream) {
+  if (p.v <= kShort)
+    return for_short(p.v, [&](auto lanes, auto values) {
+      constexpr int G = decltype(lanes)::value, E = decltype(values)::value, kRows = kBlock / G;
+      return in_launches(p, (p.rows + kRows - 1) / kRows, kBlock, [&](LogProbs a, int64_t done, dim3 grid) {
+        a.item0 = done * kRows;
+        hipLaunchKernelGGL((short_kernel<T, G, E>), grid, dim3(kBlock), 0, stream, a);
+      });
+    });
+  const int status = in_launches(p, p.rows * p.parts, kBlock, [&](LogProbs a, int64_t done, dim3 grid) {
+    a.item0 = done;
+    hipLaunchKernelGGL(long_kernel<T>, grid, dim3(kBlock), 0, stream, a);
+  });
+  if (status != HIPENVS_OK || p.parts == 1) return status;
+  return in_launches(p, p.rows, 64, [&](LogProbs a, int64_t done, dim3 grid) {
+    a.item0 = done;
+    hipLaunchKernelGGL(join_kernel<T>, grid, dim3(64), 0, stream, a);
+  });
+}
+
+template <class T>
+int gradient(const Gradient& g, hipStream_t stream) {
+  if (g.v <= kShort)
+    return for_short(g.v, [&](auto lanes, auto values) {
+      constexpr int G = decltype(lanes)::value, E = decltype(values)::value, kRows = kBlock / G;
+      return in_launches(g, (g.rows + kRows - 1) / kRows, kBlock, [&](Gradient a, int64_t done, dim3 grid) {
+        a.item0 = done * kRows;
+        hipLaunchKernelGGL((short_gradient_kernel<T, G, E>), grid, dim3(kBlock), 0, stream, a);
+      });
+    });
+  return in_launches(g, g.rows * g.pieces, kBlock, [&](Gradient a, int64_t done, dim3 grid) {
+    a.item0 = done;
+    hipLaunchKernelGGL(long_gradient_kernel<T>, grid, dim3(kBlock), 0, stream, a);
+  });
+}
+}  // namespace
+
+}  // namespace categorical
+}  // namespace hipenvs
+
+using namespace hipenvs;
+using namespace hipenvs::categorical;
+
+extern "C" int64_t hipenvs_log_probs_workspace_bytes(int64_t rows, int64_t v, int32_t top) {
+  if (!sizes_ok(0, rows, v, top)) return -1;
+  if (rows == 0) return 0;
+  LogProbs p = {};
+  return plan(&p, rows, v) == HIPENVS_OK ? lay(&p, nullptr, top) : -1;
+}
+
+extern "C" int hipenvs_log_probs(int32_t dtype, const void* logits, int64_t logits_s, const int64_t* tokens,
+                                 float* log_prob, float* entropy, float* stats, int32_t top, float* top_log_prob,
+                                 int64_t* top_index, int64_t rows, int64_t v, void* workspace,
+                                 int64_t workspace_bytes, hipenvs_stream_t stream) {
+  if (!sizes_ok(dtype, rows, v, top)) return HIPENVS_E_ARG;
+  if (rows == 0) return HIPENVS_OK;
+  if (!logits || !tokens || !log_prob || !entropy || (top > 0 && (!top_log_prob || !top_index))) return HIPENVS_E_ARG;
+  LogProbs p = {};
+  const int status = plan(&p, rows, v);
+  if (status != HIPENVS_OK) return status;
+  const int64_t need = lay(&p, (char*)workspace, top);
+  if (need > 0 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)) return HIPENVS_E_ARG;
+  p.logits = logits, p.logits_s = logits_s, p.tokens = tokens, p.log_prob = log_prob, p.entropy = entropy;
+  p.stats = stats, p.top = top, p.top_log_prob = top_log_prob, p.top_index = top_index;
+  return dtype == 1 ? forward<__bf16>(p, as_stream(stream)) : forward<float>(p, as_stream(stream));
+}
+
+extern "C" int hipenvs_log_probs_backward(int32_t dtype, const void* logits, int64_t logits_s, const int64_t* tokens,
+                                          const float* stats, const float* entropy, const float* dlog_prob,
+                                          const float* dentropy, void* dlogits, int64_t rows, int64_t v,
+                                          hipenvs_stream_t stream) {
+  if (!sizes_ok(dtype, rows, v, 0)) return HIPENVS_E_ARG;
+  if (rows == 0) return HIPENVS_OK;
+  if (!logits || !tokens || !stats || !entropy || !dlogits) return HIPENVS_E_ARG;
+  const Gradient g = {logits,   tokens,   stats,    entropy, dlog_prob, dentropy,
+                      dlogits,  logits_s, rows,     v,       0,         (int32_t)((v + kPiece - 1) / kPiece)};
+  return dtype == 1 ? gradient<__bf16>(g, as_stream(stream)) : gradient<float>(g, as_stream(stream));
+}

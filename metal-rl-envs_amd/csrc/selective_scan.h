@@ -1,0 +1,168 @@
+// The selective state space scan: what its kernels and its entry points share.
+//
+//   delta = softplus(dt + dt_bias)          h_t[n] = exp(delta rate[n]) h_{t-1}[n] + delta x write_t[n]
+//   y = sum_n read_t[n] h_t[n] + skip x     out = y silu(gate)
+//
+// for each channel of each row, with h_{t-1} left out where an episode begins at t. Channels lie
+// in g groups of dg, each with rows of write and read of its own.
+#pragma once
+
+#include "row_ops.h"
+
+namespace hipenvs {
+namespace scan {
+
+using namespace rows;
+
+constexpr int kTile = 16;        // tokens staged at once; the states before each are kept for the backward pass
+constexpr int kMaxStates = 64;
+
+struct Rows {      // (b, t, channels)
+  const void* data;
+  int64_t sb, st;
+};
+
+struct Mix {       // (b, t, g, n)
+  const void* data;
+  int64_t sb, st, sg;
+};
+
+struct Scan {
+  Rows x, dt, gate, dout;
+  Mix write, read;
+  const float *rate, *skip, *bias, *state, *dfinal;
+  const uint8_t* reset;
+  int64_t reset_sb, reset_st;
+  void* out;
+  float *final_state, *checks;     // checks (b, ceil(t / kTile), d, n), or null
+  void *dx, *ddt, *dgate, *dwrite, *dread;
+  float *dstate, *dmix, *dparams;  // dmix (tiles, b t g, 2 NP) where tiles > 1; dparams (b parts, d (n + 2))
+  float *carry, *spans;            // (b, parts, d, n): the states between the parts; (b, parts, d): their sums of delta
+  uint8_t* begun;                  // (b, parts): whether an episode begins in the part
+  int64_t b, t, part;              // part: tokens of a part, whole tiles
+  int32_t d, n, g, dg, tiles, parts;
+  int64_t item0;
+};
+
+// LPC lanes a channel, four states each; the channels of a block.
+constexpr int channels_of(int lpc) { return lpc == 16 ? 32 : 64; }
+inline int lanes_of(int n) { return n <= 4 ? 1 : n <= 8 ? 2 : n <= 16 ? 4 : n <= 32 ? 8 : 16; }
+
+template <int LPC>
+struct Shape {
+  static constexpr int CH = channels_of(LPC), kThreads = CH * LPC, kWaves = kThreads / 64, NP = 4 * LPC;
+  static constexpr int kSlots = (kTile * CH / 4 + kThreads - 1) / kThreads;   // four channels of a token each
+  static constexpr int kMixSlots = (kTile * 2 * LPC + kThreads - 1) / kThreads;
+};
+
+// Where a block is: row b, part p, group and the first of its channels within the group.
+struct Place {
+  int64_t b;
+  int p, group, first;
+};
+
+__device__ __forceinline__ Place place_of(const Scan& s, int64_t item, int parts, int channels) {
+  const int tile = (int)(item % s.tiles);
+  item /= s.tiles;
+  const int group = (int)(item % s.g);
+  item /= s.g;
+  return {item / parts, (int)(item % parts), group, tile * channels};
+}
+
+// A tile's inputs, in the registers of the threads that fetch them.
+template <class T, int LPC, bool kOut, bool kBack>
+struct Fetched {
+  using S = Shape<LPC>;
+  f32x4 x[S::kSlots], dt[S::kSlots], gate[S::kSlots], dout[S::kSlots];
+  f32x4 mix[S::kMixSlots];
+  uint32_t begins;   // a bit a token
+
+  __device__ __forceinline__ void fetch(const Scan& s, const Place& at, int64_t t0, int64_t end) {
+#pragma unroll
+    for (int i = 0; i < S::kSlots; ++i) {
+      const int slot = threadIdx.x + i * S::kThreads, tok = slot / (S::CH / 4), c = at.first + (slot % (S::CH / 4)) * 4;
+      const int64_t t = t0 + tok;
+      const int left = (tok < kTile && t < end) ? s.dg - c : 0;
+      const int64_t col = (int64_t)at.group * s.dg + c;
+      x[i] = load_upto((const T*)s.x.data + at.b * s.x.sb + t * s.x.st + col, left);
+      dt[i] = load_upto((const T*)s.dt.data + at.b * s.dt.sb + t * s.dt.st + col, left);
+      if (left <= 0) dt[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (kOut || kBack) {
+        gate[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (s.gate.data) gate[i] = load_upto((const T*)s.gate.data + at.b * s.gate.sb + t * s.gate.st + col, left);
+      }
+      if (kBack) dout[i] = load_upto((const T*)s.dout.data + at.b * s.dout.sb + t * s.dout.st + col, left);
+    }
+#pragma unroll
+    for (int i = 0; i < S::kMixSlots; ++i) {
+      const int slot = threadIdx.x + i * S::kThreads, tok = slot / (2 * LPC), part = slot % (2 * LPC);
+      const int64_t t = t0 + tok;
+      const bool there = tok < kTile && t < end;
+      const int n0 = (part % LPC) * 4;
+      const Mix& m = part < LPC ? s.write : s.read;
+      mix[i] = load_upto((const T*)m.data + at.b * m.sb + t * m.st + at.group * m.sg + n0, there ? s.n - n0 : 0);
+    }
+    begins = 0;
+    if (s.reset) {
+      const int tok = threadIdx.x & 63;
+      bool here = false;
+      if (tok < kTile && t0 + tok < end) here = s.reset[at.b * s.reset_sb + (t0 + tok) * s.reset_st] != 0;
+      begins = (uint32_t)__builtin_amdgcn_ballot_w64(here);
+    }
+  }
+};
+
+template <class T, int LPC>
+__device__ __forceinline__ void put_mix(float (*mix)[8 * LPC], const f32x4* from) {
+  using S = Shape<LPC>;
+#pragma unroll
+  for (int i = 0; i < S::kMixSlots; ++i) {
+    const int slot = threadIdx.x + i * S::kThreads, tok = slot / (2 * LPC), part = slot % (2 * LPC);
+    if (tok < kTile) *(f32x4*)&mix[tok][part * 4] = from[i];
+  }
+}
+
+__device__ __forceinline__ f32x4 per_channel(const float* of, int64_t c, int left, float otherwise) {
+  f32x4 r = {otherwise, otherwise, otherwise, otherwise};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (of && e < left) r[e] = of[c + e];
+  return r;
+}
+
+// Sums 8 values of a lane over the channels of its wave: the lanes whose bits from log2(LPC) on
+// differ. Each step halves the values a lane keeps, until one is left; lane l then has value
+// id(l) of its states, twice over where fewer channel bits than that are left.
+template <int LPC>
+struct Across {
+  static constexpr int kLeft = LPC == 16 ? 2 : 1;
+
+  static __device__ __forceinline__ void sum(float (&v)[8], int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {   // bit 5
+      const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i + 4]), false, false);
+      v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {   // bit 4
+      const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i + 2]), false, false);
+      v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    if constexpr (LPC <= 8) {       // bit 3
+      const bool upper = lane & 8;
+      const float keep = upper ? v[1] : v[0], give = upper ? v[0] : v[1];
+      v[0] = keep + from_xor<8>(give);
+    }
+    if constexpr (LPC <= 4) v[0] += from_xor<4>(v[0]);
+    if constexpr (LPC <= 2) v[0] += from_xor<2>(v[0]);
+    if constexpr (LPC <= 1) v[0] += from_xor<1>(v[0]);
+  }
+
+  // which of the eight values `kept` of this lane is
+  static __device__ __forceinline__ int id(int lane, int kept) {
+    return ((lane >> 5) & 1) * 4 + ((lane >> 4) & 1) * 2 + (LPC <= 8 ? (lane >> 3) & 1 : kept);
+  }
+};
+
+}  // namespace scan
+}  // namespace hipenvs

@@ -1,0 +1,673 @@
+// The selective state space scan over trajectories, its gradients, and one token of every
+// environment. No reference counterpart.
+#include "selective_scan.h"
+
+namespace hipenvs {
+namespace scan {
+
+// One part of a row's tokens for a block of channels: LPC lanes hold a channel, four states each,
+// and walk token by token; delta, x, write and read come through LDS, a tile of 16 tokens at a
+// time, computed once each and fetched a tile ahead. kOut: outputs, from the states before the
+// part; otherwise the part's own state alone, from zeros, for rows walked in parts.
+template <class T, int LPC, bool kOut>
+__global__ __launch_bounds__(Shape<LPC>::kThreads) void forward_kernel(Scan s) {
+  using S = Shape<LPC>;
+  __shared__ __attribute__((aligned(16))) f32x2 steps[kTile][S::CH];      // delta, delta x; then y
+  __shared__ __attribute__((aligned(16))) float mix[kTile][2 * S::NP];
+  const int parts = kOut ? s.parts : s.parts - 1;
+  const Place at = place_of(s, s.item0 + blockIdx.x, parts, S::CH);
+  const int ch = threadIdx.x / LPC, n0 = (threadIdx.x % LPC) * 4;
+  const bool live = at.first + ch < s.dg;
+  const int64_t c = (int64_t)at.group * s.dg + at.first + ch;
+  const int64_t start = at.p * s.part, end = start + s.part < s.t ? start + s.part : s.t;
+  const int left = live ? s.n - n0 : 0;
+  f32x4 rate = load_upto(s.rate + c * s.n + n0, left) * kLog2e, h = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (kOut) {
+    if (s.parts > 1)
+      h = load_upto(s.carry + ((at.b * s.parts + at.p) * s.d + c) * s.n + n0, left);
+    else if (s.state)
+      h = load_upto(s.state + (at.b * s.d + c) * s.n + n0, left);
+  }
+  const int own = at.first + (threadIdx.x % (S::CH / 4)) * 4;   // the channels this thread fetches
+  const f32x4 bias = per_channel(s.bias, (int64_t)at.group * s.dg + own, s.dg - own, 0.0f);
+  const f32x4 skip = per_channel(s.skip, (int64_t)at.group * s.dg + own, s.dg - own, 0.0f);
+  const int64_t checks = (s.t + kTile - 1) / kTile;
+  float span = 0.0f;
+  uint32_t begun = 0;
+  Fetched<T, LPC, kOut, false> next;
+  next.fetch(s, at, start, end);
+  for (int64_t t0 = start; t0 < end; t0 += kTile) {
+    const Fetched<T, LPC, kOut, false> now = next;
+#pragma unroll
+    for (int i = 0; i < S::kSlots; ++i) {
+      const int slot = threadIdx.x + i * S::kThreads, tok = slot / (S::CH / 4), k = (slot % (S::CH / 4)) * 4;
+      if (tok >= kTile) break;
+      const bool there = t0 + tok < end;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float delta = there ? softplus(now.dt[i][e] + bias[e]) : 0.0f;   // past the end the state stays
+        steps[tok][k + e] = f32x2{delta, delta * now.x[i][e]};
+      }
+    }
+    put_mix<T, LPC>(mix, now.mix);
+    __syncthreads();
+    if (t0 + kTile < end) next.fetch(s, at, t0 + kTile, end);
+    if (kOut && s.checks)
+      store_upto(s.checks + ((at.b * checks + t0 / kTile) * s.d + c) * s.n + n0, h, left);
+    begun |= now.begins;
+#pragma unroll
+    for (int tok = 0; tok < kTile; ++tok) {
+      const f32x2 st = steps[tok][ch];
+      const f32x4 w = *(const f32x4*)&mix[tok][n0];
+      if (now.begins >> tok & 1) h = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      float y = 0.0f;
+      f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (kOut) r = *(const f32x4*)&mix[tok][S::NP + n0];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        h[e] = __builtin_fmaf(exp2_of(st.x * rate[e]), h[e], st.y * w[e]);
+        if (kOut) y = __builtin_fmaf(r[e], h[e], y);
+      }
+      if (kOut)
+        steps[tok][ch].x = lanes_sum<LPC>(y);   // the same from each of the channel's lanes
+      else
+        span += st.x;
+    }
+    __syncthreads();
+    if (kOut) {
+#pragma unroll
+      for (int i = 0; i < S::kSlots; ++i) {
+        const int slot = threadIdx.x + i * S::kThreads, tok = slot / (S::CH / 4), k = (slot % (S::CH / 4)) * 4;
+        if (tok >= kTile || t0 + tok >= end || at.first + k >= s.dg) continue;
+        f32x4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          o[e] = __builtin_fmaf(skip[e], now.x[i][e], steps[tok][k + e].x);
+          if (s.gate.data) o[e] *= now.gate[i][e] * sigmoid(now.gate[i][e]);
+        }
+        const int64_t col = (int64_t)at.group * s.dg + at.first + k;
+        store_upto((T*)s.out + (at.b * s.t + t0 + tok) * s.d + col, o, s.dg - at.first - k);
+      }
+      __syncthreads();
+    }
+  }
+  if (kOut) {
+    if (at.p == s.parts - 1) store_upto(s.final_state + (at.b * s.d + c) * s.n + n0, h, left);
+  } else {
+    const int64_t at_part = at.b * s.parts + at.p;
+    store_upto(s.carry + (at_part * s.d + c) * s.n + n0, h, left);
+    if (live && n0 == 0) s.spans[at_part * s.d + c] = span;
+    if (threadIdx.x == 0 && at.group == 0 && at.first == 0) s.begun[at_part] = begun != 0;
+  }
+}
+
+// A state carried over a part: exp(rate * the part's sum of delta) of it, and nothing over an
+// episode's beginning. Token by token, an infinite state and a zero one stay what they are, which
+// their product with a decay that leaves float32's range would not.
+__device__ __forceinline__ float carried(float rate, float span, float state) {
+  const float decay = exp2_of(span * (rate * kLog2e));
+  return state == 0.0f || __builtin_isinf(state) ? state : decay * state;
+}
+
+// The states before each part (kBack: the gradients behind it) from the parts' own: a thread for
+// each state of a row, over the parts in order.
+template <bool kBack>
+__global__ __launch_bounds__(kBlock) void join_kernel(Scan s) {
+  const int64_t each = (int64_t)s.d * s.n, i = s.item0 + (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  if (i >= s.b * each) return;
+  const int64_t b = i / each, x = i - b * each, c = x / s.n;
+  const float* first = kBack ? s.dfinal : s.state;
+  float state = first ? first[i] : 0.0f;
+  const float rate = s.rate[x];
+  constexpr int kAhead = 8;
+  for (int p0 = 0; p0 < s.parts; p0 += kAhead) {
+    float own[kAhead], span[kAhead];
+    bool begun[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int at = p0 + k, p = kBack ? s.parts - 1 - at : at;
+      own[k] = span[k] = 0.0f;
+      begun[k] = false;
+      if (at < s.parts - 1) {
+        own[k] = s.carry[(b * s.parts + p) * each + x];
+        span[k] = s.spans[(b * s.parts + p) * s.d + c];
+        begun[k] = s.begun[b * s.parts + p];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int at = p0 + k, p = kBack ? s.parts - 1 - at : at;
+      if (at < s.parts) s.carry[(b * s.parts + p) * each + x] = state;
+      state = (begun[k] ? 0.0f : carried(rate, span[k], state)) + own[k];
+    }
+  }
+}
+
+// The gradient that a part passes to the states before it where none reaches it from behind.
+template <class T, int LPC>
+__global__ __launch_bounds__(Shape<LPC>::kThreads) void passed_kernel(Scan s) {
+  using S = Shape<LPC>;
+  __shared__ __attribute__((aligned(16))) f32x2 steps[kTile][S::CH];      // delta, dy
+  __shared__ __attribute__((aligned(16))) float mix[kTile][2 * S::NP];
+  Place at = place_of(s, s.item0 + blockIdx.x, s.parts - 1, S::CH);
+  at.p += 1;
+  const int ch = threadIdx.x / LPC, n0 = (threadIdx.x % LPC) * 4;
+  const bool live = at.first + ch < s.dg;
+  const int64_t c = (int64_t)at.group * s.dg + at.first + ch;
+  const int64_t start = at.p * s.part, end = start + s.part < s.t ? start + s.part : s.t;
+  const int left = live ? s.n - n0 : 0;
+  const f32x4 rate = load_upto(s.rate + c * s.n + n0, left) * kLog2e;
+  f32x4 g = {0.0f, 0.0f, 0.0f, 0.0f};
+  const int own = at.first + (threadIdx.x % (S::CH / 4)) * 4;
+  const f32x4 bias = per_channel(s.bias, (int64_t)at.group * s.dg + own, s.dg - own, 0.0f);
+  float span = 0.0f;
+  uint32_t begun = 0;
+  Fetched<T, LPC, true, true> next;
+  int64_t t0 = start + (end - start - 1) / kTile * kTile;
+  next.fetch(s, at, t0, end);
+  for (; t0 >= start; t0 -= kTile) {
+    const Fetched<T, LPC, true, true> now = next;
+#pragma unroll
+    for (int i = 0; i < S::kSlots; ++i) {
+      const int slot = threadIdx.x + i * S::kThreads, tok = slot / (S::CH / 4), k = (slot % (S::CH / 4)) * 4;
+      if (tok >= kTile) break;
+      const bool there = t0 + tok < end;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float z = now.gate[i][e];
+        steps[tok][k + e] = f32x2{there ? softplus(now.dt[i][e] + bias[e]) : 0.0f,
+                                  s.gate.data ? now.dout[i][e] * (z * sigmoid(z)) : now.dout[i][e]};
+      }
+    }
+    put_mix<T, LPC>(mix, now.mix);
+    __syncthreads();
+    if (t0 - kTile >= start) next.fetch(s, at, t0 - kTile, end);
+    begun |= now.begins;
+#pragma unroll
+    for (int tok = kTile - 1; tok >= 0; --tok) {
+      const f32x2 st = steps[tok][ch];
+      const f32x4 r = *(const f32x4*)&mix[tok][S::NP + n0];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) g[e] = exp2_of(st.x * rate[e]) * __builtin_fmaf(r[e], st.y, g[e]);
+      if (now.begins >> tok & 1) g = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      span += st.x;
+    }
+    __syncthreads();
+  }
+  const int64_t at_part = at.b * s.parts + at.p;
+  store_upto(s.carry + (at_part * s.d + c) * s.n + n0, g, left);
+  if (live && n0 == 0) s.spans[at_part * s.d + c] = span;
+  if (threadIdx.x == 0 && at.group == 0 && at.first == 0) s.begun[at_part] = begun != 0;
+}
+
+// The gradients of one part for a block of channels, tile by tile from its end: the tile's states
+// again from the one kept before it, decays and what they leave in registers, then back through them.
+//
+//   g_t = read dy + a_{t+1} g_{t+1}     dread = sum_c h dy        dwrite = sum_c g delta x
+//   dx = skip dy + delta sum_n g write  ddelta = sum_n g (rate a h_{t-1} + x write)
+//   drate = sum g a h_{t-1} delta       ddt = ddelta sigmoid(dt + bias)
+//
+// Sums over a channel's states stay within its lanes; sums over channels go lane by lane within the
+// wave, then through LDS, then (dmix) over the blocks of a group.
+template <class T, int LPC>
+__global__ __launch_bounds__(Shape<LPC>::kThreads) void backward_kernel(Scan s) {
+  using S = Shape<LPC>;
+  __shared__ __attribute__((aligned(16))) f32x4 steps[kTile][S::CH];   // delta, delta x, dy; then delta, sum g write, ddelta's states, y
+  __shared__ __attribute__((aligned(16))) float mix[kTile][2 * S::NP];
+  __shared__ __attribute__((aligned(16))) float sums[S::kWaves][kTile][2 * S::NP];
+  const Place at = place_of(s, s.item0 + blockIdx.x, s.parts, S::CH);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int ch = threadIdx.x / LPC, n0 = (threadIdx.x % LPC) * 4;
+  const bool live = at.first + ch < s.dg;
+  const int64_t c = (int64_t)at.group * s.dg + at.first + ch;
+  const int64_t start = at.p * s.part, end = start + s.part < s.t ? start + s.part : s.t;
+  const int left = live ? s.n - n0 : 0;
+  const f32x4 rate = load_upto(s.rate + c * s.n + n0, left);
+  f32x4 g = {0.0f, 0.0f, 0.0f, 0.0f}, drate = g;
+  if (s.parts > 1)
+    g = load_upto(s.carry + ((at.b * s.parts + at.p) * s.d + c) * s.n + n0, left);
+  else if (s.dfinal)
+    g = load_upto(s.dfinal + (at.b * s.d + c) * s.n + n0, left);
+  const int own = at.first + (threadIdx.x % (S::CH / 4)) * 4;
+  const f32x4 bias = per_channel(s.bias, (int64_t)at.group * s.dg + own, s.dg - own, 0.0f);
+  const f32x4 skip = per_channel(s.skip, (int64_t)at.group * s.dg + own, s.dg - own, 0.0f);
+  f32x4 dskip = {0.0f, 0.0f, 0.0f, 0.0f}, dbias = dskip;
+  const int64_t checks = (s.t + kTile - 1) / kTile;
+  Fetched<T, LPC, true, true> next;
+  int64_t t0 = start + (end - start - 1) / kTile * kTile;
+  f32x4 h_next = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (end > start) {
+    next.fetch(s, at, t0, end);
+    h_next = load_upto(s.checks + ((at.b * checks + t0 / kTile) * s.d + c) * s.n + n0, left);
+  }
+  for (; end > start && t0 >= start; t0 -= kTile) {
+    const Fetched<T, LPC, true, true> now = next;
+#pragma unroll
+    for (int i = 0; i < S::kSlots; ++i) {
+      const int slot = threadIdx.x + i * S::kThreads, tok = slot / (S::CH / 4), k = (slot % (S::CH / 4)) * 4;
+      if (tok >= kTile) break;
+      const bool there = t0 + tok < end;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float z = now.gate[i][e], delta = there ? softplus(now.dt[i][e] + bias[e]) : 0.0f;
+        steps[tok][k + e] = f32x4{delta, delta * now.x[i][e],
+                                  s.gate.data ? now.dout[i][e] * (z * sigmoid(z)) : now.dout[i][e], 0.0f};
+      }
+    }
+    put_mix<T, LPC>(mix, now.mix);
+    f32x4 h = h_next;
+    __syncthreads();
+    if (t0 - kTile >= start) {
+      next.fetch(s, at, t0 - kTile, end);
+      h_next = load_upto(s.checks + ((at.b * checks + t0 / kTile - 1) * s.d + c) * s.n + n0, left);
+    }
+    f32x4 a[kTile], kept[kTile];   // of the state before: its decay, and what is left of it
+#pragma unroll
+    for (int tok = 0; tok < kTile; ++tok) {
+      const f32x2 st = *(const f32x2*)&steps[tok][ch];
+      const f32x4 w = *(const f32x4*)&mix[tok][n0];
+      const bool begins = now.begins >> tok & 1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        a[tok][e] = exp2_of(st.x * (rate[e] * kLog2e));
+        kept[tok][e] = begins ? 0.0f : a[tok][e] * h[e];
+        h[e] = __builtin_fmaf(st.y, w[e], kept[tok][e]);
+      }
+    }
+#pragma unroll
+    for (int tok = kTile - 1; tok >= 0; --tok) {
+      const f32x4 st = steps[tok][ch];
+      const f32x4 w = *(const f32x4*)&mix[tok][n0], r = *(const f32x4*)&mix[tok][S::NP + n0];
+      float y = 0.0f, into = 0.0f, dd = 0.0f, v[8];
+      const bool begins = now.begins >> tok & 1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float state = __builtin_fmaf(st.y, w[e], kept[tok][e]);
+        g[e] = __builtin_fmaf(r[e], st.z, g[e]);
+        y = __builtin_fmaf(r[e], state, y);
+        into = __builtin_fmaf(g[e], w[e], into);
+        v[e] = g[e] * st.y;
+        v[4 + e] = state * st.z;
+        // of what is left of the state before, whose size may be far below the state's: kept by itself,
+        // as their difference would lose its last bits
+        const float through = g[e] * kept[tok][e];
+        drate[e] = __builtin_fmaf(through, st.x, drate[e]);
+        dd = __builtin_fmaf(through, rate[e], dd);
+        g[e] = begins ? 0.0f : g[e] * a[tok][e];
+      }
+      y = lanes_sum<LPC>(y);
+      into = lanes_sum<LPC>(into);
+      dd = lanes_sum<LPC>(dd);
+      steps[tok][ch] = f32x4{st.x, into, dd, y};
+      Across<LPC>::sum(v, lane);
+#pragma unroll
+      for (int k = 0; k < Across<LPC>::kLeft; ++k) {
+        const int id = Across<LPC>::id(lane, k);
+        sums[wave][tok][(id >> 2) * S::NP + n0 + (id & 3)] = v[k];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < S::kSlots; ++i) {
+      const int slot = threadIdx.x + i * S::kThreads, tok = slot / (S::CH / 4), k = (slot % (S::CH / 4)) * 4;
+      if (tok >= kTile || t0 + tok >= end || at.first + k >= s.dg) continue;
+      f32x4 dx, ddt, dgate;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const f32x4 st = steps[tok][k + e];
+        const float x = now.x[i][e], z = now.gate[i][e], dout = now.dout[i][e];
+        const float one = sigmoid(z), dy = s.gate.data ? dout * (z * one) : dout;
+        dx[e] = __builtin_fmaf(st.x, st.y, skip[e] * dy);
+        ddt[e] = __builtin_fmaf(st.y, x, st.z) * sigmoid(now.dt[i][e] + bias[e]);
+        const float y = __builtin_fmaf(skip[e], x, st.w);
+        dgate[e] = dout * y * (one * (1.0f + z * (1.0f - one)));
+        if (at.first + k + e < s.dg) {
+          dskip[e] = __builtin_fmaf(dy, x, dskip[e]);
+          dbias[e] += ddt[e];
+        }
+      }
+      const int64_t col = (int64_t)at.group * s.dg + at.first + k, to = (at.b * s.t + t0 + tok) * s.d + col;
+      const int own_left = s.dg - at.first - k;
+      store_upto((T*)s.dx + to, dx, own_left);
+      store_upto((T*)s.ddt + to, ddt, own_left);
+      if (s.gate.data) store_upto((T*)s.dgate + to, dgate, own_left);
+    }
+    for (int i = threadIdx.x; i < kTile * 2 * S::NP; i += S::kThreads) {
+      const int tok = i / (2 * S::NP), which = i % (2 * S::NP), n = which % S::NP;
+      if (t0 + tok >= end) continue;
+      float sum = 0.0f;
+#pragma unroll
+      for (int k = 0; k < S::kWaves; ++k) sum += sums[k][tok][which];
+      const int64_t row = (at.b * s.t + t0 + tok) * s.g + at.group;
+      if (s.tiles > 1)
+        s.dmix[((int64_t)(at.first / S::CH) * (s.b * s.t * s.g) + row) * (2 * S::NP) + which] = sum;
+      else if (n < s.n)
+        ((T*)(which < S::NP ? s.dwrite : s.dread))[row * s.n + n] = (T)sum;
+    }
+    __syncthreads();
+  }
+  const int64_t at_part = at.b * s.parts + at.p;
+  if (at.p == 0) store_upto(s.dstate + (at.b * s.d + c) * s.n + n0, g, left);
+  float* params = s.dparams + at_part * ((int64_t)s.d * (s.n + 2));
+  store_upto(params + c * s.n + n0, drate, left);
+  // the threads of the same four channels, one after another
+  f32x4* meet = &steps[0][0];
+  constexpr int kQuads = S::CH / 4, kRows = S::kThreads / kQuads;
+  static_assert(kRows * kQuads <= kTile * S::CH, "the sums of all threads fit the tile's place");
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    meet[threadIdx.x] = which ? dbias : dskip;
+    __syncthreads();
+    if (threadIdx.x < kQuads) {
+      f32x4 sum = meet[threadIdx.x];
+      for (int k = 1; k < kRows; ++k) sum += meet[threadIdx.x + k * kQuads];
+      store_upto(params + (int64_t)s.d * (s.n + which) + (int64_t)at.group * s.dg + own, sum, s.dg - own);
+    }
+    __syncthreads();
+  }
+}
+
+// The sums over a group's blocks of channels, rounded to the result's type.
+template <class T>
+__global__ __launch_bounds__(kBlock) void mix_sums_kernel(Scan s, int np) {
+  const int64_t i = s.item0 + (int64_t)blockIdx.x * kBlock + threadIdx.x, rows = s.b * s.t * s.g, row = i / (2 * np);
+  if (row >= rows) return;
+  const int which = (int)(i - row * 2 * np), n = which % np;
+  if (n >= s.n) return;
+  float sum = 0.0f;
+  for (int k = 0; k < s.tiles; ++k) sum += s.dmix[((int64_t)k * rows + row) * (2 * np) + which];
+  ((T*)(which < np ? s.dwrite : s.dread))[row * s.n + n] = (T)sum;
+}
+
+// One token of every environment: LPC lanes a channel, each with four states, which are read once and
+// written once, bound by that. next may be state itself: a thread writes only what it has read.
+struct Step {
+  const void *x, *dt, *gate, *write, *read;
+  int64_t x_s, dt_s, gate_s, write_s, write_sg, read_s, read_sg, reset_s;
+  const float *rate, *skip, *bias, *state;
+  const uint8_t* reset;
+  void* out;
+  float* next;
+  int64_t count, item0;   // count: environments times channels
+  int32_t d, n, dg;
+};
+
+template <class T, int LPC>
+__global__ __launch_bounds__(kBlock) void step_kernel(Step s) {
+  const int64_t item = s.item0 + (int64_t)blockIdx.x * (kBlock / LPC) + threadIdx.x / LPC;
+  if (item >= s.count) return;   // all of a channel's lanes
+  const int64_t env = (uint32_t)item / (uint32_t)s.d;
+  const int c = (int)(item - env * s.d), group = c / s.dg, n0 = (threadIdx.x % LPC) * 4, left = s.n - n0;
+  const bool begins = s.reset && s.reset[env * s.reset_s];
+  f32x4 h = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (!begins) h = load_upto(s.state + item * s.n + n0, left);
+  const f32x4 rate = load_upto(s.rate + (int64_t)c * s.n + n0, left);
+  const f32x4 w = load_upto((const T*)s.write + env * s.write_s + group * s.write_sg + n0, left);
+  const f32x4 r = load_upto((const T*)s.read + env * s.read_s + group * s.read_sg + n0, left);
+  const float x = (float)((const T*)s.x)[env * s.x_s + c], dt = (float)((const T*)s.dt)[env * s.dt_s + c];
+  const float delta = softplus(dt + (s.bias ? s.bias[c] : 0.0f)), du = delta * x;
+  float y = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    h[e] = __builtin_fmaf(exp2_of(delta * (rate[e] * kLog2e)), h[e], du * w[e]);
+    y = __builtin_fmaf(r[e], h[e], y);
+  }
+  store_upto(s.next + item * s.n + n0, h, left);
+  y = lanes_sum<LPC>(y);
+  if (n0 == 0) {
+    if (s.skip) y = __builtin_fmaf(s.skip[c], x, y);
+    if (s.gate) {
+      const float z = (float)((const T*)s.gate)[env * s.gate_s + c];
+      y *= z * sigmoid(z);
+    }
+    ((T*)s.out)[item] = (T)y;
+  }
+}
+
+namespace {
+bool dims_ok(int32_t dtype, int64_t d, int64_t n, int64_t g) {
+  return (dtype == 0 || dtype == 1) && d >= 1 && d <= 65536 && n >= 1 && n <= kMaxStates && g >= 1 && g <= d && d % g == 0;
+}
+
+bool sequence_ok(int32_t dtype, int64_t b, int64_t t, int32_t d, int32_t n, int32_t g) {
+  return dims_ok(dtype, d, n, g) && b >= 0 && b <= 0x7FFFFFFF && t >= 0 && t <= 0x7FFFFFFF && b * d <= 0x7FFFFFFF;
+}
+
+int64_t blocks_of(const Scan& s, int64_t parts) { return s.b * parts * s.g * s.tiles; }
+
+// Sizes, and the parts of a row: as many as give the card eight waves a CU, no part below 64 tokens.
+int plan(Scan* s, int64_t b, int64_t t, int32_t d, int32_t n, int32_t g) {
+  int cus = 0;
+  const int status = device_cus(&cus);
+  if (status != HIPENVS_OK) return status;
+  const int lpc = lanes_of(n), ch = channels_of(lpc);
+  s->b = b, s->t = t, s->d = d, s->n = n, s->g = g, s->dg = d / g;
+  s->tiles = (s->dg + ch - 1) / ch;
+  const int64_t waves = b * g * s->tiles * (ch * lpc / 64), want = (int64_t)cus * 8;
+  int64_t parts = 1;
+  if (waves > 0 && waves * 2 <= want) {
+    parts = want / waves;
+    if (parts > t / 64) parts = t / 64;
+    if (parts < 1) parts = 1;
+  }
+  s->part = ((t + parts - 1) / parts + kTile - 1) / kTile * kTile;
+  if (s->part < kTile) s->part = kTile;
+  s->parts = t > 0 ? (int32_t)((t + s->part - 1) / s->part) : 1;
+  return HIPENVS_OK;
+}
+
+int64_t round16(int64_t x) { return (x + 15) / 16 * 16; }
+
+// Where the states between the parts lie in `workspace`; the bytes used.
+int64_t lay_parts(Scan* s, char* at) {
+  if (s->parts <= 1) return 0;
+  const int64_t carry = round16(s->b * s->parts * s->d * s->n * 4), spans = round16(s->b * s->parts * s->d * 4);
+  s->carry = (float*)at;
+  s->spans = (float*)(at + carry);
+  s->begun = (uint8_t*)(at + carry + spans);
+  return carry + spans + round16(s->b * s->parts);
+}
+
+// The same of the backward pass, with its partial sums; *between is what the columns' sums need.
+int64_t lay_back(Scan* s, char* at, float** between) {
+  int64_t used = lay_parts(s, at);
+  const int np = 4 * lanes_of(s->n);
+  s->dmix = (float*)(at + used);
+  if (s->tiles > 1) used += round16(s->tiles * s->b * s->t * s->g * 2 * np * 4);
+  s->dparams = (float*)(at + used);
+  const int64_t rows = s->b * s->parts, width = (int64_t)s->d * (s->n + 2);
+  used += round16(rows * width * 4);
+  *between = (float*)(at + used);
+  return used + column_sums_bytes(rows, width);
+}
+
+template <class F>
+int in_launches(Scan s, int64_t blocks, int threads, const F& launch) {
+  const int64_t most = kMostThreads / threads;
+  for (s.item0 = 0; s.item0 < blocks; s.item0 += most) {
+    launch(s, dim3((unsigned)(blocks - s.item0 < most ? blocks - s.item0 : most)));
+    const int status = launch_status();
+    if (status != HIPENVS_OK) return status;
+  }
+  return HIPENVS_OK;
+}
+
+template <class F>
+int for_lanes(int lpc, const F& f) {
+  switch (lpc) {
+    case 1: return f(std::integral_constant<int, 1>());
+    case 2: return f(std::integral_constant<int, 2>());
+    case 4: return f(std::integral_constant<int, 4>());
+    case 8: return f(std::integral_constant<int, 8>());
+    default: return f(std::integral_constant<int, 16>());
+  }
+}
+
+template <bool kBack>
+int join(const Scan& s, hipStream_t stream) {
+  Scan one = s;
+  const int64_t items = s.b * s.d * s.n;
+  for (one.item0 = 0; one.item0 < items; one.item0 += kMostThreads) {
+    const int64_t own = items - one.item0 < kMostThreads ? items - one.item0 : kMostThreads;
+    hipLaunchKernelGGL(join_kernel<kBack>, dim3(grid_for(own)), dim3(kBlock), 0, stream, one);
+    const int status = launch_status();
+    if (status != HIPENVS_OK) return status;
+  }
+  return HIPENVS_OK;
+}
+
+template <class T>
+int forward(const Scan& s, hipStream_t stream) {
+  return for_lanes(lanes_of(s.n), [&](auto lanes) {
+    constexpr int LPC = decltype(lanes)::value, kThreads = Shape<LPC>::kThreads;
+    if (s.parts > 1) {
+      int status = in_launches(s, blocks_of(s, s.parts - 1), kThreads, [&](const Scan& a, dim3 grid) {
+        hipLaunchKernelGGL((forward_kernel<T, LPC, false>), grid, dim3(kThreads), 0, stream, a);
+      });
+      if (status == HIPENVS_OK) status = join<false>(s, stream);
+      if (status != HIPENVS_OK) return status;
+    }
+    return in_launches(s, blocks_of(s, s.parts), kThreads, [&](const Scan& a, dim3 grid) {
+      hipLaunchKernelGGL((forward_kernel<T, LPC, true>), grid, dim3(kThreads), 0, stream, a);
+    });
+  });
+}
+
+template <class T>
+int backward(const Scan& s, hipStream_t stream) {
+  const int walked = for_lanes(lanes_of(s.n), [&](auto lanes) {
+    constexpr int LPC = decltype(lanes)::value, kThreads = Shape<LPC>::kThreads;
+    if (s.parts > 1) {
+      int status = in_launches(s, blocks_of(s, s.parts - 1), kThreads, [&](const Scan& a, dim3 grid) {
+        hipLaunchKernelGGL((passed_kernel<T, LPC>), grid, dim3(kThreads), 0, stream, a);
+      });
+      if (status == HIPENVS_OK) status = join<true>(s, stream);
+      if (status != HIPENVS_OK) return status;
+    }
+    return in_launches(s, blocks_of(s, s.parts), kThreads, [&](const Scan& a, dim3 grid) {
+      hipLaunchKernelGGL((backward_kernel<T, LPC>), grid, dim3(kThreads), 0, stream, a);
+    });
+  });
+  if (walked != HIPENVS_OK || s.tiles <= 1 || s.t == 0) return walked;
+  Scan one = s;
+  const int np = 4 * lanes_of(s.n);
+  const int64_t items = s.b * s.t * s.g * 2 * np;
+  for (one.item0 = 0; one.item0 < items; one.item0 += kMostThreads) {
+    const int64_t own = items - one.item0 < kMostThreads ? items - one.item0 : kMostThreads;
+    hipLaunchKernelGGL(mix_sums_kernel<T>, dim3(grid_for(own)), dim3(kBlock), 0, stream, one, np);
+    const int status = launch_status();
+    if (status != HIPENVS_OK) return status;
+  }
+  return HIPENVS_OK;
+}
+
+// x, dt, gate (and dout): b, t of each; write, read: b, t, g of each; reset: b, t.
+void strided(Scan* s, const int64_t* st, bool back) {
+  s->x.sb = st[0], s->x.st = st[1], s->dt.sb = st[2], s->dt.st = st[3], s->gate.sb = st[4], s->gate.st = st[5];
+  s->write.sb = st[6], s->write.st = st[7], s->write.sg = st[8];
+  s->read.sb = st[9], s->read.st = st[10], s->read.sg = st[11];
+  s->reset_sb = st[12], s->reset_st = st[13];
+  if (back) s->dout.sb = st[14], s->dout.st = st[15];
+}
+}  // namespace
+
+}  // namespace scan
+}  // namespace hipenvs
+
+using namespace hipenvs;
+using namespace hipenvs::scan;
+
+extern "C" int64_t hipenvs_selective_scan_workspace_bytes(int32_t which, int64_t b, int64_t t, int32_t d, int32_t n,
+                                                          int32_t g) {
+  if (!sequence_ok(0, b, t, d, n, g) || which < 0 || which > 2) return -1;
+  if (b == 0) return 0;
+  if (which == 1) return b * ((t + kTile - 1) / kTile) * d * n * (int64_t)sizeof(float);
+  Scan s = {};
+  if (plan(&s, b, t, d, n, g) != HIPENVS_OK) return -1;
+  float* between = nullptr;
+  return which == 0 ? lay_parts(&s, nullptr) : lay_back(&s, nullptr, &between);
+}
+
+extern "C" int hipenvs_selective_scan(int32_t dtype, const void* x, const void* dt, const float* rate,
+                                      const void* write, const void* read, const float* skip, const void* gate,
+                                      const float* dt_bias, const float* state, const uint8_t* reset,
+                                      const int64_t* strides, void* out, float* final_state, float* checks, int64_t b,
+                                      int64_t t, int32_t d, int32_t n, int32_t g, void* workspace,
+                                      int64_t workspace_bytes, hipenvs_stream_t stream) {
+  if (!sequence_ok(dtype, b, t, d, n, g)) return HIPENVS_E_ARG;
+  if (b == 0) return HIPENVS_OK;
+  if (!rate || !final_state || (t > 0 && (!x || !dt || !write || !read || !out || !strides))) return HIPENVS_E_ARG;
+  Scan s = {};
+  const int status = plan(&s, b, t, d, n, g);
+  if (status != HIPENVS_OK) return status;
+  const int64_t need = lay_parts(&s, (char*)workspace);
+  if (need > 0 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)) return HIPENVS_E_ARG;
+  static const int64_t none[14] = {};
+  s.x.data = x, s.dt.data = dt, s.gate.data = t > 0 ? gate : nullptr, s.write.data = write, s.read.data = read;
+  strided(&s, t > 0 ? strides : none, false);
+  s.rate = rate, s.skip = skip, s.bias = dt_bias, s.state = state, s.reset = reset;
+  s.out = out, s.final_state = final_state, s.checks = checks;
+  return dtype == 1 ? forward<__bf16>(s, as_stream(stream)) : forward<float>(s, as_stream(stream));
+}
+
+extern "C" int hipenvs_selective_scan_backward(int32_t dtype, const void* x, const void* dt, const float* rate,
+                                               const void* write, const void* read, const float* skip,
+                                               const void* gate, const float* dt_bias, const uint8_t* reset,
+                                               const void* dout, const float* dfinal, const float* checks,
+                                               const int64_t* strides, void* dx, void* ddt, void* dwrite, void* dread,
+                                               void* dgate, float* dparams, float* dstate, int64_t b, int64_t t,
+                                               int32_t d, int32_t n, int32_t g, void* workspace,
+                                               int64_t workspace_bytes, hipenvs_stream_t stream) {
+  if (!sequence_ok(dtype, b, t, d, n, g)) return HIPENVS_E_ARG;
+  if (!dparams) return HIPENVS_E_ARG;
+  const int64_t width = (int64_t)d * (n + 2);
+  if (b == 0) return column_sums<float>(nullptr, 0, width, 1.0f, dparams, nullptr, as_stream(stream));
+  if (!rate || !dstate || (t > 0 && (!x || !dt || !write || !read || !dout || !checks || !dx || !ddt || !dwrite ||
+                                     !dread || !strides || (gate && !dgate))))
+    return HIPENVS_E_ARG;
+  Scan s = {};
+  int status = plan(&s, b, t, d, n, g);
+  if (status != HIPENVS_OK) return status;
+  float* between = nullptr;
+  const int64_t need = lay_back(&s, (char*)workspace, &between);
+  if (need > 0 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)) return HIPENVS_E_ARG;
+  static const int64_t none[16] = {};
+  s.x.data = x, s.dt.data = dt, s.gate.data = t > 0 ? gate : nullptr, s.write.data = write, s.read.data = read;
+  s.dout.data = dout;
+  strided(&s, t > 0 ? strides : none, true);
+  s.rate = rate, s.skip = skip, s.bias = dt_bias, s.reset = reset, s.dfinal = dfinal;
+  s.checks = const_cast<float*>(checks);
+  s.dx = dx, s.ddt = ddt, s.dwrite = dwrite, s.dread = dread, s.dgate = dgate, s.dstate = dstate;
+  const hipStream_t on = as_stream(stream);
+  status = dtype == 1 ? backward<__bf16>(s, on) : backward<float>(s, on);
+  if (status != HIPENVS_OK) return status;
+  return column_sums<float>(s.dparams, b * s.parts, width, 1.0f, dparams, between, on);
+}
+
+extern "C" int hipenvs_selective_scan_step(int32_t dtype, const void* x, const void* dt, const float* rate,
+                                           const void* write, const void* read, const float* skip, const void* gate,
+                                           const float* dt_bias, const float* state, const uint8_t* reset,
+                                           const int64_t* strides, void* out, float* next_state, int64_t count,
+                                           int32_t d, int32_t n, int32_t g, hipenvs_stream_t stream) {
+  if (!dims_ok(dtype, d, n, g) || count < 0 || count > 0x7FFFFFFF || count * d > 0x7FFFFFFF) return HIPENVS_E_ARG;
+  if (count == 0) return HIPENVS_OK;
+  if (!x || !dt || !rate || !write || !read || !state || !strides || !out || !next_state) return HIPENVS_E_ARG;
+  Step s = {x,          dt,         gate,       write,      read,       strides[0], strides[1], strides[2], strides[3],
+            strides[4], strides[5], strides[6], strides[7], rate,       skip,       dt_bias,    state,      reset,
+            out,        next_state, count * d,  0,          d,          n,          d / g};
+  return for_lanes(lanes_of(n), [&](auto lanes) {
+    constexpr int LPC = decltype(lanes)::value, kChannels = kBlock / LPC;
+    const int64_t most = kMostThreads / kBlock * kChannels;
+    for (s.item0 = 0; s.item0 < s.count; s.item0 += most) {
+      const int64_t own = s.count - s.item0 < most ? s.count - s.item0 : most;
+      const dim3 grid((unsigned)((own + kChannels - 1) / kChannels)), block(kBlock);
+      if (dtype == 1)
+        hipLaunchKernelGGL((step_kernel<__bf16, LPC>), grid, block, 0, as_stream(stream), s);
+      else
+        hipLaunchKernelGGL((step_kernel<float, LPC>), grid, block, 0, as_stream(stream), s);
+      const int status = launch_status();
+      if (status != HIPENVS_OK) return status;
+    }
+    return (int)HIPENVS_OK;
+  });
+}

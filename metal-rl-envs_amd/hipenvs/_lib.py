@@ -79,6 +79,20 @@ SIGNATURES = {
     "hipenvs_adamw_step": [_I32, _I32, _P, _P, _P, _P, _P, _P, ctypes.c_double, ctypes.c_double, ctypes.c_double,
                            ctypes.c_double, _P, _P, _P, _P, _P],
     "hipenvs_adamw_decode": [_P, _P, _P, _P, _I64, _P, _P, _P],
+    "hipenvs_selective_scan": [_I32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I32, _I32,
+                               _I32, _P, _I64, _P],
+    "hipenvs_selective_scan_backward": [_I32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P,
+                                        _P, _P, _I64, _I64, _I32, _I32, _I32, _P, _I64, _P],
+    "hipenvs_selective_scan_step": [_I32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32,
+                                    _P],
+    "hipenvs_causal_conv": [_I32, _P, _P, _P, _P, _P, _P, _I32, _P, _P, _I64, _I64, _I32, _I32, _P],
+    "hipenvs_causal_conv_backward": [_I32, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _P, _P, _P, _I64, _I64, _I32, _I32,
+                                     _P, _I64, _P],
+    "hipenvs_causal_conv_step": [_I32, _P, _I64, _P, _P, _P, _P, _I64, _I32, _P, _P, _I64, _I32, _I32, _P],
+    "hipenvs_embedding": [_I32, _P, _I32, _P, _I64, _F32, _P, _I64, _I64, _I32, _P],
+    "hipenvs_embedding_backward": [_I32, _P, _I32, _P, _I64, _F32, _P, _I64, _I64, _I32, _P, _I64, _P],
+    "hipenvs_log_probs": [_I32, _P, _I64, _P, _P, _P, _P, _I32, _P, _P, _I64, _I64, _P, _I64, _P],
+    "hipenvs_log_probs_backward": [_I32, _P, _I64, _P, _P, _P, _P, _P, _P, _I64, _I64, _P],
 }
 
 # entry points that return a value rather than a status
@@ -86,6 +100,10 @@ VALUE_SIGNATURES = {
     "hipenvs_legged_es_rollout_workspace_bytes": (ctypes.c_int64, [_I32, _I32, _I64]),
     "hipenvs_es_update_workspace_bytes": (ctypes.c_int64, [_I64, _I64]),
     "hipenvs_decay_attention_workspace_bytes": (ctypes.c_int64, [_I32, _I64, _I64, _I32, _I32, _I32]),
+    "hipenvs_selective_scan_workspace_bytes": (ctypes.c_int64, [_I32, _I64, _I64, _I32, _I32, _I32]),
+    "hipenvs_causal_conv_workspace_bytes": (ctypes.c_int64, [_I64, _I64, _I32, _I32]),
+    "hipenvs_embedding_workspace_bytes": (ctypes.c_int64, [_I64, _I64, _I32]),
+    "hipenvs_log_probs_workspace_bytes": (ctypes.c_int64, [_I64, _I64, _I32]),
 }
 
 
