@@ -186,6 +186,24 @@ __global__ __launch_bounds__(kBlock) void short_kernel(LogProbs p) {
   }
 }
 
+// Four values from i on of a row of at least four, at its end or past it the last four: no branch before
+// the load.
+template <class T>
+__device__ __forceinline__ typename Raw<T>::type fetch_piece(const T* x, int64_t i, int64_t v) {
+  return *(const typename Raw<T>::any*)(x + (i < v - 4 ? i : v - 4));
+}
+
+template <class T>
+__device__ __forceinline__ f32x4 piece_values(typename Raw<T>::type raw, int64_t i, int64_t v) {
+  f32x4 x = __builtin_convertvector(raw, f32x4);
+  if (i > v - 4) {   // only a row's last thread
+    const int by = (int)(i - (v - 4));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = by == 1 && e < 3 ? x[(e + 1) & 3] : by == 2 && e < 2 ? x[(e + 2) & 3] : by == 3 ? x[3] : x[e];
+  }
+  return x;
+}
+
 // Long rows: a block takes a part of a row, every wave with its own sums and its own best.
 template <class T>
 __global__ __launch_bounds__(kBlock) void long_kernel(LogProbs p) {
@@ -197,9 +215,11 @@ __global__ __launch_bounds__(kBlock) void long_kernel(LogProbs p) {
   const int64_t first = part * p.part, end = first + p.part < p.v ? first + p.part : p.v;
   Sums a = none();
   Best b = {0, 0};
+  typename Raw<T>::type next = fetch_piece(x, first + threadIdx.x * 4, p.v);
   for (int64_t at = first; at < end; at += kBlock * 4) {
     const int64_t i = at + threadIdx.x * 4;
-    f32x4 own = load_upto(x + i, end - i);
+    f32x4 own = piece_values<T>(next, i, p.v);
+    next = fetch_piece(x, i + kBlock * 4, p.v);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (i + e >= end) own[e] = -__builtin_inff();
@@ -319,11 +339,15 @@ __global__ __launch_bounds__(kBlock) void long_gradient_kernel(Gradient g) {
   const T* x = (const T*)g.logits + row * g.logits_s;
   T* dx = (T*)g.dlogits + row * g.v;
   const RowGradient of(g, row);
+  typename Raw<T>::type pieces[kPiece / (kBlock * 4)];
+#pragma unroll
+  for (int k = 0; k < kPiece / (kBlock * 4); ++k)
+    pieces[k] = fetch_piece(x, first + k * (kBlock * 4) + threadIdx.x * 4, g.v);
 #pragma unroll
   for (int k = 0; k < kPiece / (kBlock * 4); ++k) {
     const int64_t j = first + k * (kBlock * 4) + threadIdx.x * 4;
     if (j >= g.v) break;
-    f32x4 own = load_upto(x + j, g.v - j);
+    f32x4 own = piece_values<T>(pieces[k], j, g.v);
 #pragma unroll
     for (int e = 0; e < 4; ++e) own[e] = of.of(own[e], j + e);
     store_upto(dx + j, own, g.v - j);

@@ -65,25 +65,45 @@ __device__ __forceinline__ void push(f32x4 (&hist)[W], f32x4 x, bool begins) {
   hist[0] = x;
 }
 
+// kCount tokens of a row as they come, all of their loads in flight; those past `end` read the last one.
+template <class T, int kCount>
+struct Piece {
+  typename Raw<T>::type x[kCount], dout[kCount];
+  uint8_t begins[kCount];
+
+  template <bool kBack = false>
+  __device__ __forceinline__ void fetch(const Conv& s, int64_t b, int64_t first, int64_t end, int c) {
+#pragma unroll
+    for (int k = 0; k < kCount; ++k) {
+      const int64_t t = first + k < end ? first + k : end - 1;
+      x[k] = fetch4((const T*)s.x + b * s.x_sb + t * s.x_st, c, s.d);
+      if (kBack) dout[k] = fetch4((const T*)s.dout + b * s.dout_sb + t * s.dout_st, c, s.d);
+      begins[k] = s.reset ? s.reset[b * s.reset_sb + t * s.reset_st] : 0;
+    }
+  }
+
+  __device__ __forceinline__ f32x4 value(int k, int c, int d) const { return values<T>(x[k], c, d); }
+};
+
 // hist as it is before token t0: hist[i] then holds the value of token t0 - 1 - i.
 template <class T, int W>
 __device__ __forceinline__ void before(const Conv& s, int64_t b, int64_t t0, int c, f32x4 (&hist)[W]) {
   const int left = s.d - c;
 #pragma unroll
   for (int i = 0; i < W; ++i) hist[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  if (t0 == 0) {   // a run has more tokens than a window: the others' windows lie within the row
 #pragma unroll
-  for (int k = 0; k < W - 1; ++k) {
-    const int64_t t = t0 - (W - 1) + k;
-    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-    bool begins = false;
-    if (t >= 0) {
-      x = load_upto((const T*)s.x + b * s.x_sb + t * s.x_st + c, left);
-      begins = s.reset && s.reset[b * s.reset_sb + t * s.reset_st];
-    } else if (s.state) {
-      x = load_upto(s.state + (b * (W - 1) + (t + W - 1)) * s.d + c, left);
+    for (int k = 0; k < W - 1; ++k) {
+      f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (s.state) x = load_upto(s.state + (b * (W - 1) + k) * s.d + c, left);
+      push(hist, x, false);
     }
-    push(hist, x, begins);
+    return;
   }
+  Piece<T, W> piece;
+  piece.fetch(s, b, t0 - (W - 1), t0, c);
+#pragma unroll
+  for (int k = 0; k < W - 1; ++k) push(hist, piece.value(k, c, s.d), piece.begins[k]);
 }
 
 template <class T, int W>
@@ -96,19 +116,15 @@ __global__ __launch_bounds__(kBlock) void forward_kernel(Conv s) {
   const Taps<W> taps(s, c);
   f32x4 hist[W];
   before<T, W>(s, b, t0, c, hist);
+  Piece<T, kAhead> next;
+  if (t0 < t1) next.fetch(s, b, t0, t1, c);
   for (int64_t first = t0; first < t1; first += kAhead) {
-    f32x4 x[kAhead];
-    bool begins[kAhead];
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int64_t t = first + k;
-      x[k] = load_upto((const T*)s.x + b * s.x_sb + t * s.x_st + c, t < t1 ? left : 0);
-      begins[k] = t < t1 && s.reset && s.reset[b * s.reset_sb + t * s.reset_st];
-    }
+    const Piece<T, kAhead> now = next;
+    if (first + kAhead < t1) next.fetch(s, b, first + kAhead, t1, c);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       if (first + k >= t1) break;
-      push(hist, x[k], begins[k]);
+      push(hist, now.value(k, c, s.d), now.begins[k]);
       f32x4 pre = taps.apply(hist);
       if (s.silu)
 #pragma unroll
@@ -147,23 +163,18 @@ __global__ __launch_bounds__(kBlock) void backward_kernel(Conv s) {
       store_upto((T*)s.dx + (b * s.t + u) * s.d + c, grad, left);
   };
   int since = W;   // tokens since the episode's first
+  Piece<T, kAhead> next;
+  if (t0 < past) next.template fetch<true>(s, b, t0, past, c);
   for (int64_t first = t0; first < past; first += kAhead) {
-    f32x4 x[kAhead], dout[kAhead];
-    bool begins[kAhead];
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int64_t t = first + k;
-      x[k] = load_upto((const T*)s.x + b * s.x_sb + t * s.x_st + c, t < past ? left : 0);
-      dout[k] = load_upto((const T*)s.dout + b * s.dout_sb + t * s.dout_st + c, t < past ? left : 0);
-      begins[k] = t < past && s.reset && s.reset[b * s.reset_sb + t * s.reset_st];
-    }
+    const Piece<T, kAhead> now = next;
+    if (first + kAhead < past) next.template fetch<true>(s, b, first + kAhead, past, c);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       const int64_t t = first + k;
       if (t >= past) break;
-      push(hist, x[k], begins[k]);
-      since = begins[k] ? 0 : since < W ? since + 1 : W;
-      f32x4 grad = dout[k];
+      push(hist, now.value(k, c, s.d), now.begins[k]);
+      since = now.begins[k] ? 0 : since < W ? since + 1 : W;
+      f32x4 grad = values<T>(now.dout[k], c, s.d);
       if (s.silu) {
         const f32x4 pre = taps.apply(hist);
 #pragma unroll

@@ -30,11 +30,11 @@ __global__ __launch_bounds__(kBlock) void lookup_kernel(Tokens tokens, const T* 
   if (i >= count) return;
   const int c = (int)(item - i * quads) * 4;
   const int64_t token = tokens[i];
-  f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (token >= v)
-    x += __builtin_nanf("");
-  else if (token >= 0)
-    x = load_upto(table + token * table_sv + c, d - c) * scale;
+  const bool there = token >= 0 && token < v;
+  const f32x4 row = values<T>(fetch4(table + (there ? token : 0) * table_sv, c, d), c, d);
+  f32x4 x;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = there ? row[e] * scale : token < 0 ? 0.0f : __builtin_nanf("");
   store_upto(out + i * d + c, x, d - c);
 }
 
@@ -200,15 +200,12 @@ __global__ __launch_bounds__(kBlock) void chunks_kernel(Sums s) {
   constexpr int kAhead = 8;
   for (int64_t i0 = first; i0 < end; i0 += kAhead) {
     uint32_t key[kAhead];
-    f32x4 x[kAhead];
+    typename Raw<T>::type x[kAhead];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      key[k] = none;
-      x[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      if (i0 + k < end) {
-        key[k] = s.keys[i0 + k];
-        if (key[k] != none) x[k] = load_upto((const T*)s.dout + (int64_t)s.places[i0 + k] * s.dout_s + c, left);
-      }
+    for (int k = 0; k < kAhead; ++k) {   // past the end, the last one: all loads in flight
+      const int64_t i = i0 + k < end ? i0 + k : end - 1;
+      key[k] = s.keys[i];
+      x[k] = fetch4((const T*)s.dout + (int64_t)s.places[i] * s.dout_s, c, s.d);
     }
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
@@ -218,7 +215,7 @@ __global__ __launch_bounds__(kBlock) void chunks_kernel(Sums s) {
         current = key[k], opened = true;
         sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       }
-      sum += x[k];
+      sum += values<T>(x[k], c, s.d);
     }
   }
   close(true);
@@ -250,9 +247,10 @@ __global__ __launch_bounds__(kBlock) void across_kernel(Sums s) {
   for (int64_t k0 = chunk + 1; k0 <= last; k0 += kAhead) {
     f32x4 x[kAhead];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) x[k] = load_upto(s.firsts + (k0 + k) * s.d + c, k0 + k <= last ? left : 0);
+    for (int k = 0; k < kAhead; ++k) x[k] = fetch4(s.firsts + (k0 + k < last ? k0 + k : last) * s.d, c, s.d);
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) sum += x[k];
+    for (int k = 0; k < kAhead; ++k)
+      if (k0 + k <= last) sum += values<float>(x[k], c, s.d);
   }
   store_upto((T*)s.dtable + (int64_t)key * s.d + c, sum * s.scale, left);
 }

@@ -39,6 +39,47 @@ __device__ __forceinline__ f32x4 load_upto(const T* p, int64_t n) {
   return x;
 }
 
+// Four values as they lie in memory: a conversion where they are loaded would wait for each load by
+// itself.
+template <class T>
+struct Raw;
+template <>
+struct Raw<float> {
+  typedef f32x4 type;
+  typedef f32x4_any any;
+};
+template <>
+struct Raw<__bf16> {
+  typedef bf16x4 type;
+  typedef bf16x4_any any;
+};
+
+// Four values from `c` (a multiple of 4 below d) on of a row of d; at a ragged end the row's last four,
+// which values() puts in their place. No branch depends on the lane, so a caller's loads are all in
+// flight at once.
+template <class T>
+__device__ __forceinline__ typename Raw<T>::type fetch4(const T* row, int c, int d) {
+  if (d >= 4) return *(const typename Raw<T>::any*)(row + (c < d - 4 ? c : d - 4));
+  return typename Raw<T>::type{row[0], row[d > 1 ? 1 : 0], row[d > 2 ? 2 : 0], row[0]};
+}
+
+// What fetch4 read, as float32; zeros past the row.
+template <class T>
+__device__ __forceinline__ f32x4 values(typename Raw<T>::type raw, int c, int d) {
+  const f32x4 x = __builtin_convertvector(raw, f32x4);
+  if (d % 4 == 0) return x;
+  const int left = d - c, by = d >= 4 && left < 4 ? 4 - left : 0;
+  f32x4 y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    y[e] = x[e];
+#pragma unroll
+    for (int k = 1; e + k < 4; ++k) y[e] = by == k ? x[e + k] : y[e];
+    y[e] = e < left ? y[e] : 0.0f;
+  }
+  return y;
+}
+
 template <class T>
 __device__ __forceinline__ void store_upto(T* p, f32x4 x, int64_t n) {
   if (n >= 4) {

@@ -69,58 +69,64 @@ __device__ __forceinline__ Place place_of(const Scan& s, int64_t item, int parts
   return {item / parts, (int)(item % parts), group, tile * channels};
 }
 
-// A tile's inputs, in the registers of the threads that fetch them.
+// A tile's inputs as they come, in the registers of the threads that fetch them. Tokens past the end
+// read the last one, channels and states past theirs the last four, and whoever uses them leaves
+// them out.
 template <class T, int LPC, bool kOut, bool kBack>
 struct Fetched {
   using S = Shape<LPC>;
-  f32x4 x[S::kSlots], dt[S::kSlots], gate[S::kSlots], dout[S::kSlots];
-  f32x4 mix[S::kMixSlots];
-  uint32_t begins;   // a bit a token
+  typename Raw<T>::type x[S::kSlots], dt[S::kSlots], gate[S::kSlots], dout[S::kSlots], mix[S::kMixSlots];
+  uint8_t begins;   // of the token of this lane
 
   __device__ __forceinline__ void fetch(const Scan& s, const Place& at, int64_t t0, int64_t end) {
+    const int64_t last = end - 1;
 #pragma unroll
     for (int i = 0; i < S::kSlots; ++i) {
-      const int slot = threadIdx.x + i * S::kThreads, tok = slot / (S::CH / 4), c = at.first + (slot % (S::CH / 4)) * 4;
-      const int64_t t = t0 + tok;
-      const int left = (tok < kTile && t < end) ? s.dg - c : 0;
-      const int64_t col = (int64_t)at.group * s.dg + c;
-      x[i] = load_upto((const T*)s.x.data + at.b * s.x.sb + t * s.x.st + col, left);
-      dt[i] = load_upto((const T*)s.dt.data + at.b * s.dt.sb + t * s.dt.st + col, left);
-      if (left <= 0) dt[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      if (kOut || kBack) {
-        gate[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (s.gate.data) gate[i] = load_upto((const T*)s.gate.data + at.b * s.gate.sb + t * s.gate.st + col, left);
-      }
-      if (kBack) dout[i] = load_upto((const T*)s.dout.data + at.b * s.dout.sb + t * s.dout.st + col, left);
+      const int slot = threadIdx.x + i * S::kThreads, c = at.first + (slot % (S::CH / 4)) * 4;
+      const int own = c < s.dg ? c : 0;
+      int64_t t = t0 + slot / (S::CH / 4);
+      t = t < last ? t : last;
+      const int64_t col = (int64_t)at.group * s.dg;
+      x[i] = fetch4((const T*)s.x.data + at.b * s.x.sb + t * s.x.st + col, own, s.dg);
+      dt[i] = fetch4((const T*)s.dt.data + at.b * s.dt.sb + t * s.dt.st + col, own, s.dg);
+      if ((kOut || kBack) && s.gate.data)
+        gate[i] = fetch4((const T*)s.gate.data + at.b * s.gate.sb + t * s.gate.st + col, own, s.dg);
+      if (kBack) dout[i] = fetch4((const T*)s.dout.data + at.b * s.dout.sb + t * s.dout.st + col, own, s.dg);
     }
 #pragma unroll
     for (int i = 0; i < S::kMixSlots; ++i) {
-      const int slot = threadIdx.x + i * S::kThreads, tok = slot / (2 * LPC), part = slot % (2 * LPC);
-      const int64_t t = t0 + tok;
-      const bool there = tok < kTile && t < end;
-      const int n0 = (part % LPC) * 4;
+      const int slot = threadIdx.x + i * S::kThreads, part = slot % (2 * LPC), n0 = (part % LPC) * 4;
+      int64_t t = t0 + slot / (2 * LPC);
+      t = t < last ? t : last;
       const Mix& m = part < LPC ? s.write : s.read;
-      mix[i] = load_upto((const T*)m.data + at.b * m.sb + t * m.st + at.group * m.sg + n0, there ? s.n - n0 : 0);
+      mix[i] = fetch4((const T*)m.data + at.b * m.sb + t * m.st + at.group * m.sg, n0 < s.n ? n0 : 0, s.n);
     }
     begins = 0;
     if (s.reset) {
-      const int tok = threadIdx.x & 63;
-      bool here = false;
-      if (tok < kTile && t0 + tok < end) here = s.reset[at.b * s.reset_sb + (t0 + tok) * s.reset_st] != 0;
-      begins = (uint32_t)__builtin_amdgcn_ballot_w64(here);
+      int64_t t = t0 + (threadIdx.x & 63);
+      t = t < last ? t : last;
+      begins = s.reset[at.b * s.reset_sb + t * s.reset_st];
+    }
+  }
+
+  // a bit for each token of the tile that begins an episode
+  __device__ __forceinline__ uint32_t begun(int64_t t0, int64_t end) const {
+    const int tok = threadIdx.x & 63;
+    return (uint32_t)__builtin_amdgcn_ballot_w64(tok < kTile && t0 + tok < end && begins != 0);
+  }
+
+  // write and read to LDS, zeros past the end and past the states
+  __device__ __forceinline__ void put_mix(const Scan& s, int64_t t0, int64_t end, float (*to)[8 * LPC]) const {
+#pragma unroll
+    for (int i = 0; i < S::kMixSlots; ++i) {
+      const int slot = threadIdx.x + i * S::kThreads, tok = slot / (2 * LPC), part = slot % (2 * LPC);
+      const int n0 = (part % LPC) * 4;
+      f32x4 m = values<T>(mix[i], n0 < s.n ? n0 : 0, s.n);
+      if (t0 + tok >= end || n0 >= s.n) m = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (tok < kTile) *(f32x4*)&to[tok][part * 4] = m;
     }
   }
 };
-
-template <class T, int LPC>
-__device__ __forceinline__ void put_mix(float (*mix)[8 * LPC], const f32x4* from) {
-  using S = Shape<LPC>;
-#pragma unroll
-  for (int i = 0; i < S::kMixSlots; ++i) {
-    const int slot = threadIdx.x + i * S::kThreads, tok = slot / (2 * LPC), part = slot % (2 * LPC);
-    if (tok < kTile) *(f32x4*)&mix[tok][part * 4] = from[i];
-  }
-}
 
 __device__ __forceinline__ f32x4 per_channel(const float* of, int64_t c, int left, float otherwise) {
   f32x4 r = {otherwise, otherwise, otherwise, otherwise};

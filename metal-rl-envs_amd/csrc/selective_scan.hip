@@ -35,31 +35,34 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void forward_kernel(Scan s) {
   float span = 0.0f;
   uint32_t begun = 0;
   Fetched<T, LPC, kOut, false> next;
-  next.fetch(s, at, start, end);
+  if (start < end) next.fetch(s, at, start, end);
   for (int64_t t0 = start; t0 < end; t0 += kTile) {
     const Fetched<T, LPC, kOut, false> now = next;
+    const uint32_t begins = now.begun(t0, end);
 #pragma unroll
     for (int i = 0; i < S::kSlots; ++i) {
       const int slot = threadIdx.x + i * S::kThreads, tok = slot / (S::CH / 4), k = (slot % (S::CH / 4)) * 4;
       if (tok >= kTile) break;
-      const bool there = t0 + tok < end;
+      const bool there = t0 + tok < end && at.first + k < s.dg;   // past the end the state stays
+      const f32x4 x = values<T>(now.x[i], there ? at.first + k : 0, s.dg);
+      const f32x4 dt = values<T>(now.dt[i], there ? at.first + k : 0, s.dg);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float delta = there ? softplus(now.dt[i][e] + bias[e]) : 0.0f;   // past the end the state stays
-        steps[tok][k + e] = f32x2{delta, delta * now.x[i][e]};
+        const float delta = softplus(dt[e] + bias[e]);
+        steps[tok][k + e] = there ? f32x2{delta, delta * x[e]} : f32x2{0.0f, 0.0f};
       }
     }
-    put_mix<T, LPC>(mix, now.mix);
+    now.put_mix(s, t0, end, mix);
     __syncthreads();
     if (t0 + kTile < end) next.fetch(s, at, t0 + kTile, end);
     if (kOut && s.checks)
       store_upto(s.checks + ((at.b * checks + t0 / kTile) * s.d + c) * s.n + n0, h, left);
-    begun |= now.begins;
+    begun |= begins;
 #pragma unroll
     for (int tok = 0; tok < kTile; ++tok) {
       const f32x2 st = steps[tok][ch];
       const f32x4 w = *(const f32x4*)&mix[tok][n0];
-      if (now.begins >> tok & 1) h = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (begins >> tok & 1) h = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       float y = 0.0f;
       f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
       if (kOut) r = *(const f32x4*)&mix[tok][S::NP + n0];
@@ -79,11 +82,13 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void forward_kernel(Scan s) {
       for (int i = 0; i < S::kSlots; ++i) {
         const int slot = threadIdx.x + i * S::kThreads, tok = slot / (S::CH / 4), k = (slot % (S::CH / 4)) * 4;
         if (tok >= kTile || t0 + tok >= end || at.first + k >= s.dg) continue;
-        f32x4 o;
+        const f32x4 x = values<T>(now.x[i], at.first + k, s.dg);
+        f32x4 o, z = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (s.gate.data) z = values<T>(now.gate[i], at.first + k, s.dg);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          o[e] = __builtin_fmaf(skip[e], now.x[i][e], steps[tok][k + e].x);
-          if (s.gate.data) o[e] *= now.gate[i][e] * sigmoid(now.gate[i][e]);
+          o[e] = __builtin_fmaf(skip[e], x[e], steps[tok][k + e].x);
+          if (s.gate.data) o[e] *= z[e] * sigmoid(z[e]);
         }
         const int64_t col = (int64_t)at.group * s.dg + at.first + k;
         store_upto((T*)s.out + (at.b * s.t + t0 + tok) * s.d + col, o, s.dg - at.first - k);
@@ -167,29 +172,35 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void passed_kernel(Scan s) {
   next.fetch(s, at, t0, end);
   for (; t0 >= start; t0 -= kTile) {
     const Fetched<T, LPC, true, true> now = next;
+    const uint32_t begins = now.begun(t0, end);
 #pragma unroll
     for (int i = 0; i < S::kSlots; ++i) {
       const int slot = threadIdx.x + i * S::kThreads, tok = slot / (S::CH / 4), k = (slot % (S::CH / 4)) * 4;
       if (tok >= kTile) break;
-      const bool there = t0 + tok < end;
+      const bool there = t0 + tok < end && at.first + k < s.dg;
+      const int c0 = there ? at.first + k : 0;
+      const f32x4 dt = values<T>(now.dt[i], c0, s.dg);
+      f32x4 dy = values<T>(now.dout[i], c0, s.dg);
+      if (s.gate.data) {
+        const f32x4 z = values<T>(now.gate[i], c0, s.dg);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float z = now.gate[i][e];
-        steps[tok][k + e] = f32x2{there ? softplus(now.dt[i][e] + bias[e]) : 0.0f,
-                                  s.gate.data ? now.dout[i][e] * (z * sigmoid(z)) : now.dout[i][e]};
+        for (int e = 0; e < 4; ++e) dy[e] *= z[e] * sigmoid(z[e]);
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        steps[tok][k + e] = there ? f32x2{softplus(dt[e] + bias[e]), dy[e]} : f32x2{0.0f, 0.0f};
     }
-    put_mix<T, LPC>(mix, now.mix);
+    now.put_mix(s, t0, end, mix);
     __syncthreads();
     if (t0 - kTile >= start) next.fetch(s, at, t0 - kTile, end);
-    begun |= now.begins;
+    begun |= begins;
 #pragma unroll
     for (int tok = kTile - 1; tok >= 0; --tok) {
       const f32x2 st = steps[tok][ch];
       const f32x4 r = *(const f32x4*)&mix[tok][S::NP + n0];
 #pragma unroll
       for (int e = 0; e < 4; ++e) g[e] = exp2_of(st.x * rate[e]) * __builtin_fmaf(r[e], st.y, g[e]);
-      if (now.begins >> tok & 1) g = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (begins >> tok & 1) g = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       span += st.x;
     }
     __syncthreads();
@@ -210,7 +221,7 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void passed_kernel(Scan s) {
 // Sums over a channel's states stay within its lanes; sums over channels go lane by lane within the
 // wave, then through LDS, then (dmix) over the blocks of a group.
 template <class T, int LPC>
-__global__ __launch_bounds__(Shape<LPC>::kThreads) void backward_kernel(Scan s) {
+__global__ __launch_bounds__(Shape<LPC>::kThreads, 2) void backward_kernel(Scan s) {
   using S = Shape<LPC>;
   __shared__ __attribute__((aligned(16))) f32x4 steps[kTile][S::CH];   // delta, delta x, dy; then delta, sum g write, ddelta's states, y
   __shared__ __attribute__((aligned(16))) float mix[kTile][2 * S::NP];
@@ -242,19 +253,27 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void backward_kernel(Scan s) 
   }
   for (; end > start && t0 >= start; t0 -= kTile) {
     const Fetched<T, LPC, true, true> now = next;
+    const uint32_t begun = now.begun(t0, end);
 #pragma unroll
     for (int i = 0; i < S::kSlots; ++i) {
       const int slot = threadIdx.x + i * S::kThreads, tok = slot / (S::CH / 4), k = (slot % (S::CH / 4)) * 4;
       if (tok >= kTile) break;
-      const bool there = t0 + tok < end;
+      const bool there = t0 + tok < end && at.first + k < s.dg;
+      const int c0 = there ? at.first + k : 0;
+      const f32x4 x = values<T>(now.x[i], c0, s.dg), dt = values<T>(now.dt[i], c0, s.dg);
+      f32x4 dy = values<T>(now.dout[i], c0, s.dg);
+      if (s.gate.data) {
+        const f32x4 z = values<T>(now.gate[i], c0, s.dg);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dy[e] *= z[e] * sigmoid(z[e]);
+      }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float z = now.gate[i][e], delta = there ? softplus(now.dt[i][e] + bias[e]) : 0.0f;
-        steps[tok][k + e] = f32x4{delta, delta * now.x[i][e],
-                                  s.gate.data ? now.dout[i][e] * (z * sigmoid(z)) : now.dout[i][e], 0.0f};
+        const float delta = softplus(dt[e] + bias[e]);
+        steps[tok][k + e] = there ? f32x4{delta, delta * x[e], dy[e], 0.0f} : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       }
     }
-    put_mix<T, LPC>(mix, now.mix);
+    now.put_mix(s, t0, end, mix);
     f32x4 h = h_next;
     __syncthreads();
     if (t0 - kTile >= start) {
@@ -266,7 +285,7 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void backward_kernel(Scan s) 
     for (int tok = 0; tok < kTile; ++tok) {
       const f32x2 st = *(const f32x2*)&steps[tok][ch];
       const f32x4 w = *(const f32x4*)&mix[tok][n0];
-      const bool begins = now.begins >> tok & 1;
+      const bool begins = begun >> tok & 1;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         a[tok][e] = exp2_of(st.x * (rate[e] * kLog2e));
@@ -279,7 +298,7 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void backward_kernel(Scan s) 
       const f32x4 st = steps[tok][ch];
       const f32x4 w = *(const f32x4*)&mix[tok][n0], r = *(const f32x4*)&mix[tok][S::NP + n0];
       float y = 0.0f, into = 0.0f, dd = 0.0f, v[8];
-      const bool begins = now.begins >> tok & 1;
+      const bool begins = begun >> tok & 1;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float state = __builtin_fmaf(st.y, w[e], kept[tok][e]);
@@ -311,18 +330,20 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void backward_kernel(Scan s) 
     for (int i = 0; i < S::kSlots; ++i) {
       const int slot = threadIdx.x + i * S::kThreads, tok = slot / (S::CH / 4), k = (slot % (S::CH / 4)) * 4;
       if (tok >= kTile || t0 + tok >= end || at.first + k >= s.dg) continue;
-      f32x4 dx, ddt, dgate;
+      const f32x4 x = values<T>(now.x[i], at.first + k, s.dg), dt = values<T>(now.dt[i], at.first + k, s.dg);
+      const f32x4 dout = values<T>(now.dout[i], at.first + k, s.dg);
+      f32x4 dx, ddt, dgate, z = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (s.gate.data) z = values<T>(now.gate[i], at.first + k, s.dg);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const f32x4 st = steps[tok][k + e];
-        const float x = now.x[i][e], z = now.gate[i][e], dout = now.dout[i][e];
-        const float one = sigmoid(z), dy = s.gate.data ? dout * (z * one) : dout;
+        const float one = sigmoid(z[e]), dy = s.gate.data ? dout[e] * (z[e] * one) : dout[e];
         dx[e] = __builtin_fmaf(st.x, st.y, skip[e] * dy);
-        ddt[e] = __builtin_fmaf(st.y, x, st.z) * sigmoid(now.dt[i][e] + bias[e]);
-        const float y = __builtin_fmaf(skip[e], x, st.w);
-        dgate[e] = dout * y * (one * (1.0f + z * (1.0f - one)));
+        ddt[e] = __builtin_fmaf(st.y, x[e], st.z) * sigmoid(dt[e] + bias[e]);
+        const float y = __builtin_fmaf(skip[e], x[e], st.w);
+        dgate[e] = dout[e] * y * (one * (1.0f + z[e] * (1.0f - one)));
         if (at.first + k + e < s.dg) {
-          dskip[e] = __builtin_fmaf(dy, x, dskip[e]);
+          dskip[e] = __builtin_fmaf(dy, x[e], dskip[e]);
           dbias[e] += ddt[e];
         }
       }
