@@ -50,10 +50,16 @@ struct Sums {
     }
   }
 
-  __device__ __forceinline__ void add(float x) {   // after raise(x)
-    const float t = at_least(x - (m == -__builtin_inff() ? 0.0f : m)), e = exp2_of(t * kLog2e);
-    s += e;
-    w = __builtin_fmaf(e, t, w);
+  // after raise(x): values of which none is above m. The exponential of a NaN keeps it in both sums.
+  template <int kCount>
+  __device__ __forceinline__ void add(const float (&x)[kCount]) {
+    const float base = m == -__builtin_inff() ? 0.0f : m;
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+      const float t = x[i] - base, e = exp2_of(t * kLog2e);
+      s += e;
+      w = __builtin_fmaf(e, __builtin_fmaxf(t, -160.0f), w);
+    }
   }
 
   __device__ __forceinline__ void join(Sums o) {
@@ -104,6 +110,40 @@ __device__ __forceinline__ uint64_t lane_value(uint64_t v, int lane) {
          (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
 }
 
+template <int kXor>
+__device__ __forceinline__ uint32_t key_from_xor(uint32_t v, int lane) {
+  if constexpr (kXor == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return lane & 32 ? r[0] : r[1];
+  } else if constexpr (kXor == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return lane & 16 ? r[0] : r[1];
+  } else {
+    return __float_as_uint(from_xor<kXor>(__uint_as_float(v)));
+  }
+}
+
+// One step of a bitonic sort over the wave, largest first in runs of kRun.
+template <int kRun, int kXor>
+__device__ __forceinline__ void sort_step(uint32_t& v, int lane) {
+  const uint32_t o = key_from_xor<kXor>(v, lane);
+  const bool larger = ((lane & kXor) == 0) == (kRun == 64 || (lane & kRun) == 0);
+  v = larger ? (v > o ? v : o) : (v < o ? v : o);
+  if constexpr (kXor > 1) sort_step<kRun, kXor / 2>(v, lane);
+}
+
+__device__ __forceinline__ void sort_wave(uint32_t& v, int lane) {
+  sort_step<2, 1>(v, lane), sort_step<4, 2>(v, lane), sort_step<8, 4>(v, lane);
+  sort_step<16, 8>(v, lane), sort_step<32, 16>(v, lane), sort_step<64, 32>(v, lane);
+}
+
+// The lane before's value; 0 in the first.
+__device__ __forceinline__ uint64_t from_before(uint64_t v) {
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), 0x138, 0xF, 0xF, false);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x138, 0xF, 0xF, false);
+  return (uint64_t)hi << 32 | lo;
+}
+
 // The most likely so far, one a lane, in order; empty places are 0.
 struct Best {
   uint64_t own, least;   // least: the last that is kept, in all lanes
@@ -114,11 +154,30 @@ struct Best {
     while (better) {
       const uint64_t v = lane_value(candidate, __builtin_ctzll(better));
       const int at = __popcll(__builtin_amdgcn_ballot_w64(own > v));
-      const uint64_t before = __shfl_up(own, 1);
+      const uint64_t before = from_before(own);
       own = lane < at ? own : lane == at ? v : before;
       least = lane_value(own, top - 1);
       better &= better - 1;
       better &= __builtin_amdgcn_ballot_w64(candidate > least);
+    }
+  }
+
+  // A batch of candidates, a lane's largest given. At least `top` candidates reach the top-th of the
+  // lanes' largest, so the rest of the first batch need no look: about 25 of 1,024 are offered for 20
+  // where each wave's running best alone would take about 100.
+  template <class F>
+  __device__ __forceinline__ void offer_batch(uint64_t largest, int count, int top, int lane, const F& candidate) {
+    uint32_t bound = (uint32_t)(least >> 32);
+    if (__builtin_amdgcn_ballot_w64((uint32_t)(largest >> 32) >= bound && largest != 0) == 0) return;
+    if (least == 0) {
+      uint32_t sorted = (uint32_t)(largest >> 32);
+      sort_wave(sorted, lane);
+      bound = (uint32_t)__builtin_amdgcn_readlane((int)sorted, top - 1);
+    }
+#pragma unroll
+    for (int e = 0; e < count; ++e) {
+      const uint64_t c = candidate(e);
+      offer((uint32_t)(c >> 32) >= bound ? c : 0, top, lane);
     }
   }
 };
@@ -159,8 +218,7 @@ __global__ __launch_bounds__(kBlock) void short_kernel(LogProbs p) {
   for (int e = 0; e < E; ++e) own[e] = e * G + lane < v ? (float)x[e * G + lane] : -__builtin_inff();
 #pragma unroll
   for (int e = 0; e < E; ++e) a.m = own[e] > a.m ? own[e] : a.m;
-#pragma unroll
-  for (int e = 0; e < E; ++e) a.add(own[e]);
+  a.add(own);
   a = joined<G>(a);
   if (lane == 0) write_row(p, row, a, token >= 0 && token < p.v ? (float)x[token] : 0.0f, token);
   uint32_t taken = 0;
@@ -204,34 +262,55 @@ __device__ __forceinline__ f32x4 piece_values(typename Raw<T>::type raw, int64_t
   return x;
 }
 
-// Long rows: a block takes a part of a row, every wave with its own sums and its own best.
+// Long rows: a block takes a part of a row, every wave with its own sums and its own best, in batches of
+// 16 values a lane, the next one's loads in flight.
 template <class T>
 __global__ __launch_bounds__(kBlock) void long_kernel(LogProbs p) {
   __shared__ Sums sums[4];
   __shared__ uint64_t best[4][kMaxTop];
+  constexpr int kLoads = 4, kStep = kBlock * 4;
   const int64_t item = p.item0 + blockIdx.x, row = item / p.parts;
   const int part = (int)(item - row * p.parts), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const T* x = (const T*)p.logits + row * p.logits_s;
   const int64_t first = part * p.part, end = first + p.part < p.v ? first + p.part : p.v;
   Sums a = none();
   Best b = {0, 0};
-  typename Raw<T>::type next = fetch_piece(x, first + threadIdx.x * 4, p.v);
-  for (int64_t at = first; at < end; at += kBlock * 4) {
-    const int64_t i = at + threadIdx.x * 4;
-    f32x4 own = piece_values<T>(next, i, p.v);
-    next = fetch_piece(x, i + kBlock * 4, p.v);
+  typename Raw<T>::type next[kLoads];
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (i + e >= end) own[e] = -__builtin_inff();
+  for (int k = 0; k < kLoads; ++k) next[k] = fetch_piece(x, first + k * kStep + threadIdx.x * 4, p.v);
+  for (int64_t at = first; at < end; at += kLoads * kStep) {
+    const int64_t i = at + threadIdx.x * 4;
+    float own[kLoads * 4];
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) {
+      const f32x4 y = piece_values<T>(next[k], i + k * kStep, p.v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) own[k * 4 + e] = y[e];
+    }
+    if (at + kLoads * kStep < end)
+#pragma unroll
+      for (int k = 0; k < kLoads; ++k) next[k] = fetch_piece(x, i + (kLoads + k) * kStep, p.v);
+    if (at + kLoads * kStep > end)
+#pragma unroll
+      for (int k = 0; k < kLoads; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (i + k * kStep + e >= end) own[k * 4 + e] = -__builtin_inff();
     float m = own[0];
 #pragma unroll
-    for (int e = 1; e < 4; ++e) m = own[e] > m ? own[e] : m;
+    for (int e = 1; e < kLoads * 4; ++e) m = own[e] > m ? own[e] : m;
     a.raise(m);
+    a.add(own);
+    if (p.top) {
+      const auto candidate = [&](int e) {
+        const int64_t j = i + (e / 4) * kStep + e % 4;
+        return j < end ? ranked(own[e], (uint32_t)j) : 0;
+      };
+      uint64_t largest = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) a.add(own[e]);
-    if (p.top)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) b.offer(i + e < end ? ranked(own[e], (uint32_t)(i + e)) : 0, p.top, lane);
+      for (int e = 0; e < kLoads * 4; ++e) largest = candidate(e) > largest ? candidate(e) : largest;
+      b.offer_batch(largest, kLoads * 4, p.top, lane, candidate);
+    }
   }
   a = joined<64>(a);
   if (lane == 0) sums[wave] = a;
@@ -273,11 +352,22 @@ __global__ __launch_bounds__(64) void join_kernel(LogProbs p) {
     }
   }
   a = joined<64>(a);
-  if (p.top)
-    for (int64_t k0 = 0; k0 < (int64_t)p.parts * p.top; k0 += 64) {
-      const int64_t k = k0 + lane;
-      b.offer(k < (int64_t)p.parts * p.top ? p.tops[row * p.parts * p.top + k] : 0, p.top, lane);
+  if (p.top) {
+    constexpr int kLoads = 16;
+    const int64_t count = (int64_t)p.parts * p.top;
+    const uint64_t* from = p.tops + row * count;
+    for (int64_t k0 = lane; k0 - lane < count; k0 += kLoads * 64) {
+      uint64_t own[kLoads], largest = 0;
+#pragma unroll
+      for (int e = 0; e < kLoads; ++e) own[e] = from[k0 + e * 64 < count ? k0 + e * 64 : count - 1];
+#pragma unroll
+      for (int e = 0; e < kLoads; ++e) {
+        own[e] = k0 + e * 64 < count ? own[e] : 0;
+        largest = own[e] > largest ? own[e] : largest;
+      }
+      b.offer_batch(largest, kLoads, p.top, lane, [&](int e) { return own[e]; });
     }
+  }
   const int64_t token = p.tokens[row];
   if (lane == 0)
     write_row(p, row, a, token >= 0 && token < p.v ? (float)((const T*)p.logits)[row * p.logits_s + token] : 0.0f, token);

@@ -61,8 +61,12 @@ struct Taps {
 template <int W>
 __device__ __forceinline__ void push(f32x4 (&hist)[W], f32x4 x, bool begins) {
 #pragma unroll
-  for (int i = W - 1; i > 0; --i) hist[i] = begins ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : hist[i - 1];
+  for (int i = W - 1; i > 0; --i) hist[i] = hist[i - 1];
   hist[0] = x;
+  if (__builtin_amdgcn_ballot_w64(begins)) {   // seldom
+#pragma unroll
+    for (int i = 1; i < W; ++i) hist[i] = begins ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : hist[i];
+  }
 }
 
 // kCount tokens of a row as they come, all of their loads in flight; those past `end` read the last one.
@@ -128,7 +132,7 @@ __global__ __launch_bounds__(kBlock) void forward_kernel(Conv s) {
       f32x4 pre = taps.apply(hist);
       if (s.silu)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) pre[e] *= sigmoid(pre[e]);
+        for (int e = 0; e < 4; ++e) pre[e] *= sigmoid_for<T>(pre[e]);
       store_upto((T*)s.out + (b * s.t + first + k) * s.d + c, pre, left);
     }
   }
@@ -179,23 +183,33 @@ __global__ __launch_bounds__(kBlock) void backward_kernel(Conv s) {
         const f32x4 pre = taps.apply(hist);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float one = sigmoid(pre[e]);
+          const float one = sigmoid_for<T>(pre[e]);
           grad[e] *= one * (1.0f + pre[e] * (1.0f - one));
         }
       }
 #pragma unroll
       for (int i = W - 1; i > 0; --i) late[i] = late[i - 1];
       late[0] = zero;
+      if (__builtin_amdgcn_ballot_w64(since < W - 1 || t >= t1) == 0) {   // whole windows of own tokens
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        if (i <= since)
+        for (int i = 0; i < W; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) late[i][e] = __builtin_fmaf(taps.w[W - 1 - i][e], grad[e], late[i][e]);
-        if (t < t1 && i <= since)
+          for (int e = 0; e < 4; ++e) {
+            late[i][e] = __builtin_fmaf(taps.w[W - 1 - i][e], grad[e], late[i][e]);
+            dweight[i][e] = __builtin_fmaf(hist[i][e], grad[e], dweight[i][e]);
+          }
+        dbias += grad;
+      } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) dweight[i][e] = __builtin_fmaf(hist[i][e], grad[e], dweight[i][e]);
+        for (int i = 0; i < W; ++i)
+          if (i <= since)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              late[i][e] = __builtin_fmaf(taps.w[W - 1 - i][e], grad[e], late[i][e]);
+              if (t < t1) dweight[i][e] = __builtin_fmaf(hist[i][e], grad[e], dweight[i][e]);
+            }
+        if (t < t1) dbias += grad;
       }
-      if (t < t1) dbias += grad;
       emit(t - (W - 1), late[W - 1]);
     }
   }
@@ -245,7 +259,7 @@ __global__ __launch_bounds__(kBlock) void step_kernel(Step s) {
   f32x4 pre = taps.apply(hist);
   if (s.silu)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) pre[e] *= sigmoid(pre[e]);
+    for (int e = 0; e < 4; ++e) pre[e] *= sigmoid_for<T>(pre[e]);
   store_upto((T*)s.out + env * s.d + c, pre, left);
 #pragma unroll
   for (int k = 0; k < W - 1; ++k) store_upto(s.next + (env * (W - 1) + k) * s.d + c, hist[W - 2 - k], left);

@@ -40,15 +40,15 @@ __global__ __launch_bounds__(kBlock) void lookup_kernel(Tokens tokens, const T* 
 
 // ---- sorting the tokens ---------------------------------------------------------------
 // Least digit first, 8 bits a pass, each pass stable, so a token's places stay in their order. Keys
-// are tokens, v where there is none. A pass counts the digits of each tile of 4,096, sums the
-// counts up, digit by digit and tile by tile, and moves each key with its place.
+// are tokens, v where there is none. A pass counts the digits of each tile of kRounds x 256 keys,
+// sums each digit's counts up over the tiles, and moves each key with its place.
 
-constexpr int kDigit = 256, kRounds = 16, kSortTile = kBlock * kRounds;
+constexpr int kDigit = 256;
 
 struct Sort {
   Tokens tokens;
   const uint32_t *keys, *places;   // null in the first pass: the tokens as they come
-  uint32_t *keys_out, *places_out, *counts;
+  uint32_t *keys_out, *places_out, *counts;   // counts (256, tiles), then the digits' totals (256)
   int64_t count, v, tiles;
   int shift;
 
@@ -59,33 +59,36 @@ struct Sort {
   }
 };
 
+// The tile's digits.
+template <int kRounds>
 __global__ __launch_bounds__(kBlock) void count_kernel(Sort s) {
   __shared__ uint32_t counts[kDigit];
   counts[threadIdx.x] = 0;
   __syncthreads();
-  const int64_t first = (int64_t)blockIdx.x * kSortTile;
+  const int64_t first = (int64_t)blockIdx.x * (kBlock * kRounds) + threadIdx.x;
+  uint32_t keys[kRounds];
+#pragma unroll
   for (int r = 0; r < kRounds; ++r) {
-    const int64_t i = first + r * kBlock + threadIdx.x;
-    if (i < s.count) atomicAdd(&counts[(s.key(i) >> s.shift) & 255], 1u);
+    const int64_t i = first + r * kBlock;
+    keys[r] = s.key(i < s.count ? i : s.count - 1);
   }
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r)
+    if (first + r * kBlock < s.count) atomicAdd(&counts[(keys[r] >> s.shift) & 255], 1u);
   __syncthreads();
   s.counts[threadIdx.x * s.tiles + blockIdx.x] = counts[threadIdx.x];
 }
 
-// counts -> the sums of those before, in place; one block.
-__global__ __launch_bounds__(1024) void sum_up_kernel(uint32_t* counts, int64_t n) {
-  __shared__ uint32_t totals[16];
+// A block for each digit: its tiles' counts -> the sums of those before, in place; and its total.
+__global__ __launch_bounds__(kBlock) void sum_up_kernel(Sort s) {
+  __shared__ uint32_t totals[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t* counts = s.counts + blockIdx.x * s.tiles;
   uint32_t before = 0;
-  for (int64_t first = 0; first < n; first += 4096) {
-    const int64_t i = first + threadIdx.x * 4;
-    uint32_t x[4], sum = 0;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      x[k] = i + k < n ? counts[i + k] : 0u;
-      sum += x[k];
-    }
-    uint32_t upto = sum;
+  for (int64_t first = 0; first < s.tiles; first += kBlock) {
+    const int64_t i = first + threadIdx.x;
+    const uint32_t own = i < s.tiles ? counts[i] : 0u;
+    uint32_t upto = own;
 #pragma unroll
     for (int step = 1; step < 64; step *= 2) {
       const uint32_t other = __shfl_up(upto, step);
@@ -93,37 +96,48 @@ __global__ __launch_bounds__(1024) void sum_up_kernel(uint32_t* counts, int64_t 
     }
     if (lane == 63) totals[wave] = upto;
     __syncthreads();
-    uint32_t at = before + upto - sum, all = 0;
-    for (int k = 0; k < 16; ++k) {
-      if (k < wave) at += totals[k];
-      all += totals[k];
-    }
+    uint32_t at = before + upto - own;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      if (i + k < n) counts[i + k] = at;
-      at += x[k];
+      if (k < wave) at += totals[k];
+      before += totals[k];
     }
-    before += all;
+    if (i < s.tiles) counts[i] = at;
     __syncthreads();
   }
+  if (threadIdx.x == 0) s.counts[kDigit * s.tiles + blockIdx.x] = before;
 }
 
+template <int kRounds>
 __global__ __launch_bounds__(kBlock) void move_kernel(Sort s) {
-  __shared__ uint32_t at[4][kDigit];
+  __shared__ uint32_t at[4][kDigit], totals[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int k = 0; k < 4; ++k) at[k][threadIdx.x] = 0;
-  __syncthreads();
-  // a wave moves 1,024 neighbouring keys, so that the order of the places holds across waves
-  const int64_t first = (int64_t)blockIdx.x * kSortTile + wave * (kRounds * 64) + lane;
-  uint32_t keys[kRounds];
+  // a wave moves kRounds x 64 neighbouring keys, so that the order of the places holds across waves
+  const int64_t first = (int64_t)blockIdx.x * (kBlock * kRounds) + wave * (kRounds * 64) + lane;
+  uint32_t keys[kRounds], places[kRounds];
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
-    const int64_t i = first + r * 64;
-    keys[r] = i < s.count ? s.key(i) : 0u;
-    if (i < s.count) atomicAdd(&at[wave][(keys[r] >> s.shift) & 255], 1u);
+    const int64_t i = first + r * 64 < s.count ? first + r * 64 : s.count - 1;
+    keys[r] = s.key(i);
+    places[r] = s.places ? s.places[i] : (uint32_t)i;
   }
+  // the keys of lower digits, by the digits' totals
+  const uint32_t total = s.counts[kDigit * s.tiles + threadIdx.x];
+  uint32_t upto = total;
+#pragma unroll
+  for (int step = 1; step < 64; step *= 2) {
+    const uint32_t other = __shfl_up(upto, step);
+    if (lane >= step) upto += other;
+  }
+  if (lane == 63) totals[wave] = upto;
+  for (int k = 0; k < 4; ++k) at[k][threadIdx.x] = 0;
   __syncthreads();
-  uint32_t base = s.counts[threadIdx.x * s.tiles + blockIdx.x];
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r)
+    if (first + r * 64 < s.count) atomicAdd(&at[wave][(keys[r] >> s.shift) & 255], 1u);
+  uint32_t base = upto - total + s.counts[threadIdx.x * s.tiles + blockIdx.x];
+  for (int k = 0; k < wave; ++k) base += totals[k];
+  __syncthreads();
   for (int k = 0; k < 4; ++k) {
     const uint32_t own = at[k][threadIdx.x];
     at[k][threadIdx.x] = base;
@@ -144,7 +158,7 @@ __global__ __launch_bounds__(kBlock) void move_kernel(Sort s) {
     if (i < s.count) {
       const uint32_t to = at[wave][digit] + (uint32_t)__popcll(below);
       s.keys_out[to] = keys[r];
-      s.places_out[to] = s.places ? s.places[i] : (uint32_t)i;
+      s.places_out[to] = places[r];
     }
     __builtin_amdgcn_wave_barrier();
     if (i < s.count && below == 0) at[wave][digit] += (uint32_t)__popcll(same);
@@ -157,7 +171,7 @@ __global__ __launch_bounds__(kBlock) void move_kernel(Sort s) {
 // that they name. A run of equal keys within the chunk is finished; the sum of one that reaches over
 // the chunk's beginning or end goes to `firsts` or `lasts`, which a second kernel adds in order.
 
-constexpr int kChunk = 64;
+constexpr int kChunk = 32;
 
 struct Sums {
   const uint32_t *keys, *places;
@@ -221,38 +235,102 @@ __global__ __launch_bounds__(kBlock) void chunks_kernel(Sums s) {
   close(true);
 }
 
-// The runs that reach over chunks, each by the group of the chunk where it begins.
+// The runs that reach over chunks, each by the block of the chunk where it begins: its groups of lanes
+// add up every so many of its chunks, and their sums meet in LDS.
 template <class T>
 __global__ __launch_bounds__(kBlock) void across_kernel(Sums s) {
-  const int64_t item = (s.item0 + (int64_t)blockIdx.x * kBlock + threadIdx.x) / s.group;
-  const int64_t chunk = item / s.columns;
-  const int quad = (int)(item - chunk * s.columns) * s.group + threadIdx.x % s.group;
-  if (chunk >= s.chunks || quad >= s.quads) return;
-  const int c = quad * 4, left = s.d - c;
+  __shared__ f32x4 share[kBlock];
+  const int64_t item = s.item0 + blockIdx.x, chunk = item / s.columns;
+  const int rows = kBlock / s.group, row = threadIdx.x / s.group, lane = threadIdx.x % s.group;
+  const int quad = (int)(item - chunk * s.columns) * s.group + lane, c = (quad < s.quads ? quad : 0) * 4;
   const int64_t first = chunk * kChunk, end = first + kChunk;
-  if (end >= s.count) return;
+  if (end >= s.count) return;   // the conditions are the block's
   const uint32_t key = s.keys[end - 1];
   if (key == (uint32_t)s.v || s.keys[end] != key) return;
   if (first > 0 && s.keys[first - 1] == key) return;   // it began before this chunk
-  // the last of its chunks: the one that holds the last key not above it
   int64_t low = end, high = s.count;                    // keys[low] == key, keys[high] > key
   while (high - low > 1) {
     const int64_t mid = (low + high) / 2;
     if (s.keys[mid] == key) low = mid;
     else high = mid;
   }
-  const int64_t last = low / kChunk;
-  f32x4 sum = load_upto(s.lasts + chunk * s.d + c, left);
+  const int64_t last = low / kChunk;   // of the run's chunks
+  f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (row == 0) sum = values<float>(fetch4(s.lasts + chunk * s.d, c, s.d), c, s.d);
   constexpr int kAhead = 8;
-  for (int64_t k0 = chunk + 1; k0 <= last; k0 += kAhead) {
+  for (int64_t k0 = chunk + 1 + row; k0 <= last; k0 += kAhead * rows) {
     f32x4 x[kAhead];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) x[k] = fetch4(s.firsts + (k0 + k < last ? k0 + k : last) * s.d, c, s.d);
+    for (int k = 0; k < kAhead; ++k) {
+      const int64_t at = k0 + k * rows;
+      x[k] = fetch4(s.firsts + (at < last ? at : last) * s.d, c, s.d);
+    }
+    f32x4 some = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k)
-      if (k0 + k <= last) sum += values<float>(x[k], c, s.d);
+    for (int k = 0; k < kAhead; ++k) {
+      const f32x4 y = values<float>(x[k], c, s.d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) some[e] += k0 + k * rows <= last ? y[e] : 0.0f;
+    }
+    sum += some;
   }
-  store_upto((T*)s.dtable + (int64_t)key * s.d + c, sum * s.scale, left);
+  share[threadIdx.x] = sum;
+  __syncthreads();
+  for (int half = rows / 2; half > 0; half /= 2) {
+    if (row < half) share[threadIdx.x] += share[threadIdx.x + half * s.group];
+    __syncthreads();
+  }
+  if (row == 0 && quad < s.quads) store_upto((T*)s.dtable + (int64_t)key * s.d + c, share[threadIdx.x] * s.scale, s.d - c);
+}
+
+// ---- small tables ----------------------------------------------------------------------
+// A table of at most kSmall rows is summed without sorting: each group of lanes of a block takes every
+// so many of its tokens and adds their rows to sums of its own in LDS; a block's groups then meet, and the
+// blocks' sums are the rows of a matrix whose columns are added up. 524,288 tokens of 3 x 64 float32:
+// TIMING_SMALL against TIMING_SORTED sorted.
+
+constexpr int kSmall = 16;
+
+struct Small {
+  Tokens tokens;
+  const void* dout;
+  float* partial;   // (blocks, v d)
+  int64_t count, each, dout_s;   // each: tokens of a block
+  int32_t v, d, quads, group;
+};
+
+template <class T>
+__global__ __launch_bounds__(kBlock) void small_kernel(Small s) {
+  extern __shared__ __attribute__((aligned(16))) f32x4 sums[];   // (v, 256)
+  const int rows = kBlock / s.group, row = threadIdx.x / s.group;
+  const int quad = blockIdx.y * s.group + threadIdx.x % s.group, c = (quad < s.quads ? quad : 0) * 4;
+  for (int k = 0; k < s.v; ++k) sums[k * kBlock + threadIdx.x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const int64_t first = blockIdx.x * s.each, end = first + s.each < s.count ? first + s.each : s.count;
+  constexpr int kAhead = 8;
+  for (int64_t i0 = first + row; i0 < end; i0 += kAhead * rows) {
+    int64_t token[kAhead];
+    typename Raw<T>::type x[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int64_t i = i0 + k * rows < end ? i0 + k * rows : end - 1;
+      token[k] = s.tokens[i];
+      x[k] = fetch4((const T*)s.dout + i * s.dout_s, c, s.d);
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const f32x4 y = values<T>(x[k], c, s.d);
+      if (i0 + k * rows < end && token[k] >= 0 && token[k] < s.v) sums[token[k] * kBlock + threadIdx.x] += y;
+    }
+  }
+  __syncthreads();
+  for (int half = rows / 2; half > 0; half /= 2) {
+    if (row < half)
+      for (int k = 0; k < s.v; ++k) sums[k * kBlock + threadIdx.x] += sums[k * kBlock + threadIdx.x + half * s.group];
+    __syncthreads();
+  }
+  if (row == 0 && quad < s.quads)
+    for (int k = 0; k < s.v; ++k)
+      store_upto(s.partial + ((int64_t)blockIdx.x * s.v + k) * s.d + c, sums[k * kBlock + threadIdx.x], s.d - c);
 }
 
 namespace {
@@ -263,14 +341,33 @@ bool sizes_ok(int32_t dtype, int64_t count, int64_t v, int32_t d) {
 
 int64_t round16(int64_t x) { return (x + 15) / 16 * 16; }
 
+int group_of(int quads) {
+  int group = 1;
+  while (group < 64 && group < quads) group *= 2;
+  return group;
+}
+
+// Blocks of a small table's sums: four a CU of 256, but no fewer than eight tokens for a group of lanes.
+int64_t small_blocks(int64_t count, int32_t d) {
+  const int64_t least = 8 * (kBlock / group_of((d + 3) / 4)), blocks = (count + least - 1) / least;
+  return blocks < 1024 ? blocks : 1024;
+}
+
+int rounds_of(int64_t count) { return count < (1 << 18) ? 4 : 16; }
+
 struct Laid {
   int64_t keys, counts, partial, bytes;
 };
 
-// keys and places twice, the digits' counts, the chunks' partial sums
-Laid lay(int64_t count, int32_t d) {
-  const int64_t tiles = (count + kSortTile - 1) / kSortTile, chunks = (count + kChunk - 1) / kChunk;
-  Laid l = {round16(count * 4), round16(tiles * kDigit * 4), round16(chunks * d * 4), 0};
+// keys and places twice, the digits' counts, the chunks' partial sums; or a small table's partial sums
+Laid lay(int64_t count, int64_t v, int32_t d) {
+  if (v <= kSmall) {
+    const int64_t blocks = small_blocks(count, d), partial = round16(blocks * v * d * 4);
+    return {0, 0, partial, partial + column_sums_bytes(blocks, v * d)};
+  }
+  const int64_t tile = kBlock * rounds_of(count), tiles = (count + tile - 1) / tile;
+  const int64_t chunks = (count + kChunk - 1) / kChunk;
+  Laid l = {round16(count * 4), round16((tiles + 1) * kDigit * 4), round16(chunks * d * 4), 0};
   l.bytes = 4 * l.keys + l.counts + 2 * l.partial;
   return l;
 }
@@ -287,45 +384,70 @@ int in_launches(int64_t items, const F& launch) {
 }
 
 template <class T>
+int small_gradient(Tokens tokens, const void* dout, int64_t dout_s, float scale, void* dtable, int64_t count, int64_t v,
+                   int32_t d, char* workspace, hipStream_t stream) {
+  const Laid l = lay(count, v, d);
+  const int quads = (d + 3) / 4, group = group_of(quads);
+  const int64_t blocks = small_blocks(count, d);
+  const Small s = {tokens, dout, (float*)workspace, count, (count + blocks - 1) / blocks, dout_s, (int32_t)v, d, quads,
+                   group};
+  hipLaunchKernelGGL(small_kernel<T>, dim3((unsigned)blocks, (unsigned)((quads + group - 1) / group)), dim3(kBlock),
+                     (size_t)v * kBlock * sizeof(f32x4), stream, s);
+  const int status = launch_status();
+  if (status != HIPENVS_OK) return status;
+  return column_sums<T>(s.partial, blocks, v * d, scale, (T*)dtable, (float*)(workspace + l.partial), stream);
+}
+
+template <class T>
 int gradient(Tokens tokens, const void* dout, int64_t dout_s, float scale, void* dtable, int64_t count, int64_t v,
              int32_t d, char* workspace, hipStream_t stream) {
+  if (v <= kSmall && count > 0)
+    return small_gradient<T>(tokens, dout, dout_s, scale, dtable, count, v, d, workspace, stream);
   const int64_t values = v * d;
   int status = in_launches((values + 3) / 4, [&](int64_t item0, dim3 grid) {
     hipLaunchKernelGGL(clear_kernel<T>, grid, dim3(kBlock), 0, stream, (T*)dtable, values, item0);
   });
   if (status != HIPENVS_OK || count == 0) return status;
-  const Laid l = lay(count, d);
+  const Laid l = lay(count, v, d);
+  const int rounds = rounds_of(count);
   uint32_t* keys[2] = {(uint32_t*)workspace, (uint32_t*)(workspace + l.keys)};
   uint32_t* places[2] = {(uint32_t*)(workspace + 2 * l.keys), (uint32_t*)(workspace + 3 * l.keys)};
   Sort sort = {tokens, nullptr, nullptr, nullptr, nullptr, (uint32_t*)(workspace + 4 * l.keys), count, v,
-               (count + kSortTile - 1) / kSortTile, 0};
+               (count + kBlock * rounds - 1) / (kBlock * rounds), 0};
   int to = 0;
   for (; (v >> sort.shift) > 0; sort.shift += 8, to ^= 1) {
     sort.keys_out = keys[to], sort.places_out = places[to];
-    const dim3 tiles((unsigned)sort.tiles);
-    hipLaunchKernelGGL(count_kernel, tiles, dim3(kBlock), 0, stream, sort);
-    hipLaunchKernelGGL(sum_up_kernel, dim3(1), dim3(1024), 0, stream, sort.counts, sort.tiles * kDigit);
-    hipLaunchKernelGGL(move_kernel, tiles, dim3(kBlock), 0, stream, sort);
+    const dim3 tiles((unsigned)sort.tiles), block(kBlock);
+    if (rounds == 4)
+      hipLaunchKernelGGL(count_kernel<4>, tiles, block, 0, stream, sort);
+    else
+      hipLaunchKernelGGL(count_kernel<16>, tiles, block, 0, stream, sort);
+    hipLaunchKernelGGL(sum_up_kernel, dim3(kDigit), block, 0, stream, sort);
+    if (rounds == 4)
+      hipLaunchKernelGGL(move_kernel<4>, tiles, block, 0, stream, sort);
+    else
+      hipLaunchKernelGGL(move_kernel<16>, tiles, block, 0, stream, sort);
     status = launch_status();
     if (status != HIPENVS_OK) return status;
     sort.keys = keys[to], sort.places = places[to];
   }
   char* partial = workspace + 4 * l.keys + l.counts;
-  const int quads = (d + 3) / 4;
-  int group = 1;
-  while (group < 64 && group < quads) group *= 2;
+  const int quads = (d + 3) / 4, group = group_of(quads);
   Sums s = {sort.keys, sort.places, dout, dtable, (float*)partial, (float*)(partial + l.partial), count, v,
             (count + kChunk - 1) / kChunk, dout_s, 0, d, quads, group, (quads + group - 1) / group, scale};
-  const int64_t items = s.chunks * s.columns * group;
-  status = in_launches(items, [&](int64_t item0, dim3 grid) {
+  status = in_launches(s.chunks * s.columns * group, [&](int64_t item0, dim3 grid) {
     s.item0 = item0;
     hipLaunchKernelGGL(chunks_kernel<T>, grid, dim3(kBlock), 0, stream, s);
   });
   if (status != HIPENVS_OK || s.chunks == 1) return status;
-  return in_launches(items, [&](int64_t item0, dim3 grid) {
-    s.item0 = item0;
+  const int64_t blocks = s.chunks * s.columns, most = kMostThreads / kBlock;
+  for (s.item0 = 0; s.item0 < blocks; s.item0 += most) {
+    const dim3 grid((unsigned)(blocks - s.item0 < most ? blocks - s.item0 : most));
     hipLaunchKernelGGL(across_kernel<T>, grid, dim3(kBlock), 0, stream, s);
-  });
+    status = launch_status();
+    if (status != HIPENVS_OK) return status;
+  }
+  return HIPENVS_OK;
 }
 }  // namespace
 
@@ -355,7 +477,7 @@ extern "C" int hipenvs_embedding(int32_t dtype, const void* tokens, int32_t toke
 
 extern "C" int64_t hipenvs_embedding_workspace_bytes(int64_t count, int64_t v, int32_t d) {
   if (!sizes_ok(0, count, v, d)) return -1;
-  return count == 0 ? 0 : lay(count, d).bytes;
+  return count == 0 ? 0 : lay(count, v, d).bytes;
 }
 
 extern "C" int hipenvs_embedding_backward(int32_t dtype, const void* tokens, int32_t token_bytes, const void* dout,
@@ -364,7 +486,7 @@ extern "C" int hipenvs_embedding_backward(int32_t dtype, const void* tokens, int
                                           hipenvs_stream_t stream) {
   if (!sizes_ok(dtype, count, v, d) || (token_bytes != 4 && token_bytes != 8) || !dtable) return HIPENVS_E_ARG;
   if (count > 0 && (!tokens || !dout || !workspace || ((uintptr_t)workspace & 15) ||
-                    workspace_bytes < lay(count, d).bytes))
+                    workspace_bytes < lay(count, v, d).bytes))
     return HIPENVS_E_ARG;
   const Tokens of = {tokens, token_bytes == 8};
   return dtype == 1 ? gradient<__bf16>(of, dout, dout_s, scale, dtable, count, v, d, (char*)workspace, as_stream(stream))

@@ -88,7 +88,7 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void forward_kernel(Scan s) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           o[e] = __builtin_fmaf(skip[e], x[e], steps[tok][k + e].x);
-          if (s.gate.data) o[e] *= z[e] * sigmoid(z[e]);
+          if (s.gate.data) o[e] *= z[e] * sigmoid_for<T>(z[e]);
         }
         const int64_t col = (int64_t)at.group * s.dg + at.first + k;
         store_upto((T*)s.out + (at.b * s.t + t0 + tok) * s.d + col, o, s.dg - at.first - k);
@@ -184,7 +184,7 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void passed_kernel(Scan s) {
       if (s.gate.data) {
         const f32x4 z = values<T>(now.gate[i], c0, s.dg);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) dy[e] *= z[e] * sigmoid(z[e]);
+        for (int e = 0; e < 4; ++e) dy[e] *= z[e] * sigmoid_for<T>(z[e]);
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -265,7 +265,7 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads, 2) void backward_kernel(Scan 
       if (s.gate.data) {
         const f32x4 z = values<T>(now.gate[i], c0, s.dg);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) dy[e] *= z[e] * sigmoid(z[e]);
+        for (int e = 0; e < 4; ++e) dy[e] *= z[e] * sigmoid_for<T>(z[e]);
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -337,9 +337,9 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads, 2) void backward_kernel(Scan 
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const f32x4 st = steps[tok][k + e];
-        const float one = sigmoid(z[e]), dy = s.gate.data ? dout[e] * (z[e] * one) : dout[e];
+        const float one = sigmoid_for<T>(z[e]), dy = s.gate.data ? dout[e] * (z[e] * one) : dout[e];
         dx[e] = __builtin_fmaf(st.x, st.y, skip[e] * dy);
-        ddt[e] = __builtin_fmaf(st.y, x[e], st.z) * sigmoid(dt[e] + bias[e]);
+        ddt[e] = __builtin_fmaf(st.y, x[e], st.z) * sigmoid_for<T>(dt[e] + bias[e]);
         const float y = __builtin_fmaf(skip[e], x[e], st.w);
         dgate[e] = dout[e] * y * (one * (1.0f + z[e] * (1.0f - one)));
         if (at.first + k + e < s.dg) {
@@ -439,7 +439,7 @@ __global__ __launch_bounds__(kBlock) void step_kernel(Step s) {
     if (s.skip) y = __builtin_fmaf(s.skip[c], x, y);
     if (s.gate) {
       const float z = (float)((const T*)s.gate)[env * s.gate_s + c];
-      y *= z * sigmoid(z);
+      y *= z * sigmoid_for<T>(z);
     }
     ((T*)s.out)[item] = (T)y;
   }
