@@ -32,8 +32,11 @@ struct LogProbs {
 };
 
 // Differences of logits reach -inf, and a zero times that is no number; exp(-160) and
-// 2^-160 are 0 in float32.
-__device__ __forceinline__ float at_least(float x) { return x < -160.0f ? -160.0f : x; }
+// 2^-160 are 0 in float32. The median of three is one instruction, with a NaN's others where one is a
+// NaN; the exponential beside it keeps the NaN.
+__device__ __forceinline__ float at_least(float x) { return __builtin_amdgcn_fmed3f(x, -160.0f, __builtin_inff()); }
+
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, __builtin_inff()); }
 
 // m, s and w of some of a row's values.
 struct Sums {
@@ -58,7 +61,7 @@ struct Sums {
     for (int i = 0; i < kCount; ++i) {
       const float t = x[i] - base, e = exp2_of(t * kLog2e);
       s += e;
-      w = __builtin_fmaf(e, __builtin_fmaxf(t, -160.0f), w);
+      w = __builtin_fmaf(e, at_least(t), w);
     }
   }
 
@@ -217,7 +220,7 @@ __global__ __launch_bounds__(kBlock) void short_kernel(LogProbs p) {
 #pragma unroll
   for (int e = 0; e < E; ++e) own[e] = e * G + lane < v ? (float)x[e * G + lane] : -__builtin_inff();
 #pragma unroll
-  for (int e = 0; e < E; ++e) a.m = own[e] > a.m ? own[e] : a.m;
+  for (int e = 0; e < E; ++e) a.m = larger(own[e], a.m);
   a.add(own);
   a = joined<G>(a);
   if (lane == 0) write_row(p, row, a, token >= 0 && token < p.v ? (float)x[token] : 0.0f, token);
@@ -247,15 +250,16 @@ __global__ __launch_bounds__(kBlock) void short_kernel(LogProbs p) {
 // Four values from i on of a row of at least four, at its end or past it the last four: no branch before
 // the load.
 template <class T>
-__device__ __forceinline__ typename Raw<T>::type fetch_piece(const T* x, int64_t i, int64_t v) {
+__device__ __forceinline__ typename Raw<T>::type fetch_piece(const T* x, uint32_t i, uint32_t v) {
   return *(const typename Raw<T>::any*)(x + (i < v - 4 ? i : v - 4));
 }
 
-template <class T>
-__device__ __forceinline__ f32x4 piece_values(typename Raw<T>::type raw, int64_t i, int64_t v) {
+// What fetch_piece read, kEnd: where the row's end may be among it.
+template <class T, bool kEnd>
+__device__ __forceinline__ f32x4 piece_values(typename Raw<T>::type raw, uint32_t i, uint32_t v) {
   f32x4 x = __builtin_convertvector(raw, f32x4);
-  if (i > v - 4) {   // only a row's last thread
-    const int by = (int)(i - (v - 4));
+  if (kEnd && i > v - 4) {   // only a row's last thread
+    const uint32_t by = i - (v - 4);
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = by == 1 && e < 3 ? x[(e + 1) & 3] : by == 2 && e < 2 ? x[(e + 2) & 3] : by == 3 ? x[3] : x[e];
   }
@@ -264,67 +268,66 @@ __device__ __forceinline__ f32x4 piece_values(typename Raw<T>::type raw, int64_t
 
 // Long rows: a block takes a part of a row, every wave with its own sums and its own best, in batches of
 // 16 values a lane, the next one's loads in flight.
-template <class T>
-__global__ __launch_bounds__(kBlock) void long_kernel(LogProbs p) {
+template <class T, bool kTop>
+__global__ __launch_bounds__(kBlock, kTop ? 4 : 8) void long_kernel(LogProbs p) {
   __shared__ Sums sums[4];
-  __shared__ uint64_t best[4][kMaxTop];
-  constexpr int kLoads = 4, kStep = kBlock * 4;
+  __shared__ uint64_t best[4][kTop ? kMaxTop : 1];
+  constexpr uint32_t kLoads = 4, kStep = kBlock * 4, kBatch = kLoads * kStep;
   const int64_t item = p.item0 + blockIdx.x, row = item / p.parts;
   const int part = (int)(item - row * p.parts), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const T* x = (const T*)p.logits + row * p.logits_s;
-  const int64_t first = part * p.part, end = first + p.part < p.v ? first + p.part : p.v;
+  const uint32_t v = (uint32_t)p.v, first = part * (uint32_t)p.part;
+  const uint32_t end = v - first > (uint32_t)p.part ? first + (uint32_t)p.part : v;
   Sums a = none();
   Best b = {0, 0};
   typename Raw<T>::type next[kLoads];
 #pragma unroll
-  for (int k = 0; k < kLoads; ++k) next[k] = fetch_piece(x, first + k * kStep + threadIdx.x * 4, p.v);
-  for (int64_t at = first; at < end; at += kLoads * kStep) {
-    const int64_t i = at + threadIdx.x * 4;
+  for (uint32_t k = 0; k < kLoads; ++k) next[k] = fetch_piece(x, first + k * kStep + threadIdx.x * 4, v);
+  const auto batch = [&](uint32_t at, auto last) {
+    constexpr bool kEnd = decltype(last)::value;   // some of the batch may lie past the part
+    const uint32_t i = at + threadIdx.x * 4;
     float own[kLoads * 4];
 #pragma unroll
-    for (int k = 0; k < kLoads; ++k) {
-      const f32x4 y = piece_values<T>(next[k], i + k * kStep, p.v);
+    for (uint32_t k = 0; k < kLoads; ++k) {
+      const f32x4 y = piece_values<T, kEnd>(next[k], i + k * kStep, v);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) own[k * 4 + e] = y[e];
+      for (uint32_t e = 0; e < 4; ++e) own[k * 4 + e] = kEnd && i + k * kStep + e >= end ? -__builtin_inff() : y[e];
     }
-    if (at + kLoads * kStep < end)
+    if (!kEnd)
 #pragma unroll
-      for (int k = 0; k < kLoads; ++k) next[k] = fetch_piece(x, i + (kLoads + k) * kStep, p.v);
-    if (at + kLoads * kStep > end)
-#pragma unroll
-      for (int k = 0; k < kLoads; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (i + k * kStep + e >= end) own[k * 4 + e] = -__builtin_inff();
+      for (uint32_t k = 0; k < kLoads; ++k) next[k] = fetch_piece(x, i + kBatch + k * kStep, v);
     float m = own[0];
 #pragma unroll
-    for (int e = 1; e < kLoads * 4; ++e) m = own[e] > m ? own[e] : m;
+    for (uint32_t e = 1; e < kLoads * 4; ++e) m = larger(own[e], m);
     a.raise(m);
     a.add(own);
-    if (p.top) {
+    if constexpr (kTop) {
       const auto candidate = [&](int e) {
-        const int64_t j = i + (e / 4) * kStep + e % 4;
-        return j < end ? ranked(own[e], (uint32_t)j) : 0;
+        const uint32_t j = i + (uint32_t)(e / 4) * kStep + (uint32_t)(e % 4);
+        return !kEnd || j < end ? ranked(own[e], j) : 0;
       };
       uint64_t largest = 0;
 #pragma unroll
-      for (int e = 0; e < kLoads * 4; ++e) largest = candidate(e) > largest ? candidate(e) : largest;
+      for (int e = 0; e < (int)kLoads * 4; ++e) largest = candidate(e) > largest ? candidate(e) : largest;
       b.offer_batch(largest, kLoads * 4, p.top, lane, candidate);
     }
-  }
+  };
+  uint32_t at = first;   // rows end below 2^31
+  for (; end - at >= kBatch; at += kBatch) batch(at, std::false_type());
+  if (at < end) batch(at, std::true_type());
   a = joined<64>(a);
   if (lane == 0) sums[wave] = a;
-  if (lane < p.top) best[wave][lane] = b.own;
+  if (kTop && lane < p.top) best[wave][kTop ? lane : 0] = b.own;
   __syncthreads();
   if (wave != 0) return;
   for (int k = 1; k < 4; ++k) {
     a.join(sums[k]);
-    if (p.top) b.offer(lane < p.top ? best[k][lane] : 0, p.top, lane);
+    if constexpr (kTop) b.offer(lane < p.top ? best[k][lane] : 0, p.top, lane);
   }
   if (p.parts == 1) {
     const int64_t token = p.tokens[row];
     if (lane == 0) write_row(p, row, a, token >= 0 && token < p.v ? (float)x[token] : 0.0f, token);
-    if (lane < p.top) {
+    if (kTop && lane < p.top) {
       p.top_log_prob[row * p.top + lane] = top_log_prob(b.own, a);
       p.top_index[row * p.top + lane] = place_in(b.own);
     }
@@ -334,7 +337,7 @@ __global__ __launch_bounds__(kBlock) void long_kernel(LogProbs p) {
     float* to = p.partial + item * 4;
     to[0] = a.m, to[1] = a.s, to[2] = a.w;
   }
-  if (lane < p.top) p.tops[item * p.top + lane] = b.own;
+  if (kTop && lane < p.top) p.tops[item * p.top + lane] = b.own;
 }
 
 // The parts of a row together, a wave for each.
@@ -386,23 +389,24 @@ struct Gradient {
   int32_t pieces;
 };
 
-// What a row's gradient takes: dx = chosen dlog_prob - p (dlog_prob + dentropy (log p + H)).
+// What a row's gradient takes: dx = chosen dlog_prob - p (dlog_prob + dentropy (log p + H)), the bracket as
+// one product and a sum of log2 p.
 struct RowGradient {
-  float m, log_s, h, dlp, dh;
+  float m, log_s, slope, level, dlp;
   int64_t token;
 
   __device__ __forceinline__ RowGradient(const Gradient& g, int64_t row) {
     m = g.stats[2 * row], log_s = g.stats[2 * row + 1];
     token = g.tokens[row];
-    h = g.entropy[row];
     dlp = g.dlog_prob && token >= 0 && log_s != __builtin_inff() ? g.dlog_prob[row] : 0.0f;
-    dh = g.dentropy ? g.dentropy[row] : 0.0f;
+    const float dh = g.dentropy ? g.dentropy[row] : 0.0f;
+    slope = dh * kLn2;
+    level = __builtin_fmaf(dh, g.entropy[row], dlp);
   }
 
-  __device__ __forceinline__ float of(float x, int64_t j) const {
-    const float log2_p = at_least(__builtin_fmaf(x - m, kLog2e, -log_s));
-    const float through = -exp2_of(log2_p) * __builtin_fmaf(dh, __builtin_fmaf(log2_p, kLn2, h), dlp);
-    return j == token ? through + dlp : through;
+  __device__ __forceinline__ float of(float x) const {
+    const float log2_p = __builtin_fmaf(x - m, kLog2e, -log_s);
+    return -exp2_of(log2_p) * __builtin_fmaf(at_least(log2_p), slope, level);
   }
 };
 
@@ -417,7 +421,7 @@ __global__ __launch_bounds__(kBlock) void short_gradient_kernel(Gradient g) {
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int j = e * G + lane;
-    if (j < (int)g.v) dx[j] = (T)of.of((float)x[j], j);
+    if (j < (int)g.v) dx[j] = (T)(of.of((float)x[j]) + (j == of.token ? of.dlp : 0.0f));
   }
 }
 
@@ -429,19 +433,33 @@ __global__ __launch_bounds__(kBlock) void long_gradient_kernel(Gradient g) {
   const T* x = (const T*)g.logits + row * g.logits_s;
   T* dx = (T*)g.dlogits + row * g.v;
   const RowGradient of(g, row);
-  typename Raw<T>::type pieces[kPiece / (kBlock * 4)];
+  // a token that is none or past the row is no thread's: they begin below 2^31 + 4096
+  const uint32_t token = of.token >= 0 && of.token < g.v ? (uint32_t)of.token : 0xFFFFFFFFu;
+  constexpr uint32_t kLoads = kPiece / (kBlock * 4), kStep = kBlock * 4;
+  const uint32_t v = (uint32_t)g.v, j0 = (uint32_t)first + threadIdx.x * 4;
+  typename Raw<T>::type pieces[kLoads];
 #pragma unroll
-  for (int k = 0; k < kPiece / (kBlock * 4); ++k)
-    pieces[k] = fetch_piece(x, first + k * (kBlock * 4) + threadIdx.x * 4, g.v);
+  for (uint32_t k = 0; k < kLoads; ++k) pieces[k] = fetch_piece(x, j0 + k * kStep, v);
+  const auto put = [&](auto last) {
+    constexpr bool kEnd = decltype(last)::value;
 #pragma unroll
-  for (int k = 0; k < kPiece / (kBlock * 4); ++k) {
-    const int64_t j = first + k * (kBlock * 4) + threadIdx.x * 4;
-    if (j >= g.v) break;
-    f32x4 own = piece_values<T>(pieces[k], j, g.v);
+    for (uint32_t k = 0; k < kLoads; ++k) {
+      const uint32_t j = j0 + k * kStep;
+      if (kEnd && j >= v) break;
+      f32x4 own = piece_values<T, kEnd>(pieces[k], j, v);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) own[e] = of.of(own[e], j + e);
-    store_upto(dx + j, own, g.v - j);
-  }
+      for (int e = 0; e < 4; ++e) own[e] = of.of(own[e]);
+      const uint32_t at = token - j;
+      if (at < 4)   // one thread of the row
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) own[e] += at == e ? of.dlp : 0.0f;
+      store_upto(dx + j, own, kEnd ? (int64_t)v - j : 4);
+    }
+  };
+  if (v - (uint32_t)first >= (uint32_t)kPiece)
+    put(std::false_type());
+  else
+    put(std::true_type());
 }
 
 namespace {
@@ -512,7 +530,10 @@ int forward(const LogProbs& p, hipStream_t stream) {
     });
   const int status = in_launches(p, p.rows * p.parts, kBlock, [&](LogProbs a, int64_t done, dim3 grid) {
     a.item0 = done;
-    hipLaunchKernelGGL(long_kernel<T>, grid, dim3(kBlock), 0, stream, a);
+    if (p.top > 0)
+      hipLaunchKernelGGL((long_kernel<T, true>), grid, dim3(kBlock), 0, stream, a);
+    else
+      hipLaunchKernelGGL((long_kernel<T, false>), grid, dim3(kBlock), 0, stream, a);
   });
   if (status != HIPENVS_OK || p.parts == 1) return status;
   return in_launches(p, p.rows, 64, [&](LogProbs a, int64_t done, dim3 grid) {

@@ -24,8 +24,8 @@ struct Conv {
   const float *weight, *bias, *state, *dfinal;
   const uint8_t* reset;
   void *out, *dx;
-  float *final_state, *dstate, *dparams;   // dparams (b runs, d (W + 1)): weight (d, W), then bias
-  int64_t b, t, run, runs, item0;
+  float *final_state, *dstate, *dparams;   // dparams (runs b, d (W + 1)): weight (d, W), then bias
+  int64_t b, t, run, runs, across, item0;   // across: blocks that hold a run of every row
   int32_t d, quads;
   bool silu;
 };
@@ -69,128 +69,166 @@ __device__ __forceinline__ void push(f32x4 (&hist)[W], f32x4 x, bool begins) {
   }
 }
 
-// kCount tokens of a row as they come, all of their loads in flight; those past `end` read the last one.
-template <class T, int kCount>
-struct Piece {
-  typename Raw<T>::type x[kCount], dout[kCount];
-  uint8_t begins[kCount];
+// A thread's place: a run of tokens, the same for its block, and four channels of a row.
+struct Place {
+  int64_t run, t0, t1, b;
+  int c;
+  bool there;
 
-  template <bool kBack = false>
-  __device__ __forceinline__ void fetch(const Conv& s, int64_t b, int64_t first, int64_t end, int c) {
-#pragma unroll
-    for (int k = 0; k < kCount; ++k) {
-      const int64_t t = first + k < end ? first + k : end - 1;
-      x[k] = fetch4((const T*)s.x + b * s.x_sb + t * s.x_st, c, s.d);
-      if (kBack) dout[k] = fetch4((const T*)s.dout + b * s.dout_sb + t * s.dout_st, c, s.d);
-      begins[k] = s.reset ? s.reset[b * s.reset_sb + t * s.reset_st] : 0;
-    }
+  __device__ __forceinline__ explicit Place(const Conv& s) {
+    const int64_t block = s.item0 + blockIdx.x;
+    run = block / s.across;
+    t0 = run * s.run;
+    t1 = t0 + s.run < s.t ? t0 + s.run : s.t;
+    const int64_t item = (block - run * s.across) * kBlock + threadIdx.x;
+    b = item / s.quads;
+    there = b < s.b;
+    c = (int)(item - b * s.quads) * 4;
   }
-
-  __device__ __forceinline__ f32x4 value(int k, int c, int d) const { return values<T>(x[k], c, d); }
 };
 
-// hist as it is before token t0: hist[i] then holds the value of token t0 - 1 - i.
-template <class T, int W>
-__device__ __forceinline__ void before(const Conv& s, int64_t b, int64_t t0, int c, f32x4 (&hist)[W]) {
-  const int left = s.d - c;
+// A row's tokens for four channels, fetched kAhead at once; those past `end` are the last one again.
+template <class T, bool kWide, bool kBack>
+struct Tokens {
+  const T *x, *dout;
+  const uint8_t* reset;
+  int64_t x_st, dout_st, reset_st;
+  FourOf<T, kWide> four;
+
+  struct Piece {
+    typename Raw<T>::type x[kAhead], dout[kAhead];
+    uint8_t begins[kAhead];
+  };
+
+  __device__ __forceinline__ Tokens(const Conv& s, int64_t b, int c) : four(c, s.d) {
+    x = (const T*)s.x + b * s.x_sb + four.from;
+    dout = kBack ? (const T*)s.dout + b * s.dout_sb + four.from : nullptr;
+    reset = s.reset ? s.reset + b * s.reset_sb : nullptr;
+    x_st = s.x_st, dout_st = s.dout_st, reset_st = s.reset_st;
+  }
+
+  __device__ __forceinline__ void fetch(Piece& to, int64_t first, int64_t end) const {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int64_t t = first + k < end ? first + k : end - 1;   // the same for every lane
+      to.x[k] = four.fetch(x + t * x_st);
+      if (kBack) to.dout[k] = four.fetch(dout + t * dout_st);
+      to.begins[k] = reset ? reset[t * reset_st] : 0;
+    }
+  }
+};
+
+// hist as it is before token t0: hist[i] then holds the value of token t0 - 1 - i. A run has more tokens
+// than a window: windows of all runs but the first lie within the row.
+template <class T, int W, bool kWide, bool kBack>
+__device__ __forceinline__ void before(const Conv& s, const Tokens<T, kWide, kBack>& of, int64_t b, int64_t t0, int c,
+                                       f32x4 (&hist)[W]) {
 #pragma unroll
   for (int i = 0; i < W; ++i) hist[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  if (t0 == 0) {   // a run has more tokens than a window: the others' windows lie within the row
+  if (t0 == 0) {
 #pragma unroll
     for (int k = 0; k < W - 1; ++k) {
       f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (s.state) x = load_upto(s.state + (b * (W - 1) + k) * s.d + c, left);
+      if (s.state) x = load_upto(s.state + (b * (W - 1) + k) * s.d + c, s.d - c);
       push(hist, x, false);
     }
     return;
   }
-  Piece<T, W> piece;
-  piece.fetch(s, b, t0 - (W - 1), t0, c);
+  typename Raw<T>::type x[W];
+  uint8_t begins[W];
 #pragma unroll
-  for (int k = 0; k < W - 1; ++k) push(hist, piece.value(k, c, s.d), piece.begins[k]);
+  for (int k = 0; k < W - 1; ++k) {
+    const int64_t t = t0 - (W - 1) + k;
+    x[k] = of.four.fetch(of.x + t * of.x_st);
+    begins[k] = of.reset ? of.reset[t * of.reset_st] : 0;
+  }
+#pragma unroll
+  for (int k = 0; k < W - 1; ++k) push(hist, of.four.value(x[k]), begins[k]);
 }
 
-template <class T, int W>
+template <class T, int W, bool kWide>
 __global__ __launch_bounds__(kBlock) void forward_kernel(Conv s) {
-  const int64_t item = s.item0 + (int64_t)blockIdx.x * kBlock + threadIdx.x;
-  const int64_t row = item / s.quads, b = row / s.runs;
-  if (b >= s.b) return;
-  const int c = (int)(item - row * s.quads) * 4, left = s.d - c;
-  const int64_t t0 = (row - b * s.runs) * s.run, t1 = t0 + s.run < s.t ? t0 + s.run : s.t;
-  const Taps<W> taps(s, c);
+  const Place at(s);
+  if (!at.there) return;
+  const int left = s.d - at.c;
+  const Taps<W> taps(s, at.c);
+  const Tokens<T, kWide, false> of(s, at.b, at.c);
   f32x4 hist[W];
-  before<T, W>(s, b, t0, c, hist);
-  Piece<T, kAhead> next;
-  if (t0 < t1) next.fetch(s, b, t0, t1, c);
-  for (int64_t first = t0; first < t1; first += kAhead) {
-    const Piece<T, kAhead> now = next;
-    if (first + kAhead < t1) next.fetch(s, b, first + kAhead, t1, c);
+  before(s, of, at.b, at.t0, at.c, hist);
+  typename Tokens<T, kWide, false>::Piece next;
+  if (at.t0 < at.t1) of.fetch(next, at.t0, at.t1);
+  T* out = (T*)s.out + at.b * s.t * s.d + at.c;
+  for (int64_t first = at.t0; first < at.t1; first += kAhead) {
+    const auto now = next;
+    if (first + kAhead < at.t1) of.fetch(next, first + kAhead, at.t1);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      if (first + k >= t1) break;
-      push(hist, now.value(k, c, s.d), now.begins[k]);
+      if (first + k >= at.t1) break;
+      push(hist, of.four.value(now.x[k]), now.begins[k]);
       f32x4 pre = taps.apply(hist);
       if (s.silu)
 #pragma unroll
         for (int e = 0; e < 4; ++e) pre[e] *= sigmoid_for<T>(pre[e]);
-      store_upto((T*)s.out + (b * s.t + first + k) * s.d + c, pre, left);
+      store_upto(out + (first + k) * s.d, pre, left);
     }
   }
-  if (t1 == s.t)
+  if (at.t1 == s.t)
 #pragma unroll
     for (int k = 0; k < W - 1; ++k)
-      store_upto(s.final_state + (b * (W - 1) + k) * s.d + c, hist[W - 2 - k], left);
+      store_upto(s.final_state + (at.b * (W - 1) + k) * s.d + at.c, hist[W - 2 - k], left);
 }
 
 // Gradients of a run: token t's reaches the W tokens up to t, as far as its episode does. A run's own
 // tokens wait in `late` for those behind them, W - 1 past its end; the first run has the state's
 // values among its own, and what a row's last values leave in the final state comes last.
-template <class T, int W>
-__global__ __launch_bounds__(kBlock) void backward_kernel(Conv s) {
-  const int64_t item = s.item0 + (int64_t)blockIdx.x * kBlock + threadIdx.x;
-  const int64_t row = item / s.quads, b = row / s.runs;
-  if (b >= s.b) return;
-  const int c = (int)(item - row * s.quads) * 4, left = s.d - c;
-  const int64_t t0 = (row - b * s.runs) * s.run, t1 = t0 + s.run < s.t ? t0 + s.run : s.t;
-  const int64_t past = t1 + W - 1 < s.t ? t1 + W - 1 : s.t, first_own = t0 == 0 ? -(W - 1) : t0;
+template <class T, int W, bool kWide>
+__global__ __launch_bounds__(kBlock, 2) void backward_kernel(Conv s) {
+  const Place at(s);
+  if (!at.there) return;
+  const int left = s.d - at.c;
+  const int64_t t0 = at.t0, t1 = at.t1, past = t1 + W - 1 < s.t ? t1 + W - 1 : s.t;
+  const int64_t first_own = t0 == 0 ? -(W - 1) : t0;
   const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-  const Taps<W> taps(s, c);
+  const Taps<W> taps(s, at.c);
+  const Tokens<T, kWide, true> of(s, at.b, at.c);
   f32x4 hist[W], late[W], dweight[W], dbias = zero;   // late[i]: the gradient of token t - i
-  before<T, W>(s, b, t0, c, hist);
+  before(s, of, at.b, t0, at.c, hist);
 #pragma unroll
   for (int i = 0; i < W; ++i) late[i] = dweight[i] = zero;
-  const auto emit = [&](int64_t u, f32x4 grad) {
+  T* dx = (T*)s.dx + at.b * s.t * s.d + at.c;
+  float* dstate = s.dstate + at.b * (W - 1) * s.d + at.c;
+  const auto emit = [&](int64_t u, f32x4 grad) {   // u is the same for every lane
     if (u < first_own || u >= t1) return;
     if (u < 0)
-      store_upto(s.dstate + (b * (W - 1) + u + W - 1) * s.d + c, grad, left);
+      store_upto(dstate + (u + W - 1) * s.d, grad, left);
     else
-      store_upto((T*)s.dx + (b * s.t + u) * s.d + c, grad, left);
+      store_upto(dx + u * s.d, grad, left);
   };
   int since = W;   // tokens since the episode's first
-  Piece<T, kAhead> next;
-  if (t0 < past) next.template fetch<true>(s, b, t0, past, c);
+  typename Tokens<T, kWide, true>::Piece next;
+  if (t0 < past) of.fetch(next, t0, past);
   for (int64_t first = t0; first < past; first += kAhead) {
-    const Piece<T, kAhead> now = next;
-    if (first + kAhead < past) next.template fetch<true>(s, b, first + kAhead, past, c);
+    const auto now = next;
+    if (first + kAhead < past) of.fetch(next, first + kAhead, past);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       const int64_t t = first + k;
       if (t >= past) break;
-      push(hist, now.value(k, c, s.d), now.begins[k]);
+      push(hist, of.four.value(now.x[k]), now.begins[k]);
       since = now.begins[k] ? 0 : since < W ? since + 1 : W;
-      f32x4 grad = values<T>(now.dout[k], c, s.d);
+      f32x4 grad = of.four.value(now.dout[k]);
       if (s.silu) {
         const f32x4 pre = taps.apply(hist);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float one = sigmoid_for<T>(pre[e]);
-          grad[e] *= one * (1.0f + pre[e] * (1.0f - one));
+          grad[e] *= one * __builtin_fmaf(pre[e], 1.0f - one, 1.0f);
         }
       }
 #pragma unroll
       for (int i = W - 1; i > 0; --i) late[i] = late[i - 1];
       late[0] = zero;
-      if (__builtin_amdgcn_ballot_w64(since < W - 1 || t >= t1) == 0) {   // whole windows of own tokens
+      if (t < t1 && __builtin_amdgcn_ballot_w64(since < W - 1) == 0) {   // whole windows of own tokens
 #pragma unroll
         for (int i = 0; i < W; ++i)
 #pragma unroll
@@ -217,16 +255,16 @@ __global__ __launch_bounds__(kBlock) void backward_kernel(Conv s) {
 #pragma unroll
     for (int i = W - 2; i >= 0; --i) {
       f32x4 grad = late[i];
-      if (s.dfinal && i <= since) grad += load_upto(s.dfinal + (b * (W - 1) + (W - 2 - i)) * s.d + c, left);
+      if (s.dfinal && i <= since) grad += load_upto(s.dfinal + (at.b * (W - 1) + (W - 2 - i)) * s.d + at.c, left);
       emit(s.t - 1 - i, grad);
     }
-  float* params = s.dparams + row * ((int64_t)s.d * (W + 1));
+  float* params = s.dparams + (at.run * s.b + at.b) * ((int64_t)s.d * (W + 1));
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (e < left) {
 #pragma unroll
-      for (int j = 0; j < W; ++j) params[(int64_t)(c + e) * W + j] = dweight[W - 1 - j][e];
-      params[(int64_t)s.d * W + c + e] = dbias[e];
+      for (int j = 0; j < W; ++j) params[(int64_t)(at.c + e) * W + j] = dweight[W - 1 - j][e];
+      params[(int64_t)s.d * W + at.c + e] = dbias[e];
     }
 }
 
@@ -245,7 +283,7 @@ struct Step {
 
 template <class T, int W>
 __global__ __launch_bounds__(kBlock) void step_kernel(Step s) {
-  const int64_t item = s.item0 + (int64_t)blockIdx.x * kBlock + threadIdx.x, env = item / s.quads;
+  const int64_t item = (s.item0 + blockIdx.x) * kBlock + threadIdx.x, env = item / s.quads;
   if (env >= s.n) return;
   const int c = (int)(item - env * s.quads) * 4, left = s.d - c;
   Conv of = {};
@@ -283,6 +321,7 @@ int plan(Conv* s, int64_t b, int64_t t, int32_t d) {
   s->run = 64;
   while (s->run > 8 && b * s->quads * ((t + s->run - 1) / s->run) < (int64_t)cus * 8 * 64) s->run /= 2;
   s->runs = t > 0 ? (t + s->run - 1) / s->run : 1;
+  s->across = (b * s->quads + kBlock - 1) / kBlock;
   return HIPENVS_OK;
 }
 
@@ -297,10 +336,10 @@ int for_taps(int w, const F& f) {
 }
 
 template <class S, class F>
-int in_launches(S s, int64_t items, const F& launch) {
-  for (s.item0 = 0; s.item0 < items; s.item0 += kMostThreads) {
-    const int64_t own = items - s.item0 < kMostThreads ? items - s.item0 : kMostThreads;
-    launch(s, dim3(grid_for(own)));
+int in_launches(S s, int64_t blocks, const F& launch) {
+  constexpr int64_t kMost = kMostThreads / kBlock;
+  for (s.item0 = 0; s.item0 < blocks; s.item0 += kMost) {
+    launch(s, dim3((unsigned)(blocks - s.item0 < kMost ? blocks - s.item0 : kMost)));
     const int status = launch_status();
     if (status != HIPENVS_OK) return status;
   }
@@ -338,11 +377,16 @@ extern "C" int hipenvs_causal_conv(int32_t dtype, const void* x, const float* we
   if (t > 0) s.x_sb = strides[0], s.x_st = strides[1], s.reset_sb = strides[2], s.reset_st = strides[3];
   return for_taps(w, [&](auto taps) {
     constexpr int W = decltype(taps)::value;
-    return in_launches(s, b * s.runs * s.quads, [&](const Conv& a, dim3 grid) {
-      if (dtype == 1)
-        hipLaunchKernelGGL((forward_kernel<__bf16, W>), grid, dim3(kBlock), 0, as_stream(stream), a);
+    return in_launches(s, s.runs * s.across, [&](const Conv& a, dim3 grid) {
+      const bool wide = d >= 4;
+      if (dtype == 1 && wide)
+        hipLaunchKernelGGL((forward_kernel<__bf16, W, true>), grid, dim3(kBlock), 0, as_stream(stream), a);
+      else if (dtype == 1)
+        hipLaunchKernelGGL((forward_kernel<__bf16, W, false>), grid, dim3(kBlock), 0, as_stream(stream), a);
+      else if (wide)
+        hipLaunchKernelGGL((forward_kernel<float, W, true>), grid, dim3(kBlock), 0, as_stream(stream), a);
       else
-        hipLaunchKernelGGL((forward_kernel<float, W>), grid, dim3(kBlock), 0, as_stream(stream), a);
+        hipLaunchKernelGGL((forward_kernel<float, W, false>), grid, dim3(kBlock), 0, as_stream(stream), a);
     });
   });
 }
@@ -369,11 +413,16 @@ extern "C" int hipenvs_causal_conv_backward(int32_t dtype, const void* x, const 
     s.dout_st = strides[5];
   status = for_taps(w, [&](auto taps) {
     constexpr int W = decltype(taps)::value;
-    return in_launches(s, rows * s.quads, [&](const Conv& a, dim3 grid) {
-      if (dtype == 1)
-        hipLaunchKernelGGL((backward_kernel<__bf16, W>), grid, dim3(kBlock), 0, as_stream(stream), a);
+    return in_launches(s, s.runs * s.across, [&](const Conv& a, dim3 grid) {
+      const bool wide = d >= 4;
+      if (dtype == 1 && wide)
+        hipLaunchKernelGGL((backward_kernel<__bf16, W, true>), grid, dim3(kBlock), 0, as_stream(stream), a);
+      else if (dtype == 1)
+        hipLaunchKernelGGL((backward_kernel<__bf16, W, false>), grid, dim3(kBlock), 0, as_stream(stream), a);
+      else if (wide)
+        hipLaunchKernelGGL((backward_kernel<float, W, true>), grid, dim3(kBlock), 0, as_stream(stream), a);
       else
-        hipLaunchKernelGGL((backward_kernel<float, W>), grid, dim3(kBlock), 0, as_stream(stream), a);
+        hipLaunchKernelGGL((backward_kernel<float, W, false>), grid, dim3(kBlock), 0, as_stream(stream), a);
     });
   });
   if (status != HIPENVS_OK) return status;
@@ -390,7 +439,7 @@ extern "C" int hipenvs_causal_conv_step(int32_t dtype, const void* x, int64_t x_
   Step s = {x, x_sn, reset_sn, weight, bias, state, reset, out, next_state, n, 0, d, (d + 3) / 4, silu != 0};
   return for_taps(w, [&](auto taps) {
     constexpr int W = decltype(taps)::value;
-    return in_launches(s, n * s.quads, [&](const Step& a, dim3 grid) {
+    return in_launches(s, (n * s.quads + kBlock - 1) / kBlock, [&](const Step& a, dim3 grid) {
       if (dtype == 1)
         hipLaunchKernelGGL((step_kernel<__bf16, W>), grid, dim3(kBlock), 0, as_stream(stream), a);
       else

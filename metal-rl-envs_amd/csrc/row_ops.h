@@ -81,6 +81,42 @@ __device__ __forceinline__ f32x4 values(typename Raw<T>::type raw, int c, int d)
   return y;
 }
 
+// The same for a thread that walks down a column of rows: where its four values lie is worked out once.
+// kWide: rows of four values and more.
+template <class T, bool kWide>
+struct FourOf {
+  int from, by, left;   // the first read, how far the values lie behind it, and how many there are
+  bool ragged;          // of any lane of the wave
+
+  __device__ __forceinline__ FourOf(int c, int d) {
+    left = d - c;
+    from = kWide && left < 4 ? d - 4 : c;
+    by = kWide && left < 4 ? 4 - left : 0;
+    ragged = __builtin_amdgcn_ballot_w64(left < 4) != 0;
+  }
+
+  __device__ __forceinline__ typename Raw<T>::type fetch(const T* row) const {   // row: from `from` on
+    if constexpr (kWide)
+      return *(const typename Raw<T>::any*)row;
+    else
+      return typename Raw<T>::type{row[0], row[left > 1 ? 1 : 0], row[left > 2 ? 2 : 0], row[0]};
+  }
+
+  __device__ __forceinline__ f32x4 value(typename Raw<T>::type raw) const {
+    const f32x4 x = __builtin_convertvector(raw, f32x4);
+    if (!ragged) return x;
+    f32x4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      y[e] = x[e];
+#pragma unroll
+      for (int k = 1; e + k < 4; ++k) y[e] = by == k ? x[e + k] : y[e];
+      y[e] = e < left ? y[e] : 0.0f;
+    }
+    return y;
+  }
+};
+
 template <class T>
 __device__ __forceinline__ void store_upto(T* p, f32x4 x, int64_t n) {
   if (n >= 4) {
