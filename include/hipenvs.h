@@ -450,7 +450,7 @@ int64_t hipenvs_selective_scan_workspace_bytes(int32_t which, int64_t b, int64_t
  * dtype 0: x, dt, gate (b, t, d), write, read (b, t, g, n) and out f32; 1: bfloat16 (raw 16 bits), each
  * with unit stride in the last axis and any strides (in elements) in the others; channel c reads
  * group c / (d / g). `strides`, a host array: b, t of x, of dt, of gate, then b, t, g of write, of
- * read, then b, t of reset. rate (d, n), skip, dt_bias (d) f32 contiguous; skip, gate, dt_bias, reset
+ * read, then b, t of reset; those of t below 2^31 in size. rate (d, n), skip, dt_bias (d) f32 contiguous; skip, gate, dt_bias, reset
  * (b, t) u8 or NULL (left out); state (b, d, n) f32 contiguous or NULL (zeros).
  * -> out (b, t, d) contiguous, final_state (b, d, n) f32 (not `state`), checks (which 1 above, 16-byte
  * aligned) or NULL. 1 <= n <= 64, d <= 65536, g divides d. workspace: 16-byte aligned. What a token

@@ -189,13 +189,20 @@ __device__ __forceinline__ float sigmoid_for(float x) {
     return sigmoid(x);
 }
 
-// log(1 + exp(x)) = max(x, 0) + log(1 + e), e = exp(-|x|). The rounding of u = 1 + e is made good
-// by e / (u - 1), whose divisor is exact.
-__device__ __forceinline__ float softplus(float x) {
-  const float e = exp_negative(x), u = 1.0f + e, d = u - 1.0f;
-  const float l = d == 0.0f ? e : __builtin_amdgcn_logf(u) * kLn2 * (e * __builtin_amdgcn_rcpf(d));
-  return (x > 0.0f ? x : 0.0f) + l;
-}
+// log(1 + exp(x)) = max(x, 0) + log(1 + e), e = exp(-|x|), and its slope, the sigmoid. The rounding of
+// u = 1 + e is made good by (e - (u - 1)) / u, the slope of the logarithm there.
+struct Softplus {
+  float value, slope;
+
+  __device__ __forceinline__ explicit Softplus(float x) {
+    const float e = exp_negative(x), u = 1.0f + e, r = __builtin_amdgcn_rcpf(u);
+    const float l = __builtin_fmaf(e - (u - 1.0f), r, __builtin_amdgcn_logf(u) * kLn2);
+    value = __builtin_amdgcn_fmed3f(x, 0.0f, __builtin_inff()) + l;   // a NaN is in l
+    slope = x >= 0.0f ? r : e * r;
+  }
+};
+
+__device__ __forceinline__ float softplus(float x) { return Softplus(x).value; }
 
 // Sums of the columns of `from` (count, width) f32, in an order that depends on the sizes alone:
 // block (i, j) sums rows i * each .. of 64 columns, four rows at once, into row i of `to`.

@@ -46,7 +46,7 @@ struct Scan {
 
 // LPC lanes a channel, four states each; the channels of a block.
 constexpr int channels_of(int lpc) { return lpc == 16 ? 32 : 64; }
-inline int lanes_of(int n) { return n <= 4 ? 1 : n <= 8 ? 2 : n <= 16 ? 4 : n <= 32 ? 8 : 16; }
+inline int lanes_of(int n) { return n <= 8 ? 2 : n <= 16 ? 4 : n <= 32 ? 8 : 16; }
 
 template <int LPC>
 struct Shape {
@@ -69,44 +69,97 @@ __device__ __forceinline__ Place place_of(const Scan& s, int64_t item, int parts
   return {item / parts, (int)(item % parts), group, tile * channels};
 }
 
-// A tile's inputs as they come, in the registers of the threads that fetch them. Tokens past the end
-// read the last one, channels and states past theirs the last four, and whoever uses them leaves
-// them out.
+// What a thread fetches of every tile: its slots of four channels of a token, and of four states of write or
+// read. Rows lie at a block's own address plus token times stride, one instruction: strides of t are
+// below 2^31. Channels and states past theirs read the last four, and whoever uses them leaves them out.
+template <int LPC>
+struct Slots {
+  using S = Shape<LPC>;
+
+  static __device__ __forceinline__ int token(int i) {   // of slot i; kTile and more: none
+    return (threadIdx.x + i * S::kThreads) / (S::CH / 4);
+  }
+  static __device__ __forceinline__ int channel() { return threadIdx.x % (S::CH / 4) * 4; }   // within the block
+  static __device__ __forceinline__ int mix_token(int i) { return (threadIdx.x + i * S::kThreads) / (2 * LPC); }
+  static __device__ __forceinline__ int mix_part() { return threadIdx.x % (2 * LPC); }   // below LPC: write
+  static __device__ __forceinline__ int mix_state() { return threadIdx.x % LPC * 4; }
+};
+
+// The same number, about which the compiler knows nothing: addresses that it works out once for all of a
+// loop's rounds would take the registers of the states.
+__device__ __forceinline__ int64_t anew(int64_t x) {
+  uint32_t lo = (uint32_t)x, hi = (uint32_t)((uint64_t)x >> 32);
+  asm volatile("" : "+s"(lo), "+s"(hi));
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+template <class T>
+__device__ __forceinline__ const T* row_at(const T* base, int token, int64_t stride) {
+  return (const T*)((const char*)base + (int64_t)(token * (int)sizeof(T)) * (int64_t)(int32_t)stride);
+}
+
 template <class T, int LPC, bool kOut, bool kBack>
 struct Fetched {
   using S = Shape<LPC>;
+  using At = Slots<LPC>;
   typename Raw<T>::type x[S::kSlots], dt[S::kSlots], gate[S::kSlots], dout[S::kSlots], mix[S::kMixSlots];
   uint8_t begins;   // of the token of this lane
 
-  __device__ __forceinline__ void fetch(const Scan& s, const Place& at, int64_t t0, int64_t end) {
-    const int64_t last = end - 1;
+  // kWhole: four channels and four states at least, and a tile that ends before `end`; otherwise tokens
+  // past the end are the last one again
+  template <bool kWhole>
+  __device__ __forceinline__ void load(const Scan& s, const Place& at, int64_t t0, int64_t end) {
+    const int last = kWhole ? kTile - 1 : (int)(end - 1 - t0 < kTile - 1 ? end - 1 - t0 : kTile - 1);
+    const int64_t col = (int64_t)at.group * s.dg;
+    const T* x0 = (const T*)s.x.data + at.b * s.x.sb + t0 * s.x.st + col;
+    const T* dt0 = (const T*)s.dt.data + at.b * s.dt.sb + t0 * s.dt.st + col;
+    const T* gate0 = (const T*)s.gate.data + at.b * s.gate.sb + t0 * s.gate.st + col;
+    const T* dout0 = (const T*)s.dout.data + at.b * s.dout.sb + t0 * s.dout.st + col;
+    int c = at.first + At::channel();
+    c = c < s.dg ? c : 0;
+    if (kWhole) c = c < s.dg - 4 ? c : s.dg - 4;
+    const auto four = [&](const T* base, int token, int64_t stride) {
+      const T* row = row_at(base, token < last ? token : last, stride);
+      if constexpr (kWhole)
+        return *(const typename Raw<T>::any*)(row + c);
+      else
+        return fetch4(row, c, s.dg);
+    };
 #pragma unroll
     for (int i = 0; i < S::kSlots; ++i) {
-      const int slot = threadIdx.x + i * S::kThreads, c = at.first + (slot % (S::CH / 4)) * 4;
-      const int own = c < s.dg ? c : 0;
-      int64_t t = t0 + slot / (S::CH / 4);
-      t = t < last ? t : last;
-      const int64_t col = (int64_t)at.group * s.dg;
-      x[i] = fetch4((const T*)s.x.data + at.b * s.x.sb + t * s.x.st + col, own, s.dg);
-      dt[i] = fetch4((const T*)s.dt.data + at.b * s.dt.sb + t * s.dt.st + col, own, s.dg);
-      if ((kOut || kBack) && s.gate.data)
-        gate[i] = fetch4((const T*)s.gate.data + at.b * s.gate.sb + t * s.gate.st + col, own, s.dg);
-      if (kBack) dout[i] = fetch4((const T*)s.dout.data + at.b * s.dout.sb + t * s.dout.st + col, own, s.dg);
+      x[i] = four(x0, At::token(i), s.x.st);
+      dt[i] = four(dt0, At::token(i), s.dt.st);
+      if ((kOut || kBack) && s.gate.data) gate[i] = four(gate0, At::token(i), s.gate.st);
+      if (kBack) dout[i] = four(dout0, At::token(i), s.dout.st);
     }
+    const bool writes = At::mix_part() < LPC;
+    const T* write0 = (const T*)s.write.data + at.b * s.write.sb + t0 * s.write.st + at.group * s.write.sg;
+    const T* read0 = (const T*)s.read.data + at.b * s.read.sb + t0 * s.read.st + at.group * s.read.sg;
+    const T* mix0 = writes ? write0 : read0;
+    const int32_t mix_st = writes ? (int32_t)s.write.st : (int32_t)s.read.st;
+    int n0 = At::mix_state();
+    n0 = n0 < s.n ? n0 : 0;
+    if (kWhole) n0 = n0 < s.n - 4 ? n0 : s.n - 4;
 #pragma unroll
     for (int i = 0; i < S::kMixSlots; ++i) {
-      const int slot = threadIdx.x + i * S::kThreads, part = slot % (2 * LPC), n0 = (part % LPC) * 4;
-      int64_t t = t0 + slot / (2 * LPC);
-      t = t < last ? t : last;
-      const Mix& m = part < LPC ? s.write : s.read;
-      mix[i] = fetch4((const T*)m.data + at.b * m.sb + t * m.st + at.group * m.sg, n0 < s.n ? n0 : 0, s.n);
+      const T* row = row_at(mix0, At::mix_token(i) < last ? At::mix_token(i) : last, mix_st);
+      if constexpr (kWhole)
+        mix[i] = *(const typename Raw<T>::any*)(row + n0);
+      else
+        mix[i] = fetch4(row, n0, s.n);
     }
     begins = 0;
     if (s.reset) {
-      int64_t t = t0 + (threadIdx.x & 63);
-      t = t < last ? t : last;
-      begins = s.reset[at.b * s.reset_sb + t * s.reset_st];
+      const int tok = threadIdx.x & 63;
+      begins = *row_at(s.reset + at.b * s.reset_sb + t0 * s.reset_st, tok < last ? tok : last, s.reset_st);
     }
+  }
+
+  __device__ __forceinline__ void fetch(const Scan& s, const Place& at, int64_t t0, int64_t end) {
+    if (t0 + kTile <= end && s.dg >= 4 && s.n >= 4)
+      load<true>(s, at, t0, end);
+    else
+      load<false>(s, at, t0, end);
   }
 
   // a bit for each token of the tile that begins an episode
@@ -117,13 +170,13 @@ struct Fetched {
 
   // write and read to LDS, zeros past the end and past the states
   __device__ __forceinline__ void put_mix(const Scan& s, int64_t t0, int64_t end, float (*to)[8 * LPC]) const {
+    const int n0 = At::mix_state();
 #pragma unroll
     for (int i = 0; i < S::kMixSlots; ++i) {
-      const int slot = threadIdx.x + i * S::kThreads, tok = slot / (2 * LPC), part = slot % (2 * LPC);
-      const int n0 = (part % LPC) * 4;
+      const int tok = At::mix_token(i);
       f32x4 m = values<T>(mix[i], n0 < s.n ? n0 : 0, s.n);
       if (t0 + tok >= end || n0 >= s.n) m = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      if (tok < kTile) *(f32x4*)&to[tok][part * 4] = m;
+      if (tok < kTile) *(f32x4*)&to[tok][At::mix_part() * 4] = m;
     }
   }
 };
@@ -161,7 +214,6 @@ struct Across {
     }
     if constexpr (LPC <= 4) v[0] += from_xor<4>(v[0]);
     if constexpr (LPC <= 2) v[0] += from_xor<2>(v[0]);
-    if constexpr (LPC <= 1) v[0] += from_xor<1>(v[0]);
   }
 
   // which of the eight values `kept` of this lane is

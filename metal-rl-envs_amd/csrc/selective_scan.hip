@@ -12,6 +12,7 @@ namespace scan {
 template <class T, int LPC, bool kOut>
 __global__ __launch_bounds__(Shape<LPC>::kThreads) void forward_kernel(Scan s) {
   using S = Shape<LPC>;
+  using At = Slots<LPC>;
   __shared__ __attribute__((aligned(16))) f32x2 steps[kTile][S::CH];      // delta, delta x; then y
   __shared__ __attribute__((aligned(16))) float mix[kTile][2 * S::NP];
   const int parts = kOut ? s.parts : s.parts - 1;
@@ -28,7 +29,7 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void forward_kernel(Scan s) {
     else if (s.state)
       h = load_upto(s.state + (at.b * s.d + c) * s.n + n0, left);
   }
-  const int own = at.first + (threadIdx.x % (S::CH / 4)) * 4;   // the channels this thread fetches
+  const int own = at.first + At::channel();   // the channels this thread fetches
   const f32x4 bias = per_channel(s.bias, (int64_t)at.group * s.dg + own, s.dg - own, 0.0f);
   const f32x4 skip = per_channel(s.skip, (int64_t)at.group * s.dg + own, s.dg - own, 0.0f);
   const int64_t checks = (s.t + kTile - 1) / kTile;
@@ -36,20 +37,23 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void forward_kernel(Scan s) {
   uint32_t begun = 0;
   Fetched<T, LPC, kOut, false> next;
   if (start < end) next.fetch(s, at, start, end);
-  for (int64_t t0 = start; t0 < end; t0 += kTile) {
+  for (int64_t tile = start; tile < end; tile += kTile) {
+    const int64_t t0 = anew(tile);
     const Fetched<T, LPC, kOut, false> now = next;
     const uint32_t begins = now.begun(t0, end);
+    const int k = At::channel();
+    f32x4 x[S::kSlots];
 #pragma unroll
     for (int i = 0; i < S::kSlots; ++i) {
-      const int slot = threadIdx.x + i * S::kThreads, tok = slot / (S::CH / 4), k = (slot % (S::CH / 4)) * 4;
+      const int tok = At::token(i);
       if (tok >= kTile) break;
       const bool there = t0 + tok < end && at.first + k < s.dg;   // past the end the state stays
-      const f32x4 x = values<T>(now.x[i], there ? at.first + k : 0, s.dg);
+      x[i] = values<T>(now.x[i], there ? at.first + k : 0, s.dg);
       const f32x4 dt = values<T>(now.dt[i], there ? at.first + k : 0, s.dg);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float delta = softplus(dt[e] + bias[e]);
-        steps[tok][k + e] = there ? f32x2{delta, delta * x[e]} : f32x2{0.0f, 0.0f};
+        steps[tok][k + e] = there ? f32x2{delta, delta * x[i][e]} : f32x2{0.0f, 0.0f};
       }
     }
     now.put_mix(s, t0, end, mix);
@@ -58,40 +62,45 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void forward_kernel(Scan s) {
     if (kOut && s.checks)
       store_upto(s.checks + ((at.b * checks + t0 / kTile) * s.d + c) * s.n + n0, h, left);
     begun |= begins;
+    const auto walk = [&](auto with_resets) {
 #pragma unroll
-    for (int tok = 0; tok < kTile; ++tok) {
-      const f32x2 st = steps[tok][ch];
-      const f32x4 w = *(const f32x4*)&mix[tok][n0];
-      if (begins >> tok & 1) h = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      float y = 0.0f;
-      f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (kOut) r = *(const f32x4*)&mix[tok][S::NP + n0];
+      for (int tok = 0; tok < kTile; ++tok) {
+        const f32x2 st = steps[tok][ch];
+        const f32x4 w = *(const f32x4*)&mix[tok][n0];
+        if (decltype(with_resets)::value && (begins >> tok & 1)) h = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        float y = 0.0f;
+        f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (kOut) r = *(const f32x4*)&mix[tok][S::NP + n0];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        h[e] = __builtin_fmaf(exp2_of(st.x * rate[e]), h[e], st.y * w[e]);
-        if (kOut) y = __builtin_fmaf(r[e], h[e], y);
+        for (int e = 0; e < 4; ++e) {
+          h[e] = __builtin_fmaf(exp2_of(st.x * rate[e]), h[e], st.y * w[e]);
+          if (kOut) y = e ? __builtin_fmaf(r[e], h[e], y) : r[e] * h[e];
+        }
+        if (kOut)
+          steps[tok][ch].x = lanes_sum<LPC>(y);   // the same from each of the channel's lanes
+        else
+          span += st.x;
       }
-      if (kOut)
-        steps[tok][ch].x = lanes_sum<LPC>(y);   // the same from each of the channel's lanes
-      else
-        span += st.x;
-    }
+    };
+    if (begins)
+      walk(std::true_type());
+    else
+      walk(std::false_type());
     __syncthreads();
     if (kOut) {
 #pragma unroll
       for (int i = 0; i < S::kSlots; ++i) {
-        const int slot = threadIdx.x + i * S::kThreads, tok = slot / (S::CH / 4), k = (slot % (S::CH / 4)) * 4;
+        const int tok = At::token(i);
         if (tok >= kTile || t0 + tok >= end || at.first + k >= s.dg) continue;
-        const f32x4 x = values<T>(now.x[i], at.first + k, s.dg);
         f32x4 o, z = {0.0f, 0.0f, 0.0f, 0.0f};
         if (s.gate.data) z = values<T>(now.gate[i], at.first + k, s.dg);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          o[e] = __builtin_fmaf(skip[e], x[e], steps[tok][k + e].x);
+          o[e] = __builtin_fmaf(skip[e], x[i][e], steps[tok][k + e].x);
           if (s.gate.data) o[e] *= z[e] * sigmoid_for<T>(z[e]);
         }
-        const int64_t col = (int64_t)at.group * s.dg + at.first + k;
-        store_upto((T*)s.out + (at.b * s.t + t0 + tok) * s.d + col, o, s.dg - at.first - k);
+        T* out = (T*)s.out + (at.b * s.t + t0) * s.d + (int64_t)at.group * s.dg + at.first;
+        store_upto((T*)row_at(out, tok, s.d) + k, o, s.dg - at.first - k);
       }
       __syncthreads();
     }
@@ -124,20 +133,16 @@ __global__ __launch_bounds__(kBlock) void join_kernel(Scan s) {
   const float* first = kBack ? s.dfinal : s.state;
   float state = first ? first[i] : 0.0f;
   const float rate = s.rate[x];
-  constexpr int kAhead = 8;
+  constexpr int kAhead = 32;
   for (int p0 = 0; p0 < s.parts; p0 += kAhead) {
     float own[kAhead], span[kAhead];
     bool begun[kAhead];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int at = p0 + k, p = kBack ? s.parts - 1 - at : at;
-      own[k] = span[k] = 0.0f;
-      begun[k] = false;
-      if (at < s.parts - 1) {
-        own[k] = s.carry[(b * s.parts + p) * each + x];
-        span[k] = s.spans[(b * s.parts + p) * s.d + c];
-        begun[k] = s.begun[b * s.parts + p];
-      }
+    for (int k = 0; k < kAhead; ++k) {   // past the last but one, that one again: all loads in flight
+      const int at = p0 + k < s.parts - 1 ? p0 + k : s.parts - 2, p = kBack ? s.parts - 1 - at : at;
+      own[k] = s.carry[(b * s.parts + p) * each + x];
+      span[k] = s.spans[(b * s.parts + p) * s.d + c];
+      begun[k] = s.begun[b * s.parts + p];
     }
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
@@ -152,6 +157,7 @@ __global__ __launch_bounds__(kBlock) void join_kernel(Scan s) {
 template <class T, int LPC>
 __global__ __launch_bounds__(Shape<LPC>::kThreads) void passed_kernel(Scan s) {
   using S = Shape<LPC>;
+  using At = Slots<LPC>;
   __shared__ __attribute__((aligned(16))) f32x2 steps[kTile][S::CH];      // delta, dy
   __shared__ __attribute__((aligned(16))) float mix[kTile][2 * S::NP];
   Place at = place_of(s, s.item0 + blockIdx.x, s.parts - 1, S::CH);
@@ -163,19 +169,21 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void passed_kernel(Scan s) {
   const int left = live ? s.n - n0 : 0;
   const f32x4 rate = load_upto(s.rate + c * s.n + n0, left) * kLog2e;
   f32x4 g = {0.0f, 0.0f, 0.0f, 0.0f};
-  const int own = at.first + (threadIdx.x % (S::CH / 4)) * 4;
+  const int own = at.first + At::channel();
   const f32x4 bias = per_channel(s.bias, (int64_t)at.group * s.dg + own, s.dg - own, 0.0f);
   float span = 0.0f;
   uint32_t begun = 0;
   Fetched<T, LPC, true, true> next;
   int64_t t0 = start + (end - start - 1) / kTile * kTile;
   next.fetch(s, at, t0, end);
-  for (; t0 >= start; t0 -= kTile) {
+  for (int64_t tile = t0; tile >= start; tile -= kTile) {
+    const int64_t t0 = anew(tile);
     const Fetched<T, LPC, true, true> now = next;
     const uint32_t begins = now.begun(t0, end);
+    const int k = At::channel();
 #pragma unroll
     for (int i = 0; i < S::kSlots; ++i) {
-      const int slot = threadIdx.x + i * S::kThreads, tok = slot / (S::CH / 4), k = (slot % (S::CH / 4)) * 4;
+      const int tok = At::token(i);
       if (tok >= kTile) break;
       const bool there = t0 + tok < end && at.first + k < s.dg;
       const int c0 = there ? at.first + k : 0;
@@ -223,7 +231,11 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void passed_kernel(Scan s) {
 template <class T, int LPC>
 __global__ __launch_bounds__(Shape<LPC>::kThreads, 2) void backward_kernel(Scan s) {
   using S = Shape<LPC>;
-  __shared__ __attribute__((aligned(16))) f32x4 steps[kTile][S::CH];   // delta, delta x, dy; then delta, sum g write, ddelta's states, y
+  using At = Slots<LPC>;
+  // delta, delta x, dy; then delta, sum g write, sum g rate a h_{t-1}, sum read h
+  __shared__ __attribute__((aligned(16))) f32x4 steps[kTile][S::CH];
+  // of each slot, for its outputs: x, dy, the slope of softplus, dout times that of the gate's silu
+  __shared__ __attribute__((aligned(16))) f32x4 held[4][kTile * S::CH / 4];
   __shared__ __attribute__((aligned(16))) float mix[kTile][2 * S::NP];
   __shared__ __attribute__((aligned(16))) float sums[S::kWaves][kTile][2 * S::NP];
   const Place at = place_of(s, s.item0 + blockIdx.x, s.parts, S::CH);
@@ -234,15 +246,21 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads, 2) void backward_kernel(Scan 
   const int64_t start = at.p * s.part, end = start + s.part < s.t ? start + s.part : s.t;
   const int left = live ? s.n - n0 : 0;
   const f32x4 rate = load_upto(s.rate + c * s.n + n0, left);
+  const f32x4 rate2 = rate * kLog2e;
   f32x4 g = {0.0f, 0.0f, 0.0f, 0.0f}, drate = g;
   if (s.parts > 1)
     g = load_upto(s.carry + ((at.b * s.parts + at.p) * s.d + c) * s.n + n0, left);
   else if (s.dfinal)
     g = load_upto(s.dfinal + (at.b * s.d + c) * s.n + n0, left);
-  const int own = at.first + (threadIdx.x % (S::CH / 4)) * 4;
-  const f32x4 bias = per_channel(s.bias, (int64_t)at.group * s.dg + own, s.dg - own, 0.0f);
-  const f32x4 skip = per_channel(s.skip, (int64_t)at.group * s.dg + own, s.dg - own, 0.0f);
-  f32x4 dskip = {0.0f, 0.0f, 0.0f, 0.0f}, dbias = dskip;
+  const int own = at.first + At::channel();   // the channels this thread fetches
+  // out of the registers: of those channels dt_bias and skip, and of this thread the sums of their gradients
+  __shared__ __attribute__((aligned(16))) f32x4 params[2][S::CH / 4], grads[2][S::kThreads];
+  if (threadIdx.x < S::CH / 4) {
+    params[0][threadIdx.x] = per_channel(s.bias, (int64_t)at.group * s.dg + own, s.dg - own, 0.0f);
+    params[1][threadIdx.x] = per_channel(s.skip, (int64_t)at.group * s.dg + own, s.dg - own, 0.0f);
+  }
+  grads[0][threadIdx.x] = grads[1][threadIdx.x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  __syncthreads();
   const int64_t checks = (s.t + kTile - 1) / kTile;
   Fetched<T, LPC, true, true> next;
   int64_t t0 = start + (end - start - 1) / kTile * kTile;
@@ -251,153 +269,181 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads, 2) void backward_kernel(Scan 
     next.fetch(s, at, t0, end);
     h_next = load_upto(s.checks + ((at.b * checks + t0 / kTile) * s.d + c) * s.n + n0, left);
   }
-  for (; end > start && t0 >= start; t0 -= kTile) {
-    const Fetched<T, LPC, true, true> now = next;
-    const uint32_t begun = now.begun(t0, end);
+  for (int64_t tile = t0; end > start && tile >= start; tile -= kTile) {
+    const int64_t t0 = anew(tile);
+    uint32_t begun;
+    const int k = At::channel();
+    {
+      const Fetched<T, LPC, true, true>& now = next;
+      begun = now.begun(t0, end);
+      const f32x4 bias = params[0][k / 4];
 #pragma unroll
-    for (int i = 0; i < S::kSlots; ++i) {
-      const int slot = threadIdx.x + i * S::kThreads, tok = slot / (S::CH / 4), k = (slot % (S::CH / 4)) * 4;
-      if (tok >= kTile) break;
-      const bool there = t0 + tok < end && at.first + k < s.dg;
-      const int c0 = there ? at.first + k : 0;
-      const f32x4 x = values<T>(now.x[i], c0, s.dg), dt = values<T>(now.dt[i], c0, s.dg);
-      f32x4 dy = values<T>(now.dout[i], c0, s.dg);
-      if (s.gate.data) {
-        const f32x4 z = values<T>(now.gate[i], c0, s.dg);
+      for (int i = 0; i < S::kSlots; ++i) {
+        const int tok = At::token(i), slot = tok * (S::CH / 4) + k / 4;
+        if (tok >= kTile) break;
+        const bool there = t0 + tok < end && at.first + k < s.dg;
+        const int c0 = there ? at.first + k : 0;
+        const f32x4 x = values<T>(now.x[i], c0, s.dg), dt = values<T>(now.dt[i], c0, s.dg);
+        const f32x4 dout = values<T>(now.dout[i], c0, s.dg);
+        f32x4 dy = dout, slope, of_gate;
+        if (s.gate.data) {
+          const f32x4 z = values<T>(now.gate[i], c0, s.dg);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) dy[e] *= z[e] * sigmoid_for<T>(z[e]);
+          for (int e = 0; e < 4; ++e) {
+            const float one = sigmoid_for<T>(z[e]);
+            dy[e] = dout[e] * (z[e] * one);
+            of_gate[e] = dout[e] * (one * __builtin_fmaf(z[e], 1.0f - one, 1.0f));
+          }
+          held[3][slot] = of_gate;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const Softplus delta(dt[e] + bias[e]);
+          slope[e] = delta.slope;
+          steps[tok][k + e] = there ? f32x4{delta.value, delta.value * x[e], dy[e], 0.0f} : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        held[0][slot] = x, held[1][slot] = dy, held[2][slot] = slope;
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float delta = softplus(dt[e] + bias[e]);
-        steps[tok][k + e] = there ? f32x4{delta, delta * x[e], dy[e], 0.0f} : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      }
+      now.put_mix(s, t0, end, mix);
     }
-    now.put_mix(s, t0, end, mix);
     f32x4 h = h_next;
     __syncthreads();
     if (t0 - kTile >= start) {
       next.fetch(s, at, t0 - kTile, end);
       h_next = load_upto(s.checks + ((at.b * checks + t0 / kTile - 1) * s.d + c) * s.n + n0, left);
     }
-    f32x4 a[kTile], kept[kTile];   // of the state before: its decay, and what is left of it
+    const auto walk = [&](auto with_resets) {
+      constexpr bool kResets = decltype(with_resets)::value;
+      f32x4 a[kTile], kept[kTile];   // of the state before: its decay, and what is left of it
 #pragma unroll
-    for (int tok = 0; tok < kTile; ++tok) {
-      const f32x2 st = *(const f32x2*)&steps[tok][ch];
-      const f32x4 w = *(const f32x4*)&mix[tok][n0];
-      const bool begins = begun >> tok & 1;
+      for (int tok = 0; tok < kTile; ++tok) {
+        const f32x2 st = *(const f32x2*)&steps[tok][ch];
+        const f32x4 w = *(const f32x4*)&mix[tok][n0];
+        const bool begins = kResets && (begun >> tok & 1);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        a[tok][e] = exp2_of(st.x * (rate[e] * kLog2e));
-        kept[tok][e] = begins ? 0.0f : a[tok][e] * h[e];
-        h[e] = __builtin_fmaf(st.y, w[e], kept[tok][e]);
+        for (int e = 0; e < 4; ++e) {
+          a[tok][e] = exp2_of(st.x * rate2[e]);
+          kept[tok][e] = begins ? 0.0f : a[tok][e] * h[e];
+          h[e] = __builtin_fmaf(st.y, w[e], kept[tok][e]);
+        }
+        if (tok % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // loads moved further ahead would spill
       }
-    }
 #pragma unroll
-    for (int tok = kTile - 1; tok >= 0; --tok) {
-      const f32x4 st = steps[tok][ch];
-      const f32x4 w = *(const f32x4*)&mix[tok][n0], r = *(const f32x4*)&mix[tok][S::NP + n0];
-      float y = 0.0f, into = 0.0f, dd = 0.0f, v[8];
-      const bool begins = begun >> tok & 1;
+      for (int tok = kTile - 1; tok >= 0; --tok) {
+        const f32x4 st = steps[tok][ch];
+        const f32x4 w = *(const f32x4*)&mix[tok][n0], r = *(const f32x4*)&mix[tok][S::NP + n0];
+        float y = 0.0f, into = 0.0f, dd = 0.0f, v[8];
+        const bool begins = kResets && (begun >> tok & 1);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float state = __builtin_fmaf(st.y, w[e], kept[tok][e]);
-        g[e] = __builtin_fmaf(r[e], st.z, g[e]);
-        y = __builtin_fmaf(r[e], state, y);
-        into = __builtin_fmaf(g[e], w[e], into);
-        v[e] = g[e] * st.y;
-        v[4 + e] = state * st.z;
-        // of what is left of the state before, whose size may be far below the state's: kept by itself,
-        // as their difference would lose its last bits
-        const float through = g[e] * kept[tok][e];
-        drate[e] = __builtin_fmaf(through, st.x, drate[e]);
-        dd = __builtin_fmaf(through, rate[e], dd);
-        g[e] = begins ? 0.0f : g[e] * a[tok][e];
+        for (int e = 0; e < 4; ++e) {
+          const float state = __builtin_fmaf(st.y, w[e], kept[tok][e]);
+          g[e] = __builtin_fmaf(r[e], st.z, g[e]);
+          y = e ? __builtin_fmaf(r[e], state, y) : r[e] * state;
+          into = e ? __builtin_fmaf(g[e], w[e], into) : g[e] * w[e];
+          v[e] = g[e] * st.y;
+          v[4 + e] = state * st.z;
+          // of what is left of the state before, whose size may be far below the state's: kept by itself,
+          // as their difference would lose its last bits
+          const float through = g[e] * kept[tok][e];
+          drate[e] = __builtin_fmaf(through, st.x, drate[e]);
+          dd = e ? __builtin_fmaf(through, rate[e], dd) : through * rate[e];
+          g[e] = begins ? 0.0f : g[e] * a[tok][e];
+        }
+        y = lanes_sum<LPC>(y);
+        into = lanes_sum<LPC>(into);
+        dd = lanes_sum<LPC>(dd);
+        steps[tok][ch] = f32x4{st.x, into, dd, y};
+        Across<LPC>::sum(v, lane);
+#pragma unroll
+        for (int kk = 0; kk < Across<LPC>::kLeft; ++kk) {
+          const int id = Across<LPC>::id(lane, kk);
+          sums[wave][tok][(id >> 2) * S::NP + n0 + (id & 3)] = v[kk];
+        }
+        if (tok % 4 == 0) __builtin_amdgcn_sched_barrier(0);
       }
-      y = lanes_sum<LPC>(y);
-      into = lanes_sum<LPC>(into);
-      dd = lanes_sum<LPC>(dd);
-      steps[tok][ch] = f32x4{st.x, into, dd, y};
-      Across<LPC>::sum(v, lane);
-#pragma unroll
-      for (int k = 0; k < Across<LPC>::kLeft; ++k) {
-        const int id = Across<LPC>::id(lane, k);
-        sums[wave][tok][(id >> 2) * S::NP + n0 + (id & 3)] = v[k];
-      }
-    }
+    };
+    if (begun)
+      walk(std::true_type());
+    else
+      walk(std::false_type());
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < S::kSlots; ++i) {
-      const int slot = threadIdx.x + i * S::kThreads, tok = slot / (S::CH / 4), k = (slot % (S::CH / 4)) * 4;
+      const int tok = At::token(i), slot = tok * (S::CH / 4) + k / 4;
       if (tok >= kTile || t0 + tok >= end || at.first + k >= s.dg) continue;
-      const f32x4 x = values<T>(now.x[i], at.first + k, s.dg), dt = values<T>(now.dt[i], at.first + k, s.dg);
-      const f32x4 dout = values<T>(now.dout[i], at.first + k, s.dg);
-      f32x4 dx, ddt, dgate, z = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (s.gate.data) z = values<T>(now.gate[i], at.first + k, s.dg);
+      const f32x4 x = held[0][slot], dy = held[1][slot], slope = held[2][slot], skip = params[1][k / 4];
+      f32x4 dx, ddt, dgate, dskip = grads[0][threadIdx.x];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const f32x4 st = steps[tok][k + e];
-        const float one = sigmoid_for<T>(z[e]), dy = s.gate.data ? dout[e] * (z[e] * one) : dout[e];
-        dx[e] = __builtin_fmaf(st.x, st.y, skip[e] * dy);
-        ddt[e] = __builtin_fmaf(st.y, x[e], st.z) * sigmoid_for<T>(dt[e] + bias[e]);
-        const float y = __builtin_fmaf(skip[e], x[e], st.w);
-        dgate[e] = dout[e] * y * (one * (1.0f + z[e] * (1.0f - one)));
-        if (at.first + k + e < s.dg) {
-          dskip[e] = __builtin_fmaf(dy, x[e], dskip[e]);
-          dbias[e] += ddt[e];
-        }
+        dx[e] = __builtin_fmaf(st.x, st.y, skip[e] * dy[e]);
+        ddt[e] = __builtin_fmaf(st.y, x[e], st.z) * slope[e];
+        dgate[e] = __builtin_fmaf(skip[e], x[e], st.w);
       }
-      const int64_t col = (int64_t)at.group * s.dg + at.first + k, to = (at.b * s.t + t0 + tok) * s.d + col;
-      const int own_left = s.dg - at.first - k;
-      store_upto((T*)s.dx + to, dx, own_left);
-      store_upto((T*)s.ddt + to, ddt, own_left);
-      if (s.gate.data) store_upto((T*)s.dgate + to, dgate, own_left);
-    }
-    for (int i = threadIdx.x; i < kTile * 2 * S::NP; i += S::kThreads) {
-      const int tok = i / (2 * S::NP), which = i % (2 * S::NP), n = which % S::NP;
-      if (t0 + tok >= end) continue;
-      float sum = 0.0f;
 #pragma unroll
-      for (int k = 0; k < S::kWaves; ++k) sum += sums[k][tok][which];
-      const int64_t row = (at.b * s.t + t0 + tok) * s.g + at.group;
-      if (s.tiles > 1)
-        s.dmix[((int64_t)(at.first / S::CH) * (s.b * s.t * s.g) + row) * (2 * S::NP) + which] = sum;
-      else if (n < s.n)
-        ((T*)(which < S::NP ? s.dwrite : s.dread))[row * s.n + n] = (T)sum;
+      for (int e = 0; e < 4; ++e) dskip[e] = __builtin_fmaf(dy[e], x[e], dskip[e]);
+      grads[0][threadIdx.x] = dskip;
+      grads[1][threadIdx.x] += ddt;
+      const int64_t col = (int64_t)at.group * s.dg + at.first;
+      const int64_t row = (at.b * s.t + t0) * s.d + col;
+      const int own_left = s.dg - at.first - k;
+      store_upto((T*)row_at((T*)s.dx + row, tok, s.d) + k, dx, own_left);
+      store_upto((T*)row_at((T*)s.ddt + row, tok, s.d) + k, ddt, own_left);
+      if (s.gate.data) {
+        const f32x4 of_gate = held[3][slot];
+        store_upto((T*)row_at((T*)s.dgate + row, tok, s.d) + k, dgate * of_gate, own_left);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < S::kMixSlots; ++i) {
+      const int tok = At::mix_token(i), part = At::mix_part(), n = At::mix_state();
+      if (tok >= kTile || t0 + tok >= end) continue;
+      f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < S::kWaves; ++w) sum += *(const f32x4*)&sums[w][tok][part * 4];
+      const int64_t row = (at.b * s.t + t0) * s.g + at.group;
+      if (s.tiles > 1) {
+        float* to = s.dmix + ((int64_t)(at.first / S::CH) * (s.b * s.t * s.g) + row) * (2 * S::NP);
+        *(f32x4*)(row_at(to, tok, (int64_t)s.g * (2 * S::NP)) + part * 4) = sum;
+      } else {
+        T* to = (T*)(part < LPC ? s.dwrite : s.dread) + row * s.n;
+        store_upto((T*)row_at(to, tok, (int64_t)s.g * s.n) + n, sum, s.n - n);
+      }
     }
     __syncthreads();
   }
   const int64_t at_part = at.b * s.parts + at.p;
   if (at.p == 0) store_upto(s.dstate + (at.b * s.d + c) * s.n + n0, g, left);
-  float* params = s.dparams + at_part * ((int64_t)s.d * (s.n + 2));
-  store_upto(params + c * s.n + n0, drate, left);
+  float* params_to = s.dparams + at_part * ((int64_t)s.d * (s.n + 2));
+  store_upto(params_to + c * s.n + n0, drate, left);
   // the threads of the same four channels, one after another
-  f32x4* meet = &steps[0][0];
-  constexpr int kQuads = S::CH / 4, kRows = S::kThreads / kQuads;
-  static_assert(kRows * kQuads <= kTile * S::CH, "the sums of all threads fit the tile's place");
-#pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    meet[threadIdx.x] = which ? dbias : dskip;
-    __syncthreads();
-    if (threadIdx.x < kQuads) {
-      f32x4 sum = meet[threadIdx.x];
-      for (int k = 1; k < kRows; ++k) sum += meet[threadIdx.x + k * kQuads];
-      store_upto(params + (int64_t)s.d * (s.n + which) + (int64_t)at.group * s.dg + own, sum, s.dg - own);
-    }
-    __syncthreads();
+  constexpr int kQuads = S::CH / 4;
+  if (threadIdx.x < 2 * kQuads) {
+    const int which = threadIdx.x / kQuads, quad = threadIdx.x % kQuads, of = at.first + quad * 4;
+    f32x4 sum = grads[which][quad];
+    for (int i = 1; i < S::kThreads / kQuads; ++i) sum += grads[which][quad + i * kQuads];
+    store_upto(params_to + (int64_t)s.d * (s.n + which) + (int64_t)at.group * s.dg + of, sum, s.dg - of);
   }
 }
 
-// The sums over a group's blocks of channels, rounded to the result's type.
-template <class T>
-__global__ __launch_bounds__(kBlock) void mix_sums_kernel(Scan s, int np) {
-  const int64_t i = s.item0 + (int64_t)blockIdx.x * kBlock + threadIdx.x, rows = s.b * s.t * s.g, row = i / (2 * np);
+// The sums over a group's blocks of channels, rounded to the result's type: four values a thread.
+template <class T, int LPC>
+__global__ __launch_bounds__(kBlock) void mix_sums_kernel(Scan s) {
+  constexpr int NP = 4 * LPC;
+  const int64_t rows = s.b * s.t * s.g, i = s.item0 + (int64_t)blockIdx.x * kBlock + threadIdx.x, row = i / (2 * LPC);
   if (row >= rows) return;
-  const int which = (int)(i - row * 2 * np), n = which % np;
-  if (n >= s.n) return;
-  float sum = 0.0f;
-  for (int k = 0; k < s.tiles; ++k) sum += s.dmix[((int64_t)k * rows + row) * (2 * np) + which];
-  ((T*)(which < np ? s.dwrite : s.dread))[row * s.n + n] = (T)sum;
+  const int part = (int)(i % (2 * LPC)), n = part % LPC * 4;
+  f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int k0 = 0; k0 < s.tiles; k0 += 4) {
+    f32x4 x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      x[k] = *(const f32x4*)(s.dmix + ((int64_t)(k0 + k < s.tiles ? k0 + k : k0) * rows + row) * (2 * NP) + part * 4);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k0 + k < s.tiles) sum += x[k];
+  }
+  store_upto((T*)(part < LPC ? s.dwrite : s.dread) + row * s.n + n, sum, s.n - n);
 }
 
 // One token of every environment: LPC lanes a channel, each with four states, which are read once and
@@ -456,17 +502,18 @@ bool sequence_ok(int32_t dtype, int64_t b, int64_t t, int32_t d, int32_t n, int3
 
 int64_t blocks_of(const Scan& s, int64_t parts) { return s.b * parts * s.g * s.tiles; }
 
-// Sizes, and the parts of a row: as many as give the card eight waves a CU, no part below 64 tokens.
-int plan(Scan* s, int64_t b, int64_t t, int32_t d, int32_t n, int32_t g) {
+// Sizes, and the parts of a row: as many as fill the card with the waves that a CU holds of the pass, 16
+// forwards and 8 backwards, no part below 64 tokens.
+int plan(Scan* s, int64_t b, int64_t t, int32_t d, int32_t n, int32_t g, bool back) {
   int cus = 0;
   const int status = device_cus(&cus);
   if (status != HIPENVS_OK) return status;
   const int lpc = lanes_of(n), ch = channels_of(lpc);
   s->b = b, s->t = t, s->d = d, s->n = n, s->g = g, s->dg = d / g;
   s->tiles = (s->dg + ch - 1) / ch;
-  const int64_t waves = b * g * s->tiles * (ch * lpc / 64), want = (int64_t)cus * 8;
+  const int64_t waves = b * g * s->tiles * (ch * lpc / 64), want = (int64_t)cus * (back ? 8 : 16);
   int64_t parts = 1;
-  if (waves > 0 && waves * 2 <= want) {
+  if (waves > 0 && waves <= (int64_t)cus * 4) {
     parts = want / waves;
     if (parts > t / 64) parts = t / 64;
     if (parts < 1) parts = 1;
@@ -516,7 +563,6 @@ int in_launches(Scan s, int64_t blocks, int threads, const F& launch) {
 template <class F>
 int for_lanes(int lpc, const F& f) {
   switch (lpc) {
-    case 1: return f(std::integral_constant<int, 1>());
     case 2: return f(std::integral_constant<int, 2>());
     case 4: return f(std::integral_constant<int, 4>());
     case 8: return f(std::integral_constant<int, 8>());
@@ -570,16 +616,25 @@ int backward(const Scan& s, hipStream_t stream) {
     });
   });
   if (walked != HIPENVS_OK || s.tiles <= 1 || s.t == 0) return walked;
-  Scan one = s;
-  const int np = 4 * lanes_of(s.n);
-  const int64_t items = s.b * s.t * s.g * 2 * np;
-  for (one.item0 = 0; one.item0 < items; one.item0 += kMostThreads) {
-    const int64_t own = items - one.item0 < kMostThreads ? items - one.item0 : kMostThreads;
-    hipLaunchKernelGGL(mix_sums_kernel<T>, dim3(grid_for(own)), dim3(kBlock), 0, stream, one, np);
-    const int status = launch_status();
-    if (status != HIPENVS_OK) return status;
-  }
-  return HIPENVS_OK;
+  return for_lanes(lanes_of(s.n), [&](auto lanes) {
+    constexpr int LPC = decltype(lanes)::value;
+    Scan one = s;
+    const int64_t items = s.b * s.t * s.g * 2 * LPC;
+    for (one.item0 = 0; one.item0 < items; one.item0 += kMostThreads) {
+      const int64_t own = items - one.item0 < kMostThreads ? items - one.item0 : kMostThreads;
+      hipLaunchKernelGGL((mix_sums_kernel<T, LPC>), dim3(grid_for(own)), dim3(kBlock), 0, stream, one);
+      const int status = launch_status();
+      if (status != HIPENVS_OK) return status;
+    }
+    return (int)HIPENVS_OK;
+  });
+}
+
+// Whether the strides of t (of dout too, where `back`) fit the kernels' 32 bits.
+bool near(const int64_t* st, bool back) {
+  for (const int i : {1, 3, 5, 7, 10, 13, 15})
+    if ((i < 15 || back) && (st[i] > 0x7FFFFFFF || st[i] < -0x7FFFFFFF)) return false;
+  return true;
 }
 
 // x, dt, gate (and dout): b, t of each; write, read: b, t, g of each; reset: b, t.
@@ -604,7 +659,7 @@ extern "C" int64_t hipenvs_selective_scan_workspace_bytes(int32_t which, int64_t
   if (b == 0) return 0;
   if (which == 1) return b * ((t + kTile - 1) / kTile) * d * n * (int64_t)sizeof(float);
   Scan s = {};
-  if (plan(&s, b, t, d, n, g) != HIPENVS_OK) return -1;
+  if (plan(&s, b, t, d, n, g, which == 2) != HIPENVS_OK) return -1;
   float* between = nullptr;
   return which == 0 ? lay_parts(&s, nullptr) : lay_back(&s, nullptr, &between);
 }
@@ -619,10 +674,11 @@ extern "C" int hipenvs_selective_scan(int32_t dtype, const void* x, const void* 
   if (b == 0) return HIPENVS_OK;
   if (!rate || !final_state || (t > 0 && (!x || !dt || !write || !read || !out || !strides))) return HIPENVS_E_ARG;
   Scan s = {};
-  const int status = plan(&s, b, t, d, n, g);
+  const int status = plan(&s, b, t, d, n, g, false);
   if (status != HIPENVS_OK) return status;
   const int64_t need = lay_parts(&s, (char*)workspace);
   if (need > 0 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)) return HIPENVS_E_ARG;
+  if (t > 0 && !near(strides, false)) return HIPENVS_E_ARG;
   static const int64_t none[14] = {};
   s.x.data = x, s.dt.data = dt, s.gate.data = t > 0 ? gate : nullptr, s.write.data = write, s.read.data = read;
   strided(&s, t > 0 ? strides : none, false);
@@ -647,11 +703,12 @@ extern "C" int hipenvs_selective_scan_backward(int32_t dtype, const void* x, con
                                      !dread || !strides || (gate && !dgate))))
     return HIPENVS_E_ARG;
   Scan s = {};
-  int status = plan(&s, b, t, d, n, g);
+  int status = plan(&s, b, t, d, n, g, true);
   if (status != HIPENVS_OK) return status;
   float* between = nullptr;
   const int64_t need = lay_back(&s, (char*)workspace, &between);
   if (need > 0 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)) return HIPENVS_E_ARG;
+  if (t > 0 && !near(strides, true)) return HIPENVS_E_ARG;
   static const int64_t none[16] = {};
   s.x.data = x, s.dt.data = dt, s.gate.data = t > 0 ? gate : nullptr, s.write.data = write, s.read.data = read;
   s.dout.data = dout;

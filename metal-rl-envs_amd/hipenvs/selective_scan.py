@@ -73,6 +73,11 @@ def _strides(x, dt, write, read, gate, reset, dout=None):
     return _STRIDES[len(flat)](*flat)
 
 
+def _near(x):
+    """x, copied where its tokens lie further apart than the kernels' offsets reach."""
+    return x if x is None or -0x80000000 < x.stride(1) < 0x80000000 else x.contiguous()
+
+
 def _workspace(which, b, t, d, n, g, device):
     """(address, bytes, tensor): the workspace of a pass (0 forward, 2 backward), or the states that the
     backward pass starts from (1)."""
@@ -87,6 +92,7 @@ def _forward(x, dt, rate, write, read, skip, gate, dt_bias, state, reset, train)
     b, t, d = x.shape
     g, n = write.shape[2:]
     ptr = _lib.ptr
+    x, dt, write, read, gate, reset = (_near(y) for y in (x, dt, write, read, gate, reset))
     out = torch.empty((b, t, d), dtype=x.dtype, device=x.device)
     final = torch.empty((b, d, n), dtype=torch.float32, device=x.device)
     with _lib.on(x.device):
@@ -114,6 +120,7 @@ def _backward(ctx, dout, dfinal):
     if dout is None:
         dout = torch.zeros((b, t, d), dtype=dtype, device=device)
     dout = _checks.rows(dout, "the gradient", dtype, (b, t, d), index)
+    x, dt, write, read, gate, reset, dout = (_near(y) for y in (x, dt, write, read, gate, reset, dout))
     dfinal = _checks.f32(dfinal, "the gradient", (b, d, n), index)
     dx, ddt = (torch.empty((b, t, d), dtype=dtype, device=device) for _ in range(2))
     dgate = torch.empty((b, t, d), dtype=dtype, device=device) if gate is not None else None
