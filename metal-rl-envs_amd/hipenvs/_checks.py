@@ -42,6 +42,16 @@ def f32(x, name, shape, device, first="x"):
     return rows(x, name, torch.float32, shape, device, first).contiguous()
 
 
+def saved(x, dtype, shape, device):
+    """A tensor that autograd hands back, or a gradient: contiguous, of the type, shape and GPU that the
+    call works with. Hooks on saved tensors may hand back others of the same values, laid out in their own
+    way; anything else is refused. In the engine's thread each call costs several times what it does in the
+    caller's, so there is one for the ordinary case. None stays None."""
+    if x is None or (x.dtype is dtype and x.shape == shape and x.is_contiguous() and x.get_device() == device):
+        return x
+    return rows(x, "a tensor of the backward pass", dtype, shape, device, "the forward pass").contiguous()
+
+
 def resets(reset, shape, device, first="x"):
     if reset is None:
         return None

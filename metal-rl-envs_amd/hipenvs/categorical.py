@@ -40,12 +40,14 @@ def _forward(logits, tokens, top, train):
 def _backward(ctx, dlog_prob, dentropy, *_):
     logits, tokens, stats, entropy = ctx.saved_tensors
     dtype, (rows, v), index = ctx.ready
-    logits = _checks.rows(logits, "the saved logits", dtype, (rows, v), index, "logits")
-    tokens = _checks.rows(tokens, "the saved tokens", torch.int64, (rows,), index, "logits")
-    stats = _checks.f32(stats, "the saved sums", (rows, 2), index, "logits")
-    entropy = _checks.f32(entropy, "the saved entropy", (rows,), index, "logits")
+    if logits.dtype is not dtype or logits.shape != (rows, v) or logits.stride(1) != 1 or logits.get_device() != index:
+        logits = _checks.saved(logits, dtype, (rows, v), index)
+    tokens = _checks.saved(tokens, torch.int64, (rows,), index)
+    stats = _checks.saved(stats, torch.float32, (rows, 2), index)
+    entropy = _checks.saved(entropy, torch.float32, (rows,), index)
     _checks.refuse_tangents("the gradient of log_probs", dlog_prob, dentropy)
-    dlog_prob, dentropy = (_checks.f32(y, "the gradient", (rows,), index, "logits") for y in (dlog_prob, dentropy))
+    dlog_prob = _checks.saved(dlog_prob, torch.float32, (rows,), index)
+    dentropy = _checks.saved(dentropy, torch.float32, (rows,), index)
     ptr = _lib.ptr
     dlogits = torch.empty((rows, v), dtype=dtype, device=logits.device)
     with _lib.on(logits.device):
@@ -90,10 +92,14 @@ def log_probs(logits, tokens, top=0):
     if tokens.numel() > 0x7FFFFFFF:
         raise ValueError(f"there must be fewer than 2^31 rows, got {tokens.numel()}")
     _checks.refuse_tangents("log_probs", logits)
-    flat = logits.reshape(-1, v) if tokens.numel() else logits.reshape(0, v)
-    if flat.stride(-1) != 1 and v > 1:
+    flat = logits
+    if len(lead) != 1:
+        flat = logits.reshape(-1, v) if tokens.numel() else logits.reshape(0, v)
+        tokens = tokens.reshape(-1)
+    if flat.stride(-1) != 1:
         flat = flat.contiguous()
-    tokens = tokens.reshape(-1).to(torch.int64).contiguous()
+    if tokens.dtype is not torch.int64 or not tokens.is_contiguous():
+        tokens = tokens.to(torch.int64).contiguous()
     if _checks.wants_grad(flat):
         found = _LogProbs.apply(flat, tokens, top)
     else:

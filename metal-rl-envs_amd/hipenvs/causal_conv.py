@@ -65,17 +65,20 @@ def _forward(x, weight, bias, state, reset, silu):
 def _backward(ctx, dout, dfinal):
     x, weight, bias, state, reset = ctx.saved_tensors
     dtype, (b, t, d, w), index, silu = ctx.ready
-    x = _checks.rows(x, "the saved x", dtype, (b, t, d), index)
-    weight = _checks.f32(weight, "the saved weight", (d, w), index)
-    bias = _checks.f32(bias, "the saved bias", (d,), index)
-    state = _checks.f32(state, "the saved state", (b, w - 1, d), index)
-    reset = _checks.resets(reset, (b, t), index)
+    if x.dtype is not dtype or x.shape != (b, t, d) or x.stride(2) != 1 or x.get_device() != index:
+        x = _checks.saved(x, dtype, (b, t, d), index)
+    weight = _checks.saved(weight, torch.float32, (d, w), index)
+    bias = _checks.saved(bias, torch.float32, (d,), index)
+    state = _checks.saved(state, torch.float32, (b, w - 1, d), index)
+    if reset is not None:
+        reset = _checks.resets(reset, (b, t), index)
     _checks.refuse_tangents("the gradient of sequence", dout, dfinal)
     device, ptr = x.device, _lib.ptr
     if dout is None:
         dout = torch.zeros((b, t, d), dtype=dtype, device=device)
-    dout = _checks.rows(dout, "the gradient", dtype, (b, t, d), index)
-    dfinal = _checks.f32(dfinal, "the gradient", (b, w - 1, d), index)
+    elif dout.dtype is not dtype or dout.shape != (b, t, d) or dout.stride(2) != 1 or dout.get_device() != index:
+        dout = _checks.saved(dout, dtype, (b, t, d), index)
+    dfinal = _checks.saved(dfinal, torch.float32, (b, w - 1, d), index)
     dx = torch.empty((b, t, d), dtype=dtype, device=device)
     dparams = torch.empty(d * (w + 1), dtype=torch.float32, device=device)
     dstate = torch.empty((b, w - 1, d), dtype=torch.float32, device=device)

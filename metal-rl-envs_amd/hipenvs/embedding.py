@@ -33,7 +33,7 @@ def _backward(ctx, dout):
         return None, None, None
     tokens = _tokens(tokens, device.index)
     _checks.refuse_tangents("the gradient of lookup", dout)
-    dout = _checks.rows(dout, "the gradient", dtype, (*shape, d), device.index).reshape(-1, d)
+    dout = _checks.saved(dout, dtype, (*shape, d), device.index).view(-1, d) if tokens.numel() else dout.reshape(0, d)
     dtable = torch.empty((v, d), dtype=dtype, device=device)
     with _lib.on(device):
         nbytes = _lib.lib().hipenvs_embedding_workspace_bytes(tokens.numel(), v, d)

@@ -78,6 +78,14 @@ def _near(x):
     return x if x is None or -0x80000000 < x.stride(1) < 0x80000000 else x.contiguous()
 
 
+def _laid(x, dtype, shape, device):
+    """A tensor of the backward pass whose tokens the kernels reach: any strides, a contiguous last axis."""
+    if x is None or (x.dtype is dtype and x.shape == shape and x.stride(-1) == 1 and x.get_device() == device
+                     and -0x80000000 < x.stride(1) < 0x80000000):
+        return x
+    return _checks.saved(x, dtype, shape, device).contiguous()
+
+
 def _workspace(which, b, t, d, n, g, device):
     """(address, bytes, tensor): the workspace of a pass (0 forward, 2 backward), or the states that the
     backward pass starts from (1)."""
@@ -107,21 +115,18 @@ def _forward(x, dt, rate, write, read, skip, gate, dt_bias, state, reset, train)
 def _backward(ctx, dout, dfinal):
     x, dt, rate, write, read, skip, gate, dt_bias, reset, checks = ctx.saved_tensors
     dtype, (b, t, d, n, g), index, nchecks, has_state = ctx.ready
-    # hooks on saved tensors may hand back others of the same values, laid out in their own way
-    x, dt, gate = (y if y is None else _checks.rows(y, "a saved tensor", dtype, (b, t, d), index) for y in (x, dt, gate))
-    write, read = (_checks.rows(y, "a saved tensor", dtype, (b, t, g, n), index) for y in (write, read))
-    rate = _checks.f32(rate, "the saved rate", (d, n), index)
-    skip, dt_bias = (_checks.f32(y, "a saved tensor", (d,), index) for y in (skip, dt_bias))
-    reset = _checks.resets(reset, (b, t), index)
-    if checks is not None:
-        checks = _checks.rows(checks, "the saved states", torch.uint8, (nchecks,), index)
+    shape, mixed = (b, t, d), (b, t, g, n)
+    x, dt, gate = _laid(x, dtype, shape, index), _laid(dt, dtype, shape, index), _laid(gate, dtype, shape, index)
+    write, read = _laid(write, dtype, mixed, index), _laid(read, dtype, mixed, index)
+    rate = _checks.saved(rate, torch.float32, (d, n), index)
+    skip, dt_bias = _checks.saved(skip, torch.float32, (d,), index), _checks.saved(dt_bias, torch.float32, (d,), index)
+    if reset is not None:
+        reset = _near(_checks.resets(reset, (b, t), index))
+    checks = _checks.saved(checks, torch.uint8, (nchecks,), index)
     _checks.refuse_tangents("the gradient of sequence", dout, dfinal)
     device, ptr = x.device, _lib.ptr
-    if dout is None:
-        dout = torch.zeros((b, t, d), dtype=dtype, device=device)
-    dout = _checks.rows(dout, "the gradient", dtype, (b, t, d), index)
-    x, dt, write, read, gate, reset, dout = (_near(y) for y in (x, dt, write, read, gate, reset, dout))
-    dfinal = _checks.f32(dfinal, "the gradient", (b, d, n), index)
+    dout = torch.zeros(shape, dtype=dtype, device=device) if dout is None else _laid(dout, dtype, shape, index)
+    dfinal = _checks.saved(dfinal, torch.float32, (b, d, n), index)
     dx, ddt = (torch.empty((b, t, d), dtype=dtype, device=device) for _ in range(2))
     dgate = torch.empty((b, t, d), dtype=dtype, device=device) if gate is not None else None
     dwrite, dread = (torch.empty((b, t, g, n), dtype=dtype, device=device) for _ in range(2))
