@@ -521,7 +521,7 @@ int64_t hipenvs_embedding_workspace_bytes(int64_t count, int64_t v, int32_t d);
 
 /* dtable (v, d) = scale * the sums of the rows of dout (count, d), dout_s elements apart, over equal
  * tokens, zeros where there is none; f32 sums in an order that depends on the tokens alone. Tokens that
- * are negative or past the table add to nothing. workspace: 16-byte aligned. */
+ * are negative or past the table add to nothing. dtable and workspace: 16-byte aligned. */
 int hipenvs_embedding_backward(int32_t dtype, const void* tokens, int32_t token_bytes, const void* dout,
                                int64_t dout_s, float scale, void* dtable, int64_t count, int64_t v, int32_t d,
                                void* workspace, int64_t workspace_bytes, hipenvs_stream_t stream);

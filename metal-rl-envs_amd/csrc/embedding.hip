@@ -41,16 +41,21 @@ __global__ __launch_bounds__(kBlock) void lookup_kernel(Tokens tokens, const T* 
 // ---- sorting the tokens ---------------------------------------------------------------
 // Least digit first, 8 bits a pass, each pass stable, so a token's places stay in their order. Keys
 // are tokens, v where there is none. A pass counts the digits of each tile of kRounds x 256 keys,
-// sums each digit's counts up over the tiles, and moves each key with its place.
+// sums each digit's counts up over the tiles (where they are few, in every block that moves) and
+// moves each key with its place.
 
-constexpr int kDigit = 256;
+constexpr int kDigit = 256, kFewTiles = 64;
 
 struct Sort {
   Tokens tokens;
   const uint32_t *keys, *places;   // null in the first pass: the tokens as they come
-  uint32_t *keys_out, *places_out, *counts;   // counts (256, tiles), then the digits' totals (256)
+  uint32_t *keys_out, *places_out, *counts;   // counts (tiles, 256), then the digits' totals (256)
   int64_t count, v, tiles;
   int shift;
+  bool summed;   // counts are those of the tiles before; otherwise of the tile itself, at most kFewTiles of them
+  void* clear;   // in the first pass, what becomes zeros: the gradient, of `words` 32-bit words and a half of one
+  int64_t words;
+  bool half;
 
   __device__ __forceinline__ uint32_t key(int64_t i) const {
     if (keys) return keys[i];
@@ -59,10 +64,18 @@ struct Sort {
   }
 };
 
-// The tile's digits.
+// The tile's digits; and in the first pass zeros over the gradient, by as many blocks as that takes.
 template <int kRounds>
 __global__ __launch_bounds__(kBlock) void count_kernel(Sort s) {
   __shared__ uint32_t counts[kDigit];
+  if (s.clear) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    const int64_t step = (int64_t)gridDim.x * kBlock, first = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    for (int64_t i = first; i < s.words / 4; i += step) ((u32x4*)s.clear)[i] = u32x4{0, 0, 0, 0};
+    if (first < s.words % 4) ((uint32_t*)s.clear)[s.words / 4 * 4 + first] = 0;
+    if (first == 0 && s.half) ((uint16_t*)s.clear)[2 * s.words] = 0;
+  }
+  if (blockIdx.x >= s.tiles) return;
   counts[threadIdx.x] = 0;
   __syncthreads();
   const int64_t first = (int64_t)blockIdx.x * (kBlock * kRounds) + threadIdx.x;
@@ -76,18 +89,18 @@ __global__ __launch_bounds__(kBlock) void count_kernel(Sort s) {
   for (int r = 0; r < kRounds; ++r)
     if (first + r * kBlock < s.count) atomicAdd(&counts[(keys[r] >> s.shift) & 255], 1u);
   __syncthreads();
-  s.counts[threadIdx.x * s.tiles + blockIdx.x] = counts[threadIdx.x];
+  s.counts[blockIdx.x * kDigit + threadIdx.x] = counts[threadIdx.x];
 }
 
 // A block for each digit: its tiles' counts -> the sums of those before, in place; and its total.
 __global__ __launch_bounds__(kBlock) void sum_up_kernel(Sort s) {
   __shared__ uint32_t totals[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint32_t* counts = s.counts + blockIdx.x * s.tiles;
+  uint32_t* counts = s.counts + blockIdx.x;
   uint32_t before = 0;
   for (int64_t first = 0; first < s.tiles; first += kBlock) {
     const int64_t i = first + threadIdx.x;
-    const uint32_t own = i < s.tiles ? counts[i] : 0u;
+    const uint32_t own = i < s.tiles ? counts[i * kDigit] : 0u;
     uint32_t upto = own;
 #pragma unroll
     for (int step = 1; step < 64; step *= 2) {
@@ -102,7 +115,7 @@ __global__ __launch_bounds__(kBlock) void sum_up_kernel(Sort s) {
       if (k < wave) at += totals[k];
       before += totals[k];
     }
-    if (i < s.tiles) counts[i] = at;
+    if (i < s.tiles) counts[i * kDigit] = at;
     __syncthreads();
   }
   if (threadIdx.x == 0) s.counts[kDigit * s.tiles + blockIdx.x] = before;
@@ -122,7 +135,23 @@ __global__ __launch_bounds__(kBlock) void move_kernel(Sort s) {
     places[r] = s.places ? s.places[i] : (uint32_t)i;
   }
   // the keys of lower digits, by the digits' totals
-  const uint32_t total = s.counts[kDigit * s.tiles + threadIdx.x];
+  uint32_t total = 0, base = 0;
+  if (s.summed) {
+    total = s.counts[kDigit * s.tiles + threadIdx.x];
+    base = s.counts[blockIdx.x * kDigit + threadIdx.x];
+  } else {
+    const int tiles = (int)s.tiles;
+    for (int k0 = 0; k0 < tiles; k0 += 16) {
+      uint32_t own[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) own[k] = s.counts[(k0 + k < tiles ? k0 + k : tiles - 1) * kDigit + threadIdx.x];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        if (k0 + k < tiles) total += own[k];
+        if (k0 + k < (int)blockIdx.x) base += own[k];
+      }
+    }
+  }
   uint32_t upto = total;
 #pragma unroll
   for (int step = 1; step < 64; step *= 2) {
@@ -135,7 +164,7 @@ __global__ __launch_bounds__(kBlock) void move_kernel(Sort s) {
 #pragma unroll
   for (int r = 0; r < kRounds; ++r)
     if (first + r * 64 < s.count) atomicAdd(&at[wave][(keys[r] >> s.shift) & 255], 1u);
-  uint32_t base = upto - total + s.counts[threadIdx.x * s.tiles + blockIdx.x];
+  base += upto - total;
   for (int k = 0; k < wave; ++k) base += totals[k];
   __syncthreads();
   for (int k = 0; k < 4; ++k) {
@@ -182,12 +211,6 @@ struct Sums {
   int32_t d, quads, group, columns;   // group: lanes that share a chunk; columns: groups for a row
   float scale;
 };
-
-template <class T>
-__global__ __launch_bounds__(kBlock) void clear_kernel(T* x, int64_t n, int64_t item0) {
-  const int64_t i = (item0 + (int64_t)blockIdx.x * kBlock + threadIdx.x) * 4;
-  if (i < n) store_upto(x + i, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, n - i);
-}
 
 template <class T>
 __global__ __launch_bounds__(kBlock) void chunks_kernel(Sums s) {
@@ -248,11 +271,11 @@ __global__ __launch_bounds__(kBlock) void across_kernel(Sums s) {
   const uint32_t key = s.keys[end - 1];
   if (key == (uint32_t)s.v || s.keys[end] != key) return;
   if (first > 0 && s.keys[first - 1] == key) return;   // it began before this chunk
-  int64_t low = end, high = s.count;                    // keys[low] == key, keys[high] > key
+  int64_t low = end, high = s.count;   // keys[low] == key, keys[high] is above it: 256 probes a round
   while (high - low > 1) {
-    const int64_t mid = (low + high) / 2;
-    if (s.keys[mid] == key) low = mid;
-    else high = mid;
+    const int64_t step = (high - low + kBlock - 1) / kBlock, at = low + (threadIdx.x + 1) * step;
+    low += __syncthreads_count(at < high && s.keys[at] == key) * step;
+    high = low + step < high ? low + step : high;
   }
   const int64_t last = low / kChunk;   // of the run's chunks
   f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -353,7 +376,7 @@ int64_t small_blocks(int64_t count, int32_t d) {
   return blocks < 1024 ? blocks : 1024;
 }
 
-int rounds_of(int64_t count) { return count < (1 << 18) ? 4 : 16; }
+int rounds_of(int64_t count) { return count <= 4 * kBlock * kFewTiles ? 4 : 16; }
 
 struct Laid {
   int64_t keys, counts, partial, bytes;
@@ -403,26 +426,34 @@ int gradient(Tokens tokens, const void* dout, int64_t dout_s, float scale, void*
              int32_t d, char* workspace, hipStream_t stream) {
   if (v <= kSmall && count > 0)
     return small_gradient<T>(tokens, dout, dout_s, scale, dtable, count, v, d, workspace, stream);
-  const int64_t values = v * d;
-  int status = in_launches((values + 3) / 4, [&](int64_t item0, dim3 grid) {
-    hipLaunchKernelGGL(clear_kernel<T>, grid, dim3(kBlock), 0, stream, (T*)dtable, values, item0);
-  });
-  if (status != HIPENVS_OK || count == 0) return status;
-  const Laid l = lay(count, v, d);
+  const int64_t bytes = v * d * (int64_t)sizeof(T);
+  // 16 KiB a block, at most eight blocks a CU
+  const unsigned clears = (unsigned)(bytes / 16384 < 2047 ? bytes / 16384 + 1 : 2048);
   const int rounds = rounds_of(count);
+  if (count == 0) {
+    Sort nothing = {};
+    nothing.clear = dtable, nothing.words = bytes / 4, nothing.half = bytes % 4 != 0;
+    hipLaunchKernelGGL(count_kernel<4>, dim3(clears), dim3(kBlock), 0, stream, nothing);
+    return launch_status();
+  }
+  int status = HIPENVS_OK;
+  const Laid l = lay(count, v, d);
   uint32_t* keys[2] = {(uint32_t*)workspace, (uint32_t*)(workspace + l.keys)};
   uint32_t* places[2] = {(uint32_t*)(workspace + 2 * l.keys), (uint32_t*)(workspace + 3 * l.keys)};
   Sort sort = {tokens, nullptr, nullptr, nullptr, nullptr, (uint32_t*)(workspace + 4 * l.keys), count, v,
-               (count + kBlock * rounds - 1) / (kBlock * rounds), 0};
+               (count + kBlock * rounds - 1) / (kBlock * rounds), 0, false, dtable, bytes / 4, bytes % 4 != 0};
+  sort.summed = sort.tiles > kFewTiles;
   int to = 0;
   for (; (v >> sort.shift) > 0; sort.shift += 8, to ^= 1) {
     sort.keys_out = keys[to], sort.places_out = places[to];
     const dim3 tiles((unsigned)sort.tiles), block(kBlock);
+    const dim3 counting(sort.clear && clears > tiles.x ? clears : tiles.x);
     if (rounds == 4)
-      hipLaunchKernelGGL(count_kernel<4>, tiles, block, 0, stream, sort);
+      hipLaunchKernelGGL(count_kernel<4>, counting, block, 0, stream, sort);
     else
-      hipLaunchKernelGGL(count_kernel<16>, tiles, block, 0, stream, sort);
-    hipLaunchKernelGGL(sum_up_kernel, dim3(kDigit), block, 0, stream, sort);
+      hipLaunchKernelGGL(count_kernel<16>, counting, block, 0, stream, sort);
+    sort.clear = nullptr;
+    if (sort.summed) hipLaunchKernelGGL(sum_up_kernel, dim3(kDigit), block, 0, stream, sort);
     if (rounds == 4)
       hipLaunchKernelGGL(move_kernel<4>, tiles, block, 0, stream, sort);
     else
@@ -488,6 +519,7 @@ extern "C" int hipenvs_embedding_backward(int32_t dtype, const void* tokens, int
   if (count > 0 && (!tokens || !dout || !workspace || ((uintptr_t)workspace & 15) ||
                     workspace_bytes < lay(count, v, d).bytes))
     return HIPENVS_E_ARG;
+  if ((uintptr_t)dtable & 15) return HIPENVS_E_ARG;
   const Tokens of = {tokens, token_bytes == 8};
   return dtype == 1 ? gradient<__bf16>(of, dout, dout_s, scale, dtable, count, v, d, (char*)workspace, as_stream(stream))
                     : gradient<float>(of, dout, dout_s, scale, dtable, count, v, d, (char*)workspace, as_stream(stream));

@@ -447,7 +447,8 @@ __global__ __launch_bounds__(kBlock) void mix_sums_kernel(Scan s) {
 }
 
 // One token of every environment: LPC lanes a channel, each with four states, which are read once and
-// written once, bound by that. next may be state itself: a thread writes only what it has read.
+// written once, bound by that. A thread takes its channel of kEnvs environments, so that as many states are
+// in flight. next may be state itself: a thread writes only what it has read.
 struct Step {
   const void *x, *dt, *gate, *write, *read;
   int64_t x_s, dt_s, gate_s, write_s, write_sg, read_s, read_sg, reset_s;
@@ -455,39 +456,53 @@ struct Step {
   const uint8_t* reset;
   void* out;
   float* next;
-  int64_t count, item0;   // count: environments times channels
+  int64_t count, items, item0;   // count: environments; items: channels of groups of kEnvs
   int32_t d, n, dg;
 };
 
-template <class T, int LPC>
+template <class T, int LPC, int kEnvs>
 __global__ __launch_bounds__(kBlock) void step_kernel(Step s) {
   const int64_t item = s.item0 + (int64_t)blockIdx.x * (kBlock / LPC) + threadIdx.x / LPC;
-  if (item >= s.count) return;   // all of a channel's lanes
-  const int64_t env = (uint32_t)item / (uint32_t)s.d;
-  const int c = (int)(item - env * s.d), group = c / s.dg, n0 = (threadIdx.x % LPC) * 4, left = s.n - n0;
-  const bool begins = s.reset && s.reset[env * s.reset_s];
-  f32x4 h = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (!begins) h = load_upto(s.state + item * s.n + n0, left);
-  const f32x4 rate = load_upto(s.rate + (int64_t)c * s.n + n0, left);
-  const f32x4 w = load_upto((const T*)s.write + env * s.write_s + group * s.write_sg + n0, left);
-  const f32x4 r = load_upto((const T*)s.read + env * s.read_s + group * s.read_sg + n0, left);
-  const float x = (float)((const T*)s.x)[env * s.x_s + c], dt = (float)((const T*)s.dt)[env * s.dt_s + c];
-  const float delta = softplus(dt + (s.bias ? s.bias[c] : 0.0f)), du = delta * x;
-  float y = 0.0f;
+  if (item >= s.items) return;   // all of a channel's lanes
+  const int64_t env0 = (int64_t)((uint32_t)item / (uint32_t)s.d) * kEnvs;
+  const int c = (int)(item % (uint32_t)s.d), group = c / s.dg, n0 = (threadIdx.x % LPC) * 4, left = s.n - n0;
+  f32x4 h[kEnvs];
+  typename Raw<T>::type w[kEnvs], r[kEnvs];
+  T x[kEnvs], dt[kEnvs], z[kEnvs];
+  uint8_t begins[kEnvs];
+  const int from = n0 < s.n ? n0 : 0;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    h[e] = __builtin_fmaf(exp2_of(delta * (rate[e] * kLog2e)), h[e], du * w[e]);
-    y = __builtin_fmaf(r[e], h[e], y);
+  for (int k = 0; k < kEnvs; ++k) {   // past the last environment, that one again: all loads in flight
+    const int64_t env = env0 + k < s.count ? env0 + k : s.count - 1;
+    h[k] = fetch4(s.state + (env * s.d + c) * s.n, from, s.n);
+    w[k] = fetch4((const T*)s.write + env * s.write_s + group * s.write_sg, from, s.n);
+    r[k] = fetch4((const T*)s.read + env * s.read_s + group * s.read_sg, from, s.n);
+    x[k] = ((const T*)s.x)[env * s.x_s + c];
+    dt[k] = ((const T*)s.dt)[env * s.dt_s + c];
+    z[k] = s.gate ? ((const T*)s.gate)[env * s.gate_s + c] : (T)0.0f;
+    begins[k] = s.reset ? s.reset[env * s.reset_s] : 0;
   }
-  store_upto(s.next + item * s.n + n0, h, left);
-  y = lanes_sum<LPC>(y);
-  if (n0 == 0) {
-    if (s.skip) y = __builtin_fmaf(s.skip[c], x, y);
-    if (s.gate) {
-      const float z = (float)((const T*)s.gate)[env * s.gate_s + c];
-      y *= z * sigmoid_for<T>(z);
+  const f32x4 rate = load_upto(s.rate + (int64_t)c * s.n + n0, left);
+  const float bias = s.bias ? s.bias[c] : 0.0f, skip = s.skip ? s.skip[c] : 0.0f;
+#pragma unroll
+  for (int k = 0; k < kEnvs; ++k) {
+    if (env0 + k >= s.count) break;
+    const float delta = softplus((float)dt[k] + bias), du = delta * (float)x[k];
+    f32x4 state = values<float>(h[k], from, s.n), wk = values<T>(w[k], from, s.n), rk = values<T>(r[k], from, s.n);
+    if (n0 >= s.n) wk = rk = state = f32x4{0.0f, 0.0f, 0.0f, 0.0f};   // a lane without states
+    float y = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      state[e] = __builtin_fmaf(exp2_of(delta * (rate[e] * kLog2e)), begins[k] ? 0.0f : state[e], du * wk[e]);
+      y = __builtin_fmaf(rk[e], state[e], y);
     }
-    ((T*)s.out)[item] = (T)y;
+    store_upto(s.next + ((env0 + k) * s.d + c) * s.n + n0, state, left);
+    y = lanes_sum<LPC>(y);
+    if (n0 == 0) {
+      y = __builtin_fmaf(skip, (float)x[k], y);
+      if (s.gate) y *= (float)z[k] * sigmoid_for<T>((float)z[k]);
+      ((T*)s.out)[(env0 + k) * s.d + c] = (T)y;
+    }
   }
 }
 
@@ -730,21 +745,31 @@ extern "C" int hipenvs_selective_scan_step(int32_t dtype, const void* x, const v
   if (!dims_ok(dtype, d, n, g) || count < 0 || count > 0x7FFFFFFF || count * d > 0x7FFFFFFF) return HIPENVS_E_ARG;
   if (count == 0) return HIPENVS_OK;
   if (!x || !dt || !rate || !write || !read || !state || !strides || !out || !next_state) return HIPENVS_E_ARG;
+  int cus = 0;
+  const int status = device_cus(&cus);
+  if (status != HIPENVS_OK) return status;
   Step s = {x,          dt,         gate,       write,      read,       strides[0], strides[1], strides[2], strides[3],
             strides[4], strides[5], strides[6], strides[7], rate,       skip,       dt_bias,    state,      reset,
-            out,        next_state, count * d,  0,          d,          n,          d / g};
+            out,        next_state, count,      0,          0,          d,          n,          d / g};
   return for_lanes(lanes_of(n), [&](auto lanes) {
     constexpr int LPC = decltype(lanes)::value, kChannels = kBlock / LPC;
+    // four environments a thread where that leaves 32 blocks a CU
+    const bool many = count * d / 4 >= (int64_t)cus * 32 * kChannels;
+    s.items = (many ? (count + 3) / 4 : count) * d;
     const int64_t most = kMostThreads / kBlock * kChannels;
-    for (s.item0 = 0; s.item0 < s.count; s.item0 += most) {
-      const int64_t own = s.count - s.item0 < most ? s.count - s.item0 : most;
+    for (s.item0 = 0; s.item0 < s.items; s.item0 += most) {
+      const int64_t own = s.items - s.item0 < most ? s.items - s.item0 : most;
       const dim3 grid((unsigned)((own + kChannels - 1) / kChannels)), block(kBlock);
-      if (dtype == 1)
-        hipLaunchKernelGGL((step_kernel<__bf16, LPC>), grid, block, 0, as_stream(stream), s);
+      if (dtype == 1 && many)
+        hipLaunchKernelGGL((step_kernel<__bf16, LPC, 4>), grid, block, 0, as_stream(stream), s);
+      else if (dtype == 1)
+        hipLaunchKernelGGL((step_kernel<__bf16, LPC, 1>), grid, block, 0, as_stream(stream), s);
+      else if (many)
+        hipLaunchKernelGGL((step_kernel<float, LPC, 4>), grid, block, 0, as_stream(stream), s);
       else
-        hipLaunchKernelGGL((step_kernel<float, LPC>), grid, block, 0, as_stream(stream), s);
-      const int status = launch_status();
-      if (status != HIPENVS_OK) return status;
+        hipLaunchKernelGGL((step_kernel<float, LPC, 1>), grid, block, 0, as_stream(stream), s);
+      const int launched = launch_status();
+      if (launched != HIPENVS_OK) return launched;
     }
     return (int)HIPENVS_OK;
   });

@@ -422,3 +422,21 @@ def test_refusals(dev):
     with torch.autograd.forward_ad.dual_level():
         dual = torch.autograd.forward_ad.make_dual(c["x"], torch.ones_like(c["x"]))
         refused(ValueError, x=dual)
+
+
+@pytest.mark.parametrize("count,d,n,g", [(4099, 256, 16, 2), (3001, 200, 5, 1), (8190, 64, 40, 4)])
+def test_steps_of_many_environments(dev, count, d, n, g):
+    """Several environments a thread, the last group not whole, against the definition."""
+    from hipenvs import selective_scan
+
+    for dtype in (F32, BF16):
+        c = make(dev, 2 * g, count, 1, d, n, g, dtype, "fused", 3)
+        one = {k: (v[:, 0] if k in ("x", "dt", "write", "read", "gate", "reset") else v) for k, v in c.items()}
+        out, state = selective_scan.step(**one)
+        f64 = to_np(c)
+        want = oss.sequence(**f64)
+        size = oss.magnitudes(*f64.values(), np.zeros((count, 1, d)), np.zeros((count, d, n)))
+        close(out[:, None], want[0], size[0], dtype, units(1, d, n))
+        close(state, want[1], size[1], F32, units(1, d, n))
+        again, same = selective_scan.step(**one, next_state=one["state"])
+        assert torch.equal(again, out) and torch.equal(same, state)
