@@ -58,7 +58,7 @@ def make(dev, seed, count, v, d, dtype, wide=True, past=0, absent=0.1, skew=1.0)
 
 
 CASES = [  # tokens, rows of the table, width
-    (1, 1, 1), (5, 3, 4), (63, 2, 64), (64, 3, 65), (65, 1, 7), (1000, 3, 64), (4097, 255, 3), (5000, 256, 130),
+    (1, 1, 1), (5, 3, 4), (3000, 16, 300), (3000, 17, 300), (63, 2, 64), (64, 3, 65), (65, 1, 7), (1000, 3, 64), (4097, 255, 3), (5000, 256, 130),
     (9000, 257, 32), (20000, 70000, 12), (3000, 65535, 8), (700, 5, 513), (129, 17000000, 1), (70000, 2, 5), (30000, 65536, 2),
 ]
 

@@ -215,6 +215,47 @@ def test_what_a_reset_leaves_out(dev, t):
         assert torch.isfinite(a).all() and torch.equal(a, e)
 
 
+@pytest.mark.parametrize("n", [3, 5, 8, 12, 16, 24, 40, 64])
+def test_infinities_reach_what_they_should(dev, n):
+    """An infinite x of one channel: its outputs and states are infinite until the episode ends, and no other
+    channel's or later token's is touched; an infinite dt decays all of a state, past n too."""
+    from hipenvs import selective_scan
+
+    b, t, d = 1, 40, 6
+    x, dt = torch.ones(b, t, d, device=dev), torch.zeros(b, t, d, device=dev)
+    mix = torch.ones(b, t, n, device=dev)
+    rate = -torch.full((d, n), 0.01, device=dev)
+    reset = torch.zeros(b, t, dtype=torch.bool, device=dev)
+    reset[0, 30] = True
+    clean, _ = selective_scan.sequence(x, dt, rate, mix, mix, reset=reset)
+    x[0, 3, 2] = float("inf")
+    out, final = selective_scan.sequence(x, dt, rate, mix, mix, reset=reset)
+    assert torch.isinf(out[0, 3:30, 2]).all() and torch.isfinite(final).all()
+    keep = torch.ones(b, t, d, dtype=torch.bool, device=dev)
+    keep[0, 3:30, 2] = False
+    assert torch.equal(out[keep], clean[keep])
+    state = torch.zeros(1, d, n, device=dev)
+    acted = []
+    for i in range(t):
+        o, _ = selective_scan.step(x[:, i], dt[:, i], rate, mix[:, i], mix[:, i], state=state, reset=reset[:, i],
+                                   next_state=state)
+        acted.append(o)
+    acted = torch.stack(acted, 1)
+    assert torch.equal(torch.isinf(acted), ~keep) and torch.isfinite(state).all()
+    # the gradients of a clean window before and behind it, an infinite dout of one token among them
+    x = torch.ones(b, t, d, device=dev, requires_grad=True)
+    dout = torch.ones(b, t, d, device=dev)
+    dout[0, 35, 1] = float("inf")
+    out, _ = selective_scan.sequence(x, dt, rate, mix, mix, reset=reset)
+    dx, = torch.autograd.grad(out, x, dout)
+    assert torch.isinf(dx[0, 30:36, 1]).all() and torch.isfinite(dx[0, :30]).all() and torch.isfinite(dx[0, 36:]).all()
+    # an infinite dt: the state before is gone, the token's own is infinite
+    dt = dt.clone()
+    dt[0, 5, 4] = float("inf")
+    out, _ = selective_scan.sequence(x.detach(), dt, rate, mix, mix, reset=reset)
+    assert torch.isinf(out[0, 5:30, 4]).all() and torch.isfinite(out[0, 30:]).all() and torch.isfinite(out[0, :5]).all()
+
+
 def test_infinite_and_zero_states_pass_parts(dev):
     """An infinite state stays infinite and a zero one zero over parts whose decay leaves float32's
     range, as token by token."""
