@@ -7,7 +7,10 @@
 // row's first token come from `state`, the W - 1 values before it.
 //
 // A thread walks a run of tokens of four channels with the last W - 1 values in registers, so each
-// value is read once but for the W - 1 at a run's borders; bound by memory.
+// value is read once but for the W - 1 at a run's borders. A block's threads walk the same tokens, so
+// what depends on the token alone is scalar. 64 x 1,000 tokens of 501 channels, bfloat16 at odd addresses: 41 us,
+// 3.1 TB/s, and 76 + 10 backwards, 2.5 TB/s, bound by vector instructions (about 55 and 60 % of the time) and
+// by the latency that two waves a SIMD leave backwards (200 registers; three waves spill: 180 us).
 #include "row_ops.h"
 
 namespace hipenvs {

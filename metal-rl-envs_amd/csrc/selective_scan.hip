@@ -7,18 +7,24 @@ namespace scan {
 
 // What a tile's walk has to leave out. States past n have no write and no read, but zero times an
 // infinity is no number: where there are any, they are kept at zero, by whole lanes that see neither delta x
-// nor dy (n a multiple of four) or one by one. 4,096 x 128 x 128, float32, a third of the tiles with
-// beginnings: 1,440 us with every tile as kAny, 1,268 so (backwards).
-enum Kind { kPlain, kLanes, kAny };   // nothing; lanes without states; beginnings, or single states too
+// nor dy (n a multiple of four) or one by one. 64 x 1,000 tokens of 500 channels of 12 states, bfloat16:
+// 264 and 635 us forwards and backwards with every tile as kAny, 230 and 565 so.
+// kFull: n is all the lanes' states, and there are none past it.
+enum Kind { kPlain, kLanes, kBegins, kAny };   // nothing; lanes without states; beginnings; single states too
 
-template <class F>
-__device__ __forceinline__ void for_kind(uint32_t begins, int n, int np, const F& walk) {
-  if (begins || n % 4 != 0)
-    walk(std::integral_constant<int, kAny>());
-  else if (n < np)
-    walk(std::integral_constant<int, kLanes>());
-  else
-    walk(std::integral_constant<int, kPlain>());
+template <bool kFull, class F>
+__device__ __forceinline__ void for_kind(uint32_t begins, int n, const F& walk) {
+  if constexpr (kFull) {
+    if (begins)
+      walk(std::integral_constant<int, kBegins>());
+    else
+      walk(std::integral_constant<int, kPlain>());
+  } else {
+    if (begins || n % 4 != 0)
+      walk(std::integral_constant<int, kAny>());
+    else
+      walk(std::integral_constant<int, kLanes>());
+  }
 }
 
 // Four states' rates; those past n decay, so that an infinite delta leaves them at zero.
@@ -33,7 +39,14 @@ __device__ __forceinline__ f32x4 rates_of(const Scan& s, int64_t c, int n0, int 
 // and walk token by token; delta, x, write and read come through LDS, a tile of 16 tokens at a
 // time, computed once each and fetched a tile ahead. kOut: outputs, from the states before the
 // part; otherwise the part's own state alone, from zeros, for rows walked in parts.
-template <class T, int LPC, bool kOut>
+//
+// Bound by its vector instructions (97 % of the time at 4,096 x 128 tokens of 128 channels, float32): 26 a
+// token for 16 channels of 16 states, two of them for each exponential, and as much again a token for what a
+// tile's elements take (softplus, the gate, addresses). 375 us there, 2.5 TB/s; 16,381 tokens of 512 channels
+// in parts 36 + 15 + 51 us. Tiles of eight tokens took 442, of one row in fewer parts (eight waves a CU
+// instead of 16) 41 + 9 + 64. Loads that a branch or a conversion separates wait for each other: 73 us for the
+// 51 before they went.
+template <class T, int LPC, bool kFull, bool kOut>
 __global__ __launch_bounds__(Shape<LPC>::kThreads) void forward_kernel(Scan s) {
   using S = Shape<LPC>;
   using At = Slots<LPC>;
@@ -94,7 +107,7 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void forward_kernel(Scan s) {
         f32x2 st = steps[tok][ch];
         const f32x4 w = *(const f32x4*)&mix[tok][n0];
         if (kKind == kLanes) st.y = left > 0 ? st.y : 0.0f;
-        if (kKind == kAny && (begins >> tok & 1)) h = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (kKind >= kBegins && (begins >> tok & 1)) h = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         float y = 0.0f;
         f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
         if (kOut) r = *(const f32x4*)&mix[tok][S::NP + n0];
@@ -110,7 +123,7 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void forward_kernel(Scan s) {
           span += st.x;
       }
     };
-    for_kind(begins, s.n, S::NP, walk);
+    for_kind<kFull>(begins, s.n, walk);
     __syncthreads();
     if (kOut) {
 #pragma unroll
@@ -254,11 +267,16 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void passed_kernel(Scan s) {
 //
 // Sums over a channel's states stay within its lanes; sums over channels go lane by lane within the
 // wave, then through LDS, then (dmix) over the blocks of a group.
-template <class T, int LPC>
+//
+// Bound by instruction issue at the two waves a SIMD that 128 registers of decays and states leave (some
+// instruction issues 88 % of the time, a vector one 69 %): 1,300 us for 4,096 x 128 tokens of 128 channels,
+// float32, of which the sums over channels take 190, the exponentials 155 and the outputs 165. Three waves with
+// the decays computed again instead of held: 1,340; tiles of eight tokens, three waves: 1,620.
+template <class T, int LPC, bool kFull>
 __global__ __launch_bounds__(Shape<LPC>::kThreads, 2) void backward_kernel(Scan s) {
   using S = Shape<LPC>;
   using At = Slots<LPC>;
-  // delta, delta x, dy; then delta, sum g write, sum g rate a h_{t-1}, sum read h
+  // delta, delta x, dy; then delta, sum g write, sum g rate a h_{t-1} / ln 2, sum read h
   __shared__ __attribute__((aligned(16))) f32x4 steps[kTile][S::CH];
   // of each slot, for its outputs: x, dy, the slope of softplus, dout times that of the gate's silu
   __shared__ __attribute__((aligned(16))) f32x4 held[4][kTile * S::CH / 4];
@@ -271,8 +289,7 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads, 2) void backward_kernel(Scan 
   const int64_t c = (int64_t)at.group * s.dg + at.first + ch;
   const int64_t start = at.p * s.part, end = start + s.part < s.t ? start + s.part : s.t;
   const int left = live ? s.n - n0 : 0;
-  const f32x4 rate = rates_of(s, c, n0, left);
-  const f32x4 rate2 = rate * kLog2e;
+  const f32x4 rate = rates_of(s, c, n0, left) * kLog2e;
   f32x4 g = {0.0f, 0.0f, 0.0f, 0.0f}, drate = g;
   if (s.parts > 1)
     g = load_upto(s.carry + ((at.b * s.parts + at.p) * s.d + c) * s.n + n0, left);
@@ -345,11 +362,11 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads, 2) void backward_kernel(Scan 
       for (int tok = 0; tok < kTile; ++tok) {
         f32x2 st = *(const f32x2*)&steps[tok][ch];
         const f32x4 w = *(const f32x4*)&mix[tok][n0];
-        const bool begins = kKind == kAny && (begun >> tok & 1);
+        const bool begins = kKind >= kBegins && (begun >> tok & 1);
         if (kKind == kLanes) st.y = left > 0 ? st.y : 0.0f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          a[tok][e] = exp2_of(st.x * rate2[e]);
+          a[tok][e] = exp2_of(st.x * rate[e]);
           kept[tok][e] = begins ? 0.0f : a[tok][e] * h[e];
           h[e] = __builtin_fmaf(st.y, w[e], kept[tok][e]);
           if (kKind == kAny) h[e] = e < left ? h[e] : 0.0f;
@@ -361,7 +378,7 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads, 2) void backward_kernel(Scan 
         f32x4 st = steps[tok][ch];
         const f32x4 w = *(const f32x4*)&mix[tok][n0], r = *(const f32x4*)&mix[tok][S::NP + n0];
         float y = 0.0f, into = 0.0f, dd = 0.0f, v[8];
-        const bool begins = kKind == kAny && (begun >> tok & 1);
+        const bool begins = kKind >= kBegins && (begun >> tok & 1);
         if (kKind == kLanes) st.y = left > 0 ? st.y : 0.0f, st.z = left > 0 ? st.z : 0.0f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -392,7 +409,7 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads, 2) void backward_kernel(Scan 
         if (tok % 4 == 0) __builtin_amdgcn_sched_barrier(0);
       }
     };
-    for_kind(begun, s.n, S::NP, walk);
+    for_kind<kFull>(begun, s.n, walk);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < S::kSlots; ++i) {
@@ -408,7 +425,7 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads, 2) void backward_kernel(Scan 
           dx[e] = __builtin_fmaf(skip[e], dy[e], dx[e]);
           dgate[e] = __builtin_fmaf(skip[e], x[e], dgate[e]);
         }
-        ddt[e] = __builtin_fmaf(st.y, x[e], st.z) * slope[e];
+        ddt[e] = __builtin_fmaf(st.z, kLn2, st.y * x[e]) * slope[e];
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) dskip[e] = __builtin_fmaf(dy[e], x[e], dskip[e]);
@@ -478,7 +495,7 @@ __global__ __launch_bounds__(kBlock) void mix_sums_kernel(Scan s) {
 
 // One token of every environment: LPC lanes a channel, each with four states, which are read once and
 // written once, bound by that. A thread takes its channel of kEnvs environments, so that as many states are
-// in flight. next may be state itself: a thread writes only what it has read.
+// in flight: 4,096 x 512 x 16 states in 70 us, 4.1 TB/s, where one a thread takes 79. next may be state itself: a thread writes only what it has read.
 struct Step {
   const void *x, *dt, *gate, *write, *read;
   int64_t x_s, dt_s, gate_s, write_s, write_sg, read_s, read_sg, reset_s;
@@ -618,6 +635,14 @@ int for_lanes(int lpc, const F& f) {
   }
 }
 
+// f(lanes of a channel, whether n is all of their states)
+template <class F>
+int for_states(int n, const F& f) {
+  return for_lanes(lanes_of(n), [&](auto lanes) {
+    return n == 4 * decltype(lanes)::value ? f(lanes, std::true_type()) : f(lanes, std::false_type());
+  });
+}
+
 template <bool kBack>
 int join(const Scan& s, hipStream_t stream) {
   Scan one = s;
@@ -633,25 +658,27 @@ int join(const Scan& s, hipStream_t stream) {
 
 template <class T>
 int forward(const Scan& s, hipStream_t stream) {
-  return for_lanes(lanes_of(s.n), [&](auto lanes) {
+  return for_states(s.n, [&](auto lanes, auto full) {
     constexpr int LPC = decltype(lanes)::value, kThreads = Shape<LPC>::kThreads;
+    constexpr bool kFull = decltype(full)::value;
     if (s.parts > 1) {
       int status = in_launches(s, blocks_of(s, s.parts - 1), kThreads, [&](const Scan& a, dim3 grid) {
-        hipLaunchKernelGGL((forward_kernel<T, LPC, false>), grid, dim3(kThreads), 0, stream, a);
+        hipLaunchKernelGGL((forward_kernel<T, LPC, kFull, false>), grid, dim3(kThreads), 0, stream, a);
       });
       if (status == HIPENVS_OK) status = join<false>(s, stream);
       if (status != HIPENVS_OK) return status;
     }
     return in_launches(s, blocks_of(s, s.parts), kThreads, [&](const Scan& a, dim3 grid) {
-      hipLaunchKernelGGL((forward_kernel<T, LPC, true>), grid, dim3(kThreads), 0, stream, a);
+      hipLaunchKernelGGL((forward_kernel<T, LPC, kFull, true>), grid, dim3(kThreads), 0, stream, a);
     });
   });
 }
 
 template <class T>
 int backward(const Scan& s, hipStream_t stream) {
-  const int walked = for_lanes(lanes_of(s.n), [&](auto lanes) {
+  const int walked = for_states(s.n, [&](auto lanes, auto full) {
     constexpr int LPC = decltype(lanes)::value, kThreads = Shape<LPC>::kThreads;
+    constexpr bool kFull = decltype(full)::value;
     if (s.parts > 1) {
       int status = in_launches(s, blocks_of(s, s.parts - 1), kThreads, [&](const Scan& a, dim3 grid) {
         hipLaunchKernelGGL((passed_kernel<T, LPC>), grid, dim3(kThreads), 0, stream, a);
@@ -660,7 +687,7 @@ int backward(const Scan& s, hipStream_t stream) {
       if (status != HIPENVS_OK) return status;
     }
     return in_launches(s, blocks_of(s, s.parts), kThreads, [&](const Scan& a, dim3 grid) {
-      hipLaunchKernelGGL((backward_kernel<T, LPC>), grid, dim3(kThreads), 0, stream, a);
+      hipLaunchKernelGGL((backward_kernel<T, LPC, kFull>), grid, dim3(kThreads), 0, stream, a);
     });
   });
   if (walked != HIPENVS_OK || s.tiles <= 1 || s.t == 0) return walked;
