@@ -87,39 +87,90 @@ struct Slots {
 
 // The same number, about which the compiler knows nothing: addresses that it works out once for all of a
 // loop's rounds would take the registers of the states.
+__device__ __forceinline__ int32_t anew(int32_t x) {
+  asm volatile("" : "+s"(x));
+  return x;
+}
+
 __device__ __forceinline__ int64_t anew(int64_t x) {
-  uint32_t lo = (uint32_t)x, hi = (uint32_t)((uint64_t)x >> 32);
-  asm volatile("" : "+s"(lo), "+s"(hi));
+  const uint32_t lo = (uint32_t)anew((int32_t)x), hi = (uint32_t)anew((int32_t)(x >> 32));
   return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
-template <class T>
-__device__ __forceinline__ const T* row_at(const T* base, int token, int64_t stride) {
-  return (const T*)((const char*)base + (int64_t)(token * (int)sizeof(T)) * (int64_t)(int32_t)stride);
+// A use of a loaded value: the wait for it comes here, and not behind the stores that follow, which a later
+// one would wait for as well.
+template <class V>
+__device__ __forceinline__ void settle(V& x) {
+  static_assert(sizeof(V) == 8 || sizeof(V) == 16, "four values");
+  typedef uint32_t bits __attribute__((ext_vector_type(sizeof(V) / 4)));
+  bits held = __builtin_bit_cast(bits, x);
+  asm volatile("" : "+v"(held));
+  x = __builtin_bit_cast(V, held);
 }
 
-template <class T, int LPC, bool kOut, bool kBack>
+template <class T>
+__device__ __forceinline__ const T* row_at(const T* base, int token, int32_t stride) {
+  return (const T*)((const char*)base + (int64_t)(token * (int)sizeof(T)) * (int64_t)stride);
+}
+
+// Where a tile's first token lies, and how far apart tokens are.
+template <class T>
+struct Source {
+  const T* at;
+  int32_t st;
+
+  __device__ __forceinline__ void set(const void* data, int64_t offset, int64_t t0, int64_t stride) {
+    at = (const T*)data + offset + t0 * stride;
+    st = (int32_t)stride;
+  }
+  __device__ __forceinline__ void move(int tokens) { at = row_at(at, tokens, st); }
+};
+
+// A block's sources, a tile after another. Without a gate its place is x, read again and not used: a
+// branch would keep the loads behind it from being in flight with those before.
+template <class T, bool kGate, bool kBack>
+struct Sources {
+  Source<T> x, dt, gate, dout, write, read;
+  Source<uint8_t> reset;
+
+  __device__ __forceinline__ Sources(const Scan& s, const Place& at, int64_t t0) {
+    const int64_t col = (int64_t)at.group * s.dg;
+    x.set(s.x.data, at.b * s.x.sb + col, t0, s.x.st);
+    dt.set(s.dt.data, at.b * s.dt.sb + col, t0, s.dt.st);
+    const Rows& z = s.gate.data ? s.gate : s.x;
+    if (kGate) gate.set(z.data, at.b * z.sb + col, t0, z.st);
+    if (kBack) dout.set(s.dout.data, at.b * s.dout.sb + col, t0, s.dout.st);
+    write.set(s.write.data, at.b * s.write.sb + at.group * s.write.sg, t0, s.write.st);
+    read.set(s.read.data, at.b * s.read.sb + at.group * s.read.sg, t0, s.read.st);
+    reset.at = nullptr, reset.st = 0;
+    if (s.reset) reset.set(s.reset, at.b * s.reset_sb, t0, s.reset_st);
+  }
+
+  __device__ __forceinline__ void move(int tokens) {
+    x.move(tokens), dt.move(tokens), write.move(tokens), read.move(tokens);
+    if (kGate) gate.move(tokens);
+    if (kBack) dout.move(tokens);
+    reset.move(tokens);
+  }
+};
+
+template <class T, int LPC, bool kGate, bool kBack>
 struct Fetched {
   using S = Shape<LPC>;
   using At = Slots<LPC>;
   typename Raw<T>::type x[S::kSlots], dt[S::kSlots], gate[S::kSlots], dout[S::kSlots], mix[S::kMixSlots];
   uint8_t begins;   // of the token of this lane
 
-  // kWhole: four channels and four states at least, and a tile that ends before `end`; otherwise tokens
-  // past the end are the last one again
+  // kWhole: four channels and four states at least, and `count`, the tokens from the tile's first on, a whole
+  // tile; otherwise tokens past the end are the last one again
   template <bool kWhole>
-  __device__ __forceinline__ void load(const Scan& s, const Place& at, int64_t t0, int64_t end) {
-    const int last = kWhole ? kTile - 1 : (int)(end - 1 - t0 < kTile - 1 ? end - 1 - t0 : kTile - 1);
-    const int64_t col = (int64_t)at.group * s.dg;
-    const T* x0 = (const T*)s.x.data + at.b * s.x.sb + t0 * s.x.st + col;
-    const T* dt0 = (const T*)s.dt.data + at.b * s.dt.sb + t0 * s.dt.st + col;
-    const T* gate0 = (const T*)s.gate.data + at.b * s.gate.sb + t0 * s.gate.st + col;
-    const T* dout0 = (const T*)s.dout.data + at.b * s.dout.sb + t0 * s.dout.st + col;
-    int c = at.first + At::channel();
+  __device__ __forceinline__ void load(const Scan& s, const Sources<T, kGate, kBack>& of, int first, int64_t count) {
+    const int last = kWhole || count > kTile ? kTile - 1 : (int)count - 1;
+    int c = first + At::channel();
     c = c < s.dg ? c : 0;
     if (kWhole) c = c < s.dg - 4 ? c : s.dg - 4;
-    const auto four = [&](const T* base, int token, int64_t stride) {
-      const T* row = row_at(base, token < last ? token : last, stride);
+    const auto four = [&](const Source<T>& source, int token) {
+      const T* row = row_at(source.at, token < last ? token : last, anew(source.st));
       if constexpr (kWhole)
         return *(const typename Raw<T>::any*)(row + c);
       else
@@ -127,16 +178,14 @@ struct Fetched {
     };
 #pragma unroll
     for (int i = 0; i < S::kSlots; ++i) {
-      x[i] = four(x0, At::token(i), s.x.st);
-      dt[i] = four(dt0, At::token(i), s.dt.st);
-      if ((kOut || kBack) && s.gate.data) gate[i] = four(gate0, At::token(i), s.gate.st);
-      if (kBack) dout[i] = four(dout0, At::token(i), s.dout.st);
+      x[i] = four(of.x, At::token(i));
+      dt[i] = four(of.dt, At::token(i));
+      if (kGate) gate[i] = four(of.gate, At::token(i));
+      if (kBack) dout[i] = four(of.dout, At::token(i));
     }
     const bool writes = At::mix_part() < LPC;
-    const T* write0 = (const T*)s.write.data + at.b * s.write.sb + t0 * s.write.st + at.group * s.write.sg;
-    const T* read0 = (const T*)s.read.data + at.b * s.read.sb + t0 * s.read.st + at.group * s.read.sg;
-    const T* mix0 = writes ? write0 : read0;
-    const int32_t mix_st = writes ? (int32_t)s.write.st : (int32_t)s.read.st;
+    const T* mix0 = writes ? of.write.at : of.read.at;
+    const int32_t mix_st = writes ? anew(of.write.st) : anew(of.read.st);
     int n0 = At::mix_state();
     n0 = n0 < s.n ? n0 : 0;
     if (kWhole) n0 = n0 < s.n - 4 ? n0 : s.n - 4;
@@ -149,17 +198,31 @@ struct Fetched {
         mix[i] = fetch4(row, n0, s.n);
     }
     begins = 0;
-    if (s.reset) {
+    if (of.reset.at) {
       const int tok = threadIdx.x & 63;
-      begins = *row_at(s.reset + at.b * s.reset_sb + t0 * s.reset_st, tok < last ? tok : last, s.reset_st);
+      begins = *row_at(of.reset.at, tok < last ? tok : last, anew(of.reset.st));
     }
   }
 
-  __device__ __forceinline__ void fetch(const Scan& s, const Place& at, int64_t t0, int64_t end) {
-    if (t0 + kTile <= end && s.dg >= 4 && s.n >= 4)
-      load<true>(s, at, t0, end);
+  __device__ __forceinline__ void fetch(const Scan& s, const Sources<T, kGate, kBack>& of, int first, int64_t count) {
+    if (count >= kTile && s.dg >= 4 && s.n >= 4)
+      load<true>(s, of, first, count);
     else
-      load<false>(s, at, t0, end);
+      load<false>(s, of, first, count);
+  }
+
+  __device__ __forceinline__ void arrive() {
+#pragma unroll
+    for (int i = 0; i < S::kSlots; ++i) {
+      settle(x[i]), settle(dt[i]);
+      if (kGate) settle(gate[i]);
+      if (kBack) settle(dout[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < S::kMixSlots; ++i) settle(mix[i]);
+    uint32_t held = begins;
+    asm volatile("" : "+v"(held));
+    begins = (uint8_t)held;
   }
 
   // a bit for each token of the tile that begins an episode

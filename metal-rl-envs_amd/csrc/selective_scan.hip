@@ -73,8 +73,9 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void forward_kernel(Scan s) {
   const int64_t checks = (s.t + kTile - 1) / kTile;
   float span = 0.0f;
   uint32_t begun = 0;
+  Sources<T, kOut, false> of(s, at, start);
   Fetched<T, LPC, kOut, false> next;
-  if (start < end) next.fetch(s, at, start, end);
+  if (start < end) next.fetch(s, of, at.first, end - start);
   for (int64_t tile = start; tile < end; tile += kTile) {
     const int64_t t0 = anew(tile);
     const Fetched<T, LPC, kOut, false> now = next;
@@ -96,7 +97,10 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void forward_kernel(Scan s) {
     }
     now.put_mix(s, t0, end, mix);
     __syncthreads();
-    if (t0 + kTile < end) next.fetch(s, at, t0 + kTile, end);
+    if (t0 + kTile < end) {
+      of.move(kTile);
+      next.fetch(s, of, at.first, end - t0 - kTile);
+    }
     if (kOut && s.checks)
       store_upto(s.checks + ((at.b * checks + t0 / kTile) * s.d + c) * s.n + n0, h, left);
     begun |= begins;
@@ -126,6 +130,7 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void forward_kernel(Scan s) {
     for_kind<kFull>(begins, s.n, walk);
     __syncthreads();
     if (kOut) {
+      next.arrive();
 #pragma unroll
       for (int i = 0; i < S::kSlots; ++i) {
         const int tok = At::token(i);
@@ -139,7 +144,7 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void forward_kernel(Scan s) {
           if (s.gate.data) o[e] *= z[e] * sigmoid_for<T>(z[e]);
         }
         T* out = (T*)s.out + (at.b * s.t + t0) * s.d + (int64_t)at.group * s.dg + at.first;
-        store_upto((T*)row_at(out, tok, s.d) + k, o, s.dg - at.first - k);
+        store_upto(const_cast<T*>(row_at(out, tok, anew(s.d))) + k, o, s.dg - at.first - k);
       }
       __syncthreads();
     }
@@ -212,9 +217,10 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void passed_kernel(Scan s) {
   const f32x4 bias = per_channel(s.bias, (int64_t)at.group * s.dg + own, s.dg - own, 0.0f);
   float span = 0.0f;
   uint32_t begun = 0;
-  Fetched<T, LPC, true, true> next;
   int64_t t0 = start + (end - start - 1) / kTile * kTile;
-  next.fetch(s, at, t0, end);
+  Sources<T, true, true> of(s, at, t0);
+  Fetched<T, LPC, true, true> next;
+  next.fetch(s, of, at.first, end - t0);
   for (int64_t tile = t0; tile >= start; tile -= kTile) {
     const int64_t t0 = anew(tile);
     const Fetched<T, LPC, true, true> now = next;
@@ -239,7 +245,10 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void passed_kernel(Scan s) {
     }
     now.put_mix(s, t0, end, mix);
     __syncthreads();
-    if (t0 - kTile >= start) next.fetch(s, at, t0 - kTile, end);
+    if (t0 - kTile >= start) {
+      of.move(-kTile);
+      next.fetch(s, of, at.first, end - t0 + kTile);
+    }
     begun |= begins;
 #pragma unroll
     for (int tok = kTile - 1; tok >= 0; --tok) {
@@ -305,12 +314,17 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads, 2) void backward_kernel(Scan 
   grads[0][threadIdx.x] = grads[1][threadIdx.x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   __syncthreads();
   const int64_t checks = (s.t + kTile - 1) / kTile;
+  const int64_t t0 = end > start ? start + (end - start - 1) / kTile * kTile : start;
+  Sources<T, true, true> of(s, at, t0);
   Fetched<T, LPC, true, true> next;
-  int64_t t0 = start + (end - start - 1) / kTile * kTile;
+  // the states before each tile, of the last ones where there are none
+  const int c_in = at.first + ch < s.dg ? at.first + ch : 0, n_in = n0 < s.n ? n0 : 0;
+  const float* check = s.checks + ((at.b * checks + t0 / kTile) * s.d + (int64_t)at.group * s.dg) * s.n;
+  const auto fetch_check = [&]() { return fetch4(check + c_in * s.n, n_in, s.n); };
   f32x4 h_next = {0.0f, 0.0f, 0.0f, 0.0f};
   if (end > start) {
-    next.fetch(s, at, t0, end);
-    h_next = load_upto(s.checks + ((at.b * checks + t0 / kTile) * s.d + c) * s.n + n0, left);
+    next.fetch(s, of, at.first, end - t0);
+    h_next = fetch_check();
   }
   for (int64_t tile = t0; end > start && tile >= start; tile -= kTile) {
     const int64_t t0 = anew(tile);
@@ -349,11 +363,14 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads, 2) void backward_kernel(Scan 
       }
       now.put_mix(s, t0, end, mix);
     }
-    f32x4 h = h_next;
+    f32x4 h = values<float>(h_next, n_in, s.n);
+    if (left <= 0) h = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     __syncthreads();
     if (t0 - kTile >= start) {
-      next.fetch(s, at, t0 - kTile, end);
-      h_next = load_upto(s.checks + ((at.b * checks + t0 / kTile - 1) * s.d + c) * s.n + n0, left);
+      of.move(-kTile);
+      check -= (int64_t)s.d * s.n;
+      next.fetch(s, of, at.first, end - t0 + kTile);
+      h_next = fetch_check();
     }
     const auto walk = [&](auto kind) {
       constexpr int kKind = decltype(kind)::value;
@@ -411,6 +428,8 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads, 2) void backward_kernel(Scan 
     };
     for_kind<kFull>(begun, s.n, walk);
     __syncthreads();
+    next.arrive();
+    settle(h_next);
 #pragma unroll
     for (int i = 0; i < S::kSlots; ++i) {
       const int tok = At::token(i), slot = tok * (S::CH / 4) + k / 4;
@@ -434,11 +453,12 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads, 2) void backward_kernel(Scan 
       const int64_t col = (int64_t)at.group * s.dg + at.first;
       const int64_t row = (at.b * s.t + t0) * s.d + col;
       const int own_left = s.dg - at.first - k;
-      store_upto((T*)row_at((T*)s.dx + row, tok, s.d) + k, dx, own_left);
-      store_upto((T*)row_at((T*)s.ddt + row, tok, s.d) + k, ddt, own_left);
+      const int64_t to = (int64_t)tok * anew(s.d) + row + k;
+      store_upto((T*)s.dx + to, dx, own_left);
+      store_upto((T*)s.ddt + to, ddt, own_left);
       if (s.gate.data) {
         const f32x4 of_gate = held[3][slot];
-        store_upto((T*)row_at((T*)s.dgate + row, tok, s.d) + k, dgate * of_gate, own_left);
+        store_upto((T*)s.dgate + to, dgate * of_gate, own_left);
       }
     }
 #pragma unroll
@@ -451,10 +471,10 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads, 2) void backward_kernel(Scan 
       const int64_t row = (at.b * s.t + t0) * s.g + at.group;
       if (s.tiles > 1) {
         float* to = s.dmix + ((int64_t)(at.first / S::CH) * (s.b * s.t * s.g) + row) * (2 * S::NP);
-        *(f32x4*)(row_at(to, tok, (int64_t)s.g * (2 * S::NP)) + part * 4) = sum;
+        *(f32x4*)(to + (int64_t)tok * anew(s.g * (2 * S::NP)) + part * 4) = sum;
       } else {
         T* to = (T*)(part < LPC ? s.dwrite : s.dread) + row * s.n;
-        store_upto((T*)row_at(to, tok, (int64_t)s.g * s.n) + n, sum, s.n - n);
+        store_upto(to + (int64_t)tok * anew(s.g * s.n) + n, sum, s.n - n);
       }
     }
     __syncthreads();
