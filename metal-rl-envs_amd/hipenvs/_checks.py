@@ -26,6 +26,9 @@ def first(x, name, axes):
 
 def rows(x, name, dtype, shape, device, first="x"):
     """A tensor of that type, shape and GPU; copied where its last axis is not contiguous."""
+    if (isinstance(x, torch.Tensor) and x.dtype is dtype and x.shape == shape and x.get_device() == device
+            and x.stride(-1) == 1):
+        return x
     if tensor(x, name).dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {x.dtype}")
     if x.shape != shape:
@@ -37,8 +40,9 @@ def rows(x, name, dtype, shape, device, first="x"):
 
 def f32(x, name, shape, device, first="x"):
     """A float32 tensor of that shape and GPU; copied where it is not contiguous. None stays None."""
-    if x is None:
-        return None
+    if x is None or (isinstance(x, torch.Tensor) and x.dtype is torch.float32 and x.shape == shape
+                     and x.get_device() == device and x.is_contiguous()):
+        return x
     return rows(x, name, torch.float32, shape, device, first).contiguous()
 
 

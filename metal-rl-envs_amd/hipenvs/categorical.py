@@ -31,9 +31,9 @@ def _forward(logits, tokens, top, train):
         if nbytes < 0:
             raise _lib.HipEnvsError(f"hipenvs_log_probs: unsupported sizes ({rows}, {v}, {top})")
         held = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-        _lib.call("hipenvs_log_probs", _checks.DTYPES[logits.dtype], ptr(logits), logits.stride(0), ptr(tokens),
-                  ptr(log_prob), ptr(entropy), ptr(stats), top, ptr(top_log_prob), ptr(top_index), rows, v, ptr(held),
-                  nbytes, _lib.stream_of(device))
+        _lib.call("hipenvs_log_probs", _checks.DTYPES[logits.dtype], logits.data_ptr(), logits.stride(0),
+                  tokens.data_ptr(), log_prob.data_ptr(), entropy.data_ptr(), ptr(stats), top, ptr(top_log_prob),
+                  ptr(top_index), rows, v, ptr(held), nbytes, _lib.stream_of(device))
     return log_prob, entropy, top_log_prob, top_index, stats
 
 
@@ -51,9 +51,9 @@ def _backward(ctx, dlog_prob, dentropy, *_):
     ptr = _lib.ptr
     dlogits = torch.empty((rows, v), dtype=dtype, device=logits.device)
     with _lib.on(logits.device):
-        _lib.call("hipenvs_log_probs_backward", _checks.DTYPES[dtype], ptr(logits), logits.stride(0), ptr(tokens),
-                  ptr(stats), ptr(entropy), ptr(dlog_prob), ptr(dentropy), ptr(dlogits), rows, v,
-                  _lib.stream_of(logits.device))
+        _lib.call("hipenvs_log_probs_backward", _checks.DTYPES[dtype], logits.data_ptr(), logits.stride(0),
+                  tokens.data_ptr(), ptr(stats), entropy.data_ptr(), ptr(dlog_prob), ptr(dentropy), dlogits.data_ptr(),
+                  rows, v, _lib.stream_of(logits.device))
     return dlogits, None, None
 
 

@@ -57,8 +57,9 @@ def _forward(x, weight, bias, state, reset, silu):
     out = torch.empty((b, t, d), dtype=x.dtype, device=x.device)
     final = torch.empty((b, w - 1, d), dtype=torch.float32, device=x.device)
     with _lib.on(x.device):
-        _lib.call("hipenvs_causal_conv", _checks.DTYPES[x.dtype], ptr(x), ptr(weight), ptr(bias), ptr(state), ptr(reset),
-                  _strides(x, reset), silu, ptr(out), ptr(final), b, t, d, w, _lib.stream_of(x.device))
+        _lib.call("hipenvs_causal_conv", _checks.DTYPES[x.dtype], x.data_ptr(), weight.data_ptr(), ptr(bias),
+                  ptr(state), ptr(reset), _strides(x, reset), silu, out.data_ptr(), final.data_ptr(), b, t, d, w,
+                  _lib.stream_of(x.device))
     return out, final
 
 
@@ -87,9 +88,9 @@ def _backward(ctx, dout, dfinal):
         if nbytes < 0:
             raise _lib.HipEnvsError(f"hipenvs_causal_conv: unsupported sequence ({b}, {t}, {d}, {w})")
         held = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-        _lib.call("hipenvs_causal_conv_backward", _checks.DTYPES[dtype], ptr(x), ptr(weight), ptr(bias), ptr(state),
-                  ptr(reset), ptr(dout), ptr(dfinal), _strides(x, reset, dout), silu, ptr(dx), ptr(dparams), ptr(dstate),
-                  b, t, d, w, ptr(held), nbytes, _lib.stream_of(device))
+        _lib.call("hipenvs_causal_conv_backward", _checks.DTYPES[dtype], x.data_ptr(), weight.data_ptr(), ptr(bias),
+                  ptr(state), ptr(reset), dout.data_ptr(), ptr(dfinal), _strides(x, reset, dout), silu, dx.data_ptr(),
+                  dparams.data_ptr(), dstate.data_ptr(), b, t, d, w, ptr(held), nbytes, _lib.stream_of(device))
     dweight, dbias = torch.split(dparams, (d * w, d))
     return (dx, dweight.view(d, w), dbias if bias is not None else None, dstate if state is not None else None, None,
             None)
@@ -138,7 +139,7 @@ def step(x, weight, bias=None, state=None, reset=None, silu=True, next_state=Non
         _checks.target(next_state, "next_state", (n, w - 1, d), device)
     out = torch.empty((n, d), dtype=x.dtype, device=on)
     with _lib.on(on):
-        _lib.call("hipenvs_causal_conv_step", _checks.DTYPES[x.dtype], ptr(x), x.stride(0), ptr(weight), ptr(bias),
-                  ptr(state), ptr(reset), reset.stride(0) if reset is not None else 0, bool(silu), ptr(out),
-                  ptr(next_state), n, d, w, _lib.stream_of(on))
+        _lib.call("hipenvs_causal_conv_step", _checks.DTYPES[x.dtype], x.data_ptr(), x.stride(0), weight.data_ptr(),
+                  ptr(bias), ptr(state), ptr(reset), reset.stride(0) if reset is not None else 0, bool(silu),
+                  out.data_ptr(), next_state.data_ptr(), n, d, w, _lib.stream_of(on))
     return out, next_state

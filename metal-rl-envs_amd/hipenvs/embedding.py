@@ -20,8 +20,8 @@ def _forward(tokens, table, scale):
     v, d = table.shape
     out = torch.empty((*tokens.shape, d), dtype=table.dtype, device=table.device)
     with _lib.on(table.device):
-        _lib.call("hipenvs_embedding", _checks.DTYPES[table.dtype], _lib.ptr(tokens), tokens.element_size(),
-                  _lib.ptr(table), table.stride(0), scale, _lib.ptr(out), tokens.numel(), v, d,
+        _lib.call("hipenvs_embedding", _checks.DTYPES[table.dtype], tokens.data_ptr(), tokens.element_size(),
+                  table.data_ptr(), table.stride(0), scale, out.data_ptr(), tokens.numel(), v, d,
                   _lib.stream_of(table.device))
     return out
 
@@ -40,9 +40,9 @@ def _backward(ctx, dout):
         if nbytes < 0:
             raise _lib.HipEnvsError(f"hipenvs_embedding: unsupported sizes ({tokens.numel()}, {v}, {d})")
         held = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-        _lib.call("hipenvs_embedding_backward", _checks.DTYPES[dtype], _lib.ptr(tokens), tokens.element_size(),
-                  _lib.ptr(dout), dout.stride(0), scale, _lib.ptr(dtable), tokens.numel(), v, d, _lib.ptr(held), nbytes,
-                  _lib.stream_of(device))
+        _lib.call("hipenvs_embedding_backward", _checks.DTYPES[dtype], tokens.data_ptr(), tokens.element_size(),
+                  dout.data_ptr(), dout.stride(0), scale, dtable.data_ptr(), tokens.numel(), v, d, _lib.ptr(held),
+                  nbytes, _lib.stream_of(device))
     return None, dtable, None
 
 

@@ -24,7 +24,8 @@ from dataclasses import dataclass
 
 import torch
 
-from . import _lib, acrobot, adamw, adapter, cartpole, categorical, causal_conv, decay_attention, embedding, selective_scan
+from . import _lib, acrobot, adamw, adapter, cartpole
+from . import categorical, causal_conv, decay_attention, embedding, selective_scan
 
 # body, the rows of its state that the policy sees, actions. The angles and positions alone:
 # velocities have to be inferred from the steps before.
@@ -203,8 +204,8 @@ class Learner:
         self.env = adapter.DeviceEnv(body, cfg.envs, seed=cfg.seed + 1, device=device)
         self.generator = torch.Generator(device=device)
         self.generator.manual_seed(cfg.seed)
-        self.policy = Policy(len(seen), actions, cfg.width, cfg.heads, cfg.layers, self.generator, cfg.memory, cfg.states,
-                             cfg.previous_action)
+        self.policy = Policy(len(seen), actions, cfg.width, cfg.heads, cfg.layers, self.generator, cfg.memory,
+                             cfg.states, cfg.previous_action)
         self.optimizer = adamw.AdamW(self.policy.parameters(), lr=cfg.lr, weight_decay=cfg.weight_decay, bits=cfg.bits)
         self.memory = self.policy.initial_state(cfg.envs)
         self.begins = torch.ones(cfg.envs, dtype=torch.bool, device=device)
@@ -297,8 +298,8 @@ def main(argv=None):
     p.add_argument("--entropy", type=float, default=0.0)
     a = p.parse_args(argv)
     cfg = Config(task=a.task, envs=a.envs, horizon=a.horizon, width=a.width, heads=a.heads, layers=a.layers, lr=a.lr,
-                 bits=a.bits, seed=a.seed, memory=a.memory, states=a.states, previous_action=a.previous_action, clip=a.clip,
-                 epochs=a.epochs, entropy=a.entropy)
+                 bits=a.bits, seed=a.seed, memory=a.memory, states=a.states, previous_action=a.previous_action,
+                 clip=a.clip, epochs=a.epochs, entropy=a.entropy)
     return train(cfg, a.updates, lambda i, lasted: print(f"update {i:4d}  steps an episode {lasted:7.1f}", flush=True))
 
 

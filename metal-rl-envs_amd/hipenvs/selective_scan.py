@@ -106,9 +106,10 @@ def _forward(x, dt, rate, write, read, skip, gate, dt_bias, state, reset, train)
     with _lib.on(x.device):
         at, nbytes, held = _workspace(0, b, t, d, n, g, x.device)
         checks = _workspace(1, b, t, d, n, g, x.device)[2] if train else None
-        _lib.call("hipenvs_selective_scan", _checks.DTYPES[x.dtype], ptr(x), ptr(dt), ptr(rate), ptr(write), ptr(read),
-                  ptr(skip), ptr(gate), ptr(dt_bias), ptr(state), ptr(reset), _strides(x, dt, write, read, gate, reset),
-                  ptr(out), ptr(final), ptr(checks), b, t, d, n, g, at, nbytes, _lib.stream_of(x.device))
+        _lib.call("hipenvs_selective_scan", _checks.DTYPES[x.dtype], x.data_ptr(), dt.data_ptr(), rate.data_ptr(),
+                  write.data_ptr(), read.data_ptr(), ptr(skip), ptr(gate), ptr(dt_bias), ptr(state), ptr(reset),
+                  _strides(x, dt, write, read, gate, reset), out.data_ptr(), final.data_ptr(), ptr(checks), b, t, d, n,
+                  g, at, nbytes, _lib.stream_of(x.device))
     return out, final, checks
 
 
@@ -134,10 +135,11 @@ def _backward(ctx, dout, dfinal):
     dstate = torch.empty((b, d, n), dtype=torch.float32, device=device)
     with _lib.on(device):
         at, nbytes, held = _workspace(2, b, t, d, n, g, device)
-        _lib.call("hipenvs_selective_scan_backward", _checks.DTYPES[dtype], ptr(x), ptr(dt), ptr(rate), ptr(write),
-                  ptr(read), ptr(skip), ptr(gate), ptr(dt_bias), ptr(reset), ptr(dout), ptr(dfinal), ptr(checks),
-                  _strides(x, dt, write, read, gate, reset, dout), ptr(dx), ptr(ddt), ptr(dwrite), ptr(dread), ptr(dgate),
-                  ptr(dparams), ptr(dstate), b, t, d, n, g, at, nbytes, _lib.stream_of(device))
+        _lib.call("hipenvs_selective_scan_backward", _checks.DTYPES[dtype], x.data_ptr(), dt.data_ptr(),
+                  rate.data_ptr(), write.data_ptr(), read.data_ptr(), ptr(skip), ptr(gate), ptr(dt_bias), ptr(reset),
+                  dout.data_ptr(), ptr(dfinal), ptr(checks), _strides(x, dt, write, read, gate, reset, dout),
+                  dx.data_ptr(), ddt.data_ptr(), dwrite.data_ptr(), dread.data_ptr(), ptr(dgate), dparams.data_ptr(),
+                  dstate.data_ptr(), b, t, d, n, g, at, nbytes, _lib.stream_of(device))
     drate, dskip, dbias = torch.split(dparams, (d * n, d, d))
     return (dx, ddt, drate.view(d, n), dwrite, dread, dskip if skip is not None else None, dgate,
             dbias if dt_bias is not None else None, dstate if has_state else None, None)
@@ -196,7 +198,7 @@ def step(x, dt, rate, write, read, skip=None, gate=None, dt_bias=None, state=Non
     strides = _STRIDES[8](x.stride(0), dt.stride(0), gate.stride(0) if gate is not None else 0, *write.stride()[:2],
                           *read.stride()[:2], reset.stride(0) if reset is not None else 0)
     with _lib.on(on):
-        _lib.call("hipenvs_selective_scan_step", _checks.DTYPES[x.dtype], ptr(x), ptr(dt), ptr(rate), ptr(write),
-                  ptr(read), ptr(skip), ptr(gate), ptr(dt_bias), ptr(state), ptr(reset), strides, ptr(out),
-                  ptr(next_state), count, d, n, g, _lib.stream_of(on))
+        _lib.call("hipenvs_selective_scan_step", _checks.DTYPES[x.dtype], x.data_ptr(), dt.data_ptr(), rate.data_ptr(),
+                  write.data_ptr(), read.data_ptr(), ptr(skip), ptr(gate), ptr(dt_bias), ptr(state), ptr(reset),
+                  strides, out.data_ptr(), next_state.data_ptr(), count, d, n, g, _lib.stream_of(on))
     return out, next_state
