@@ -44,13 +44,17 @@ struct Scan {
   int64_t item0;
 };
 
-// LPC lanes a channel, four states each; the channels of a block.
-constexpr int channels_of(int lpc) { return lpc == 16 ? 32 : 64; }
+// LPC lanes a channel, four states each. A block has 64 channels (32 at 16 lanes) of one group, or where a
+// group has no more than 32, as few as fill its waves: lanes without a channel cost as much as others. 128
+// channels in four groups, 1,024 x 128 tokens, forwards and backwards: 714 us in blocks of 64, 511 so; in 128
+// groups 25,300 and 6,900.
+constexpr int channels_of(int lpc, bool few) { return few ? (lpc == 2 ? 32 : 16) : lpc == 16 ? 32 : 64; }
 inline int lanes_of(int n) { return n <= 8 ? 2 : n <= 16 ? 4 : n <= 32 ? 8 : 16; }
+inline bool few_channels(int dg) { return dg <= 32; }
 
-template <int LPC>
+template <int LPC, bool kFew>
 struct Shape {
-  static constexpr int CH = channels_of(LPC), kThreads = CH * LPC, kWaves = kThreads / 64, NP = 4 * LPC;
+  static constexpr int CH = channels_of(LPC, kFew), kThreads = CH * LPC, kWaves = kThreads / 64, NP = 4 * LPC;
   static constexpr int kSlots = (kTile * CH / 4 + kThreads - 1) / kThreads;   // four channels of a token each
   static constexpr int kMixSlots = (kTile * 2 * LPC + kThreads - 1) / kThreads;
 };
@@ -72,9 +76,9 @@ __device__ __forceinline__ Place place_of(const Scan& s, int64_t item, int parts
 // What a thread fetches of every tile: its slots of four channels of a token, and of four states of write or
 // read. Rows lie at a block's own address plus token times stride, one instruction: strides of t are
 // below 2^31. Channels and states past theirs read the last four, and whoever uses them leaves them out.
-template <int LPC>
+template <int LPC, bool kFew>
 struct Slots {
-  using S = Shape<LPC>;
+  using S = Shape<LPC, kFew>;
 
   static __device__ __forceinline__ int token(int i) {   // of slot i; kTile and more: none
     return (threadIdx.x + i * S::kThreads) / (S::CH / 4);
@@ -154,10 +158,10 @@ struct Sources {
   }
 };
 
-template <class T, int LPC, bool kGate, bool kBack>
+template <class T, int LPC, bool kFew, bool kGate, bool kBack>
 struct Fetched {
-  using S = Shape<LPC>;
-  using At = Slots<LPC>;
+  using S = Shape<LPC, kFew>;
+  using At = Slots<LPC, kFew>;
   typename Raw<T>::type x[S::kSlots], dt[S::kSlots], gate[S::kSlots], dout[S::kSlots], mix[S::kMixSlots];
   uint8_t begins;   // of the token of this lane
 

@@ -46,10 +46,10 @@ __device__ __forceinline__ f32x4 rates_of(const Scan& s, int64_t c, int n0, int 
 // in parts 36 + 15 + 51 us. Tiles of eight tokens took 442, of one row in fewer parts (eight waves a CU
 // instead of 16) 41 + 9 + 64. Loads that a branch or a conversion separates wait for each other: 73 us for the
 // 51 before they went.
-template <class T, int LPC, bool kFull, bool kOut>
-__global__ __launch_bounds__(Shape<LPC>::kThreads) void forward_kernel(Scan s) {
-  using S = Shape<LPC>;
-  using At = Slots<LPC>;
+template <class T, int LPC, bool kFew, bool kFull, bool kOut>
+__global__ __launch_bounds__((Shape<LPC, kFew>::kThreads)) void forward_kernel(Scan s) {
+  using S = Shape<LPC, kFew>;
+  using At = Slots<LPC, kFew>;
   __shared__ __attribute__((aligned(16))) f32x2 steps[kTile][S::CH];      // delta, delta x; then y
   __shared__ __attribute__((aligned(16))) float mix[kTile][2 * S::NP];
   const int parts = kOut ? s.parts : s.parts - 1;
@@ -74,11 +74,11 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void forward_kernel(Scan s) {
   float span = 0.0f;
   uint32_t begun = 0;
   Sources<T, kOut, false> of(s, at, start);
-  Fetched<T, LPC, kOut, false> next;
+  Fetched<T, LPC, kFew, kOut, false> next;
   if (start < end) next.fetch(s, of, at.first, end - start);
   for (int64_t tile = start; tile < end; tile += kTile) {
     const int64_t t0 = anew(tile);
-    const Fetched<T, LPC, kOut, false> now = next;
+    const Fetched<T, LPC, kFew, kOut, false> now = next;
     const uint32_t begins = now.begun(t0, end);
     const int k = At::channel();
     f32x4 x[S::kSlots];
@@ -198,10 +198,10 @@ __global__ __launch_bounds__(kBlock) void join_kernel(Scan s) {
 }
 
 // The gradient that a part passes to the states before it where none reaches it from behind.
-template <class T, int LPC>
-__global__ __launch_bounds__(Shape<LPC>::kThreads) void passed_kernel(Scan s) {
-  using S = Shape<LPC>;
-  using At = Slots<LPC>;
+template <class T, int LPC, bool kFew>
+__global__ __launch_bounds__((Shape<LPC, kFew>::kThreads)) void passed_kernel(Scan s) {
+  using S = Shape<LPC, kFew>;
+  using At = Slots<LPC, kFew>;
   __shared__ __attribute__((aligned(16))) f32x2 steps[kTile][S::CH];      // delta, dy
   __shared__ __attribute__((aligned(16))) float mix[kTile][2 * S::NP];
   Place at = place_of(s, s.item0 + blockIdx.x, s.parts - 1, S::CH);
@@ -219,11 +219,11 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void passed_kernel(Scan s) {
   uint32_t begun = 0;
   int64_t t0 = start + (end - start - 1) / kTile * kTile;
   Sources<T, true, true> of(s, at, t0);
-  Fetched<T, LPC, true, true> next;
+  Fetched<T, LPC, kFew, true, true> next;
   next.fetch(s, of, at.first, end - t0);
   for (int64_t tile = t0; tile >= start; tile -= kTile) {
     const int64_t t0 = anew(tile);
-    const Fetched<T, LPC, true, true> now = next;
+    const Fetched<T, LPC, kFew, true, true> now = next;
     const uint32_t begins = now.begun(t0, end);
     const int k = At::channel();
 #pragma unroll
@@ -281,10 +281,10 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads) void passed_kernel(Scan s) {
 // instruction issues 88 % of the time, a vector one 69 %): 1,300 us for 4,096 x 128 tokens of 128 channels,
 // float32, of which the sums over channels take 190, the exponentials 155 and the outputs 165. Three waves with
 // the decays computed again instead of held: 1,340; tiles of eight tokens, three waves: 1,620.
-template <class T, int LPC, bool kFull>
-__global__ __launch_bounds__(Shape<LPC>::kThreads, 2) void backward_kernel(Scan s) {
-  using S = Shape<LPC>;
-  using At = Slots<LPC>;
+template <class T, int LPC, bool kFew, bool kFull>
+__global__ __launch_bounds__((Shape<LPC, kFew>::kThreads), 2) void backward_kernel(Scan s) {
+  using S = Shape<LPC, kFew>;
+  using At = Slots<LPC, kFew>;
   // delta, delta x, dy; then delta, sum g write, sum g rate a h_{t-1} / ln 2, sum read h
   __shared__ __attribute__((aligned(16))) f32x4 steps[kTile][S::CH];
   // of each slot, for its outputs: x, dy, the slope of softplus, dout times that of the gate's silu
@@ -316,7 +316,7 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads, 2) void backward_kernel(Scan 
   const int64_t checks = (s.t + kTile - 1) / kTile;
   const int64_t t0 = end > start ? start + (end - start - 1) / kTile * kTile : start;
   Sources<T, true, true> of(s, at, t0);
-  Fetched<T, LPC, true, true> next;
+  Fetched<T, LPC, kFew, true, true> next;
   // the states before each tile, of the last ones where there are none
   const int c_in = at.first + ch < s.dg ? at.first + ch : 0, n_in = n0 < s.n ? n0 : 0;
   const float* check = s.checks + ((at.b * checks + t0 / kTile) * s.d + (int64_t)at.group * s.dg) * s.n;
@@ -331,7 +331,7 @@ __global__ __launch_bounds__(Shape<LPC>::kThreads, 2) void backward_kernel(Scan 
     uint32_t begun;
     const int k = At::channel();
     {
-      const Fetched<T, LPC, true, true>& now = next;
+      const Fetched<T, LPC, kFew, true, true>& now = next;
       begun = now.begun(t0, end);
       const f32x4 bias = params[0][k / 4];
 #pragma unroll
@@ -593,7 +593,7 @@ int plan(Scan* s, int64_t b, int64_t t, int32_t d, int32_t n, int32_t g, bool ba
   int cus = 0;
   const int status = device_cus(&cus);
   if (status != HIPENVS_OK) return status;
-  const int lpc = lanes_of(n), ch = channels_of(lpc);
+  const int lpc = lanes_of(n), ch = channels_of(lpc, few_channels(d / g));
   s->b = b, s->t = t, s->d = d, s->n = n, s->g = g, s->dg = d / g;
   s->tiles = (s->dg + ch - 1) / ch;
   const int64_t waves = b * g * s->tiles * (ch * lpc / 64), want = (int64_t)cus * (back ? 8 : 16);
@@ -655,11 +655,14 @@ int for_lanes(int lpc, const F& f) {
   }
 }
 
-// f(lanes of a channel, whether n is all of their states)
+// f(lanes of a channel, whether groups have few channels, whether n is all of the lanes' states)
 template <class F>
-int for_states(int n, const F& f) {
-  return for_lanes(lanes_of(n), [&](auto lanes) {
-    return n == 4 * decltype(lanes)::value ? f(lanes, std::true_type()) : f(lanes, std::false_type());
+int for_shape(const Scan& s, const F& f) {
+  return for_lanes(lanes_of(s.n), [&](auto lanes) {
+    const bool full = s.n == 4 * decltype(lanes)::value;
+    if (few_channels(s.dg))
+      return full ? f(lanes, std::true_type(), std::true_type()) : f(lanes, std::true_type(), std::false_type());
+    return full ? f(lanes, std::false_type(), std::true_type()) : f(lanes, std::false_type(), std::false_type());
   });
 }
 
@@ -678,36 +681,38 @@ int join(const Scan& s, hipStream_t stream) {
 
 template <class T>
 int forward(const Scan& s, hipStream_t stream) {
-  return for_states(s.n, [&](auto lanes, auto full) {
-    constexpr int LPC = decltype(lanes)::value, kThreads = Shape<LPC>::kThreads;
-    constexpr bool kFull = decltype(full)::value;
+  return for_shape(s, [&](auto lanes, auto few, auto full) {
+    constexpr int LPC = decltype(lanes)::value;
+    constexpr bool kFew = decltype(few)::value, kFull = decltype(full)::value;
+    constexpr int kThreads = Shape<LPC, kFew>::kThreads;
     if (s.parts > 1) {
       int status = in_launches(s, blocks_of(s, s.parts - 1), kThreads, [&](const Scan& a, dim3 grid) {
-        hipLaunchKernelGGL((forward_kernel<T, LPC, kFull, false>), grid, dim3(kThreads), 0, stream, a);
+        hipLaunchKernelGGL((forward_kernel<T, LPC, kFew, kFull, false>), grid, dim3(kThreads), 0, stream, a);
       });
       if (status == HIPENVS_OK) status = join<false>(s, stream);
       if (status != HIPENVS_OK) return status;
     }
     return in_launches(s, blocks_of(s, s.parts), kThreads, [&](const Scan& a, dim3 grid) {
-      hipLaunchKernelGGL((forward_kernel<T, LPC, kFull, true>), grid, dim3(kThreads), 0, stream, a);
+      hipLaunchKernelGGL((forward_kernel<T, LPC, kFew, kFull, true>), grid, dim3(kThreads), 0, stream, a);
     });
   });
 }
 
 template <class T>
 int backward(const Scan& s, hipStream_t stream) {
-  const int walked = for_states(s.n, [&](auto lanes, auto full) {
-    constexpr int LPC = decltype(lanes)::value, kThreads = Shape<LPC>::kThreads;
-    constexpr bool kFull = decltype(full)::value;
+  const int walked = for_shape(s, [&](auto lanes, auto few, auto full) {
+    constexpr int LPC = decltype(lanes)::value;
+    constexpr bool kFew = decltype(few)::value, kFull = decltype(full)::value;
+    constexpr int kThreads = Shape<LPC, kFew>::kThreads;
     if (s.parts > 1) {
       int status = in_launches(s, blocks_of(s, s.parts - 1), kThreads, [&](const Scan& a, dim3 grid) {
-        hipLaunchKernelGGL((passed_kernel<T, LPC>), grid, dim3(kThreads), 0, stream, a);
+        hipLaunchKernelGGL((passed_kernel<T, LPC, kFew>), grid, dim3(kThreads), 0, stream, a);
       });
       if (status == HIPENVS_OK) status = join<true>(s, stream);
       if (status != HIPENVS_OK) return status;
     }
     return in_launches(s, blocks_of(s, s.parts), kThreads, [&](const Scan& a, dim3 grid) {
-      hipLaunchKernelGGL((backward_kernel<T, LPC, kFull>), grid, dim3(kThreads), 0, stream, a);
+      hipLaunchKernelGGL((backward_kernel<T, LPC, kFew, kFull>), grid, dim3(kThreads), 0, stream, a);
     });
   });
   if (walked != HIPENVS_OK || s.tiles <= 1 || s.t == 0) return walked;

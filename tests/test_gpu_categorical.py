@@ -122,6 +122,13 @@ def test_log_probs_and_gradients_match_the_definition(dev, shape, dtype):
     check(*make(dev, 9, rows, v, dtype), min(v, 64))
 
 
+@pytest.mark.parametrize("v", [6, 8, 9, 24, 32, 33, 66, 128, 129, 255, 400, 512, 513])
+def test_rows_of_every_number_of_lanes(dev, v):
+    for k, dtype in enumerate((F32, BF16)):
+        print("log_probs", v, dtype, flush=True)
+        check(*make(dev, 20 + k, 300, v, dtype, 0.3, 2.0, "odd"), min(v, 5))
+
+
 @pytest.mark.parametrize("v", [3, 100, 900, 5000, 20000])
 def test_rows_that_leave_nothing_and_extreme_masks(dev, v):
     """Rows of -inf alone, masks of the type's lowest value, one token left, the given token not allowed."""

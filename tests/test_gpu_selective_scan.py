@@ -131,6 +131,15 @@ def test_sequence_and_gradients_match_the_definition(dev, shape, dtype):
         check(dev, make(dev, k, *shape, dtype, layout, episode))
 
 
+# groups of few channels and of more, at every number of lanes, with all of their states and without
+@pytest.mark.parametrize("n", [6, 8, 13, 16, 27, 32, 61, 64])
+@pytest.mark.parametrize("d,g", [(1, 1), (16, 1), (31, 1), (32, 1), (33, 1), (65, 1), (96, 3), (68, 2)])
+def test_groups_of_every_width(dev, d, g, n):
+    for k, dtype in enumerate((F32, BF16)):
+        print("scan", d, g, n, dtype, flush=True)
+        check(dev, make(dev, 30 + k, 2, 19, d, n, g, dtype, ("fused", "odd")[k], 11))
+
+
 @pytest.mark.parametrize("without", [("skip",), ("gate",), ("dt_bias",), ("state",), ("skip", "gate", "dt_bias", "state")])
 def test_terms_left_out(dev, without):
     check(dev, make(dev, 3, 2, 37, 70, 16, 1, without=without))
