@@ -206,7 +206,10 @@ __device__ __forceinline__ float top_log_prob(uint64_t ranked, Sums a) {
   return (x - a.m) - __builtin_amdgcn_logf(a.s) * kLn2;
 }
 
-// Short rows: G lanes hold a row in registers, E values each.
+// Short rows: G lanes hold a row in registers, E values each, four next to each other of every 4 G, all loaded
+// before any is used. Bound by memory: 2^28 values, forwards and backwards, in rows of 1,000 in 628 us as float32
+// (5.1 TB/s) and 338 as bfloat16, in rows of 64 in 611 and 395. Values loaded one by one, each behind a
+// comparison and a conversion, took 729 and 749, 904 and 759.
 template <class T, int G, int E>
 __global__ __launch_bounds__(kBlock) void short_kernel(LogProbs p) {
   const int64_t row = p.item0 + (int64_t)blockIdx.x * (kBlock / G) + threadIdx.x / G;
@@ -215,21 +218,31 @@ __global__ __launch_bounds__(kBlock) void short_kernel(LogProbs p) {
   const T* x = (const T*)p.logits + row * p.logits_s;
   const int v = (int)p.v;
   const int64_t token = p.tokens[row];
+  const auto place = [&](int e) { return (e / 4 * G + lane) * 4 + e % 4; };
+  typename Raw<T>::type raw[E / 4];
+#pragma unroll
+  for (int k = 0; k < E / 4; ++k) raw[k] = fetch4(x, place(4 * k), v);
+  const bool has = token >= 0 && token < v;
+  const T chosen = x[has ? token : 0];
   float own[E];
   Sums a = none();
 #pragma unroll
-  for (int e = 0; e < E; ++e) own[e] = e * G + lane < v ? (float)x[e * G + lane] : -__builtin_inff();
+  for (int k = 0; k < E / 4; ++k) {
+    const f32x4 y = values<T>(raw[k], place(4 * k), v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) own[4 * k + e] = place(4 * k + e) < v ? y[e] : -__builtin_inff();
+  }
 #pragma unroll
   for (int e = 0; e < E; ++e) a.m = larger(own[e], a.m);
   a.add(own);
   a = joined<G>(a);
-  if (lane == 0) write_row(p, row, a, token >= 0 && token < p.v ? (float)x[token] : 0.0f, token);
+  if (lane == 0) write_row(p, row, a, has ? (float)chosen : 0.0f, token);
   uint32_t taken = 0;
   for (int k = 0; k < p.top; ++k) {
     uint64_t best = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const uint64_t r = e * G + lane < v && !(taken >> e & 1) ? ranked(own[e], e * G + lane) : 0;
+      const uint64_t r = place(e) < v && !(taken >> e & 1) ? ranked(own[e], place(e)) : 0;
       best = r > best ? r : best;
     }
     uint64_t all = best;
@@ -239,7 +252,7 @@ __global__ __launch_bounds__(kBlock) void short_kernel(LogProbs p) {
       all = other > all ? other : all;
     }
     const uint32_t at = place_in(all);
-    if (at % G == (uint32_t)lane) taken |= 1u << (at / G);
+    if (at / 4 % G == (uint32_t)lane) taken |= 1u << (at / (4 * G) * 4 + at % 4);
     if (lane == 0) {
       p.top_log_prob[row * p.top + k] = top_log_prob(all, a);
       p.top_index[row * p.top + k] = at;
@@ -418,11 +431,23 @@ __global__ __launch_bounds__(kBlock) void short_gradient_kernel(Gradient g) {
   if (row >= g.rows) return;
   const T* x = (const T*)g.logits + row * g.logits_s;
   T* dx = (T*)g.dlogits + row * g.v;
-  const RowGradient of(g, row);
+  const int v = (int)g.v;
+  typename Raw<T>::type raw[E / 4];
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int j = e * G + lane;
-    if (j < (int)g.v) dx[j] = (T)(of.of((float)x[j]) + (j == of.token ? of.dlp : 0.0f));
+  for (int k = 0; k < E / 4; ++k) raw[k] = fetch4(x, (k * G + lane) * 4, v);
+  const RowGradient of(g, row);
+  const uint32_t token = of.token >= 0 && of.token < v ? (uint32_t)of.token : 0xFFFFFFFFu;
+#pragma unroll
+  for (int k = 0; k < E / 4; ++k) {
+    const int j = (k * G + lane) * 4;
+    f32x4 own = values<T>(raw[k], j, v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) own[e] = of.of(own[e]);
+    const uint32_t at = token - (uint32_t)j;
+    if (at < 4)   // one thread of the row
+#pragma unroll
+      for (uint32_t e = 0; e < 4; ++e) own[e] += at == e ? of.dlp : 0.0f;
+    store_upto(dx + j, own, v - j);
   }
 }
 
@@ -513,18 +538,18 @@ int in_launches(S s, int64_t blocks, int threads, const F& launch) {
 }
 
 // f(lanes of a row, values a lane) for rows of up to kShort values: the fewer lanes, the more rows a wave's
-// joins serve, but the further apart lie the values that a load fetches. 2^28 float32 values, forwards and
-// backwards, in us, at four a lane, eight and 16: rows of 16 517, 943, 1,824; of 32 995, 1,426, 3,047; of 64 951,
-// 904, 1,466; of 128 972, 741, 898; of 256 998, 769, 680; of 512 -, 768, 684.
+// joins serve, but the further apart lie the values that a load fetches. 2^28 values, forwards and backwards, in
+// us, at four a lane, eight and 16, float32 and then bfloat16: rows of 32 747, 676, 914 and 603, 397, 482; of 64
+// 761, 611, 650 and 626, 395, 451; of 128 766, 590, 601 and 630, 397, 327; of 256 779, 601, 581 and 654, 404, 311.
 template <class F>
 int for_short(int64_t v, const F& f) {
   using std::integral_constant;
   if (v <= 4) return f(integral_constant<int, 1>(), integral_constant<int, 4>());
-  if (v <= 8) return f(integral_constant<int, 2>(), integral_constant<int, 4>());
-  if (v <= 16) return f(integral_constant<int, 4>(), integral_constant<int, 4>());
-  if (v <= 32) return f(integral_constant<int, 8>(), integral_constant<int, 4>());
+  if (v <= 8) return f(integral_constant<int, 1>(), integral_constant<int, 8>());
+  if (v <= 16) return f(integral_constant<int, 2>(), integral_constant<int, 8>());
+  if (v <= 32) return f(integral_constant<int, 4>(), integral_constant<int, 8>());
   if (v <= 64) return f(integral_constant<int, 8>(), integral_constant<int, 8>());
-  if (v <= 128) return f(integral_constant<int, 16>(), integral_constant<int, 8>());
+  if (v <= 128) return f(integral_constant<int, 8>(), integral_constant<int, 16>());
   if (v <= 256) return f(integral_constant<int, 16>(), integral_constant<int, 16>());
   if (v <= 512) return f(integral_constant<int, 32>(), integral_constant<int, 16>());
   return f(integral_constant<int, 64>(), integral_constant<int, 16>());
