@@ -8,7 +8,7 @@ namespace scan {
 // What a tile's walk has to leave out. States past n have no write and no read, but zero times an
 // infinity is no number: where there are any, they are kept at zero, by whole lanes that see neither delta x
 // nor dy (n a multiple of four) or one by one. 64 x 1,000 tokens of 500 channels of 12 states, bfloat16:
-// 264 and 635 us forwards and backwards with every tile as kAny, 230 and 565 so.
+// 264 and 635 us forwards and backwards with every tile as kAny, 230 and 575 so.
 // kFull: n is all the lanes' states, and there are none past it.
 enum Kind { kPlain, kLanes, kBegins, kAny };   // nothing; lanes without states; beginnings; single states too
 
@@ -40,9 +40,9 @@ __device__ __forceinline__ f32x4 rates_of(const Scan& s, int64_t c, int n0, int 
 // time, computed once each and fetched a tile ahead. kOut: outputs, from the states before the
 // part; otherwise the part's own state alone, from zeros, for rows walked in parts.
 //
-// Bound by its vector instructions (97 % of the time at 4,096 x 128 tokens of 128 channels, float32): 26 a
-// token for 16 channels of 16 states, two of them for each exponential, and as much again a token for what a
-// tile's elements take (softplus, the gate, addresses). 375 us there, 2.5 TB/s; 16,381 tokens of 512 channels
+// Bound by its vector instructions, which issue all of the time at 4,096 x 128 tokens of 128 channels, float32:
+// 44 a token for 16 channels of 16 states, 22 of them the walk (two for each exponential), the rest what a
+// tile's elements take (softplus, the gate, addresses). 370 us there, 2.5 TB/s; 16,381 tokens of 512 channels
 // in parts 36 + 15 + 51 us. Tiles of eight tokens took 442, of one row in fewer parts (eight waves a CU
 // instead of 16) 41 + 9 + 64. Loads that a branch or a conversion separates wait for each other: 73 us for the
 // 51 before they went.
@@ -277,10 +277,12 @@ __global__ __launch_bounds__((Shape<LPC, kFew>::kThreads)) void passed_kernel(Sc
 // Sums over a channel's states stay within its lanes; sums over channels go lane by lane within the
 // wave, then through LDS, then (dmix) over the blocks of a group.
 //
-// Bound by instruction issue at the two waves a SIMD that 128 registers of decays and states leave (some
-// instruction issues 88 % of the time, a vector one 69 %): 1,300 us for 4,096 x 128 tokens of 128 channels,
-// float32, of which the sums over channels take 190, the exponentials 155 and the outputs 165. Three waves with
-// the decays computed again instead of held: 1,340; tiles of eight tokens, three waves: 1,620.
+// Bound by instruction issue at the two waves a SIMD that 128 registers of decays and states leave (a vector
+// one 81 % of the time, 118 a token for 16 channels of 16 states): 1,190 us for 4,096 x 128 tokens of 128
+// channels, float32, of which the sums over channels take some 190, the exponentials 155 and the outputs 165.
+// Before the next tile's loads were waited for ahead of the outputs' stores, and its addresses kept from tile to
+// tile, it took 1,290; then, three waves with the decays computed again instead of held 1,340, tiles of
+// eight tokens with three waves 1,620.
 template <class T, int LPC, bool kFew, bool kFull>
 __global__ __launch_bounds__((Shape<LPC, kFew>::kThreads), 2) void backward_kernel(Scan s) {
   using S = Shape<LPC, kFew>;
@@ -515,7 +517,8 @@ __global__ __launch_bounds__(kBlock) void mix_sums_kernel(Scan s) {
 
 // One token of every environment: LPC lanes a channel, each with four states, which are read once and
 // written once, bound by that. A thread takes its channel of kEnvs environments, so that as many states are
-// in flight: 4,096 x 512 x 16 states in 70 us, 4.1 TB/s, where one a thread takes 79. next may be state itself: a thread writes only what it has read.
+// in flight: 4,096 x 512 x 16 states in 70 us, 4.1 TB/s, where one a thread takes 79. next may be state itself: a
+// thread writes only what it has read.
 struct Step {
   const void *x, *dt, *gate, *write, *read;
   int64_t x_s, dt_s, gate_s, write_s, write_sg, read_s, read_sg, reset_s;
