@@ -161,6 +161,13 @@ def test_few_long_rows(dev, dtype, n):
     check(dev, make(dev, 6, 1, 128, 8, n, 1, dtype, "fused", 0))
 
 
+@pytest.mark.parametrize("n", [3, 8, 16, 30, 32, 50, 64])
+def test_few_long_rows_of_wide_groups(dev, n):
+    for k, (b, d, g) in enumerate(((2, 80, 1), (1, 140, 2))):
+        print("long", n, d, g, flush=True)
+        check(dev, make(dev, 40 + k, b, 517, d, n, g, (F32, BF16)[k], "fused", (0, 200)[k]))
+
+
 def test_softplus_and_sigmoid_units(dev):
     """delta from one token of a zero state: within SOFTPLUS units and the four of products; and silu."""
     from hipenvs import selective_scan
