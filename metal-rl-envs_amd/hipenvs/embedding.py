@@ -32,6 +32,8 @@ def _backward(ctx, dout):
     if dout is None:
         return None, None, None
     tokens = _tokens(tokens, device.index)
+    if tokens.shape != shape:   # as many rows of dout are read as there are tokens
+        raise ValueError(f"saved tokens must have shape {tuple(shape)}, got {tuple(tokens.shape)}")
     _checks.refuse_tangents("the gradient of lookup", dout)
     dout = _checks.saved(dout, dtype, (*shape, d), device.index).view(-1, d) if tokens.numel() else dout.reshape(0, d)
     dtable = torch.empty((v, d), dtype=dtype, device=device)

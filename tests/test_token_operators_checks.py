@@ -1,0 +1,20 @@
+"""What the lookup's backward pass refuses before any launch (CPU)."""
+
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+
+def test_lookup_refuses_saved_tokens_of_another_shape():
+    """Hooks on saved tensors may hand back others: as many rows are read of the gradient as there are tokens,
+    so more of them would be read past its end."""
+    from hipenvs import embedding
+
+    here = SimpleNamespace(index=torch.zeros(1).get_device())   # a tensor of the host passes for one of this device
+    dout = torch.zeros(3, 2, 5)
+    for tokens in (torch.zeros(3, 3, dtype=torch.int64), torch.zeros(2, 3, dtype=torch.int64),
+                   torch.zeros(7, dtype=torch.int32), torch.zeros(0, dtype=torch.int64)):
+        ctx = SimpleNamespace(saved_tensors=(tokens,), ready=(torch.float32, (4, 5), (3, 2), here, 1.0))
+        with pytest.raises(ValueError, match="shape"):
+            embedding._backward(ctx, dout)
