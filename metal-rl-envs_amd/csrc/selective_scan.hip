@@ -398,6 +398,7 @@ __global__ __launch_bounds__((Shape<LPC, kFew>::kThreads), 2) void backward_kern
         const f32x4 w = *(const f32x4*)&mix[tok][n0], r = *(const f32x4*)&mix[tok][S::NP + n0];
         float y = 0.0f, into = 0.0f, dd = 0.0f, v[8];
         const bool begins = kKind >= kBegins && (begun >> tok & 1);
+        const float delta = begins ? 0.0f : st.x;   // of the state before
         if (kKind == kLanes) st.y = left > 0 ? st.y : 0.0f, st.z = left > 0 ? st.z : 0.0f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -409,9 +410,10 @@ __global__ __launch_bounds__((Shape<LPC, kFew>::kThreads), 2) void backward_kern
           v[e] = g[e] * st.y;
           v[4 + e] = state * st.z;
           // of what is left of the state before, whose size may be far below the state's: kept by itself,
-          // as their difference would lose its last bits
-          const float through = g[e] * kept[tok][e];
-          drate[e] = __builtin_fmaf(through, st.x, drate[e]);
+          // as their difference would lose its last bits. Nothing is where an episode begins, with an
+          // infinite g or delta too
+          const float through = begins ? 0.0f : g[e] * kept[tok][e];
+          drate[e] = __builtin_fmaf(through, delta, drate[e]);
           dd = e ? __builtin_fmaf(through, rate[e], dd) : through * rate[e];
           g[e] = begins ? 0.0f : g[e] * a[tok][e];
         }

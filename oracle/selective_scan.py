@@ -77,8 +77,9 @@ def _gradients(x, rate, f, one, open_, slope, g, dout, dfinal):
         dread[:, i] = states[:, i] * dy[:, i, :, None]
         dwrite[:, i] = G * (f["delta"][:, i] * x[:, i])[..., None]
         into = (G * f["write"][:, i]).sum(-1)
-        through = G * before[:, i]
-        drate += (through * f["delta"][:, i, :, None]).sum(0)
+        begins = f["begins"][:, i, None, None]   # the state before owes nothing, to an infinite G or delta neither
+        through = np.where(begins, 0.0, G * before[:, i])
+        drate += np.where(begins, 0.0, through * f["delta"][:, i, :, None]).sum(0)
         ddt[:, i] = ((through * rate).sum(-1) + into * x[:, i]) * one[:, i]
         dx[:, i] = f["skip"] * dy[:, i] + f["delta"][:, i] * into
         G = np.where(f["begins"][:, i, None, None], 0.0, G * f["keep"][:, i])

@@ -1,0 +1,82 @@
+"""Infinities where an operator over tokens has left something out (GPU): an episode's first token leaves out the
+state and the taps before it, a logit of -inf its token. What is left out owes nothing to an infinite gradient or
+decay on the other side, where zero times an infinity would be no number."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import selective_scan as oss
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+INF = float("inf")
+
+
+def to_np(x):
+    return x.detach().cpu().numpy() if x.dtype == torch.bool else x.detach().double().cpu().numpy()
+
+
+# n: two to sixteen lanes, with all of their states and without; t: in one part, and in several
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [3, 8, 12, 16, 27, 64])
+@pytest.mark.parametrize("t", [40, 900])
+def test_scan_infinite_gradient_of_an_episodes_first_token(dev, n, t, dtype):
+    """The state before is left out: rate's gradient, and all others but that token's own, are those with a
+    gradient of zero there; and the token's own are the definition's."""
+    from hipenvs import selective_scan
+
+    gen = torch.Generator().manual_seed(n)
+    b, d, at = 2, 40, t // 2 + 3
+    reset = torch.zeros(b, t, dtype=torch.bool)
+    reset[0, at] = True
+    rows = [torch.rand(b, t, w, generator=gen).add(0.1).to(dtype) for w in (d, d, n, n)]
+    given = {"x": rows[0], "dt": rows[1], "rate": -torch.rand(d, n, generator=gen) - 0.1, "write": rows[2], "read": rows[3]}
+    given = {k: v.to(dev) for k, v in given.items()}
+    grads = []
+    for first in (0.0, INF):
+        dout = torch.ones(b, t, d, dtype=dtype, device=dev)
+        dout[0, at, 5] = first
+        leaves = {k: v.detach().requires_grad_() for k, v in given.items()}
+        out, _ = selective_scan.sequence(**leaves, reset=reset.to(dev))
+        grads.append(dict(zip(leaves, torch.autograd.grad(out, list(leaves.values()), dout))))
+    zero, inf = grads
+    assert torch.isfinite(inf["rate"]).all() and torch.equal(inf["rate"], zero["rate"])
+    for name in ("x", "dt"):
+        elsewhere = torch.ones(b, t, d, dtype=torch.bool, device=dev)
+        elsewhere[0, at, 5] = False
+        assert torch.equal(inf[name][elsewhere], zero[name][elsewhere])
+        assert inf[name][0, at, 5] == INF   # x, write, read and the slope of softplus are above zero
+    for name in ("write", "read"):
+        others = torch.arange(t, device=dev) != at
+        assert torch.equal(inf[name][:, others], zero[name][:, others]) and (inf[name][0, at] == INF).all()
+    f64 = [to_np(given[k]) for k in ("x", "dt", "rate")] + [to_np(given[k])[:, :, None] for k in ("write", "read")]
+    with np.errstate(invalid="ignore"):   # the token's own sums
+        want = oss.gradients(*f64, None, None, None, None, to_np(reset), to_np(dout), np.zeros((b, d, n)))
+    assert np.isfinite(want[2]).all() and want[1][0, at, 5] == INF
+
+
+@pytest.mark.parametrize("n", [3, 8, 12, 16, 64])
+@pytest.mark.parametrize("t", [40, 900])
+def test_scan_infinite_delta_of_an_episode_of_one_token(dev, n, t):
+    """Its state is infinite and ends with it: rate's gradient is what it is with a finite delta there."""
+    from hipenvs import selective_scan
+
+    gen = torch.Generator().manual_seed(n)
+    b, d, at = 1, 40, t // 2 + 3
+    reset = torch.zeros(b, t, dtype=torch.bool)
+    reset[0, at:at + 2] = True
+    x, dt, write, read = (torch.rand(b, t, w, generator=gen).add(0.1) for w in (d, d, n, n))
+    rate = -torch.rand(d, n, generator=gen) - 0.1
+    drates = []
+    for first in (0.5, INF):
+        dt[0, at, 5] = first
+        leaf = rate.to(dev).requires_grad_()
+        out, _ = selective_scan.sequence(x.to(dev), dt.to(dev), leaf, write.to(dev), read.to(dev), reset=reset.to(dev))
+        drates.append(torch.autograd.grad(out, leaf, torch.ones_like(out))[0])
+    assert torch.isfinite(drates[1]).all() and torch.equal(*drates)
+    with np.errstate(invalid="ignore"):   # a gate of one at an infinite output
+        want = oss.gradients(*(to_np(y) for y in (x, dt, rate)), to_np(write)[:, :, None], to_np(read)[:, :, None], None,
+                             None, None, None, to_np(reset), np.ones((b, t, d)), np.zeros((b, d, n)))
+    assert np.isfinite(want[2]).all()
