@@ -122,9 +122,10 @@ struct Tokens {
 };
 
 // hist as it is before token t0: hist[i] then holds the value of token t0 - 1 - i. A run has more tokens
-// than a window: windows of all runs but the first lie within the row.
+// than a window: windows of all runs but the first lie within the row. Returns the tokens from the episode's
+// first to t0 - 1, W where it lies before the window.
 template <class T, int W, bool kWide, bool kBack>
-__device__ __forceinline__ void before(const Conv& s, const Tokens<T, kWide, kBack>& of, int64_t b, int64_t t0, int c,
+__device__ __forceinline__ int before(const Conv& s, const Tokens<T, kWide, kBack>& of, int64_t b, int64_t t0, int c,
                                        f32x4 (&hist)[W]) {
 #pragma unroll
   for (int i = 0; i < W; ++i) hist[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -135,7 +136,7 @@ __device__ __forceinline__ void before(const Conv& s, const Tokens<T, kWide, kBa
       if (s.state) x = load_upto(s.state + (b * (W - 1) + k) * s.d + c, s.d - c);
       push(hist, x, false);
     }
-    return;
+    return W;
   }
   typename Raw<T>::type x[W];
   uint8_t begins[W];
@@ -145,8 +146,13 @@ __device__ __forceinline__ void before(const Conv& s, const Tokens<T, kWide, kBa
     x[k] = of.four.fetch(of.x + t * of.x_st);
     begins[k] = of.reset ? of.reset[t * of.reset_st] : 0;
   }
+  int since = W;
 #pragma unroll
-  for (int k = 0; k < W - 1; ++k) push(hist, of.four.value(x[k]), begins[k]);
+  for (int k = 0; k < W - 1; ++k) {
+    push(hist, of.four.value(x[k]), begins[k]);
+    since = begins[k] ? 0 : since < W ? since + 1 : W;
+  }
+  return since;
 }
 
 template <class T, int W, bool kWide>
@@ -195,7 +201,7 @@ __global__ __launch_bounds__(kBlock, 2) void backward_kernel(Conv s) {
   const Taps<W> taps(s, at.c);
   const Tokens<T, kWide, true> of(s, at.b, at.c);
   f32x4 hist[W], late[W], dweight[W], dbias = zero;   // late[i]: the gradient of token t - i
-  before(s, of, at.b, t0, at.c, hist);
+  int since = before(s, of, at.b, t0, at.c, hist);   // tokens since the episode's first
 #pragma unroll
   for (int i = 0; i < W; ++i) late[i] = dweight[i] = zero;
   T* dx = (T*)s.dx + at.b * s.t * s.d + at.c;
@@ -207,7 +213,6 @@ __global__ __launch_bounds__(kBlock, 2) void backward_kernel(Conv s) {
     else
       store_upto(dx + u * s.d, grad, left);
   };
-  int since = W;   // tokens since the episode's first
   typename Tokens<T, kWide, true>::Piece next;
   if (t0 < past) of.fetch(next, t0, past);
   for (int64_t first = t0; first < past; first += kAhead) {

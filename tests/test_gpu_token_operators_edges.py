@@ -80,3 +80,32 @@ def test_scan_infinite_delta_of_an_episode_of_one_token(dev, n, t):
         want = oss.gradients(*(to_np(y) for y in (x, dt, rate)), to_np(write)[:, :, None], to_np(read)[:, :, None], None,
                              None, None, None, to_np(reset), np.ones((b, t, d)), np.zeros((b, d, n)))
     assert np.isfinite(want[2]).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("w", [2, 3, 4])
+def test_conv_infinite_gradient_next_to_an_episodes_first_tokens(dev, w, dtype):
+    """Every place of an episode's beginning and of an infinite gradient just behind it: the weights of the taps
+    that are left out have the gradient that they have without it."""
+    from hipenvs import causal_conv
+
+    gen = torch.Generator().manual_seed(w)
+    b, t, d = 1, 70, 6
+    x = torch.rand(b, t, d, generator=gen).add(0.1).to(dtype).to(dev)
+    weight = torch.rand(d, w, generator=gen).add(0.1).to(dev)
+    for begin in (0, 1, 5, 7, 8, 15, 16, 30, 31, 32, 62, 63, 64, 66):
+        reset = torch.zeros(b, t, dtype=torch.bool, device=dev)
+        reset[0, begin] = True
+        for behind in range(w - 1):
+            grads = []
+            for value in (0.0, INF):
+                dout = torch.ones(b, t, d, dtype=dtype, device=dev)
+                dout[0, begin + behind, 2] = value
+                leaf = weight.detach().requires_grad_()
+                out, _ = causal_conv.sequence(x, leaf, reset=reset, silu=False)
+                grads.append(torch.autograd.grad(out, leaf, dout)[0])
+            zero, inf = grads
+            hit = torch.zeros(d, w, dtype=torch.bool, device=dev)
+            hit[2, w - 1 - behind:] = True   # the taps within the episode
+            assert torch.equal(inf[~hit], zero[~hit]), (begin, behind)
+            assert (inf[hit] == INF).all(), (begin, behind)
