@@ -27,13 +27,24 @@ __device__ __forceinline__ void for_kind(uint32_t begins, int n, const F& walk) 
   }
 }
 
-// Four states' rates; those past n decay, so that an infinite delta leaves them at zero.
+// Four states' rates times log2(e); those past n decay, so that an infinite delta leaves them at zero. An infinite
+// one is as good as float32's largest, and times a delta of zero, which stands for that of an episode's first
+// token, it is a number.
 __device__ __forceinline__ f32x4 rates_of(const Scan& s, int64_t c, int n0, int left) {
+  constexpr float kMost = 0x1.fffffep+127f;
   f32x4 rate = load_upto(s.rate + c * s.n + n0, left);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) rate[e] = e < left ? rate[e] : -1.0f;
+  for (int e = 0; e < 4; ++e) {
+    const float x = (e < left ? rate[e] : -1.0f) * kLog2e;
+    rate[e] = x > kMost ? kMost : x < -kMost ? -kMost : x;   // a NaN stays
+  }
   return rate;
 }
+
+// x, or 0 where `bits` is 0 and not ~0. A selection of the backward pass's values by a scalar condition became
+// branches, across which 60 to 110 registers of decays and states spilled: 1,190 -> 2,000 us at 4,096 x 128 tokens of
+// 128 channels, float32.
+__device__ __forceinline__ float masked(float x, uint32_t bits) { return __uint_as_float(__float_as_uint(x) & bits); }
 
 // One part of a row's tokens for a block of channels: LPC lanes hold a channel, four states each,
 // and walk token by token; delta, x, write and read come through LDS, a tile of 16 tokens at a
@@ -59,7 +70,7 @@ __global__ __launch_bounds__((Shape<LPC, kFew>::kThreads)) void forward_kernel(S
   const int64_t c = (int64_t)at.group * s.dg + at.first + ch;
   const int64_t start = at.p * s.part, end = start + s.part < s.t ? start + s.part : s.t;
   const int left = live ? s.n - n0 : 0;
-  const f32x4 rate = rates_of(s, c, n0, left) * kLog2e;
+  const f32x4 rate = rates_of(s, c, n0, left);
   f32x4 h = {0.0f, 0.0f, 0.0f, 0.0f};
   if (kOut) {
     if (s.parts > 1)
@@ -111,7 +122,11 @@ __global__ __launch_bounds__((Shape<LPC, kFew>::kThreads)) void forward_kernel(S
         f32x2 st = steps[tok][ch];
         const f32x4 w = *(const f32x4*)&mix[tok][n0];
         if (kKind == kLanes) st.y = left > 0 ? st.y : 0.0f;
-        if (kKind >= kBegins && (begins >> tok & 1)) h = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (kKind >= kBegins) {   // no state before, and no decay that could be infinite and make zero no number
+          const bool first = begins >> tok & 1;
+          if (first) h = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          st.x = masked(st.x, first ? 0u : ~0u);
+        }
         float y = 0.0f;
         f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
         if (kOut) r = *(const f32x4*)&mix[tok][S::NP + n0];
@@ -211,7 +226,7 @@ __global__ __launch_bounds__((Shape<LPC, kFew>::kThreads)) void passed_kernel(Sc
   const int64_t c = (int64_t)at.group * s.dg + at.first + ch;
   const int64_t start = at.p * s.part, end = start + s.part < s.t ? start + s.part : s.t;
   const int left = live ? s.n - n0 : 0;
-  const f32x4 rate = rates_of(s, c, n0, left) * kLog2e;
+  const f32x4 rate = rates_of(s, c, n0, left);
   f32x4 g = {0.0f, 0.0f, 0.0f, 0.0f};
   const int own = at.first + At::channel();
   const f32x4 bias = per_channel(s.bias, (int64_t)at.group * s.dg + own, s.dg - own, 0.0f);
@@ -267,10 +282,6 @@ __global__ __launch_bounds__((Shape<LPC, kFew>::kThreads)) void passed_kernel(Sc
   if (threadIdx.x == 0 && at.group == 0 && at.first == 0) s.begun[at_part] = begun != 0;
 }
 
-// x, or 0 where `bits` is 0 and not ~0. A selection of the backward pass's values by a scalar condition became
-// branches, across which 60 to 110 registers of decays and states spilled: 1,190 -> 2,000 us at the size below.
-__device__ __forceinline__ float masked(float x, uint32_t bits) { return __uint_as_float(__float_as_uint(x) & bits); }
-
 // The gradients of one part for a block of channels, tile by tile from its end: the tile's states
 // again from the one kept before it, decays and what they leave in registers, then back through them.
 //
@@ -304,7 +315,7 @@ __global__ __launch_bounds__((Shape<LPC, kFew>::kThreads), 2) void backward_kern
   const int64_t c = (int64_t)at.group * s.dg + at.first + ch;
   const int64_t start = at.p * s.part, end = start + s.part < s.t ? start + s.part : s.t;
   const int left = live ? s.n - n0 : 0;
-  const f32x4 rate = rates_of(s, c, n0, left) * kLog2e;
+  const f32x4 rate = rates_of(s, c, n0, left);
   f32x4 g = {0.0f, 0.0f, 0.0f, 0.0f}, drate = g;
   if (s.parts > 1)
     g = load_upto(s.carry + ((at.b * s.parts + at.p) * s.d + c) * s.n + n0, left);
@@ -572,7 +583,8 @@ __global__ __launch_bounds__(kBlock) void step_kernel(Step s) {
     float y = 0.0f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      state[e] = __builtin_fmaf(exp2_of(delta * (rate[e] * kLog2e)), begins[k] ? 0.0f : state[e], du * wk[e]);
+      const float own = du * wk[e];
+      state[e] = begins[k] ? own : __builtin_fmaf(exp2_of(delta * (rate[e] * kLog2e)), state[e], own);
       state[e] = e < left ? state[e] : 0.0f;   // zero times an infinity
       y = __builtin_fmaf(rk[e], state[e], y);
     }

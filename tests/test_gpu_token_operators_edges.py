@@ -82,6 +82,33 @@ def test_scan_infinite_delta_of_an_episode_of_one_token(dev, n, t):
     assert np.isfinite(want[2]).all()
 
 
+@pytest.mark.parametrize("n", [3, 8, 12, 16, 64])
+@pytest.mark.parametrize("t", [40, 900])
+def test_scan_infinite_decay_at_an_episodes_first_token(dev, n, t):
+    """A rate above zero and a large delta: the decay of an episode's first token is infinite, and meets no state."""
+    from hipenvs import selective_scan
+
+    b, d, at = 2, 6, t // 2 + 3
+    x, dt, mix = torch.ones(b, t, d), torch.full((b, t, d), -30.0), torch.ones(b, t, n)
+    dt[:, at, 1] = 200.0
+    reset = torch.zeros(b, t, dtype=torch.bool)
+    reset[:, at] = True
+    rate, state = torch.ones(d, n), torch.ones(b, d, n)
+    given = [y.to(dev) for y in (x, dt, rate, mix, mix)]
+    out, final = selective_scan.sequence(*given, state=state.to(dev), reset=reset.to(dev))
+    f64 = {k: to_np(y) for k, y in (("x", x), ("dt", dt), ("rate", rate), ("state", state), ("reset", reset))}
+    want = oss.sequence(**f64, write=to_np(mix)[:, :, None], read=to_np(mix)[:, :, None])
+    # all terms are above zero. A state sums at most t of them and meets t decays, each within two units of
+    # 2^-24 (their exponents are below 1e-12); delta is within 8 units and its product; an output sums n states
+    assert np.isfinite(want[0]).all()
+    assert np.all(np.abs(to_np(out) - want[0]) <= (3 * t + n + 16) * 2.0 ** -24 * np.abs(want[0]))
+    assert np.all(np.abs(to_np(final) - want[1]) <= (3 * t + n + 16) * 2.0 ** -24 * np.abs(want[1]))
+    one = [y[:, at].contiguous() if y.dim() == 3 else y for y in given]
+    o, s = selective_scan.step(*one, state=state.to(dev), reset=torch.ones(b, dtype=torch.bool, device=dev))
+    assert torch.isfinite(s).all()
+    assert ((o - out[:, at]).abs() <= 2 * (n + 16) * 2.0 ** -24 * out[:, at]).all()   # the same sums, in either order
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("w", [2, 3, 4])
 def test_conv_infinite_gradient_next_to_an_episodes_first_tokens(dev, w, dtype):
