@@ -418,9 +418,10 @@ struct RowGradient {
     level = __builtin_fmaf(dh, g.entropy[row], dlp);
   }
 
+  // a token that is not allowed owes nothing, to an infinite slope or level neither
   __device__ __forceinline__ float of(float x) const {
-    const float log2_p = __builtin_fmaf(x - m, kLog2e, -log_s);
-    return -exp2_of(log2_p) * __builtin_fmaf(at_least(log2_p), slope, level);
+    const float log2_p = __builtin_fmaf(x - m, kLog2e, -log_s), p = exp2_of(log2_p);
+    return p == 0.0f ? 0.0f : -p * __builtin_fmaf(at_least(log2_p), slope, level);
   }
 };
 

@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 import torch
 
+from oracle import categorical as oca
 from oracle import selective_scan as oss
 
 pytestmark = pytest.mark.gpu
@@ -136,3 +137,28 @@ def test_conv_infinite_gradient_next_to_an_episodes_first_tokens(dev, w, dtype):
             hit[2, w - 1 - behind:] = True   # the taps within the episode
             assert torch.equal(inf[~hit], zero[~hit]), (begin, behind)
             assert (inf[hit] == INF).all(), (begin, behind)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("v", [2, 3, 7, 16, 30, 64, 100, 200, 500, 1000, 1024, 1025, 5000])
+def test_log_probs_infinite_gradients_leave_masked_tokens_at_zero(dev, v, dtype):
+    """Tokens that are not allowed, in rows with others and in rows of nothing else."""
+    from hipenvs import categorical
+
+    gen = torch.Generator().manual_seed(v)
+    x = torch.randn(6, v, generator=gen).to(dtype)
+    x[:, ::2] = -INF
+    x[2:4] = -INF
+    tokens = torch.tensor([1, 1, 1, -1, 1, 1])
+    leaf = x.to(dev).requires_grad_()
+    log_prob, entropy = categorical.log_probs(leaf, tokens.to(dev))
+    for given in ((INF, 1.0), (1.0, INF), (-INF, -INF), (float("nan"), 1.0)):
+        dlog_prob, dentropy = (torch.full((6,), y, device=dev) for y in given)
+        grad, = torch.autograd.grad((log_prob, entropy), leaf, (dlog_prob, dentropy), retain_graph=True)
+        assert (grad[:, ::2] == 0).all() and (grad[2:4] == 0).all()
+    # finite ones: a p is within 32 units of 2^-24 of itself (its exponent is below 20), the bracket below
+    # 1 + 2 log 5000 < 19 within 64 of its size: below 1e-5
+    grad, = torch.autograd.grad((log_prob, entropy), leaf, (torch.ones(6, device=dev), torch.ones(6, device=dev)))
+    want = oca.gradient(x.double().numpy(), tokens.numpy(), np.ones(6), np.ones(6))
+    off = np.abs(to_np(grad) - want)
+    assert off.max() <= 1e-5 + (2.0 ** -8 if dtype == BF16 else 0.0) * np.abs(want).max()
