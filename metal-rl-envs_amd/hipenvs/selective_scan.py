@@ -74,8 +74,11 @@ def _strides(x, dt, write, read, gate, reset, dout=None):
 
 
 def _near(x):
-    """x, copied where its tokens lie further apart than the kernels' offsets reach."""
-    return x if x is None or -0x80000000 < x.stride(1) < 0x80000000 else x.contiguous()
+    """x, copied where its tokens lie further apart than the kernels' offsets reach. A clone: a row of one
+    token is contiguous whatever its stride, and contiguous() would leave that as it is."""
+    if x is None or -0x80000000 < x.stride(1) < 0x80000000:
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
 
 
 def _laid(x, dtype, shape, device):
@@ -83,7 +86,7 @@ def _laid(x, dtype, shape, device):
     if x is None or (x.dtype is dtype and x.shape == shape and x.stride(-1) == 1 and x.get_device() == device
                      and -0x80000000 < x.stride(1) < 0x80000000):
         return x
-    return _checks.saved(x, dtype, shape, device).contiguous()
+    return _near(_checks.saved(x, dtype, shape, device).contiguous())
 
 
 def _workspace(which, b, t, d, n, g, device):

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from oracle import categorical as oca
+from oracle import causal_conv as occ
 from oracle import selective_scan as oss
 
 pytestmark = pytest.mark.gpu
@@ -162,3 +163,58 @@ def test_log_probs_infinite_gradients_leave_masked_tokens_at_zero(dev, v, dtype)
     want = oca.gradient(x.double().numpy(), tokens.numpy(), np.ones(6), np.ones(6))
     off = np.abs(to_np(grad) - want)
     assert off.max() <= 1e-5 + (2.0 ** -8 if dtype == BF16 else 0.0) * np.abs(want).max()
+
+
+def test_rows_of_tokens_far_apart(dev):
+    """Tokens 2^31 values apart, whose offsets from each other do not fit 32 bits: as they are for the
+    convolution, copied for the scan, in every input and in the gradient that comes back."""
+    from hipenvs import causal_conv, selective_scan
+
+    gen = torch.Generator().manual_seed(1)
+    d, n, t, far = 24, 4, 3, (1 << 31) + 7
+    whole = torch.empty((t - 1) * far + 6 * d, dtype=BF16, device=dev)
+    marks = torch.zeros((t - 1) * far + 2, dtype=torch.bool, device=dev)
+
+    def apart(values, at):
+        y = whole.as_strided((1, t, values.shape[-1]), (1, far, 1), at)
+        y.copy_(values)
+        return y
+
+    x, dt, gate, mix, dout = (torch.randn(1, t, w, generator=gen).to(BF16).to(dev) for w in (d, d, d, 2 * n, d))
+    reset = torch.tensor([[False, False, True]], device=dev)
+    begins = marks.as_strided((1, t), (1, far), 1)
+    begins.copy_(reset)
+    spread = [apart(y, k * d) for k, y in enumerate((x, dt, gate, mix[..., :n], mix[..., n:], dout))]
+    rate, weight = -torch.ones(d, n, device=dev), torch.randn(d, 4, generator=gen).to(dev)
+    near = (x, dt, gate, mix[..., :n].contiguous(), mix[..., n:].contiguous(), dout)
+    results = []
+    for given, r in ((near, reset), (spread, begins)):
+        a, b, c, w, o = (y.detach().requires_grad_() for y in given[:5])
+        out, final = selective_scan.sequence(a, b, rate, w, o, gate=c, reset=r)
+        conv, held = causal_conv.sequence(a, weight, reset=r)
+        grads = torch.autograd.grad((out, conv), (a, b, c, w, o), (given[5], given[5]))
+        results.append((out.detach(), final.detach(), conv.detach(), held.detach(), *grads))
+    assert all(torch.equal(a, e) for a, e in zip(*results))
+
+
+def test_rows_of_one_token_far_apart(dev):
+    """A row of one token has no next one: its stride of t may be anything."""
+    from hipenvs import selective_scan
+
+    gen = torch.Generator().manual_seed(1)
+    d, n, far = 10, 4, 1 << 33
+    x, dt, gate = (torch.randn(2, 1, d, generator=gen).to(dev) for _ in range(3))
+    write, read = (torch.randn(2, 1, 1, n, generator=gen).to(dev) for _ in range(2))
+    reset = torch.ones(2, 1, dtype=torch.bool, device=dev)
+    rate = -torch.ones(d, n, device=dev)
+    results = []
+    for apart in (False, True):
+        leaves = [y.detach().clone() for y in (x, dt, write, read, gate)]
+        begins, dout = reset, torch.ones(2, 1, d, device=dev)
+        if apart:
+            leaves = [y.as_strided(y.shape, (y.stride(0), far, *y.stride()[2:])) for y in leaves]
+            begins, dout = (y.as_strided(y.shape, (y.stride(0), far, *y.stride()[2:])) for y in (begins, dout))
+        leaves = [y.requires_grad_() for y in leaves]
+        out, final = selective_scan.sequence(leaves[0], leaves[1], rate, leaves[2], leaves[3], gate=leaves[4], reset=begins)
+        results.append((out.detach(), final.detach(), *torch.autograd.grad(out, leaves, dout)))
+    assert all(torch.equal(a, e) for a, e in zip(*results))
