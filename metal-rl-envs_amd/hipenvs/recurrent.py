@@ -194,6 +194,8 @@ class Learner:
             raise ValueError(f"task must be one of {sorted(TASKS)}, got {cfg.task}")
         if cfg.memory not in ("decay", "scan"):
             raise ValueError(f"memory must be decay or scan, got {cfg.memory}")
+        if not 0.0 <= cfg.clip < math.inf:
+            raise ValueError(f"clip must be 0 or above and finite, got {cfg.clip}")
         if cfg.epochs < 1 or (cfg.epochs > 1 and not cfg.clip > 0):
             raise ValueError(f"epochs must be 1, or more with a clip above 0, got {cfg.epochs} with clip {cfg.clip}")
         self.cfg = cfg

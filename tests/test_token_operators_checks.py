@@ -18,3 +18,13 @@ def test_lookup_refuses_saved_tokens_of_another_shape():
         ctx = SimpleNamespace(saved_tensors=(tokens,), ready=(torch.float32, (4, 5), (3, 2), here, 1.0))
         with pytest.raises(ValueError, match="shape"):
             embedding._backward(ctx, dout)
+
+
+@pytest.mark.parametrize("clip", [-0.1, -2.0, float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("epochs", [1, 2])
+def test_learner_refuses_a_clip_whose_bounds_cross(clip, epochs):
+    """clamp(1 - clip, 1 + clip) of a clip below zero is a constant, without a gradient."""
+    from hipenvs import recurrent
+
+    with pytest.raises(ValueError, match="clip"):
+        recurrent.Learner(recurrent.Config(clip=clip, epochs=epochs))
