@@ -30,6 +30,7 @@ from . import categorical, causal_conv, decay_attention, embedding, selective_sc
 # body, the rows of its state that the policy sees, actions. The angles and positions alone:
 # velocities have to be inferred from the steps before.
 TASKS = {"cartpole": (cartpole, (0, 2), 2), "acrobot": (acrobot, (0, 1), 3)}
+MEMORIES = ("decay", "scan")
 
 
 @dataclass(frozen=True)
@@ -131,6 +132,8 @@ class Policy:
 
     def __init__(self, obs_dim, actions, width, heads, layers, generator, memory="decay", states=16,
                  previous_action=False):
+        if memory not in MEMORIES:
+            raise ValueError(f"memory must be {' or '.join(MEMORIES)}, got {memory}")
         if memory == "decay" and width % heads:
             raise ValueError(f"width {width} must be a multiple of heads {heads}")
         device = generator.device
@@ -192,8 +195,8 @@ class Learner:
     def __init__(self, cfg, device=None):
         if cfg.task not in TASKS:
             raise ValueError(f"task must be one of {sorted(TASKS)}, got {cfg.task}")
-        if cfg.memory not in ("decay", "scan"):
-            raise ValueError(f"memory must be decay or scan, got {cfg.memory}")
+        if cfg.memory not in MEMORIES:
+            raise ValueError(f"memory must be {' or '.join(MEMORIES)}, got {cfg.memory}")
         if not 0.0 <= cfg.clip < math.inf:
             raise ValueError(f"clip must be 0 or above and finite, got {cfg.clip}")
         if cfg.epochs < 1 or (cfg.epochs > 1 and not cfg.clip > 0):
@@ -292,7 +295,7 @@ def main(argv=None):
     p.add_argument("--bits", type=int, choices=(8, 32), default=32)
     p.add_argument("--updates", type=int, default=100)
     p.add_argument("--seed", type=int, default=0)
-    p.add_argument("--memory", choices=("decay", "scan"), default="decay")
+    p.add_argument("--memory", choices=MEMORIES, default="decay")
     p.add_argument("--states", type=int, default=16)
     p.add_argument("--previous-action", action="store_true")
     p.add_argument("--clip", type=float, default=0.0)

@@ -28,3 +28,14 @@ def test_learner_refuses_a_clip_whose_bounds_cross(clip, epochs):
 
     with pytest.raises(ValueError, match="clip"):
         recurrent.Learner(recurrent.Config(clip=clip, epochs=epochs))
+
+
+def test_policy_refuses_an_unknown_memory():
+    """It would be given decay attention."""
+    from hipenvs import recurrent
+
+    for memory in ("scam", None, "Scan"):
+        with pytest.raises(ValueError, match="memory"):
+            recurrent.Policy(2, 3, 8, 2, 1, torch.Generator(), memory=memory)
+    for memory, count in (("decay", 5), ("scan", 11)):
+        assert len(recurrent.Policy(2, 3, 8, 2, 1, torch.Generator(), memory=memory, states=4).parameters()) == count
