@@ -535,8 +535,10 @@ __global__ __launch_bounds__(kBlock) void mix_sums_kernel(Scan s) {
 
 // One token of every environment: LPC lanes a channel, each with four states, which are read once and
 // written once, bound by that. A thread takes its channel of kEnvs environments, so that as many states are
-// in flight: 4,096 x 512 x 16 states in 70 us, 4.1 TB/s, where one a thread takes 79. next may be state itself: a
-// thread writes only what it has read.
+// in flight. Medians over replays of a graph, states in turn, one environment a thread and four: 4,096 x 512 x 16
+// with bfloat16 rows 82.3 and 79.0 us (285 MB, 3.6 TB/s), 8,192 of them 158.7 and 146.8; with float32 rows, where
+// registers for four leave fewer waves, 91.8 and 97.7 (302 MB, 3.3 TB/s), 179.8 and 186.4. next may be state itself:
+// a thread writes only what it has read.
 struct Step {
   const void *x, *dt, *gate, *write, *read;
   int64_t x_s, dt_s, gate_s, write_s, write_sg, read_s, read_sg, reset_s;
@@ -860,8 +862,8 @@ extern "C" int hipenvs_selective_scan_step(int32_t dtype, const void* x, const v
             out,        next_state, count,      0,          0,          d,          n,          d / g};
   return for_lanes(lanes_of(n), [&](auto lanes) {
     constexpr int LPC = decltype(lanes)::value, kChannels = kBlock / LPC;
-    // four environments a thread where that leaves 32 blocks a CU
-    const bool many = count * d / 4 >= (int64_t)cus * 32 * kChannels;
+    // four environments a thread for bfloat16 rows where that leaves 32 blocks a CU
+    const bool many = dtype == 1 && count * d / 4 >= (int64_t)cus * 32 * kChannels;
     s.items = (many ? (count + 3) / 4 : count) * d;
     const int64_t most = kMostThreads / kBlock * kChannels;
     for (s.item0 = 0; s.item0 < s.items; s.item0 += most) {
@@ -871,8 +873,6 @@ extern "C" int hipenvs_selective_scan_step(int32_t dtype, const void* x, const v
         hipLaunchKernelGGL((step_kernel<__bf16, LPC, 4>), grid, block, 0, as_stream(stream), s);
       else if (dtype == 1)
         hipLaunchKernelGGL((step_kernel<__bf16, LPC, 1>), grid, block, 0, as_stream(stream), s);
-      else if (many)
-        hipLaunchKernelGGL((step_kernel<float, LPC, 4>), grid, block, 0, as_stream(stream), s);
       else
         hipLaunchKernelGGL((step_kernel<float, LPC, 1>), grid, block, 0, as_stream(stream), s);
       const int launched = launch_status();
