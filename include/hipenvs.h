@@ -453,7 +453,7 @@ int64_t hipenvs_selective_scan_workspace_bytes(int32_t which, int64_t b, int64_t
  * read, then b, t of reset; those of t below 2^31 in size. rate (d, n), skip, dt_bias (d) f32 contiguous; skip, gate, dt_bias, reset
  * (b, t) u8 or NULL (left out); state (b, d, n) f32 contiguous or NULL (zeros).
  * -> out (b, t, d) contiguous, final_state (b, d, n) f32 (not `state`), checks (which 1 above, 16-byte
- * aligned) or NULL. 1 <= n <= 64, d <= 65536, g divides d. workspace: 16-byte aligned. What a token
+ * aligned) or NULL. 1 <= n <= 64, d <= 65536, b d < 2^31, g divides d. workspace: 16-byte aligned. What a token
  * before a reset or after t holds, a NaN or an infinity among it, does not reach out_t. */
 int hipenvs_selective_scan(int32_t dtype, const void* x, const void* dt, const float* rate, const void* write,
                            const void* read, const float* skip, const void* gate, const float* dt_bias,
@@ -476,7 +476,7 @@ int hipenvs_selective_scan_backward(int32_t dtype, const void* x, const void* dt
 /* One token of `count` environments: x, dt, gate (count, d), write, read (count, g, n), state
  * (count, d, n) f32 contiguous, reset (count) u8 or NULL -> out (count, d) contiguous, next_state, which
  * may be `state`. `strides`: of the environment in x, dt, gate, then of the environment and the group
- * in write, in read, then of reset. */
+ * in write, in read, then of reset. count d < 2^31. */
 int hipenvs_selective_scan_step(int32_t dtype, const void* x, const void* dt, const float* rate, const void* write,
                                 const void* read, const float* skip, const void* gate, const float* dt_bias,
                                 const float* state, const uint8_t* reset, const int64_t* strides, void* out,
@@ -488,7 +488,7 @@ int hipenvs_selective_scan_step(int32_t dtype, const void* x, const void* dt, co
  * without the taps that reach before the first token of t's episode. x (b, t, d) in dtype with unit
  * stride in the last axis; weight (d, w), bias (d) or NULL f32; state (b, w - 1, d) f32 contiguous, the
  * values before the row, or NULL (zeros); `strides`: b, t of x, then of reset (u8 or NULL)
- * -> out (b, t, d) contiguous, final_state (b, w - 1, d) f32 (not `state`). */
+ * -> out (b, t, d) contiguous, final_state (b, w - 1, d) f32 (not `state`). d <= 65536, b d < 2^31. */
 int hipenvs_causal_conv(int32_t dtype, const void* x, const float* weight, const float* bias, const float* state,
                         const uint8_t* reset, const int64_t* strides, int32_t silu, void* out, float* final_state,
                         int64_t b, int64_t t, int32_t d, int32_t w, hipenvs_stream_t stream);
@@ -506,7 +506,7 @@ int hipenvs_causal_conv_backward(int32_t dtype, const void* x, const float* weig
                                  hipenvs_stream_t stream);
 
 /* One token of n environments: x (n, d) with stride x_sn, state (n, w - 1, d) f32 contiguous -> out
- * (n, d) contiguous, next_state, which may be `state`. */
+ * (n, d) contiguous, next_state, which may be `state`. n d < 2^31. */
 int hipenvs_causal_conv_step(int32_t dtype, const void* x, int64_t x_sn, const float* weight, const float* bias,
                              const float* state, const uint8_t* reset, int64_t reset_sn, int32_t silu, void* out,
                              float* next_state, int64_t n, int32_t d, int32_t w, hipenvs_stream_t stream);

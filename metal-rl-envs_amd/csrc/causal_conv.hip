@@ -10,7 +10,8 @@
 // value is read once but for the W - 1 at a run's borders. A block's threads walk the same tokens, so
 // what depends on the token alone is scalar. 64 x 1,000 tokens of 501 channels, bfloat16 at odd addresses: 41 us,
 // 3.1 TB/s, and 76 + 10 backwards, 2.5 TB/s, bound by vector instructions (about 55 and 60 % of the time) and
-// by the latency that two waves a SIMD leave backwards (200 registers; three waves spill: 180 us).
+// by the latency that two waves a SIMD leave backwards (204 registers; three waves spill: 180 us). In float32, with
+// 248 registers backwards, 61 us, and 170 for both.
 #include "row_ops.h"
 
 namespace hipenvs {
@@ -322,7 +323,9 @@ bool sequence_ok(int32_t dtype, int64_t b, int64_t t, int32_t d, int32_t w) {
 
 // Runs of 64 tokens, shorter (down to 8) while the card has fewer waves than it holds: eight a CU
 // forwards, and half of that backwards, where a run costs a row of partial sums (64 x 1,000 x 501
-// bfloat16: 84 + 13 us with runs of 32, 76 + 10 with 64).
+// bfloat16: 84 + 13 us with runs of 32, 76 + 10 with 64). By this rule, with runs of 64 and of 8 throughout, in us,
+// bfloat16: 64 x 1,000 x 501 41, 45 and 54 (both passes 120, 120, 194), 16 x 1,000 x 501 21, 33 and 21 (55, 91, 66),
+// 1 x 16,381 x 512 18, 30 and 20 (57, 83, 79), 128 x 64 x 64 9, 26 and 9 (26, 75, 26).
 int plan(Conv* s, int64_t b, int64_t t, int32_t d, bool back) {
   int cus = 0;
   const int status = device_cus(&cus);

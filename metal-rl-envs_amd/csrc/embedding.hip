@@ -310,7 +310,9 @@ __global__ __launch_bounds__(kBlock) void across_kernel(Sums s) {
 // A table of at most kSmall rows is summed without sorting: each group of lanes of a block takes every
 // so many of its tokens and adds their rows to sums of its own in LDS; a block's groups then meet, and the
 // blocks' sums are the rows of a matrix whose columns are added up. 524,288 tokens of 3 x 64 float32, 134 MB:
-// 27 + 8 us, 4.9 TB/s, against 134 sorted. A thread's sums are its own, so their order is that of the tokens.
+// 27 + 8 us, 4.9 TB/s. The lookup and its gradient, so and sorted: that 60 and 156 us, of 8 rows 61 and 122, of
+// 16, which leave LDS for two blocks a CU, 88 and 114; 64,000 tokens of 2 x 512 bfloat16 46 and 106, of 8 53 and 72,
+// of 16 69 and 66; 3,000 of 16 x 64 float32 16 and 28. A thread's sums are its own, so their order is that of the tokens.
 
 constexpr int kSmall = 16;
 
@@ -370,7 +372,8 @@ int group_of(int quads) {
   return group;
 }
 
-// Blocks of a small table's sums: four a CU of 256, but no fewer than eight tokens for a group of lanes.
+// Blocks of a small table's sums: four a CU of 256 (from 11 rows on LDS holds fewer at once), but no fewer than
+// eight tokens for a group of lanes.
 int64_t small_blocks(int64_t count, int32_t d) {
   const int64_t least = 8 * (kBlock / group_of((d + 3) / 4)), blocks = (count + least - 1) / least;
   return blocks < 1024 ? blocks : 1024;

@@ -53,10 +53,12 @@ __device__ __forceinline__ float masked(float x, uint32_t bits) { return __uint_
 //
 // Bound by its vector instructions, which issue all of the time at 4,096 x 128 tokens of 128 channels, float32:
 // 44 a token for 16 channels of 16 states, 22 of them the walk (two for each exponential), the rest what a
-// tile's elements take (softplus, the gate, addresses). 370 us there, 2.5 TB/s; 16,381 tokens of 512 channels
-// in parts 36 + 15 + 51 us. Tiles of eight tokens took 442, of one row in fewer parts (eight waves a CU
-// instead of 16) 41 + 9 + 64. Loads that a branch or a conversion separates wait for each other: 73 us for the
-// 51 before they went.
+// tile's elements take: softplus, the gate, addresses, and reading back the scalars that spill into vector lanes
+// (53 to 82 with outputs, 21 to 41 without; none in the walks). 340 to 370 us there, 2.5 TB/s and more; 16,381
+// tokens of 512 channels in parts 36 + 15 + 51 us. n counts as the 8, 16, 32 or 64 states that the lanes hold:
+// 1,024 x 128 x 128, bfloat16, 62 us for n = 8, 96 for 9, 86 for 16, 178 for 17, 160 for 32, 352 for 33, 318 for 64.
+// Tiles of eight tokens took 442, of one row in fewer parts (eight waves a CU instead of 16) 41 + 9 + 64. Loads
+// that a branch or a conversion separates wait for each other: 73 us for the 51 before they went.
 template <class T, int LPC, bool kFew, bool kFull, bool kOut>
 __global__ __launch_bounds__((Shape<LPC, kFew>::kThreads)) void forward_kernel(Scan s) {
   using S = Shape<LPC, kFew>;
@@ -293,8 +295,11 @@ __global__ __launch_bounds__((Shape<LPC, kFew>::kThreads)) void passed_kernel(Sc
 // wave, then through LDS, then (dmix) over the blocks of a group.
 //
 // Bound by instruction issue at the two waves a SIMD that 128 registers of decays and states leave (a vector
-// one 81 % of the time, 118 a token for 16 channels of 16 states): 1,190 us for 4,096 x 128 tokens of 128
-// channels, float32, of which the sums over channels take some 190, the exponentials 155 and the outputs 165.
+// one 81 % of the time, 120 a token for 16 channels of 16 states): 1,100 to 1,200 us for 4,096 x 128 tokens of 128
+// channels, float32, of which the sums over channels take some 190, the exponentials 155 and the outputs 165. Among
+// them are the reads of 134 to 181 scalars that spill into vector lanes, none in the walks. Vector registers spill
+// in float32 with two lanes a channel, 6 to 12 of them, and 2 with eight or 16 lanes, few channels and all states:
+// 1,024 x 128 x 128 forwards and backwards 326 us for n = 8 where bfloat16, without, takes 246.
 // Before the next tile's loads were waited for ahead of the outputs' stores, and its addresses kept from tile to
 // tile, it took 1,290; then, three waves with the decays computed again instead of held 1,340, tiles of
 // eight tokens with three waves 1,620.
@@ -612,7 +617,10 @@ bool sequence_ok(int32_t dtype, int64_t b, int64_t t, int32_t d, int32_t n, int3
 int64_t blocks_of(const Scan& s, int64_t parts) { return s.b * parts * s.g * s.tiles; }
 
 // Sizes, and the parts of a row: as many as fill the card with the waves that a CU holds of the pass, 16
-// forwards and 8 backwards, no part below 64 tokens.
+// forwards and 8 backwards, no part below 64 tokens; none from more than four waves a CU on, where every token is
+// walked twice to fill what little of the card is free. Rows of 2,048 x 512 x 16, bfloat16, in parts and without, in us:
+// 32 rows, the last in parts, 277 and 331 (forwards and backwards 1,000 and 1,150); 33 rows, the first without, 371
+// and 407 (1,459 and 1,507), 48 rows 428 and 409 (1,533 and 1,524), 64 rows 495 and 411 (1,610 and 1,535).
 int plan(Scan* s, int64_t b, int64_t t, int32_t d, int32_t n, int32_t g, bool back) {
   int cus = 0;
   const int status = device_cus(&cus);
