@@ -27,17 +27,19 @@ __device__ __forceinline__ void for_kind(uint32_t begins, int n, const F& walk) 
   }
 }
 
-// Four states' rates times log2(e); those past n decay, so that an infinite delta leaves them at zero. An infinite
-// one is as good as float32's largest, and times a delta of zero, which stands for that of an episode's first
-// token, it is a number.
-__device__ __forceinline__ f32x4 rates_of(const Scan& s, int64_t c, int n0, int left) {
+// A rate times log2(e). An infinite one is as good as float32's largest, and times a delta of zero, which stands
+// for that of an episode's first token in a walk, it is a number.
+__device__ __forceinline__ float rate_of(float rate) {
   constexpr float kMost = 0x1.fffffep+127f;
-  f32x4 rate = load_upto(s.rate + c * s.n + n0, left);
+  const float x = rate * kLog2e;
+  return x > kMost ? kMost : x < -kMost ? -kMost : x;   // a NaN stays
+}
+
+// Four states' rates; those past n decay, so that an infinite delta leaves them at zero.
+__device__ __forceinline__ f32x4 rates_of(const float* from, int left) {
+  f32x4 rate = load_upto(from, left);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float x = (e < left ? rate[e] : -1.0f) * kLog2e;
-    rate[e] = x > kMost ? kMost : x < -kMost ? -kMost : x;   // a NaN stays
-  }
+  for (int e = 0; e < 4; ++e) rate[e] = rate_of(e < left ? rate[e] : -1.0f);
   return rate;
 }
 
@@ -72,7 +74,7 @@ __global__ __launch_bounds__((Shape<LPC, kFew>::kThreads)) void forward_kernel(S
   const int64_t c = (int64_t)at.group * s.dg + at.first + ch;
   const int64_t start = at.p * s.part, end = start + s.part < s.t ? start + s.part : s.t;
   const int left = live ? s.n - n0 : 0;
-  const f32x4 rate = rates_of(s, c, n0, left);
+  const f32x4 rate = rates_of(s.rate + c * s.n + n0, left);
   f32x4 h = {0.0f, 0.0f, 0.0f, 0.0f};
   if (kOut) {
     if (s.parts > 1)
@@ -176,11 +178,11 @@ __global__ __launch_bounds__((Shape<LPC, kFew>::kThreads)) void forward_kernel(S
   }
 }
 
-// A state carried over a part: exp(rate * the part's sum of delta) of it, and nothing over an
-// episode's beginning. Token by token, an infinite state and a zero one stay what they are, which
+// A state carried over a part: exp(rate * the part's sum of delta) of it, `rate` times log2(e), and nothing
+// over an episode's beginning. Token by token, an infinite state and a zero one stay what they are, which
 // their product with a decay that leaves float32's range would not.
 __device__ __forceinline__ float carried(float rate, float span, float state) {
-  const float decay = exp2_of(span * (rate * kLog2e));
+  const float decay = exp2_of(span * rate);
   return state == 0.0f || __builtin_isinf(state) ? state : decay * state;
 }
 
@@ -193,7 +195,7 @@ __global__ __launch_bounds__(kBlock) void join_kernel(Scan s) {
   const int64_t b = i / each, x = i - b * each, c = x / s.n;
   const float* first = kBack ? s.dfinal : s.state;
   float state = first ? first[i] : 0.0f;
-  const float rate = s.rate[x];
+  const float rate = rate_of(s.rate[x]);
   constexpr int kAhead = 32;
   for (int p0 = 0; p0 < s.parts; p0 += kAhead) {
     float own[kAhead], span[kAhead];
@@ -228,7 +230,7 @@ __global__ __launch_bounds__((Shape<LPC, kFew>::kThreads)) void passed_kernel(Sc
   const int64_t c = (int64_t)at.group * s.dg + at.first + ch;
   const int64_t start = at.p * s.part, end = start + s.part < s.t ? start + s.part : s.t;
   const int left = live ? s.n - n0 : 0;
-  const f32x4 rate = rates_of(s, c, n0, left);
+  const f32x4 rate = rates_of(s.rate + c * s.n + n0, left);
   f32x4 g = {0.0f, 0.0f, 0.0f, 0.0f};
   const int own = at.first + At::channel();
   const f32x4 bias = per_channel(s.bias, (int64_t)at.group * s.dg + own, s.dg - own, 0.0f);
@@ -320,7 +322,7 @@ __global__ __launch_bounds__((Shape<LPC, kFew>::kThreads), 2) void backward_kern
   const int64_t c = (int64_t)at.group * s.dg + at.first + ch;
   const int64_t start = at.p * s.part, end = start + s.part < s.t ? start + s.part : s.t;
   const int left = live ? s.n - n0 : 0;
-  const f32x4 rate = rates_of(s, c, n0, left);
+  const f32x4 rate = rates_of(s.rate + c * s.n + n0, left);
   f32x4 g = {0.0f, 0.0f, 0.0f, 0.0f}, drate = g;
   if (s.parts > 1)
     g = load_upto(s.carry + ((at.b * s.parts + at.p) * s.d + c) * s.n + n0, left);
@@ -577,9 +579,7 @@ __global__ __launch_bounds__(kBlock) void step_kernel(Step s) {
     z[k] = s.gate ? ((const T*)s.gate)[env * s.gate_s + c] : (T)0.0f;
     begins[k] = s.reset ? s.reset[env * s.reset_s] : 0;
   }
-  f32x4 rate = load_upto(s.rate + (int64_t)c * s.n + n0, left);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) rate[e] = e < left ? rate[e] : -1.0f;
+  const f32x4 rate = rates_of(s.rate + (int64_t)c * s.n + n0, left);
   const float bias = s.bias ? s.bias[c] : 0.0f, skip = s.skip ? s.skip[c] : 0.0f;
 #pragma unroll
   for (int k = 0; k < kEnvs; ++k) {
@@ -591,7 +591,7 @@ __global__ __launch_bounds__(kBlock) void step_kernel(Step s) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float own = du * wk[e];
-      state[e] = begins[k] ? own : __builtin_fmaf(exp2_of(delta * (rate[e] * kLog2e)), state[e], own);
+      state[e] = begins[k] ? own : __builtin_fmaf(exp2_of(delta * rate[e]), state[e], own);
       state[e] = e < left ? state[e] : 0.0f;   // zero times an infinity
       y = __builtin_fmaf(rk[e], state[e], y);
     }

@@ -111,6 +111,34 @@ def test_scan_infinite_decay_at_an_episodes_first_token(dev, n, t):
     assert ((o - out[:, at]).abs() <= 2 * (n + 16) * 2.0 ** -24 * out[:, at]).all()   # the same sums, in either order
 
 
+@pytest.mark.parametrize("n", [3, 16])
+@pytest.mark.parametrize("t", [40, 900])
+def test_scan_infinite_rates(dev, n, t):
+    """A rate of -inf keeps nothing of the state before, and all of it where delta is zero; walked whole, in parts
+    and step by step."""
+    from hipenvs import selective_scan
+
+    b, d = 1, 4
+    x, mix, state = torch.ones(b, t, d, device=dev), torch.ones(b, t, n, device=dev), torch.full((b, d, n), 2.0, device=dev)
+    rate = torch.full((d, n), -INF, device=dev)
+    reset = torch.zeros(b, t, dtype=torch.bool, device=dev)
+    reset[0, t // 2] = True
+    for value, want in ((-300.0, 0.0), (3.0, float(np.log1p(np.exp(3.0))))):
+        dt = torch.full((b, t, d), value, device=dev)
+        kept = value < 0
+        for begins in (None, reset):
+            out, final = selective_scan.sequence(x, dt, rate, mix, mix, state=state, reset=begins)
+            last = state if kept and begins is None else torch.full_like(state, want)
+            # one token's delta, within 8 units of 2^-24, and its product; sums of n of them
+            assert ((final - last).abs() <= 9 * 2.0 ** -24 * last).all()
+            held = state.clone()
+            for i in range(t):
+                o, _ = selective_scan.step(x[:, i], dt[:, i], rate, mix[:, i], mix[:, i], state=held,
+                                           reset=None if begins is None else begins[:, i], next_state=held)
+                assert ((o - out[:, i]).abs() <= 2 * n * 2.0 ** -24 * out[:, i]).all()
+            assert torch.equal(held, final)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("w", [2, 3, 4])
 def test_conv_infinite_gradient_next_to_an_episodes_first_tokens(dev, w, dtype):
